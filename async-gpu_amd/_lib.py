@@ -17,6 +17,7 @@ ERR_NULL_POINTER, ERR_UNSUPPORTED, ERR_WORKSPACE, ERR_DEVICE_WAIT, ERR_BUSY = -4
 EPI_NONE, EPI_GELU_TANH, EPI_GELU_QUICK, EPI_FORCE_LITERAL, EPI_FORCE_FP32_GEMV = 0, 1, 2, 0x100, 0x200
 QUANT_RUST, QUANT_SCRIPT = 0, 1
 GELU_TANH, GELU_QUICK = 0, 1
+CACHE_F32, CACHE_F16, CACHE_BF16 = 0, 1, 2
 
 
 class AgpuError(RuntimeError):
@@ -94,6 +95,10 @@ SIGNATURES = {
     "agpu_attention": (_i32, [_vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32]),
     "agpu_bench_attention": (_i32, [_vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _vp]),
     "agpu_kv_append": (_i32, [_vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32]),
+    "agpu_paged_plan": (_i32, [_vp] * 11 + [_i32] * 5),
+    "agpu_paged_kv_append": (_i32, [_vp] * 3 + [C.c_int64] * 4 + [_vp] * 2 + [C.c_int64] * 2 + [_vp] + [_i32] * 6),
+    "agpu_paged_attention": (_i32, [_vp] * 2 + [C.c_int64] * 2 + [_vp] * 2 + [C.c_int64] * 2 + [_vp] * 4 + [_i32] * 11),
+    "agpu_sample": (_i32, [_vp] * 4 + [_i32] * 2 + [_f, _i32, _f, _f] + [_vp] * 4),
     "agpu_gemm_f32": (_i32, [_vp, _vp, _vp, _vp, _i32, _i32, _i32]),
     # include/agpu_gpt2.h (first argument is the model handle, or the config / context)
     "agpu_gpt2_config_small": (_i32, [_vp]),

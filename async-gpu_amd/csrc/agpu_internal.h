@@ -96,6 +96,26 @@ struct agpu_ctx_guard {
         if (!(p)) return agpu_fail((ctx), AGPU_ERR_NULL_POINTER, "%s: null pointer " #p, __func__); \
     } while (0)
 
+// Makes the context's device the current one until the end of the scope: a launch on the default stream goes to the current device.
+struct agpu_on_device {
+    int prev = -1;
+    int32_t rc = AGPU_OK;
+    explicit agpu_on_device(agpu_ctx *ctx) {
+        int now = -1;
+        hipError_t e = hipGetDevice(&now);
+        if (e == hipSuccess && now != ctx->device) {
+            e = hipSetDevice(ctx->device);
+            if (e == hipSuccess) prev = now;
+        }
+        rc = agpu_hip(ctx, e, "hipSetDevice");
+    }
+    ~agpu_on_device() {
+        if (prev >= 0) (void)hipSetDevice(prev);
+    }
+    agpu_on_device(const agpu_on_device &) = delete;
+    agpu_on_device &operator=(const agpu_on_device &) = delete;
+};
+
 #define AGPU_LAUNCH_CHECK(ctx, name) agpu_hip((ctx), hipGetLastError(), name)
 
 // ---- device helpers ---------------------------------------------------------------
@@ -125,6 +145,13 @@ template <int CTRL, int ROW_MASK>
 __device__ __forceinline__ float dpp_move(float old, float v) {
     return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, old), __builtin_bit_cast(int, v), CTRL,
                                                                  ROW_MASK, 0xf, false));
+}
+
+// Four floats from any address (a multiple of four bytes).
+typedef float agpu_float4_u __attribute__((ext_vector_type(4), aligned(4)));
+__device__ __forceinline__ float4 load4(const float *p) {
+    const agpu_float4_u v = *reinterpret_cast<const agpu_float4_u *>(p);
+    return make_float4(v[0], v[1], v[2], v[3]);
 }
 
 // Sum / maximum over each row of 16 lanes, result in every lane of the row.

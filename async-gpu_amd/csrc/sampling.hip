@@ -21,6 +21,7 @@
 // need not be: with the row kept in registers and 52 places that gather, 25 us).  50257 logits, k = 40: 12.4 us a launch; 18.9 with a
 // barrier a bit for the bound and all of the row read twice.
 #include "agpu_internal.h"
+#include "sampling.h"
 
 #include <cmath>
 #include <cstring>
@@ -32,16 +33,6 @@ constexpr int TK_THREADS = 1024, TK_WAVES = TK_THREADS / 64, TK_MAX_N = 65536, T
 constexpr int TK_CAND = 8192;  // gathered elements LDS has room for (64 KB)
 constexpr int TK_UNROLL = 16;  // elements of the row a thread has on their way at a time, where it is read again
 constexpr int TK_RUNS = 13;     // runs of four elements a thread has on their way at a time
-
-__device__ __forceinline__ uint32_t order_key(float x) {
-    if (x != x) return 0u;
-    const uint32_t u = x == 0.0f ? 0u : __float_as_uint(x);  // -0.0 and 0.0 are one value
-    return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
-}
-
-__device__ __forceinline__ float key_value(uint32_t key) {
-    return __uint_as_float((key & 0x80000000u) ? (key & 0x7fffffffu) : ~key);
-}
 
 // Sum of one wave-uniform count per wave over the workgroup; buffers alternate so one barrier per call is enough.
 __device__ __forceinline__ int block_count(int wave_count, int (*scratch)[TK_WAVES], int &phase, int lane, int wave) {

@@ -26,7 +26,8 @@ namespace {
 #define AGPU_OPS(X)                                                                                                          \
     X(agpu_int4_linear) X(agpu_ln_int4_linear) X(agpu_layer_norm) X(agpu_add_layer_norm_dual) X(agpu_gelu)                    \
     X(agpu_add_inplace) X(agpu_bias_add) X(agpu_softmax_rows) X(agpu_embedding) X(agpu_argmax_rows) X(agpu_split_qkv)         \
-    X(agpu_concat_heads) X(agpu_attention) X(agpu_kv_append) X(agpu_gemm_f32) X(agpu_last_error_string)
+    X(agpu_concat_heads) X(agpu_attention) X(agpu_kv_append) X(agpu_gemm_f32) X(agpu_last_error_string)          \
+    X(agpu_paged_plan) X(agpu_paged_kv_append) X(agpu_paged_attention) X(agpu_sample)
 struct Lib {
 #define X(f) decltype(&f) f##_ = nullptr;
     AGPU_OPS(X)
@@ -403,6 +404,152 @@ PyObject *gemm_f32(PyObject *const *a) {
     return wrap(std::move(c));
 }
 
+// ---- several requests over a cache in pages --------------------------------------------------
+
+// A tensor of a given type and rank; sizes of -1 are any.
+const at::Tensor &typed(PyObject *o, at::ScalarType type, std::initializer_list<int64_t> sizes, const char *what) {
+    const at::Tensor &t = tensor(o);
+    bool fits = t.dim() == (int64_t)sizes.size();
+    int64_t d = 0;
+    for (const int64_t s : sizes) fits = fits && (s < 0 || t.size(d) == s), ++d;
+    if (!fits) shape_err(what, str(t.sizes()));
+    if (t.scalar_type() != type) shape_err(std::string(what) + " of " + c10::toString(type), c10::toString(t.scalar_type()));
+    return t;
+}
+const at::Tensor &ints(PyObject *o, std::initializer_list<int64_t> sizes, const char *what) {
+    const at::Tensor &t = typed(o, at::kInt, sizes, what);
+    if (!t.is_contiguous()) shape_err(std::string("contiguous ") + what, "strides " + str(t.strides()));
+    return t;
+}
+// All on one GPU: the one that the operator runs on.
+template <class... T>
+void together(const at::Tensor &first, const T &...others) {
+    if (!first.is_cuda() || !(... && (others.device() == first.device()))) {
+        PyErr_SetString(PyExc_AssertionError, "expects device tensors, all on one GPU");
+        throw PyFail();
+    }
+}
+const int32_t *ip(const at::Tensor &t) { return static_cast<const int32_t *>(t.const_data_ptr()); }
+int32_t *iw(const at::Tensor &t) { return static_cast<int32_t *>(t.mutable_data_ptr()); }
+
+// K or V in pages: [n_pages, n_kv_heads, page_size, 64], a page contiguous, pages anywhere
+const at::Tensor &pages(PyObject *o, const char *what) {
+    const at::Tensor &t = tensor(o);
+    rank(t, 4, what);
+    const auto ty = t.scalar_type();
+    if (ty != at::kFloat && ty != at::kHalf && ty != at::kBFloat16) shape_err("a cache of float32, float16 or bfloat16", c10::toString(ty));
+    const int64_t heads = t.size(1), size = t.size(2), dh = t.size(3);
+    if ((dh > 1 && t.stride(3) != 1) || (size > 1 && t.stride(2) != dh) || (heads > 1 && t.stride(1) != size * dh))
+        shape_err("contiguous pages [n_kv_heads, page_size, d_head]", "strides " + str(t.strides()));
+    return t;
+}
+int32_t cache_type(const at::Tensor &t) {
+    return t.scalar_type() == at::kFloat ? AGPU_CACHE_F32 : t.scalar_type() == at::kHalf ? AGPU_CACHE_F16 : AGPU_CACHE_BF16;
+}
+void same_cache(const at::Tensor &k, const at::Tensor &v) {
+    if (k.sizes() != v.sizes() || k.scalar_type() != v.scalar_type()) shape_err("k_cache and v_cache alike", str(k.sizes()) + ", " + str(v.sizes()));
+}
+int64_t page_stride(const at::Tensor &t) { return t.size(0) > 1 ? t.stride(0) : t.size(1) * t.size(2) * t.size(3); }
+// Rows [tokens, heads, d_head] at any two strides
+const at::Tensor &rows(PyObject *o, int64_t tokens, int64_t heads, int64_t dh, const char *what) {
+    const at::Tensor &t = typed(o, at::kFloat, {tokens, heads, dh}, what);
+    if (t.size(2) > 1 && t.stride(2) != 1) shape_err(std::string(what) + " with contiguous rows of a head", "strides " + str(t.strides()));
+    return t;
+}
+
+// cached_lens, new_lens, block_tables, free_pages, n_free, page_size, max_tokens
+PyObject *paged_plan(PyObject *const *a) {
+    const at::Tensor &tables = ints(a[2], {-1, -1}, "block_tables [batch, width]");
+    const int64_t batch = tables.size(0);
+    const at::Tensor &cached = ints(a[0], {batch}, "cached_lens [batch]"), &fresh = ints(a[1], {batch}, "new_lens [batch]");
+    const at::Tensor &stack = ints(a[3], {-1}, "free_pages [stack_size]"), &n_free = ints(a[4], {1}, "n_free [1]");
+    const int64_t max_tokens = integer(a[6]);
+    if (max_tokens < 0) shape_err("max_tokens >= 0", str(max_tokens));
+    together(tables, cached, fresh, stack, n_free);
+    std::array<at::Tensor, 5> t;
+    const int64_t sizes[5] = {batch, batch + 1, max_tokens, max_tokens, 1};
+    for (int i = 0; i < 5; ++i) t[i] = empty({sizes[i]}, tables, at::kInt);
+    int32_t *const tp = iw(tables), *const sp = iw(stack);
+    call(lib.agpu_paged_plan_, context(tables), ip(cached), ip(fresh), tp, sp, ip(n_free), iw(t[0]), iw(t[1]), iw(t[2]), iw(t[3]), iw(t[4]), i32(batch),
+         i32(tables.size(1)), i32(stack.numel()), i32(a[5]), i32(max_tokens));
+    return Py_BuildValue("(NNNNN)", wrap(std::move(t[0])), wrap(std::move(t[1])), wrap(std::move(t[2])), wrap(std::move(t[3])), wrap(std::move(t[4])));
+}
+
+// k, v, k_cache, v_cache, slots
+PyObject *paged_kv_append(PyObject *const *a) {
+    const at::Tensor &kc = pages(a[2], "k_cache [n_pages, n_kv_heads, page_size, d_head]"), &vc = pages(a[3], "v_cache [n_pages, n_kv_heads, page_size, d_head]");
+    same_cache(kc, vc);
+    const at::Tensor &slots = ints(a[4], {-1}, "slots [tokens]");
+    const int64_t tokens = slots.size(0), heads = kc.size(1), dh = kc.size(3);
+    const at::Tensor &k = rows(a[0], tokens, heads, dh, "k [tokens, n_kv_heads, d_head]"), &v = rows(a[1], tokens, heads, dh, "v [tokens, n_kv_heads, d_head]");
+    together(kc, vc, slots, k, v);
+    void *const kp = kc.mutable_data_ptr(), *const vp = vc.mutable_data_ptr();
+    call(lib.agpu_paged_kv_append_, context(kc), data(k), data(v), k.stride(0), k.stride(1), v.stride(0), v.stride(1), kp, vp, page_stride(kc), page_stride(vc),
+         ip(slots), i32(tokens), i32(heads), i32(kc.size(0)), i32(kc.size(2)), i32(dh), cache_type(kc));
+    return Py_BuildValue("(OO)", a[2], a[3]);
+}
+
+// q, k_cache, v_cache, block_tables, kv_lens, query_start, window, sinks, out
+PyObject *paged_attention(PyObject *const *a) {
+    const at::Tensor &kc = pages(a[1], "k_cache [n_pages, n_kv_heads, page_size, d_head]"), &vc = pages(a[2], "v_cache [n_pages, n_kv_heads, page_size, d_head]");
+    same_cache(kc, vc);
+    const at::Tensor &q = rows(a[0], -1, -1, kc.size(3), "q [tokens, n_heads, d_head]");
+    const at::Tensor &tables = ints(a[3], {-1, -1}, "block_tables [batch, width]");
+    const int64_t tokens = q.size(0), heads = q.size(1), batch = tables.size(0);
+    const at::Tensor &lens = ints(a[4], {batch}, "kv_lens [batch]");
+    const bool ragged = a[5] != Py_None, given = a[8] != Py_None;
+    const at::Tensor &start = ragged ? ints(a[5], {batch + 1}, "query_start [batch + 1]") : lens;
+    if (!ragged && tokens != batch) shape_err("a row for each of " + str(batch) + " requests without query_start", str(tokens));
+    if (given) {
+        const at::Tensor &o = typed(a[8], at::kFloat, {tokens, heads, q.size(2)}, "out [tokens, n_heads, d_head]");
+        if (!o.is_contiguous()) shape_err("contiguous out", "strides " + str(o.strides()));
+        for (const at::Tensor *t : {&q, &kc, &vc})
+            if (o.is_alias_of(*t)) shape_err("out with memory of its own", "that of an input");
+    }
+    together(q, kc, vc, tables, lens, start);
+    at::Tensor o = given ? tensor(a[8]) : empty(q.sizes(), q);
+    together(q, o);
+    float *const op = written(o);
+    call(lib.agpu_paged_attention_, context(q), data(q), q.stride(0), q.stride(1), kc.const_data_ptr(), vc.const_data_ptr(), page_stride(kc), page_stride(vc), ip(tables),
+         ip(lens), ragged ? ip(start) : nullptr, op, i32(tokens), i32(batch), i32(heads), i32(kc.size(1)), i32(kc.size(0)), i32(kc.size(2)), i32(tables.size(1)),
+         i32(a[6]), i32(a[7]), i32(q.size(2)), cache_type(kc));
+    return given ? same(a[8]) : wrap(std::move(o));
+}
+
+// A setting of sample: a number for all rows, or a tensor with one a row
+struct PerRow {
+    const at::Tensor *t = nullptr;
+    PerRow(PyObject *o, at::ScalarType type, int64_t n, const at::Tensor &like, const char *what) {
+        if (!THPVariable_Check(o)) return;
+        t = &typed(o, type, {n}, what);
+        if (!t->is_contiguous()) shape_err(std::string("contiguous ") + what, "strides " + str(t->strides()));
+        if (t->device() != like.device()) {
+            PyErr_SetString(PyExc_AssertionError, "expects device tensors, all on one GPU");
+            throw PyFail();
+        }
+    }
+    const float *floats() const { return t ? data(*t) : nullptr; }
+};
+
+// logits, u, temperature, top_k, top_p, min_p
+PyObject *sample(PyObject *const *a) {
+    const at::Tensor &x = tensor(a[0]), &u = tensor(a[1]);
+    const int64_t n = last(x), count = n ? x.numel() / n : 0;
+    if (x.scalar_type() != at::kFloat || u.scalar_type() != at::kFloat) shape_err("logits and u of Float", std::string(c10::toString(x.scalar_type())) + ", " + c10::toString(u.scalar_type()));
+    if (n == 0) shape_err("logits of at least one token", str(x.sizes()));
+    if (u.numel() != count) shape_err("u with a number for each of " + str(count) + " rows", str(u.sizes()));
+    if (!x.is_contiguous() || !u.is_contiguous()) shape_err("contiguous logits and u", "strides " + str(x.strides()) + ", " + str(u.strides()));
+    const PerRow temperature(a[2], at::kFloat, count, x, "temperature [rows]"), top_k(a[3], at::kInt, count, x, "top_k [rows]");
+    const PerRow top_p(a[4], at::kFloat, count, x, "top_p [rows]"), min_p(a[5], at::kFloat, count, x, "min_p [rows]");
+    const float t = temperature.t ? 1.0f : real(a[2]), p = top_p.t ? 1.0f : real(a[4]), m = min_p.t ? 0.0f : real(a[5]);
+    const int32_t k = top_k.t ? 0 : i32(a[3]);
+    together(x, u);
+    at::Tensor out = empty(x.sizes().slice(0, x.dim() - 1), x, at::kInt);
+    call(lib.agpu_sample_, context(x), data(x), data(u), iw(out), i32(count), i32(n), t, k, p, m, temperature.floats(), top_k.t ? ip(*top_k.t) : nullptr, top_p.floats(),
+         min_p.floats());
+    return wrap(std::move(out));
+}
+
 // ---- the module ---------------------------------------------------------------------------
 
 template <PyObject *(*OP)(PyObject *const *), int NARGS>
@@ -451,7 +598,7 @@ PyObject *forget(PyObject *, PyObject *handle) {
 PyMethodDef methods[] = {
     OP(int4_linear, 9), OP(layer_norm, 4), OP(add_layer_norm_dual, 6), OP(gelu, 2), OP(add_inplace, 2), OP(bias_add, 2), OP(softmax_rows, 1),
     OP(embedding, 4), OP(argmax_rows, 2), OP(split_qkv, 3), OP(concat_heads, 1), OP(attention, 6), OP(multi_head_flash_attention, 6),
-    OP(kv_append, 3), OP(gemm_f32, 2),
+    OP(kv_append, 3), OP(gemm_f32, 2), OP(paged_plan, 7), OP(paged_kv_append, 5), OP(paged_attention, 9), OP(sample, 6),
     {"bind", bind, METH_VARARGS, nullptr}, {"forget", forget, METH_O, nullptr}, {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_torch_ops", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -196,6 +196,40 @@ def gemm_f32(a, b):
     return _native.gemm_f32(a, b)
 
 
+# ---- several requests over a KV cache in pages: a step is paged_plan, then per layer paged_kv_append and paged_attention, then sample.
+# Lengths, tables and slots are int32 device tensors; nothing waits for the host.  A cache is two tensors [n_pages, n_kv_heads, page_size, 64] of
+# float32, float16 or bfloat16 whose pages may lie apart (slices of a larger pool).
+
+
+def paged_plan(cached_lens, new_lens, block_tables, free_pages, n_free, page_size, max_tokens):
+    """Pages and places for the new tokens of the requests: -> (kv_lens [batch], query_start [batch + 1], slots [max_tokens], positions
+    [max_tokens], n_free [1]).  new_lens below 0: the request has ended and gives its pages back.  block_tables [batch, width] and free_pages (a
+    stack of page ids, the first n_free of them) are updated in place; the next step takes kv_lens as cached_lens and the n_free returned.
+    Requests are served in order while pages and max_tokens last; those that were not keep their length and have no row."""
+    return _native.paged_plan(cached_lens, new_lens, block_tables, free_pages, n_free, page_size, max_tokens)
+
+
+def paged_kv_append(k, v, k_cache, v_cache, slots):
+    """K and V rows [tokens, n_kv_heads, 64] (any strides of tokens and heads, so slices of QKV rows too) into their slots of the cache, in place;
+    a slot outside of it (-1) writes nothing.  Returns (k_cache, v_cache)."""
+    return _native.paged_kv_append(k, v, k_cache, v_cache, slots)
+
+
+def paged_attention(q, k_cache, v_cache, block_tables, kv_lens, query_start=None, window=0, sinks=0, out=None):
+    """Attention of the new rows of several requests over their pages: q [tokens, n_heads, 64] (any strides of tokens and heads) -> [tokens, n_heads, 64].
+    Rows query_start[b] .. query_start[b + 1] - 1 are the last positions of the kv_lens[b] of request b; without query_start each request
+    has one row.  A row at position p sees key j <= p, with window > 0 only where p - j < window or j < sinks.  n_heads is a multiple of the
+    cache's heads.  A row that sees nothing gives zeros; rows behind the last request's are not written (`out` keeps them)."""
+    return _native.paged_attention(q, k_cache, v_cache, block_tables, kv_lens, query_start, window, sinks, out)
+
+
+def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """The next token of each row of logits [..., n] from given numbers u in [0, 1), one a row -> int32 [...].  The settings are numbers, or tensors with
+    one a row: temperature, then the top_k first candidates (0: all), of those the nucleus of top_p, of those the ones with at least min_p of the
+    first one's probability.  With the same number it draws what top_k_sample draws.  -1: no logit of the row is above -inf."""
+    return _native.sample(logits, u, temperature, top_k, top_p, min_p)
+
+
 class SimpleRng:
     """SimpleRng (nn/models/gpt2.rs:1000-1023): xorshift64; next_f32 in [0, 1)."""
 

@@ -302,6 +302,20 @@ uint32_t agpu_top_k_draw_host(const float *ranked_vals, const uint32_t *ranked_i
  * k (index, value) pairs to the host, draw with the next value of the generator.  *token_out_host on the host. */
 int32_t agpu_top_k_sample(agpu_ctx *ctx, const float *logits, int32_t n, int32_t k, float temperature,
                           uint64_t *rng_state, uint32_t *token_out_host);
+/* The next token of each row of logits [rows, n] with the given numbers u [rows] of [0, 1); all of it on the device, and without a counterpart in the
+ * reference beyond its top-k.  w_i = exp((x_i - max_j x_j) / max(temperature, 1e-8)); the candidates are ranked by x (descending; equals by index,
+ * ascending) and filtered, each filter keeping a first part of the ranking and all of them the first candidate:
+ *   top_k > 0   the top_k first
+ *   top_p < 1   those before which less than top_p times the sum of the w that top_k leaves lies
+ *   min_p > 0   those with w_i >= min_p
+ * The token is the first of them whose running sum of w exceeds u times their sum (the last one if none does: u >= 1), so that
+ * with the same number it is the one that top_k_sample draws, up to that one's rounding.  A setting is one number for all rows, or where the array
+ * behind it is not NULL one number a row (device, [rows]).  NaN ranks with -inf and is never drawn; a row without any logit above -inf gives -1.
+ * Weights are rounded to 2^-b of the first one's, b = 62 - ceil(log2 n) or 50 if that is less (46 for 50257 logits), and
+ * their sums are exact; candidates below half of that have none.  n <= 2^20. */
+int32_t agpu_sample(agpu_ctx *ctx, const float *logits, const float *u, int32_t *tokens_out, int32_t rows, int32_t n, float temperature,
+                    int32_t top_k, float top_p, float min_p, const float *temperatures, const int32_t *top_ks, const float *top_ps,
+                    const float *min_ps);
 /* softmax_max_prob (gpt2.rs:983-988), the confidence probed by the early-exit callers: conf_out[row] =
  * 1 / sum_j exp(logits[row, j] - max_j logits[row, j]), the softmax probability of the row's arg-max; idx_out
  * (optional) receives that arg-max (first index among equals).  Device pointers; conf_out [rows], idx_out [rows].
@@ -355,6 +369,55 @@ int32_t agpu_bench_attention(agpu_ctx *ctx, const float *q, const float *k, cons
  * -> cache [H, max_seq, dh] at write_pos. */
 int32_t agpu_kv_append(agpu_ctx *ctx, const float *src, float *cache, int32_t n_heads, int32_t src_stride,
                        int32_t max_seq, int32_t write_pos, int32_t d_head);
+
+/* ---- a KV cache in pages, for several requests at once ------------------------------------ */
+/* No counterpart in the reference, whose cache holds one sequence (KvCache, nn/models/gpt2.rs:1064-1117).  A step of a server:
+ * agpu_paged_plan gives the requests their pages and their new tokens their places, agpu_paged_kv_append puts K and V there,
+ * agpu_paged_attention reads them, agpu_sample draws the next tokens.  Nothing of it waits for the host: lengths, tables and slots are
+ * device data, launch shapes follow from the sizes of the arguments alone, and a step may be captured into a HIP graph.
+ *   cache         K and V each [n_pages][n_kv_heads][page_size][64] of cache_type, pages *_page_stride elements apart (a multiple of 16
+ *                 bytes, the first at 16 bytes): what may lie between pages is the other one of K and V, or other layers
+ *   block_tables  [batch][table_width] int32: position p of request b is on page block_tables[b][p / page_size].  Only entries of
+ *                 positions that the call needs are read, so the others may hold anything.
+ *   slot          page * page_size + p % page_size */
+#define AGPU_CACHE_F32 0
+#define AGPU_CACHE_F16 1
+#define AGPU_CACHE_BF16 2
+/* Pages for the new tokens of `batch` requests (4096 at most), in the order of the requests.
+ *   cached_lens [batch]   positions that a request holds already; their pages are in its row of block_tables
+ *   new_lens [batch]      new tokens; 0: none in this step; below 0: the request has ended and its pages are free again
+ *   free_pages [stack_size], n_free [1]   a stack of free page ids and how many there are
+ * Pages of ended requests go onto the stack first, in order; then each request takes those that it needs from the top.  Requests are served in
+ * order while there are pages and while their tokens, added up, do not exceed max_tokens: from the first one that does not fit on, none
+ * gets anything.  A request that would not fit its row of block_tables is left out by itself.
+ *   kv_lens [batch]            positions with the new tokens: cached_lens + new_lens where the request was served, 0 where it has ended
+ *   query_start [batch + 1]    row of its first new token; [batch] is how many there are
+ *   slots, positions [max_tokens]   of every new token; -1 and 0 behind the last one
+ *   n_free_out [1]             free pages left.  block_tables and free_pages are updated in place, the latter below n_free_out only.
+ * Where n_free + the pages given back exceeds stack_size, what has no place on the stack is lost.  The outputs do not overlap the inputs.
+ * The next step takes kv_lens as cached_lens and n_free_out as n_free. */
+int32_t agpu_paged_plan(agpu_ctx *ctx, const int32_t *cached_lens, const int32_t *new_lens, int32_t *block_tables, int32_t *free_pages,
+                        const int32_t *n_free, int32_t *kv_lens, int32_t *query_start, int32_t *slots, int32_t *positions,
+                        int32_t *n_free_out, int32_t batch, int32_t table_width, int32_t stack_size, int32_t page_size,
+                        int32_t max_tokens);
+/* K and V rows of `tokens` new tokens into their slots, rounded to the cache's type (to nearest, ties to even).  k, v: row (t, h) of 64 floats at
+ * t * token_stride + h * head_stride elements, so that both [tokens, 3d] rows of a QKV projection and [H, tokens, 64] may be read as they are.
+ * A slot outside the cache (-1: padding) writes nothing.  Which row stays where two tokens have the same slot is not defined. */
+int32_t agpu_paged_kv_append(agpu_ctx *ctx, const float *k, const float *v, int64_t k_token_stride, int64_t k_head_stride,
+                             int64_t v_token_stride, int64_t v_head_stride, void *k_cache, void *v_cache, int64_t k_page_stride,
+                             int64_t v_page_stride, const int32_t *slots, int32_t tokens, int32_t n_kv_heads, int32_t n_pages,
+                             int32_t page_size, int32_t d_head, int32_t cache_type);
+/* Attention of the new rows of several requests over their pages.  Rows query_start[b] .. query_start[b + 1] - 1 of q are the last positions of
+ * the kv_lens[b] that request b has (K and V of the new tokens among them); query_start NULL: one row each, tokens == batch.  A row at
+ * position p sees key j <= p, with window > 0 only where p - j < window or j < sinks.  Query head h reads K/V head h / (n_heads / n_kv_heads).
+ *   q   row (t, h) of 64 floats at t * q_token_stride + h * q_head_stride elements;  o [tokens][n_heads][64]
+ * A row that sees no key gives zeros.  Rows behind the last request's are left as they were.  Keys on a page id outside the cache are not seen.
+ * K and V that a row does not see do not reach it, whatever they are.  Scores, weights and sums are fp32. */
+int32_t agpu_paged_attention(agpu_ctx *ctx, const float *q, int64_t q_token_stride, int64_t q_head_stride, const void *k_cache,
+                             const void *v_cache, int64_t k_page_stride, int64_t v_page_stride, const int32_t *block_tables,
+                             const int32_t *kv_lens, const int32_t *query_start, float *o, int32_t tokens, int32_t batch, int32_t n_heads,
+                             int32_t n_kv_heads, int32_t n_pages, int32_t page_size, int32_t table_width, int32_t window, int32_t sinks,
+                             int32_t d_head, int32_t cache_type);
 
 /* ---- f32 GEMM (the reference model's f32 LM head) --------------------------------------- */
 

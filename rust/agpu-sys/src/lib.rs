@@ -68,6 +68,9 @@ pub const AGPU_QUANT_RUST: i32 = 0;
 pub const AGPU_QUANT_SCRIPT: i32 = 1;
 pub const AGPU_GELU_TANH: i32 = 0;
 pub const AGPU_GELU_QUICK: i32 = 1;
+pub const AGPU_CACHE_F32: i32 = 0;
+pub const AGPU_CACHE_F16: i32 = 1;
+pub const AGPU_CACHE_BF16: i32 = 2;
 pub const AGPU_LM_HEAD_INT4: i32 = 0;
 pub const AGPU_LM_HEAD_F32: i32 = 1;
 pub const AGPU_LINEAR_QKV: i32 = 0;
@@ -130,6 +133,10 @@ extern "C" {
     pub fn agpu_attention(ctx: *mut agpu_ctx, q: *const f32, k: *const f32, v: *const f32, o: *mut f32, n_heads: i32, q_len: i32, kv_len: i32, q_offset: i32, kv_stride: i32, d_head: i32, causal: i32) -> i32;
     pub fn agpu_bench_attention(ctx: *mut agpu_ctx, q: *const f32, k: *const f32, v: *const f32, o: *mut f32, n_heads: i32, q_len: i32, kv_len: i32, q_offset: i32, kv_stride: i32, d_head: i32, causal: i32, reps: i32, us_per_launch_out_host: *mut f32) -> i32;
     pub fn agpu_kv_append(ctx: *mut agpu_ctx, src: *const f32, cache: *mut f32, n_heads: i32, src_stride: i32, max_seq: i32, write_pos: i32, d_head: i32) -> i32;
+    pub fn agpu_paged_plan(ctx: *mut agpu_ctx, cached_lens: *const i32, new_lens: *const i32, block_tables: *mut i32, free_pages: *mut i32, n_free: *const i32, kv_lens: *mut i32, query_start: *mut i32, slots: *mut i32, positions: *mut i32, n_free_out: *mut i32, batch: i32, table_width: i32, stack_size: i32, page_size: i32, max_tokens: i32) -> i32;
+    pub fn agpu_paged_kv_append(ctx: *mut agpu_ctx, k: *const f32, v: *const f32, k_token_stride: i64, k_head_stride: i64, v_token_stride: i64, v_head_stride: i64, k_cache: *mut c_void, v_cache: *mut c_void, k_page_stride: i64, v_page_stride: i64, slots: *const i32, tokens: i32, n_kv_heads: i32, n_pages: i32, page_size: i32, d_head: i32, cache_type: i32) -> i32;
+    pub fn agpu_paged_attention(ctx: *mut agpu_ctx, q: *const f32, q_token_stride: i64, q_head_stride: i64, k_cache: *const c_void, v_cache: *const c_void, k_page_stride: i64, v_page_stride: i64, block_tables: *const i32, kv_lens: *const i32, query_start: *const i32, o: *mut f32, tokens: i32, batch: i32, n_heads: i32, n_kv_heads: i32, n_pages: i32, page_size: i32, table_width: i32, window: i32, sinks: i32, d_head: i32, cache_type: i32) -> i32;
+    pub fn agpu_sample(ctx: *mut agpu_ctx, logits: *const f32, u: *const f32, tokens_out: *mut i32, rows: i32, n: i32, temperature: f32, top_k: i32, top_p: f32, min_p: f32, temperatures: *const f32, top_ks: *const i32, top_ps: *const f32, min_ps: *const f32) -> i32;
     pub fn agpu_gemm_f32(ctx: *mut agpu_ctx, a: *const f32, b: *const f32, c: *mut f32, M: i32, N: i32, K: i32) -> i32;
     // ---- include/agpu_gpt2.h ----
     pub fn agpu_gpt2_config_small(out: *mut agpu_gpt2_config) -> i32;
