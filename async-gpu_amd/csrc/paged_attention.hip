@@ -1,8 +1,10 @@
 // Attention over a KV cache in pages, d_head = 64: o = softmax(q k / 8) v for the rows of several requests, each over the keys of its own block table.
 #include "agpu_internal.h"
+#include "gemm_bf16.h"
 #include "paged.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace {
 
@@ -22,6 +24,7 @@ struct PagedAttn {
     PageDiv div;
     int shortest_run, max_runs;  // of keys over workgroups
     float *partial;
+    int part;  // floats of an item's run there
     unsigned int *counters;
     int strict;
 };
@@ -32,12 +35,15 @@ constexpr float kQueryScale = 0.125f * 1.44269504088896340736f;
 // ---- elements of the cache, 16 bytes a lane ----
 struct F32 {
     static constexpr int EL = 4;
+    static __device__ __forceinline__ float one(const void *p, size_t i) { return static_cast<const float *>(p)[i]; }
     static __device__ __forceinline__ void floats(const uint4 &x, float (&f)[4]) {
         f[0] = __uint_as_float(x.x); f[1] = __uint_as_float(x.y); f[2] = __uint_as_float(x.z); f[3] = __uint_as_float(x.w);
     }
 };
 struct BF16 {
     static constexpr int EL = 8;
+    static constexpr uint32_t kExponent = 0x7f80;
+    static __device__ __forceinline__ float one(const void *p, size_t i) { return __uint_as_float((uint32_t)static_cast<const unsigned short *>(p)[i] << 16); }
     static __device__ __forceinline__ void floats(const uint4 &x, float (&f)[8]) {
         const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
@@ -49,6 +55,8 @@ struct BF16 {
 };
 struct F16 {
     static constexpr int EL = 8;
+    static constexpr uint32_t kExponent = 0x7c00;
+    static __device__ __forceinline__ float one(const void *p, size_t i) { return (float)static_cast<const _Float16 *>(p)[i]; }
     static __device__ __forceinline__ void floats(const uint4 &x, float (&f)[8]) {
         const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
@@ -87,20 +95,20 @@ __device__ __forceinline__ int request_of(const int *query_start, int batch, int
     return b;
 }
 
-// grid (tokens * n_kv * blocks, runs), 64 W threads: up to G query heads of a token that share a K/V head over a run of its keys.  LPK lanes share a key, 16 bytes each.
+// What a workgroup of W waves needs in LDS for a token's G query heads.
+template <int G, int W>
+struct TokenShared {
+    float o[W][G][DH], m[W][G], l[W][G];
+    unsigned int ticket;
+};
+
+// Up to G query heads of a token that share a K/V head over a run of its keys, by 64 W threads.  LPK lanes share a key, 16 bytes each.
+// h: K/V head, head0: first of the query heads, heads: how many; end: the row behind the request's last; item: place among the partial results.
 template <class T, int G, int W, int PASS>
-__global__ __launch_bounds__(64 * W) void paged_tokens_kernel(const PagedAttn p) {
+__device__ __forceinline__ void token_run(const PagedAttn &p, TokenShared<G, W> &s, int t, int b, int kv_len, int end, int h, int head0, int heads, int run, int item) {
     constexpr int EL = T::EL, LPK = DH / EL, KEYS = 64 / LPK;
-    __shared__ float s_o[W][G][DH], s_m[W][G], s_l[W][G];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int sub = lane % LPK, own = lane / LPK;
-    const int item = blockIdx.x, run = blockIdx.y;
-    const int heads_all = p.n_heads / p.n_kv, blocks = (heads_all + G - 1) / G;  // (G is the power of two that covers them, up to 8)
-    const int t = item / (p.n_kv * blocks), hb = item - t * p.n_kv * blocks, h = hb / blocks, g0 = (hb - h * blocks) * G;
-    const int heads = min(G, heads_all - g0), head0 = h * heads_all + g0;
-    const int b = request_of(p.query_start, p.batch, t, lane);
-    if (b >= p.batch) return;
-    const int kv_len = p.kv_lens[b], end = p.query_start ? p.query_start[b + 1] : t + 1;
     const Visible vis = paged::visible(kv_len - end + t, kv_len, p.held, p.window, p.sinks);
     const int keys = paged::run_of_keys(vis.count, p.shortest_run, p.max_runs), runs = max(1, (vis.count + keys - 1) / keys);
     if (run >= runs) return;
@@ -149,7 +157,7 @@ __global__ __launch_bounds__(64 * W) void paged_tokens_kernel(const PagedAttn p)
             vx[i] = *reinterpret_cast<const uint4 *>(vb + (page * p.v_page + row) * kBytes);
         }
         pages(base + own + PASS * W * KEYS);
-        float s[G][PASS];
+        float x[G][PASS];
 #pragma unroll
         for (int i = 0; i < PASS; ++i) {
             float f[EL];
@@ -159,22 +167,22 @@ __global__ __launch_bounds__(64 * W) void paged_tokens_kernel(const PagedAttn p)
                 float d = q[g][0] * f[0];
 #pragma unroll
                 for (int e = 1; e < EL; ++e) d = fmaf(q[g][e], f[e], d);
-                s[g][i] = ok[i] ? sum_of_key<LPK>(d) : -INFINITY;
+                x[g][i] = ok[i] ? sum_of_key<LPK>(d) : -INFINITY;
             }
         }
 #pragma unroll
         for (int g = 0; g < G; ++g) {
             float top = m[g];
 #pragma unroll
-            for (int i = 0; i < PASS; ++i) top = fmaxf(top, s[g][i]);
+            for (int i = 0; i < PASS; ++i) top = fmaxf(top, x[g][i]);
             const float ref = top == -INFINITY ? 0.0f : top, a = __builtin_amdgcn_exp2f(m[g] - ref);
             l[g] *= a;
 #pragma unroll
             for (int e = 0; e < EL; ++e) o[g][e] *= a;
 #pragma unroll
             for (int i = 0; i < PASS; ++i) {
-                s[g][i] = __builtin_amdgcn_exp2f(s[g][i] - ref);
-                l[g] += s[g][i];
+                x[g][i] = __builtin_amdgcn_exp2f(x[g][i] - ref);
+                l[g] += x[g][i];
             }
             m[g] = top;
         }
@@ -184,9 +192,9 @@ __global__ __launch_bounds__(64 * W) void paged_tokens_kernel(const PagedAttn p)
             T::floats(vx[i], f);
 #pragma unroll
             for (int e = 0; e < EL; ++e) {
-                const float x = ok[i] ? f[e] : 0.0f;  // (what lies behind the keys may be no number)
+                const float y = ok[i] ? f[e] : 0.0f;  // (what lies behind the keys may be no number)
 #pragma unroll
-                for (int g = 0; g < G; ++g) o[g][e] = fmaf(s[g][i], x, o[g][e]);
+                for (int g = 0; g < G; ++g) o[g][e] = fmaf(x[g][i], y, o[g][e]);
             }
         }
     }
@@ -199,25 +207,25 @@ __global__ __launch_bounds__(64 * W) void paged_tokens_kernel(const PagedAttn p)
 #pragma unroll
         for (int e = 0; e < EL; ++e) {
             const float x = over_keys<LPK>(o[g][e] * f, [](float a, float c) { return a + c; });
-            if (own == 0) s_o[wave][g][EL * sub + e] = x;
+            if (own == 0) s.o[wave][g][EL * sub + e] = x;
         }
         if (lane == 0) {
-            s_m[wave][g] = top;
-            s_l[wave][g] = sum;
+            s.m[wave][g] = top;
+            s.l[wave][g] = sum;
         }
     }
     __syncthreads();
-    auto place = [&](int r, int g) { return p.partial + (((size_t)item * p.max_runs + r) * G + g) * (DH + 2); };
+    auto place = [&](int r, int g) { return p.partial + ((size_t)item * p.max_runs + r) * p.part + g * (DH + 2); };
     float *out = p.o + ((size_t)t * p.n_heads + head0) * DH + lane;
     for (int g = wave; g < heads; g += W) {
         float top = -INFINITY, acc = 0.0f, sum = 0.0f;
 #pragma unroll
-        for (int w = 0; w < W; ++w) top = fmaxf(top, s_m[w][g]);
+        for (int w = 0; w < W; ++w) top = fmaxf(top, s.m[w][g]);
 #pragma unroll
         for (int w = 0; w < W; ++w) {
-            const float f = s_m[w][g] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s_m[w][g] - top);
-            acc = fmaf(s_o[w][g][lane], f, acc);
-            sum = fmaf(s_l[w][g], f, sum);
+            const float f = s.m[w][g] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s.m[w][g] - top);
+            acc = fmaf(s.o[w][g][lane], f, acc);
+            sum = fmaf(s.l[w][g], f, sum);
         }
         if (runs == 1) {
             out[g * DH] = sum == 0.0f ? 0.0f : acc / sum;
@@ -231,15 +239,14 @@ __global__ __launch_bounds__(64 * W) void paged_tokens_kernel(const PagedAttn p)
         }
     }
     if (runs == 1) return;
-    __shared__ unsigned int s_ticket;
     partials_published(p.strict);
     __syncthreads();
     if (tid == 0) {
-        s_ticket = take_ticket(&p.counters[item], p.strict);
-        if (s_ticket == (unsigned)(runs - 1)) __hip_atomic_store(&p.counters[item], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        s.ticket = take_ticket(&p.counters[item], p.strict);
+        if (s.ticket == (unsigned)(runs - 1)) __hip_atomic_store(&p.counters[item], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     __syncthreads();
-    if (s_ticket != (unsigned)(runs - 1)) return;
+    if (s.ticket != (unsigned)(runs - 1)) return;
     if (p.strict) __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
     for (int g = wave; g < heads; g += W) {
         auto load = [&](int r, int i) { return __hip_atomic_load(place(r, g) + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
@@ -258,19 +265,513 @@ __global__ __launch_bounds__(64 * W) void paged_tokens_kernel(const PagedAttn p)
     }
 }
 
+// grid (tokens * n_kv * blocks, runs): every row by itself, whatever request it belongs to.
+template <class T, int G, int W, int PASS>
+__global__ __launch_bounds__(64 * W) void paged_tokens_kernel(const PagedAttn p) {
+    __shared__ TokenShared<G, W> s;
+    const int item = blockIdx.x, heads_all = p.n_heads / p.n_kv, blocks = (heads_all + G - 1) / G;  // (G is the power of two that covers them, up to 8)
+    const int t = item / (p.n_kv * blocks), hb = item - t * p.n_kv * blocks, h = hb / blocks, g0 = (hb - h * blocks) * G;
+    const int b = request_of(p.query_start, p.batch, t, threadIdx.x & 63);
+    if (b >= p.batch) return;
+    const int end = p.query_start ? p.query_start[b + 1] : t + 1;
+    token_run<T, G, W, PASS>(p, s, t, b, p.kv_lens[b], end, h, h * heads_all + g0, min(G, heads_all - g0), blockIdx.y, item);
+}
+
+// ---- tiles of rows on the matrix cores ----
+// S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_32x32x16 with 32 keys and 32 rows: what a 32 x 32 result holds of a column (a row of q) in its two
+// half waves is what the second product takes, if V's keys come in the order tile_key.
+//   fp32 cache   every operand is the exact sum of three bf16 numbers (8 bits each, cut off one after the other); of the nine products of pieces the six that
+//                reach 2^-24 are formed, the smallest first
+//   bf16 cache   K and V as they are, q and the weights in three pieces: three products
+//   f16 cache    K and V as they are, q (times a power of two per row) and the weights (times 2^9) as two f16 numbers: two products.  q is good to 2^-22 of itself
+//                and 2^-40 of its largest element.
+constexpr int TILE_ROWS = 128, TILE_KEYS = 32;
+constexpr int kFrag = 4 * 2 * 32;  // 16-byte fragments of a piece of 32 keys of K, and of V
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+
+__device__ __forceinline__ int tile_key(int step, int half, int e) { return 16 * step + 8 * (e >> 2) + 4 * half + (e & 3); }
+
+__device__ __forceinline__ uint32_t upper_halves(float a, float b) { return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u); }
+__device__ __forceinline__ float without_top(float x) { return x - __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
+// Eight floats -> their three pieces, the largest first
+__device__ __forceinline__ void pieces_of(const float (&v)[8], uint4 (&piece)[3]) {
+    float r[8], t[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        r[e] = without_top(v[e]);
+        t[e] = without_top(r[e]);
+    }
+    piece[0] = make_uint4(upper_halves(v[0], v[1]), upper_halves(v[2], v[3]), upper_halves(v[4], v[5]), upper_halves(v[6], v[7]));
+    piece[1] = make_uint4(upper_halves(r[0], r[1]), upper_halves(r[2], r[3]), upper_halves(r[4], r[5]), upper_halves(r[6], r[7]));
+    piece[2] = make_uint4(upper_halves(t[0], t[1]), upper_halves(t[2], t[3]), upper_halves(t[4], t[5]), upper_halves(t[6], t[7]));
+}
+__device__ __forceinline__ void pieces_of(const float (&v)[8], uint4 (&piece)[2]) {  // f16
+    f16x8 hi, lo;
+    split_f16(v, 1.0f, hi, lo);
+    piece[0] = __builtin_bit_cast(uint4, hi);
+    piece[1] = __builtin_bit_cast(uint4, lo);
+}
+
+template <class T>
+struct Tiles;  // KP pieces of K and V, QP of q and the weights; UP: what weights are multiplied by
+template <>
+struct Tiles<F32> {
+    static constexpr int KP = 3, QP = 3;
+    static constexpr float UP = 1.0f;
+    static __device__ __forceinline__ floatx16 mfma(uint4 a, uint4 b, floatx16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    }
+};
+template <>
+struct Tiles<BF16> {
+    static constexpr int KP = 1, QP = 3;
+    static constexpr float UP = 1.0f;
+    static __device__ __forceinline__ floatx16 mfma(uint4 a, uint4 b, floatx16 c) { return Tiles<F32>::mfma(a, b, c); }
+};
+template <>
+struct Tiles<F16> {
+    static constexpr int KP = 1, QP = 2;
+    static constexpr float UP = 512.0f;
+    static __device__ __forceinline__ floatx16 mfma(uint4 a, uint4 b, floatx16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    }
+};
+
+// Eight elements of K (of one key) or of V (one dimension of eight keys) on their way from the cache to LDS.
+template <class T>
+struct Staged;
+template <>
+struct Staged<F32> {
+    float x[8];
+    __device__ __forceinline__ void row(const char *p, bool ok) {
+        const float4 a = ok ? *reinterpret_cast<const float4 *>(p) : make_float4(0.f, 0.f, 0.f, 0.f), b = ok ? *reinterpret_cast<const float4 *>(p + 16) : a;
+        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+    }
+    __device__ __forceinline__ void element(int e, const char *p, bool ok) { x[e] = ok ? *reinterpret_cast<const float *>(p) : 0.0f; }
+    __device__ __forceinline__ float trace() const {  // not a number if one of them is infinite or none
+        float t = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) t = fmaf(x[e], 0.0f, t);
+        return t;
+    }
+    // Zeros in place of those; which there were.
+    __device__ __forceinline__ uint32_t clean() {
+        uint32_t odd = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (!(fabsf(x[e]) < INFINITY)) {
+                odd |= 1u << e;
+                x[e] = 0.0f;
+            }
+        return odd;
+    }
+    __device__ __forceinline__ void store(uint4 *to) const {
+        uint4 piece[3];
+        pieces_of(x, piece);
+#pragma unroll
+        for (int i = 0; i < 3; ++i) to[i * kFrag] = piece[i];
+    }
+};
+template <class T>
+struct Staged16 {
+    uint32_t x[8];  // K: the first four, two elements each; V: one each
+    bool is_row;
+    __device__ __forceinline__ void row(const char *p, bool ok) {
+        const uint4 a = ok ? *reinterpret_cast<const uint4 *>(p) : make_uint4(0, 0, 0, 0);
+        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+        is_row = true;
+    }
+    __device__ __forceinline__ void element(int e, const char *p, bool ok) {
+        x[e] = ok ? *reinterpret_cast<const unsigned short *>(p) : 0u;
+        is_row = false;
+    }
+    __device__ __forceinline__ uint4 frag() const {
+        return is_row ? make_uint4(x[0], x[1], x[2], x[3]) : make_uint4(x[0] | x[1] << 16, x[2] | x[3] << 16, x[4] | x[5] << 16, x[6] | x[7] << 16);
+    }
+    __device__ __forceinline__ float trace() const {
+        float f[8], t = 0.0f;
+        T::floats(frag(), f);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) t = fmaf(f[e], 0.0f, t);
+        return t;
+    }
+    __device__ __forceinline__ uint32_t clean() {
+        uint32_t odd = 0;
+        constexpr uint32_t kExponent = T::kExponent;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const uint32_t bits = (is_row ? x[e >> 1] >> (16 * (e & 1)) : x[e]) & kExponent;
+            if (bits == kExponent) {
+                odd |= 1u << e;
+                if (is_row) x[e >> 1] &= e & 1 ? 0x0000ffffu : 0xffff0000u;
+                else x[e] = 0;
+            }
+        }
+        return odd;
+    }
+    __device__ __forceinline__ void store(uint4 *to) const { *to = frag(); }
+};
+template <>
+struct Staged<BF16> : Staged16<BF16> {};
+template <>
+struct Staged<F16> : Staged16<F16> {};
+
+template <class T>
+struct TileShared {
+    uint4 k[2][Tiles<T>::KP][kFrag], v[2][Tiles<T>::KP][kFrag];  // [buffer][piece]: K [d step of 16][half][key], V [32 dimensions][key step][half][dimension]
+    long long at[4][TILE_KEYS];  // of a tile's keys: where their rows begin, in elements from the head's first page, K and V
+    long long at_v[4][TILE_KEYS];
+    uint32_t seen[4];            // which of them are there
+    uint32_t odd_k[4], odd_v[4];  // of which something is infinite or not a number
+    unsigned int ticket;
+};
+
+__device__ __forceinline__ float other_half(float v, float &own) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    own = __uint_as_float(r[0]);
+    return __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float max_of_halves(float v) {
+    float own;
+    const float other = other_half(v, own);
+    return fmaxf(own, other);
+}
+__device__ __forceinline__ float sum_of_halves(float v) {
+    float own;
+    const float other = other_half(v, own);
+    return own + other;
+}
+
+// Up to 128 rows of a request (its tokens' heads of one K/V head, token by token) over a run of the keys that any of them sees, by four waves of 32 rows, which
+// share the tiles of 32 keys: what each thread has fetched goes to LDS as operands while the next tile is on its way, one barrier a tile.
+// first_row: of the rows of the request and K/V head.
+template <class T>
+__device__ __forceinline__ void tile_run(const PagedAttn &p, TileShared<T> &s, int b, int start, int q_len, int kv_len, int h, int first_row, int run, int item) {
+    constexpr int KP = Tiles<T>::KP, QP = Tiles<T>::QP;
+    constexpr int kBytes = 16 / T::EL;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 31, h2 = lane >> 5;
+    const int group = p.n_heads / p.n_kv, rows = q_len * group, last_row = min(first_row + TILE_ROWS, rows) - 1;
+    // all keys that a row of the tile sees, numbered without a gap
+    const int pos0 = kv_len - q_len + first_row / group, pos1 = kv_len - q_len + last_row / group;
+    int end = min(min(pos1 + 1, kv_len), p.held);
+    end = max(end, 0);
+    int low = p.window > 0 ? max(pos0 + 1 - p.window, 0) : 0;
+    const int first = min(min(p.sinks, low), end), gap = low - first, count = first + max(end - low, 0);
+    const int keys = paged::run_of_keys(count, p.shortest_run, p.max_runs), runs = max(1, (count + keys - 1) / keys);
+    if (run >= runs) return;
+    const int lo = run * keys, hi = min(count, lo + keys);
+    // this lane's row; rows behind the last one repeat it
+    const int row = min(first_row + 32 * wave + c, last_row), token = row / group, head = h * group + (row - token * group);
+    const bool mine = first_row + 32 * wave + c <= last_row, any = first_row + 32 * wave <= last_row;
+    const int pos = kv_len - q_len + token;
+    const int wave_pos0 = kv_len - q_len + min(first_row + 32 * wave, last_row) / group, wave_pos1 = kv_len - q_len + min(first_row + 32 * wave + 31, last_row) / group;
+    // key number v is seen if v <= v_last and (v > v_low or v < v_first)
+    const int v_last = pos - gap, v_low = p.window > 0 ? pos - p.window - gap : -1, v_first = p.window > 0 ? max(first, p.sinks - gap) : 0;
+
+    const float *q_row = p.q + (size_t)(start + token) * p.q_row + (size_t)head * p.q_head;
+    uint4 q[4][QP];
+    float unit = 1.0f;  // of the scores
+    {
+        float x[4][8], most = 0.0f;
+#pragma unroll
+        for (int ds = 0; ds < 4; ++ds) {
+            const float4 a = load4(q_row + 16 * ds + 8 * h2), d = load4(q_row + 16 * ds + 8 * h2 + 4);
+            const float y[8] = {a.x, a.y, a.z, a.w, d.x, d.y, d.z, d.w};
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                x[ds][e] = y[e] * kQueryScale;
+                most = fmaxf(most, fabsf(x[ds][e]));
+            }
+        }
+        if (QP == 2) {  // into 2^14 .. 2^15
+            const int up = max(min(141 - (int)((__float_as_uint(max_of_halves(most)) >> 23) & 255u), 100), -112);
+            const float by = __uint_as_float((uint32_t)(up + 127) << 23);
+            unit = __uint_as_float((uint32_t)(127 - up) << 23);
+#pragma unroll
+            for (int ds = 0; ds < 4; ++ds)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[ds][e] *= by;
+        }
+#pragma unroll
+        for (int ds = 0; ds < 4; ++ds) pieces_of(x[ds], q[ds]);
+    }
+
+    // keys of tile i are lo + 32 i ..; places of a tile are looked up two tiles ahead
+    const int tiles = (hi - lo + TILE_KEYS - 1) / TILE_KEYS;
+    const int *table = p.tables + (size_t)b * p.width;
+    auto look_up = [&](int i, int &id, int &off) {  // the first 32 threads
+        const int v = lo + TILE_KEYS * i + c;
+        id = -1;
+        off = 0;
+        if (v < hi) {
+            const int j = v < first ? v : v + gap, page = p.div.page(j);
+            id = table[page];
+            off = j - page * p.div.size;
+        }
+    };
+    auto leave = [&](int i, int id, int off) {
+        const bool ok = (unsigned)id < (unsigned)p.n_pages;
+        const long long at = (long long)(h * p.div.size + off) * DH;
+        s.at[i & 3][c] = ok ? id * p.k_page + at : -1;
+        s.at_v[i & 3][c] = ok ? id * p.v_page + at : -1;
+        const uint64_t who = __ballot(ok);
+        if (lane == 0) {
+            s.seen[i & 3] = (uint32_t)who;
+            s.odd_k[i & 3] = s.odd_v[i & 3] = 0;
+        }
+    };
+    int id = -1, off = 0;
+    if (tid < 32) {
+        look_up(0, id, off);
+        leave(0, id, off);
+        look_up(1, id, off);
+        leave(1, id, off);
+        look_up(2, id, off);
+    }
+    __syncthreads();
+    const char *const kb = static_cast<const char *>(p.k), *const vb = static_cast<const char *>(p.v);
+    Staged<T> sk, sv;
+    const int k_d = 16 * wave + 8 * h2, v_step = wave & 1, v_d = 32 * (wave >> 1) + c;  // what this thread fetches
+    auto fetch = [&](int i) {
+        const long long at = s.at[i & 3][c];
+        sk.row(kb + (at + k_d) * kBytes, at >= 0);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const long long to = s.at_v[i & 3][tile_key(v_step, h2, e)];
+            sv.element(e, vb + (to + v_d) * kBytes, to >= 0);
+        }
+    };
+    if (tiles > 0) fetch(0);
+
+    floatx16 o[2] = {};
+    float m = -INFINITY, l = 0.0f;
+    for (int i = 0; i < tiles; ++i) {
+        const int buf = i & 1;
+        if (__builtin_expect(__any(sk.trace() + sv.trace() != 0.0f), 0)) {
+            if (sk.clean()) atomicOr(&s.odd_k[i & 3], 1u << c);
+            const uint32_t odd = sv.clean();
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (odd >> e & 1) atomicOr(&s.odd_v[i & 3], 1u << tile_key(v_step, h2, e));
+        }
+        sk.store(&s.k[buf][0][(2 * wave + h2) * 32 + c]);
+        sv.store(&s.v[buf][0][((2 * (wave >> 1) + v_step) * 2 + h2) * 32 + c]);
+        if (i + 1 < tiles) fetch(i + 1);
+        if (tid < 32) {
+            leave(i + 2, id, off);
+            look_up(i + 3, id, off);
+        }
+        __syncthreads();
+        const int v0 = lo + TILE_KEYS * i;
+        if (!any || (v0 >= first && v0 > wave_pos1 - gap)) continue;  // (the next tile goes to the other buffer)
+        const uint32_t there = s.seen[i & 3];
+        floatx16 x = {};
+#pragma unroll
+        for (int level = QP - 1; level >= 0; --level)
+#pragma unroll
+            for (int ds = 0; ds < 4; ++ds)
+#pragma unroll
+                for (int kp = KP - 1; kp >= 0; --kp)
+                    if (level - kp >= 0 && level - kp < QP) x = Tiles<T>::mfma(s.k[buf][kp][(2 * ds + h2) * 32 + c], q[ds][level - kp], x);
+        if (QP == 2)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) x[r] *= unit;
+        // Keys with something infinite in them, or no number, went as zeros, which no row's other keys notice; their scores are formed in fp32 here, and
+        // their values are added below, for the rows that see them.
+        const uint32_t odd_k = s.odd_k[i & 3], odd_v = s.odd_v[i & 3];
+        if (__builtin_expect(odd_k != 0, 0))
+#pragma unroll 1
+            for (int kk = 0; kk < TILE_KEYS; ++kk) {
+                if (!(odd_k >> kk & 1)) continue;
+                const size_t at = (size_t)s.at[i & 3][kk];
+                float d = 0.0f;
+#pragma unroll 1
+                for (int e = 0; e < 32; ++e) d = fmaf(q_row[32 * h2 + e] * kQueryScale, T::one(kb, at + 32 * h2 + e), d);
+                d = sum_of_halves(d);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) x[r] = 8 * (r >> 2) + 4 * h2 + (r & 3) == kk ? d : x[r];
+            }
+        // only tiles at the ends of what rows see hide anything (uniform over the wave)
+        const bool whole = there == 0xffffffffu && v0 + TILE_KEYS - 1 <= wave_pos0 - gap &&
+                           (p.window == 0 || v0 > wave_pos1 - p.window - gap || v0 + TILE_KEYS <= v_first);
+        if (!whole) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int kk = 8 * (r >> 2) + 4 * h2 + (r & 3), v = v0 + kk;
+                const bool see = (there >> kk & 1) && v <= v_last && (v > v_low || v < v_first);
+                x[r] = see ? x[r] : -INFINITY;
+            }
+        }
+        float top = x[0];
+#pragma unroll
+        for (int r = 1; r < 16; ++r) top = fmaxf(top, x[r]);
+        top = max_of_halves(top);
+        if (__any(top > m + 6.0f)) {  // weights may grow to 2^6 before everything is rescaled
+            const float now = fmaxf(m, top), a = now == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - now);
+            m = now;
+            l *= a;
+#pragma unroll
+            for (int db = 0; db < 2; ++db)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[db][r] *= a;
+        }
+        const float ref = m == -INFINITY ? 0.0f : m;
+        float sum = 0.0f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            x[r] = __builtin_amdgcn_exp2f(x[r] - ref);
+            sum += x[r];
+        }
+        l += sum;
+        uint4 w[2][QP];
+#pragma unroll
+        for (int st = 0; st < 2; ++st) {
+            float y[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] = x[8 * st + e] * Tiles<T>::UP;
+            pieces_of(y, w[st]);
+        }
+#pragma unroll
+        for (int level = QP - 1; level >= 0; --level)
+#pragma unroll
+            for (int kp = KP - 1; kp >= 0; --kp)
+                if (level - kp >= 0 && level - kp < QP)
+#pragma unroll
+                    for (int st = 0; st < 2; ++st)
+#pragma unroll
+                        for (int db = 0; db < 2; ++db) o[db] = Tiles<T>::mfma(s.v[buf][kp][((2 * db + st) * 2 + h2) * 32 + c], w[st][level - kp], o[db]);
+        if (__builtin_expect(odd_v != 0, 0))
+#pragma unroll 1
+            for (int kk = 0; kk < TILE_KEYS; ++kk) {
+                const int v = v0 + kk;
+                if (!(odd_v >> kk & 1)) continue;
+                const bool see = v <= v_last && (v > v_low || v < v_first);
+                float weight = 0.0f;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) weight = 8 * (r >> 2) + 4 * h2 + (r & 3) == kk ? x[r] : weight;
+                weight = sum_of_halves(weight);  // (one of them is zero)
+                const size_t at = (size_t)s.at_v[i & 3][kk];
+#pragma unroll
+                for (int db = 0; db < 2; ++db)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const float y = T::one(vb, at + 32 * db + 8 * (r >> 2) + 4 * h2 + (r & 3));
+                        o[db][r] += see && !(fabsf(y) < INFINITY) ? weight * y : 0.0f;
+                    }
+            }
+    }
+    l = sum_of_halves(l);
+    auto store = [&](float sum) {
+        if (!mine) return;
+        const float by = sum == 0.0f ? 0.0f : 1.0f / (sum * Tiles<T>::UP);
+        float *out = p.o + ((size_t)(start + token) * p.n_heads + head) * DH + 4 * h2;
+#pragma unroll
+        for (int db = 0; db < 2; ++db)
+#pragma unroll
+            for (int r = 0; r < 16; r += 4)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) out[32 * db + 2 * r + e] = sum == 0.0f ? 0.0f : o[db][r + e] * by;
+    };
+    if (runs == 1) return store(l);
+    auto part = [&](int r) { return p.partial + ((size_t)item * p.max_runs + r) * p.part + wave * (32 * (DH + 2)); };  // [wave][dimension, or m and l][row]
+    if (any) {
+        float *to = part(run);
+#pragma unroll
+        for (int db = 0; db < 2; ++db)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                __hip_atomic_store(to + (32 * db + 8 * (r >> 2) + 4 * h2 + (r & 3)) * 32 + c, o[db][r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __hip_atomic_store(to + (DH + h2) * 32 + c, h2 == 0 ? m : l, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    partials_published(p.strict);
+    __syncthreads();
+    if (tid == 0) {
+        s.ticket = take_ticket(&p.counters[item], p.strict);
+        if (s.ticket == (unsigned)(runs - 1)) __hip_atomic_store(&p.counters[item], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    if (s.ticket != (unsigned)(runs - 1) || !any) return;
+    if (p.strict) __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+    auto load = [&](int r, int i) { return __hip_atomic_load(part(r) + i * 32 + c, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+    m = -INFINITY;
+    for (int r = 0; r < runs; ++r) m = fmaxf(m, load(r, DH));
+    l = 0.0f;
+    o[0] = o[1] = floatx16{};
+#pragma unroll 1
+    for (int r = 0; r < runs; ++r) {
+        const float mr = load(r, DH), a = mr == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mr - m);
+        l = fmaf(load(r, DH + 1), a, l);
+#pragma unroll
+        for (int db = 0; db < 2; ++db)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[db][e] = fmaf(load(r, 32 * db + 8 * (e >> 2) + 4 * h2 + (e & 3)), a, o[db][e]);
+    }
+    store(l);
+}
+
+// Requests with new rows of every number: those with up to eight rows of heads a K/V head go token by token, the others in tiles.  grid (tile places *
+// n_kv, then token places * n_kv; runs).  A request b has tile places from query_start[b] * group / 128 + b on, enough for its rows and one more than all tiles of
+// the requests before it need; and `slots` places for its tokens.
+template <class T, int G>
+__global__ __launch_bounds__(256, 2) void paged_rows_kernel(const PagedAttn p, int tile_places, int slots) {
+    union Shared {
+        TileShared<T> tiles;
+        TokenShared<G, 4> token;
+    };
+    __shared__ __align__(16) char smem[sizeof(Shared)];
+    const int lane = threadIdx.x & 63, group = p.n_heads / p.n_kv, tile_wgs = tile_places * p.n_kv;
+    // consecutive workgroups go round the XCDs; an XCD takes consecutive items, whose tiles share a head's K and V
+    int at = blockIdx.x;
+    if (at < tile_wgs) {
+        const int each = tile_wgs >> 3, rest = tile_wgs & 7, xcd = at & 7;
+        at = xcd * each + min(xcd, rest) + (at >> 3);
+        const int h = at / tile_places, place = tile_places - 1 - (at - h * tile_places);
+        int b = -1;
+        for (int i = 0; i < p.batch; i += 64) b += __popcll(__ballot(i + lane < p.batch && p.query_start[i + lane] * group / TILE_ROWS + i + lane <= place));
+        if (b < 0) return;
+        const int start = p.query_start[b], q_len = min(p.query_start[b + 1], p.tokens) - start, rows = q_len * group;
+        const int first_row = (place - start * group / TILE_ROWS - b) * TILE_ROWS;
+        if (start < 0 || q_len <= slots || first_row < 0 || first_row >= rows) return;
+        tile_run<T>(p, *reinterpret_cast<TileShared<T> *>(smem), b, start, q_len, p.kv_lens[b], h, first_row, blockIdx.y, blockIdx.x);
+    } else {
+        at -= tile_wgs;
+        const int h = at % p.n_kv, place = at / p.n_kv, b = place / slots, i = place - b * slots;
+        const int start = p.query_start[b], end = min(p.query_start[b + 1], p.tokens), q_len = end - start;
+        if (start < 0 || i >= q_len || q_len > slots) return;
+        token_run<T, G, 4, 4>(p, *reinterpret_cast<TokenShared<G, 4> *>(smem), start + i, b, p.kv_lens[b], end, h, h * group, group, blockIdx.y, blockIdx.x);
+    }
+}
+
 template <class T, int G>
 int32_t tokens_go(agpu_ctx *ctx, PagedAttn &p, int64_t longest) {
     const int64_t items = (int64_t)p.tokens * p.n_kv * ceil_div(p.n_heads / p.n_kv, G);
     const paged::Cut cut = paged::cut_keys(items, longest, 2048, 128, 64, G * (DH + 2) * sizeof(float), ctx->ws_bytes / 2, ctx->n_counters - 1);
+    p.part = G * (DH + 2);
     p.shortest_run = cut.shortest;
     p.max_runs = cut.runs;
     hipLaunchKernelGGL((paged_tokens_kernel<T, G, 4, 4>), dim3((unsigned)items, cut.runs), dim3(256), 0, ctx->stream, p);
     return AGPU_LAUNCH_CHECK(ctx, "paged_tokens_kernel");
 }
+template <class T, int G>
+int32_t rows_go(agpu_ctx *ctx, PagedAttn &p, int64_t longest) {
+    const int group = p.n_heads / p.n_kv, slots = 8 / group;  // up to eight rows: token by token
+    const int tile_places = (int)((int64_t)p.tokens * group / TILE_ROWS) + p.batch;
+    const int64_t items = ((int64_t)tile_places + (int64_t)p.batch * slots) * p.n_kv;
+    const paged::Cut cut = paged::cut_keys(items, longest, 1024, 256, 64, TILE_ROWS * (DH + 2) * sizeof(float), ctx->ws_bytes / 2, ctx->n_counters - 1);
+    p.part = TILE_ROWS * (DH + 2);  // (a token's take less)
+    p.shortest_run = cut.shortest;
+    p.max_runs = cut.runs;
+    hipLaunchKernelGGL((paged_rows_kernel<T, G>), dim3((unsigned)items, cut.runs), dim3(256), 0, ctx->stream, p, tile_places, slots);
+    return AGPU_LAUNCH_CHECK(ctx, "paged_rows_kernel");
+}
 template <class T>
 int32_t attention_go(agpu_ctx *ctx, PagedAttn &p, int64_t longest) {
     const int g = p.n_heads / p.n_kv;
-    return g == 1 ? tokens_go<T, 1>(ctx, p, longest) : g == 2 ? tokens_go<T, 2>(ctx, p, longest) : g <= 4 ? tokens_go<T, 4>(ctx, p, longest) : tokens_go<T, 8>(ctx, p, longest);
+    auto go = [&](auto heads) {
+        constexpr int G = decltype(heads)::value;
+        return p.tokens <= p.batch ? tokens_go<T, G>(ctx, p, longest) : rows_go<T, G>(ctx, p, longest);
+    };
+    return g == 1 ? go(std::integral_constant<int, 1>{}) : g == 2 ? go(std::integral_constant<int, 2>{}) : g <= 4 ? go(std::integral_constant<int, 4>{}) : go(std::integral_constant<int, 8>{});
 }
 
 }  // namespace
