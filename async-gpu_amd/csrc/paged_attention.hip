@@ -22,11 +22,15 @@ struct PagedAttn {
     float *o;  // [tokens][n_heads][64]
     int tokens, batch, n_heads, n_kv, n_pages, width, held, window, sinks;
     PageDiv div;
-    int shortest_run, max_runs;  // of keys over workgroups
+    int strict;
+};
+
+// How keys are cut into runs over workgroups, and where items of several runs leave their partial results and draw their tickets.
+struct Runs {
+    int shortest, most;
     float *partial;
     int part;  // floats of an item's run there
     unsigned int *counters;
-    int strict;
 };
 
 // Scores are in units of the binary logarithm: q is taken times log2(e) / 8.
@@ -105,12 +109,12 @@ struct TokenShared {
 // Up to G query heads of a token that share a K/V head over a run of its keys, by 64 W threads.  LPK lanes share a key, 16 bytes each.
 // h: K/V head, head0: first of the query heads, heads: how many; end: the row behind the request's last; item: place among the partial results.
 template <class T, int G, int W, int PASS>
-__device__ __forceinline__ void token_run(const PagedAttn &p, TokenShared<G, W> &s, int t, int b, int kv_len, int end, int h, int head0, int heads, int run, int item) {
+__device__ __forceinline__ void token_run(const PagedAttn &p, TokenShared<G, W> &s, const Runs &cut, int t, int b, int kv_len, int end, int h, int head0, int heads, int run, int item) {
     constexpr int EL = T::EL, LPK = DH / EL, KEYS = 64 / LPK;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int sub = lane % LPK, own = lane / LPK;
     const Visible vis = paged::visible(kv_len - end + t, kv_len, p.held, p.window, p.sinks);
-    const int keys = paged::run_of_keys(vis.count, p.shortest_run, p.max_runs), runs = max(1, (vis.count + keys - 1) / keys);
+    const int keys = paged::run_of_keys(vis.count, cut.shortest, cut.most), runs = max(1, (vis.count + keys - 1) / keys);
     if (run >= runs) return;
     const int lo = run * keys, hi = min(vis.count, lo + keys);
 
@@ -215,7 +219,7 @@ __device__ __forceinline__ void token_run(const PagedAttn &p, TokenShared<G, W> 
         }
     }
     __syncthreads();
-    auto place = [&](int r, int g) { return p.partial + ((size_t)item * p.max_runs + r) * p.part + g * (DH + 2); };
+    auto place = [&](int r, int g) { return cut.partial + ((size_t)item * cut.most + r) * cut.part + g * (DH + 2); };
     float *out = p.o + ((size_t)t * p.n_heads + head0) * DH + lane;
     for (int g = wave; g < heads; g += W) {
         float top = -INFINITY, acc = 0.0f, sum = 0.0f;
@@ -242,8 +246,8 @@ __device__ __forceinline__ void token_run(const PagedAttn &p, TokenShared<G, W> 
     partials_published(p.strict);
     __syncthreads();
     if (tid == 0) {
-        s.ticket = take_ticket(&p.counters[item], p.strict);
-        if (s.ticket == (unsigned)(runs - 1)) __hip_atomic_store(&p.counters[item], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        s.ticket = take_ticket(&cut.counters[item], p.strict);
+        if (s.ticket == (unsigned)(runs - 1)) __hip_atomic_store(&cut.counters[item], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     __syncthreads();
     if (s.ticket != (unsigned)(runs - 1)) return;
@@ -267,14 +271,14 @@ __device__ __forceinline__ void token_run(const PagedAttn &p, TokenShared<G, W> 
 
 // grid (tokens * n_kv * blocks, runs): every row by itself, whatever request it belongs to.
 template <class T, int G, int W, int PASS>
-__global__ __launch_bounds__(64 * W) void paged_tokens_kernel(const PagedAttn p) {
+__global__ __launch_bounds__(64 * W) void paged_tokens_kernel(const PagedAttn p, const Runs cut) {
     __shared__ TokenShared<G, W> s;
     const int item = blockIdx.x, heads_all = p.n_heads / p.n_kv, blocks = (heads_all + G - 1) / G;  // (G is the power of two that covers them, up to 8)
     const int t = item / (p.n_kv * blocks), hb = item - t * p.n_kv * blocks, h = hb / blocks, g0 = (hb - h * blocks) * G;
     const int b = request_of(p.query_start, p.batch, t, threadIdx.x & 63);
     if (b >= p.batch) return;
     const int end = p.query_start ? p.query_start[b + 1] : t + 1;
-    token_run<T, G, W, PASS>(p, s, t, b, p.kv_lens[b], end, h, h * heads_all + g0, min(G, heads_all - g0), blockIdx.y, item);
+    token_run<T, G, W, PASS>(p, s, cut, t, b, p.kv_lens[b], end, h, h * heads_all + g0, min(G, heads_all - g0), blockIdx.y, item);
 }
 
 // ---- tiles of rows on the matrix cores ----
@@ -446,7 +450,7 @@ __device__ __forceinline__ float sum_of_halves(float v) {
 // share the tiles of 32 keys: what each thread has fetched goes to LDS as operands while the next tile is on its way, one barrier a tile.
 // first_row: of the rows of the request and K/V head.
 template <class T>
-__device__ __forceinline__ void tile_run(const PagedAttn &p, TileShared<T> &s, int b, int start, int q_len, int kv_len, int h, int first_row, int run, int item) {
+__device__ __forceinline__ void tile_run(const PagedAttn &p, TileShared<T> &s, const Runs &cut, int b, int start, int q_len, int kv_len, int h, int first_row, int run, int item) {
     constexpr int KP = Tiles<T>::KP, QP = Tiles<T>::QP;
     constexpr int kBytes = 16 / T::EL;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 31, h2 = lane >> 5;
@@ -457,7 +461,7 @@ __device__ __forceinline__ void tile_run(const PagedAttn &p, TileShared<T> &s, i
     end = max(end, 0);
     int low = p.window > 0 ? max(pos0 + 1 - p.window, 0) : 0;
     const int first = min(min(p.sinks, low), end), gap = low - first, count = first + max(end - low, 0);
-    const int keys = paged::run_of_keys(count, p.shortest_run, p.max_runs), runs = max(1, (count + keys - 1) / keys);
+    const int keys = paged::run_of_keys(count, cut.shortest, cut.most), runs = max(1, (count + keys - 1) / keys);
     if (run >= runs) return;
     const int lo = run * keys, hi = min(count, lo + keys);
     // this lane's row; rows behind the last one repeat it
@@ -673,7 +677,7 @@ __device__ __forceinline__ void tile_run(const PagedAttn &p, TileShared<T> &s, i
                 for (int e = 0; e < 4; ++e) out[32 * db + 2 * r + e] = sum == 0.0f ? 0.0f : o[db][r + e] * by;
     };
     if (runs == 1) return store(l);
-    auto part = [&](int r) { return p.partial + ((size_t)item * p.max_runs + r) * p.part + wave * (32 * (DH + 2)); };  // [wave][dimension, or m and l][row]
+    auto part = [&](int r) { return cut.partial + ((size_t)item * cut.most + r) * cut.part + wave * (32 * (DH + 2)); };  // [wave][dimension, or m and l][row]
     if (any) {
         float *to = part(run);
 #pragma unroll
@@ -686,8 +690,8 @@ __device__ __forceinline__ void tile_run(const PagedAttn &p, TileShared<T> &s, i
     partials_published(p.strict);
     __syncthreads();
     if (tid == 0) {
-        s.ticket = take_ticket(&p.counters[item], p.strict);
-        if (s.ticket == (unsigned)(runs - 1)) __hip_atomic_store(&p.counters[item], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        s.ticket = take_ticket(&cut.counters[item], p.strict);
+        if (s.ticket == (unsigned)(runs - 1)) __hip_atomic_store(&cut.counters[item], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     __syncthreads();
     if (s.ticket != (unsigned)(runs - 1) || !any) return;
@@ -709,63 +713,68 @@ __device__ __forceinline__ void tile_run(const PagedAttn &p, TileShared<T> &s, i
     store(l);
 }
 
-// Requests with new rows of every number: those with up to eight rows of heads a K/V head go token by token, the others in tiles.  grid (tile places *
-// n_kv, then token places * n_kv; runs).  A request b has tile places from query_start[b] * group / 128 + b on, enough for its rows and one more than all tiles of
+// Requests with new rows of every number: those with up to eight rows of heads a K/V head go token by token, the others in tiles.  grid: tile places * n_kv *
+// runs, then token places * n_kv * runs.  A request b has tile places from query_start[b] * group / 128 + b on, enough for its rows and one more than all tiles of
 // the requests before it need; and `slots` places for its tokens.
 template <class T, int G>
-__global__ __launch_bounds__(256, 2) void paged_rows_kernel(const PagedAttn p, int tile_places, int slots) {
+__global__ __launch_bounds__(256, 2) void paged_rows_kernel(const PagedAttn p, const Runs tile_cut, const Runs token_cut, int tile_places, int slots) {
     union Shared {
         TileShared<T> tiles;
         TokenShared<G, 4> token;
     };
     __shared__ __align__(16) char smem[sizeof(Shared)];
-    const int lane = threadIdx.x & 63, group = p.n_heads / p.n_kv, tile_wgs = tile_places * p.n_kv;
-    // consecutive workgroups go round the XCDs; an XCD takes consecutive items, whose tiles share a head's K and V
+    const int lane = threadIdx.x & 63, group = p.n_heads / p.n_kv, tile_items = tile_places * p.n_kv, tile_wgs = tile_items * tile_cut.most;
     int at = blockIdx.x;
     if (at < tile_wgs) {
+        // consecutive workgroups go round the XCDs; an XCD takes consecutive items, whose tiles share a head's K and V
         const int each = tile_wgs >> 3, rest = tile_wgs & 7, xcd = at & 7;
         at = xcd * each + min(xcd, rest) + (at >> 3);
-        const int h = at / tile_places, place = tile_places - 1 - (at - h * tile_places);
+        const int item = at / tile_cut.most, run = at - item * tile_cut.most;
+        const int h = item / tile_places, place = tile_places - 1 - (item - h * tile_places);
         int b = -1;
         for (int i = 0; i < p.batch; i += 64) b += __popcll(__ballot(i + lane < p.batch && p.query_start[i + lane] * group / TILE_ROWS + i + lane <= place));
         if (b < 0) return;
         const int start = p.query_start[b], q_len = min(p.query_start[b + 1], p.tokens) - start, rows = q_len * group;
         const int first_row = (place - start * group / TILE_ROWS - b) * TILE_ROWS;
         if (start < 0 || q_len <= slots || first_row < 0 || first_row >= rows) return;
-        tile_run<T>(p, *reinterpret_cast<TileShared<T> *>(smem), b, start, q_len, p.kv_lens[b], h, first_row, blockIdx.y, blockIdx.x);
+        tile_run<T>(p, *reinterpret_cast<TileShared<T> *>(smem), tile_cut, b, start, q_len, p.kv_lens[b], h, first_row, run, item);
     } else {
         at -= tile_wgs;
-        const int h = at % p.n_kv, place = at / p.n_kv, b = place / slots, i = place - b * slots;
+        const int item = at / token_cut.most, run = at - item * token_cut.most;
+        const int h = item % p.n_kv, place = item / p.n_kv, b = place / slots, i = place - b * slots;
         const int start = p.query_start[b], end = min(p.query_start[b + 1], p.tokens), q_len = end - start;
         if (start < 0 || i >= q_len || q_len > slots) return;
-        token_run<T, G, 4, 4>(p, *reinterpret_cast<TokenShared<G, 4> *>(smem), start + i, b, p.kv_lens[b], end, h, h * group, group, blockIdx.y, blockIdx.x);
+        token_run<T, G, 4, 4>(p, *reinterpret_cast<TokenShared<G, 4> *>(smem), token_cut, start + i, b, p.kv_lens[b], end, h, h * group, group, run, item);
     }
 }
 
 template <class T, int G>
-int32_t tokens_go(agpu_ctx *ctx, PagedAttn &p, int64_t longest) {
+int32_t tokens_go(agpu_ctx *ctx, const PagedAttn &p, int64_t longest) {
     const int64_t items = (int64_t)p.tokens * p.n_kv * ceil_div(p.n_heads / p.n_kv, G);
-    const paged::Cut cut = paged::cut_keys(items, longest, 2048, 128, 64, G * (DH + 2) * sizeof(float), ctx->ws_bytes / 2, ctx->n_counters - 1);
-    p.part = G * (DH + 2);
-    p.shortest_run = cut.shortest;
-    p.max_runs = cut.runs;
-    hipLaunchKernelGGL((paged_tokens_kernel<T, G, 4, 4>), dim3((unsigned)items, cut.runs), dim3(256), 0, ctx->stream, p);
+    constexpr int part = G * (DH + 2);
+    const paged::Cut cut = paged::cut_keys(items, longest, 2048, 128, 64, part * sizeof(float), ctx->ws_bytes / 2, ctx->n_counters - 1);
+    const Runs runs = {cut.shortest, cut.runs, reinterpret_cast<float *>(ctx->workspace), part, ctx->counters};
+    hipLaunchKernelGGL((paged_tokens_kernel<T, G, 4, 4>), dim3((unsigned)items, cut.runs), dim3(256), 0, ctx->stream, p, runs);
     return AGPU_LAUNCH_CHECK(ctx, "paged_tokens_kernel");
 }
 template <class T, int G>
-int32_t rows_go(agpu_ctx *ctx, PagedAttn &p, int64_t longest) {
+int32_t rows_go(agpu_ctx *ctx, const PagedAttn &p, int64_t longest) {
     const int group = p.n_heads / p.n_kv, slots = 8 / group;  // up to eight rows: token by token
     const int tile_places = (int)((int64_t)p.tokens * group / TILE_ROWS) + p.batch;
-    const int64_t items = ((int64_t)tile_places + (int64_t)p.batch * slots) * p.n_kv;
-    const paged::Cut cut = paged::cut_keys(items, longest, 1024, 256, 64, TILE_ROWS * (DH + 2) * sizeof(float), ctx->ws_bytes / 2, ctx->n_counters - 1);
-    p.part = TILE_ROWS * (DH + 2);  // (a token's take less)
-    p.shortest_run = cut.shortest;
-    p.max_runs = cut.runs;
-    hipLaunchKernelGGL((paged_rows_kernel<T, G>), dim3((unsigned)items, cut.runs), dim3(256), 0, ctx->stream, p, tile_places, slots);
+    const int64_t tiles = (int64_t)tile_places * p.n_kv, tokens = (int64_t)p.batch * slots * p.n_kv;
+    constexpr int tile_part = TILE_ROWS * (DH + 2), token_part = G * (DH + 2);
+    // a quarter of the scratch and of the tickets each
+    const size_t space = ctx->ws_bytes / 4;
+    const int64_t tickets = (ctx->n_counters - 1) / 2;
+    const paged::Cut a = paged::cut_keys(tiles, longest, 1024, 256, 64, tile_part * sizeof(float), space, tickets);
+    const paged::Cut b = paged::cut_keys(tokens, longest, 2048, 128, 64, token_part * sizeof(float), space, tickets);
+    const Runs tile_cut = {a.shortest, a.runs, reinterpret_cast<float *>(ctx->workspace), tile_part, ctx->counters};
+    const Runs token_cut = {b.shortest, b.runs, reinterpret_cast<float *>(ctx->workspace + space), token_part, ctx->counters + tickets};
+    hipLaunchKernelGGL((paged_rows_kernel<T, G>), dim3((unsigned)(tiles * a.runs + tokens * b.runs)), dim3(256), 0, ctx->stream, p, tile_cut, token_cut, tile_places, slots);
     return AGPU_LAUNCH_CHECK(ctx, "paged_rows_kernel");
 }
 template <class T>
-int32_t attention_go(agpu_ctx *ctx, PagedAttn &p, int64_t longest) {
+int32_t attention_go(agpu_ctx *ctx, const PagedAttn &p, int64_t longest) {
     const int g = p.n_heads / p.n_kv;
     auto go = [&](auto heads) {
         constexpr int G = decltype(heads)::value;
@@ -799,8 +808,6 @@ AGPU_EXPORT int32_t agpu_paged_attention(agpu_ctx *ctx, const float *q, int64_t 
     p.tokens = tokens; p.batch = batch; p.n_heads = n_heads; p.n_kv = n_kv_heads; p.n_pages = n_pages;
     p.width = table_width; p.held = table_width * page_size; p.window = window; p.sinks = sinks;
     p.div = PageDiv::of(page_size);
-    p.partial = reinterpret_cast<float *>(ctx->workspace);
-    p.counters = ctx->counters;
     p.strict = ctx->strict_sync;
     const int64_t longest = paged::longest_row(p.held, window, sinks);
     return cache_type == AGPU_CACHE_F32 ? attention_go<F32>(ctx, p, longest) : cache_type == AGPU_CACHE_F16 ? attention_go<F16>(ctx, p, longest) : attention_go<BF16>(ctx, p, longest);
