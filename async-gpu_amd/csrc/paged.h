@@ -50,26 +50,34 @@ AGPU_HD Visible visible(int pos, int kv_len, int held, int window, int sinks) {
     return {first, first + rest, low - first};
 }
 
-// Keys over workgroups: a run of keys a workgroup, `most` runs at most.
-AGPU_HD int run_of_keys(int count, int shortest, int most) {
-    const int even = ((count + most - 1) / most + 31) & ~31;
-    return even > shortest ? even : shortest;
+// `count` keys over workgroups: about as many runs as there are `run` keys in them, `most` at most, of `keys` each (a multiple of 32; the last ones may be
+// empty).  More keys never make fewer runs.
+struct RunsOf {
+    int runs, keys;
+};
+AGPU_HD RunsOf runs_of(int count, int run, int most) {
+    int runs = (int)(((unsigned)count + (unsigned)run / 2) / (unsigned)run);
+    runs = runs < 1 ? 1 : runs > most ? most : runs;
+    return {runs, ((count + runs - 1) / runs + 31) & ~31};
+}
+// A run's length for `work` keys in all (added up over the items) that are to be `fill` runs or so: between `least` and what leaves no item more than `most`.
+AGPU_HD int run_for(float work, float fill, int least, int longest, int most) {
+    const float even = work / fill;
+    int run = even < 1048576.0f ? (int)even : 1048576;
+    const int needed = (longest + most - 1) / most;
+    run = run > least ? run : least;
+    run = run > needed ? run : needed;
+    return (run + 31) & ~31;
 }
 
-// The cut of a call: items (a token's query heads of one K/V head, or a tile of rows), runs of keys for each and how short a run is.
-struct Cut {
-    int shortest, runs;
-};
-// longest: the most keys a row can see.  Partial results of an item and run take item_bytes of `space`; an item of several runs needs one of `tickets`.
-inline Cut cut_keys(int64_t items, int64_t longest, int64_t fill, int64_t shortest, int64_t most_runs, size_t item_bytes, size_t space, int64_t tickets) {
-    int64_t run = (longest * items / fill + 31) & ~(int64_t)31;
-    run = run < shortest ? shortest : run > 8 * shortest ? 8 * shortest : run;
-    int64_t runs = (longest + run - 1) / run;
-    runs = runs < most_runs ? runs : most_runs;
+// How many runs an item may have at most: `longest` keys in runs of `least`, partial results of item_bytes each in `space`, a ticket for every item of several.
+inline int most_runs(int64_t items, int64_t longest, int64_t least, size_t item_bytes, size_t space, int64_t tickets) {
+    int64_t runs = (longest + least - 1) / least;
+    runs = runs < 64 ? runs : 64;
     if (items > tickets) runs = 1;
     const int64_t room = items > 0 ? (int64_t)(space / item_bytes) / items : 1;
     runs = runs < room ? runs : room;
-    return {(int)run, runs < 1 ? 1 : (int)runs};
+    return runs < 1 ? 1 : (int)runs;
 }
 // The most keys a row can see.
 inline int64_t longest_row(int64_t held, int64_t window, int64_t sinks) { return window > 0 && window + sinks < held ? window + sinks : held; }

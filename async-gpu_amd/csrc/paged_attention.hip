@@ -27,7 +27,7 @@ struct PagedAttn {
 
 // How keys are cut into runs over workgroups, and where items of several runs leave their partial results and draw their tickets.
 struct Runs {
-    int shortest, most;
+    int run, most;  // about how many keys; how many runs at most
     float *partial;
     int part;  // floats of an item's run there
     unsigned int *counters;
@@ -114,9 +114,10 @@ __device__ __forceinline__ void token_run(const PagedAttn &p, TokenShared<G, W> 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int sub = lane % LPK, own = lane / LPK;
     const Visible vis = paged::visible(kv_len - end + t, kv_len, p.held, p.window, p.sinks);
-    const int keys = paged::run_of_keys(vis.count, cut.shortest, cut.most), runs = max(1, (vis.count + keys - 1) / keys);
+    const paged::RunsOf cuts = paged::runs_of(vis.count, cut.run, cut.most);
+    const int runs = cuts.runs;
     if (run >= runs) return;
-    const int lo = run * keys, hi = min(vis.count, lo + keys);
+    const int lo = run * cuts.keys, hi = min(vis.count, lo + cuts.keys);
 
     float q[G][EL];
 #pragma unroll
@@ -269,16 +270,112 @@ __device__ __forceinline__ void token_run(const PagedAttn &p, TokenShared<G, W> 
     }
 }
 
-// grid (tokens * n_kv * blocks, runs): every row by itself, whatever request it belongs to.
+#ifndef TOKG
+#define TOKG 6
+#define FILL 4.0f
+#define ROWG 2
+#endif
+constexpr int kListed = 256;
+// The work of up to 256 entries (requests, or tokens), in LDS: running sums of their units.  A workgroup numbers all units, entry by entry, and takes
+// those of its own number, that plus the number of workgroups, and so on.
+struct Units {
+    int incl[kListed];
+    // units[j] of entry 64 j + lane, the same in every wave; returns how many there are (a barrier has to follow)
+    __device__ __forceinline__ int number(const int (&units)[4], int entries, int lane) {
+        int all = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (64 * j >= entries) break;  // uniform
+            int v = units[j];
+#pragma unroll
+            for (int by = 1; by < 64; by <<= 1) {
+                const int o = __shfl_up(v, by, kWave);
+                v += lane >= by ? o : 0;
+            }
+            incl[64 * j + lane] = v + all;
+            all += __builtin_amdgcn_readlane(v, 63);
+        }
+        return all;
+    }
+    // the entry of unit u; u becomes its number within the entry
+    __device__ __forceinline__ int entry(int &u, int lane) const {
+        int at = 0, before = 0;
+        for (int j = 0;; ++j) {
+            const int v = incl[64 * j + lane];
+            const uint64_t beyond = __ballot(v > u);
+            if (beyond != 0) {  // uniform; there is one
+                at = __builtin_ctzll(beyond);
+                if (at > 0) before = __builtin_amdgcn_readlane(v, at - 1);
+                u -= before;
+                return 64 * j + at;
+            }
+            before = __builtin_amdgcn_readlane(v, 63);
+        }
+    }
+};
+
+// What the last row of a request (or a tile of `rows` tokens) sees at most.
+__device__ __forceinline__ int keys_seen(const PagedAttn &p, int kv_len, int rows) {
+    const int held = max(min(kv_len, p.held), 0);
+    return p.window > 0 ? (int)min((long long)held, (long long)p.window + p.sinks + rows) : held;
+}
+
+// Every row by itself, whatever request it belongs to: a unit is a run of the keys of up to G query heads of a token that share a K/V head.  Up to 256 tokens
+// (`listed`) the units are numbered and a run is as long as it takes to keep the device busy; for more, there are items * cut.most.
 template <class T, int G, int W, int PASS>
-__global__ __launch_bounds__(64 * W) void paged_tokens_kernel(const PagedAttn p, const Runs cut) {
+__global__ __launch_bounds__(64 * W) void paged_tokens_kernel(const PagedAttn p, Runs cut, float fill, int least, int listed) {
     __shared__ TokenShared<G, W> s;
-    const int item = blockIdx.x, heads_all = p.n_heads / p.n_kv, blocks = (heads_all + G - 1) / G;  // (G is the power of two that covers them, up to 8)
-    const int t = item / (p.n_kv * blocks), hb = item - t * p.n_kv * blocks, h = hb / blocks, g0 = (hb - h * blocks) * G;
-    const int b = request_of(p.query_start, p.batch, t, threadIdx.x & 63);
-    if (b >= p.batch) return;
-    const int end = p.query_start ? p.query_start[b + 1] : t + 1;
-    token_run<T, G, W, PASS>(p, s, cut, t, b, p.kv_lens[b], end, h, h * heads_all + g0, min(G, heads_all - g0), blockIdx.y, item);
+    __shared__ Units list;
+    const int lane = threadIdx.x & 63, heads_all = p.n_heads / p.n_kv, blocks = (heads_all + G - 1) / G;  // (G is the power of two that covers them, up to 8)
+    const int per_token = p.n_kv * blocks;
+    int all = p.tokens * per_token * cut.most;
+    if (listed) {
+        int units[4], longest = 0;
+        float work = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            units[j] = 0;
+            const int row = 64 * j + lane;
+            if (row < p.tokens) {
+                // the request of a row that is no request's only one: its first entry of query_start beyond the row
+                int b = row;
+                if (p.query_start && !(row < p.batch && p.query_start[row] == row && p.query_start[row + 1] == row + 1)) {
+                    int lo = 0, hi = p.batch;
+                    while (lo < hi) {
+                        const int mid = (lo + hi) >> 1;
+                        if (p.query_start[mid + 1] <= row) lo = mid + 1;
+                        else hi = mid;
+                    }
+                    b = lo;
+                }
+                units[j] = b < p.batch ? max(keys_seen(p, p.kv_lens[b], 1), 1) : 0;
+            }
+            work += (float)units[j];
+            longest = max(longest, units[j]);
+        }
+        cut.run = paged::run_for(wave_sum(work) * per_token, fill, least, (int)wave_minmax_u32<true>((unsigned)longest), cut.most);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) units[j] = units[j] > 0 ? paged::runs_of(units[j], cut.run, cut.most).runs * per_token : 0;
+        all = list.number(units, p.tokens, lane);
+    }
+    for (int unit = blockIdx.x; unit < all; unit += gridDim.x) {
+        __syncthreads();  // the numbers, and what the last unit left
+        int at = unit, t, run, hb;
+        if (listed) {
+            t = list.entry(at, lane);
+            run = at / per_token;
+            hb = at - run * per_token;
+        } else {
+            run = at % cut.most;
+            at /= cut.most;
+            t = at / per_token;
+            hb = at - t * per_token;
+        }
+        const int h = hb / blocks, g0 = (hb - h * blocks) * G, b = request_of(p.query_start, p.batch, t, lane);
+        if (b >= p.batch) continue;
+        const int end = p.query_start ? p.query_start[b + 1] : t + 1;
+        token_run<T, G, W, PASS>(p, s, cut, t, b, p.kv_lens[b], end, h, h * heads_all + g0, min(G, heads_all - g0), run, t * per_token + hb);
+    }
 }
 
 // ---- tiles of rows on the matrix cores ----
@@ -347,16 +444,22 @@ struct Staged;
 template <>
 struct Staged<F32> {
     float x[8];
-    __device__ __forceinline__ void row(const char *p, bool ok) {
-        const float4 a = ok ? *reinterpret_cast<const float4 *>(p) : make_float4(0.f, 0.f, 0.f, 0.f), b = ok ? *reinterpret_cast<const float4 *>(p + 16) : a;
+    __device__ __forceinline__ void row(const char *p) {
+        const float4 a = *reinterpret_cast<const float4 *>(p), b = *reinterpret_cast<const float4 *>(p + 16);
         x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
     }
-    __device__ __forceinline__ void element(int e, const char *p, bool ok) { x[e] = ok ? *reinterpret_cast<const float *>(p) : 0.0f; }
-    __device__ __forceinline__ float trace() const {  // not a number if one of them is infinite or none
+    __device__ __forceinline__ void element(int e, const char *p) { x[e] = *reinterpret_cast<const float *>(p); }
+    __device__ __forceinline__ void clear_row() {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = 0.0f;
+    }
+    __device__ __forceinline__ void clear_element(int e) { x[e] = 0.0f; }
+    __device__ __forceinline__ void pack() {}
+    __device__ __forceinline__ bool odd() const {  // one of them is infinite or no number
         float t = 0.0f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) t = fmaf(x[e], 0.0f, t);
-        return t;
+        return t != 0.0f;
     }
     // Zeros in place of those; which there were.
     __device__ __forceinline__ uint32_t clean() {
@@ -378,42 +481,36 @@ struct Staged<F32> {
 };
 template <class T>
 struct Staged16 {
-    uint32_t x[8];  // K: the first four, two elements each; V: one each
-    bool is_row;
-    __device__ __forceinline__ void row(const char *p, bool ok) {
-        const uint4 a = ok ? *reinterpret_cast<const uint4 *>(p) : make_uint4(0, 0, 0, 0);
+    uint32_t x[8];  // a row, or elements that have been packed: the first four, two elements each; before: one each
+    __device__ __forceinline__ void row(const char *p) {
+        const uint4 a = *reinterpret_cast<const uint4 *>(p);
         x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-        is_row = true;
     }
-    __device__ __forceinline__ void element(int e, const char *p, bool ok) {
-        x[e] = ok ? *reinterpret_cast<const unsigned short *>(p) : 0u;
-        is_row = false;
-    }
-    __device__ __forceinline__ uint4 frag() const {
-        return is_row ? make_uint4(x[0], x[1], x[2], x[3]) : make_uint4(x[0] | x[1] << 16, x[2] | x[3] << 16, x[4] | x[5] << 16, x[6] | x[7] << 16);
-    }
-    __device__ __forceinline__ float trace() const {
-        float f[8], t = 0.0f;
-        T::floats(frag(), f);
+    __device__ __forceinline__ void element(int e, const char *p) { x[e] = *reinterpret_cast<const unsigned short *>(p); }
+    __device__ __forceinline__ void clear_row() { x[0] = x[1] = x[2] = x[3] = 0; }
+    __device__ __forceinline__ void clear_element(int e) { x[e] = 0; }
+    __device__ __forceinline__ void pack() {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) t = fmaf(f[e], 0.0f, t);
-        return t;
+        for (int e = 0; e < 4; ++e) x[e] = x[2 * e] | x[2 * e + 1] << 16;
+    }
+    __device__ __forceinline__ bool odd() const {  // an exponent of ones and one more is the sign bit
+        constexpr uint32_t ones = T::kExponent * 0x10001u, one = (T::kExponent & (0u - T::kExponent)) * 0x10001u;
+        uint32_t t = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) t |= (x[e] & ones) + one;
+        return (t & 0x80008000u) != 0;
     }
     __device__ __forceinline__ uint32_t clean() {
         uint32_t odd = 0;
-        constexpr uint32_t kExponent = T::kExponent;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const uint32_t bits = (is_row ? x[e >> 1] >> (16 * (e & 1)) : x[e]) & kExponent;
-            if (bits == kExponent) {
+        for (int e = 0; e < 8; ++e)
+            if ((x[e >> 1] >> (16 * (e & 1)) & T::kExponent) == T::kExponent) {
                 odd |= 1u << e;
-                if (is_row) x[e >> 1] &= e & 1 ? 0x0000ffffu : 0xffff0000u;
-                else x[e] = 0;
+                x[e >> 1] &= e & 1 ? 0x0000ffffu : 0xffff0000u;
             }
-        }
         return odd;
     }
-    __device__ __forceinline__ void store(uint4 *to) const { *to = frag(); }
+    __device__ __forceinline__ void store(uint4 *to) const { *to = make_uint4(x[0], x[1], x[2], x[3]); }
 };
 template <>
 struct Staged<BF16> : Staged16<BF16> {};
@@ -423,9 +520,8 @@ struct Staged<F16> : Staged16<F16> {};
 template <class T>
 struct TileShared {
     uint4 k[2][Tiles<T>::KP][kFrag], v[2][Tiles<T>::KP][kFrag];  // [buffer][piece]: K [d step of 16][half][key], V [32 dimensions][key step][half][dimension]
-    long long at[4][TILE_KEYS];  // of a tile's keys: where their rows begin, in elements from the head's first page, K and V
-    long long at_v[4][TILE_KEYS];
-    uint32_t seen[4];            // which of them are there
+    long long at[4][TILE_KEYS], at_v[4][TILE_KEYS];  // of a tile's keys: where their rows of K and V begin, in bytes (0 for those that are not there)
+    uint32_t seen[4];             // which of them are there
     uint32_t odd_k[4], odd_v[4];  // of which something is infinite or not a number
     unsigned int ticket;
 };
@@ -461,9 +557,10 @@ __device__ __forceinline__ void tile_run(const PagedAttn &p, TileShared<T> &s, c
     end = max(end, 0);
     int low = p.window > 0 ? max(pos0 + 1 - p.window, 0) : 0;
     const int first = min(min(p.sinks, low), end), gap = low - first, count = first + max(end - low, 0);
-    const int keys = paged::run_of_keys(count, cut.shortest, cut.most), runs = max(1, (count + keys - 1) / keys);
+    const paged::RunsOf cuts = paged::runs_of(count, cut.run, cut.most);
+    const int runs = cuts.runs;
     if (run >= runs) return;
-    const int lo = run * keys, hi = min(count, lo + keys);
+    const int lo = run * cuts.keys, hi = min(count, lo + cuts.keys);
     // this lane's row; rows behind the last one repeat it
     const int row = min(first_row + 32 * wave + c, last_row), token = row / group, head = h * group + (row - token * group);
     const bool mine = first_row + 32 * wave + c <= last_row, any = first_row + 32 * wave <= last_row;
@@ -516,8 +613,8 @@ __device__ __forceinline__ void tile_run(const PagedAttn &p, TileShared<T> &s, c
     auto leave = [&](int i, int id, int off) {
         const bool ok = (unsigned)id < (unsigned)p.n_pages;
         const long long at = (long long)(h * p.div.size + off) * DH;
-        s.at[i & 3][c] = ok ? id * p.k_page + at : -1;
-        s.at_v[i & 3][c] = ok ? id * p.v_page + at : -1;
+        s.at[i & 3][c] = ok ? (id * p.k_page + at) * kBytes : 0;
+        s.at_v[i & 3][c] = ok ? (id * p.v_page + at) * kBytes : 0;
         const uint64_t who = __ballot(ok);
         if (lane == 0) {
             s.seen[i & 3] = (uint32_t)who;
@@ -535,14 +632,15 @@ __device__ __forceinline__ void tile_run(const PagedAttn &p, TileShared<T> &s, c
     __syncthreads();
     const char *const kb = static_cast<const char *>(p.k), *const vb = static_cast<const char *>(p.v);
     Staged<T> sk, sv;
-    const int k_d = 16 * wave + 8 * h2, v_step = wave & 1, v_d = 32 * (wave >> 1) + c;  // what this thread fetches
+    // What this thread fetches: eight elements of K of key c, and eight keys of dimension `lane` of V, the same ones for the whole wave.
+    const int k_byte = (16 * wave + 8 * h2) * kBytes, v_step = wave & 1, v_half = wave >> 1;
     auto fetch = [&](int i) {
-        const long long at = s.at[i & 3][c];
-        sk.row(kb + (at + k_d) * kBytes, at >= 0);
+        sk.row(kb + s.at[i & 3][c] + k_byte);
+        const long long at = s.at_v[i & 3][tile_key(v_step, v_half, lane & 7)];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const long long to = s.at_v[i & 3][tile_key(v_step, h2, e)];
-            sv.element(e, vb + (to + v_d) * kBytes, to >= 0);
+            const uint32_t low = __builtin_amdgcn_readlane((int)(uint32_t)at, e), high = __builtin_amdgcn_readlane((int)(at >> 32), e);
+            sv.element(e, vb + (long long)((uint64_t)high << 32 | low) + lane * kBytes);
         }
     };
     if (tiles > 0) fetch(0);
@@ -551,15 +649,23 @@ __device__ __forceinline__ void tile_run(const PagedAttn &p, TileShared<T> &s, c
     float m = -INFINITY, l = 0.0f;
     for (int i = 0; i < tiles; ++i) {
         const int buf = i & 1;
-        if (__builtin_expect(__any(sk.trace() + sv.trace() != 0.0f), 0)) {
+        const uint32_t there = s.seen[i & 3];
+        if (there != 0xffffffffu) {  // uniform; zeros instead of what is not there
+            if (!(there >> c & 1)) sk.clear_row();
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (!(there >> tile_key(v_step, v_half, e) & 1)) sv.clear_element(e);
+        }
+        sv.pack();
+        if (__builtin_expect(__any(sk.odd() || sv.odd()), 0)) {
             if (sk.clean()) atomicOr(&s.odd_k[i & 3], 1u << c);
             const uint32_t odd = sv.clean();
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-                if (odd >> e & 1) atomicOr(&s.odd_v[i & 3], 1u << tile_key(v_step, h2, e));
+                if (odd >> e & 1) atomicOr(&s.odd_v[i & 3], 1u << tile_key(v_step, v_half, e));
         }
         sk.store(&s.k[buf][0][(2 * wave + h2) * 32 + c]);
-        sv.store(&s.v[buf][0][((2 * (wave >> 1) + v_step) * 2 + h2) * 32 + c]);
+        sv.store(&s.v[buf][0][((2 * h2 + v_step) * 2 + v_half) * 32 + c]);
         if (i + 1 < tiles) fetch(i + 1);
         if (tid < 32) {
             leave(i + 2, id, off);
@@ -568,7 +674,6 @@ __device__ __forceinline__ void tile_run(const PagedAttn &p, TileShared<T> &s, c
         __syncthreads();
         const int v0 = lo + TILE_KEYS * i;
         if (!any || (v0 >= first && v0 > wave_pos1 - gap)) continue;  // (the next tile goes to the other buffer)
-        const uint32_t there = s.seen[i & 3];
         floatx16 x = {};
 #pragma unroll
         for (int level = QP - 1; level >= 0; --level)
@@ -590,7 +695,7 @@ __device__ __forceinline__ void tile_run(const PagedAttn &p, TileShared<T> &s, c
                 const size_t at = (size_t)s.at[i & 3][kk];
                 float d = 0.0f;
 #pragma unroll 1
-                for (int e = 0; e < 32; ++e) d = fmaf(q_row[32 * h2 + e] * kQueryScale, T::one(kb, at + 32 * h2 + e), d);
+                for (int e = 0; e < 32; ++e) d = fmaf(q_row[32 * h2 + e] * kQueryScale, T::one(kb + at, 32 * h2 + e), d);
                 d = sum_of_halves(d);
 #pragma unroll
                 for (int r = 0; r < 16; ++r) x[r] = 8 * (r >> 2) + 4 * h2 + (r & 3) == kk ? d : x[r];
@@ -659,7 +764,7 @@ __device__ __forceinline__ void tile_run(const PagedAttn &p, TileShared<T> &s, c
                 for (int db = 0; db < 2; ++db)
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
-                        const float y = T::one(vb, at + 32 * db + 8 * (r >> 2) + 4 * h2 + (r & 3));
+                        const float y = T::one(vb + at, 32 * db + 8 * (r >> 2) + 4 * h2 + (r & 3));
                         o[db][r] += see && !(fabsf(y) < INFINITY) ? weight * y : 0.0f;
                     }
             }
@@ -677,15 +782,16 @@ __device__ __forceinline__ void tile_run(const PagedAttn &p, TileShared<T> &s, c
                 for (int e = 0; e < 4; ++e) out[32 * db + 2 * r + e] = sum == 0.0f ? 0.0f : o[db][r + e] * by;
     };
     if (runs == 1) return store(l);
-    auto part = [&](int r) { return cut.partial + ((size_t)item * cut.most + r) * cut.part + wave * (32 * (DH + 2)); };  // [wave][dimension, or m and l][row]
+    auto part = [&](int r) { return cut.partial + ((size_t)item * cut.most + r) * cut.part + wave * (32 * (DH + 2)); };  // [wave][two dimensions, or m and l][row]
+    auto pair = [](float a, float b) { return (unsigned long long)__float_as_uint(b) << 32 | __float_as_uint(a); };
+    auto place = [&](int r, int d) { return reinterpret_cast<unsigned long long *>(part(r)) + (d >> 1) * 32 + c; };  // of dimensions d and d + 1 of row c
     if (any) {
-        float *to = part(run);
 #pragma unroll
         for (int db = 0; db < 2; ++db)
 #pragma unroll
-            for (int r = 0; r < 16; ++r)
-                __hip_atomic_store(to + (32 * db + 8 * (r >> 2) + 4 * h2 + (r & 3)) * 32 + c, o[db][r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        __hip_atomic_store(to + (DH + h2) * 32 + c, h2 == 0 ? m : l, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            for (int r = 0; r < 16; r += 2)
+                __hip_atomic_store(place(run, 32 * db + 8 * (r >> 2) + 4 * h2 + (r & 3)), pair(o[db][r], o[db][r + 1]), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (h2 == 0) __hip_atomic_store(place(run, DH), pair(m, l), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     partials_published(p.strict);
     __syncthreads();
@@ -696,65 +802,146 @@ __device__ __forceinline__ void tile_run(const PagedAttn &p, TileShared<T> &s, c
     __syncthreads();
     if (s.ticket != (unsigned)(runs - 1) || !any) return;
     if (p.strict) __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
-    auto load = [&](int r, int i) { return __hip_atomic_load(part(r) + i * 32 + c, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+    auto load = [&](int r, int d, float &x, float &y) {
+        const unsigned long long v = __hip_atomic_load(place(r, d), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        x = __uint_as_float((uint32_t)v);
+        y = __uint_as_float((uint32_t)(v >> 32));
+    };
     m = -INFINITY;
-    for (int r = 0; r < runs; ++r) m = fmaxf(m, load(r, DH));
+    for (int r = 0; r < runs; ++r) {
+        float mr, lr;
+        load(r, DH, mr, lr);
+        m = fmaxf(m, mr);
+    }
     l = 0.0f;
     o[0] = o[1] = floatx16{};
 #pragma unroll 1
     for (int r = 0; r < runs; ++r) {
-        const float mr = load(r, DH), a = mr == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mr - m);
-        l = fmaf(load(r, DH + 1), a, l);
+        float mr, lr;
+        load(r, DH, mr, lr);
+        const float a = mr == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mr - m);
+        l = fmaf(lr, a, l);
 #pragma unroll
         for (int db = 0; db < 2; ++db)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) o[db][e] = fmaf(load(r, 32 * db + 8 * (e >> 2) + 4 * h2 + (e & 3)), a, o[db][e]);
+            for (int e = 0; e < 16; e += 2) {
+                float x, y;
+                load(r, 32 * db + 8 * (e >> 2) + 4 * h2 + (e & 3), x, y);
+                o[db][e] = fmaf(x, a, o[db][e]);
+                o[db][e + 1] = fmaf(y, a, o[db][e + 1]);
+            }
     }
     store(l);
 }
 
-// Requests with new rows of every number: those with up to eight rows of heads a K/V head go token by token, the others in tiles.  grid: tile places * n_kv *
-// runs, then token places * n_kv * runs.  A request b has tile places from query_start[b] * group / 128 + b on, enough for its rows and one more than all tiles of
-// the requests before it need; and `slots` places for its tokens.
+// Requests with new rows of every number: those with up to eight rows of heads a K/V head (`slots` tokens) go token by token, the others in tiles.  A
+// unit is a run of keys of a tile, or of a token, and a K/V head.  Up to 256 requests (`listed`) the units are numbered, tiles first, and runs are as long as it
+// takes to keep the device busy; for more, the grid has places for as many as there could be.  Request b's tiles have places from
+// query_start[b] * group / 128 + b on, which are enough for its rows, and more than all tiles of the requests before it need.
 template <class T, int G>
-__global__ __launch_bounds__(256, 2) void paged_rows_kernel(const PagedAttn p, const Runs tile_cut, const Runs token_cut, int tile_places, int slots) {
+__global__ __launch_bounds__(256, 2) void paged_rows_kernel(const PagedAttn p, Runs tile_cut, Runs token_cut, int tile_places, int slots, int cus, int listed) {
     union Shared {
         TileShared<T> tiles;
         TokenShared<G, 4> token;
     };
     __shared__ __align__(16) char smem[sizeof(Shared)];
-    const int lane = threadIdx.x & 63, group = p.n_heads / p.n_kv, tile_items = tile_places * p.n_kv, tile_wgs = tile_items * tile_cut.most;
-    int at = blockIdx.x;
-    if (at < tile_wgs) {
-        // consecutive workgroups go round the XCDs; an XCD takes consecutive items, whose tiles share a head's K and V
-        const int each = tile_wgs >> 3, rest = tile_wgs & 7, xcd = at & 7;
-        at = xcd * each + min(xcd, rest) + (at >> 3);
-        const int item = at / tile_cut.most, run = at - item * tile_cut.most;
-        const int h = item / tile_places, place = tile_places - 1 - (item - h * tile_places);
-        int b = -1;
-        for (int i = 0; i < p.batch; i += 64) b += __popcll(__ballot(i + lane < p.batch && p.query_start[i + lane] * group / TILE_ROWS + i + lane <= place));
-        if (b < 0) return;
-        const int start = p.query_start[b], q_len = min(p.query_start[b + 1], p.tokens) - start, rows = q_len * group;
-        const int first_row = (place - start * group / TILE_ROWS - b) * TILE_ROWS;
-        if (start < 0 || q_len <= slots || first_row < 0 || first_row >= rows) return;
-        tile_run<T>(p, *reinterpret_cast<TileShared<T> *>(smem), tile_cut, b, start, q_len, p.kv_lens[b], h, first_row, run, item);
-    } else {
-        at -= tile_wgs;
-        const int item = at / token_cut.most, run = at - item * token_cut.most;
-        const int h = item % p.n_kv, place = item / p.n_kv, b = place / slots, i = place - b * slots;
+    __shared__ Units tile_list, token_list;
+    const int lane = threadIdx.x & 63, group = p.n_heads / p.n_kv;
+    int tile_units = tile_places * p.n_kv * tile_cut.most, all = tile_units + p.batch * slots * p.n_kv * token_cut.most;
+    if (listed) {
+        int tiles[4], tokens[4], keys[4], longest = 0;
+        float tile_work = 0.0f, token_work = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            tiles[j] = tokens[j] = keys[j] = 0;
+            if (64 * j + lane < p.batch) {
+                const int start = p.query_start[64 * j + lane], q_len = min(p.query_start[64 * j + lane + 1], p.tokens) - start;
+                if (start >= 0 && q_len > 0) {
+                    keys[j] = max(keys_seen(p, p.kv_lens[64 * j + lane], q_len > slots ? min(q_len, TILE_ROWS / group + 2) : 1), 1);
+                    if (q_len > slots) tiles[j] = (q_len * group + TILE_ROWS - 1) / TILE_ROWS;
+                    else tokens[j] = q_len;
+                }
+            }
+            tile_work += (float)tiles[j] * (float)keys[j];
+            token_work += (float)tokens[j] * (float)keys[j];
+            longest = max(longest, keys[j]);
+        }
+        longest = (int)wave_minmax_u32<true>((unsigned)longest);
+        tile_cut.run = paged::run_for(wave_sum(tile_work) * p.n_kv, 2.0f * cus, 256, longest, tile_cut.most);
+        token_cut.run = paged::run_for(wave_sum(token_work) * p.n_kv, 2.0f * cus, 128, longest, token_cut.most);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            tiles[j] = tiles[j] > 0 ? tiles[j] * paged::runs_of(keys[j], tile_cut.run, tile_cut.most).runs * p.n_kv : 0;
+            tokens[j] = tokens[j] > 0 ? tokens[j] * paged::runs_of(keys[j], token_cut.run, token_cut.most).runs * p.n_kv : 0;
+        }
+        tile_units = tile_list.number(tiles, p.batch, lane);
+        all = tile_units + token_list.number(tokens, p.batch, lane);
+    }
+    for (int unit = blockIdx.x; unit < all; unit += gridDim.x) {
+        __syncthreads();  // the numbers, and what the last unit left
+        int at = unit, b, h, run, tile = -1, token = -1;
+        if (listed) {
+            if (at < tile_units) {
+                // consecutive workgroups go round the XCDs; an XCD takes consecutive units, whose tiles share a head's K and V
+                const int each = tile_units >> 3, rest = tile_units & 7, xcd = at & 7;
+                at = xcd * each + min(xcd, rest) + (at >> 3);
+                b = tile_list.entry(at, lane);
+                const int q_len = min(p.query_start[b + 1], p.tokens) - p.query_start[b], n = (q_len * group + TILE_ROWS - 1) / TILE_ROWS;
+                const int runs = paged::runs_of(max(keys_seen(p, p.kv_lens[b], min(q_len, TILE_ROWS / group + 2)), 1), tile_cut.run, tile_cut.most).runs;
+                h = at / (n * runs);
+                at -= h * n * runs;
+                tile = n - 1 - at / runs;
+                run = at % runs;
+            } else {
+                at -= tile_units;
+                b = token_list.entry(at, lane);
+                const int runs = paged::runs_of(max(keys_seen(p, p.kv_lens[b], 1), 1), token_cut.run, token_cut.most).runs;
+                token = at / (runs * p.n_kv);
+                at -= token * runs * p.n_kv;
+                run = at / p.n_kv;
+                h = at - run * p.n_kv;
+            }
+        } else if (at < tile_units) {
+            run = at % tile_cut.most;
+            at /= tile_cut.most;
+            h = at / tile_places;
+            const int place = tile_places - 1 - (at - h * tile_places);
+            b = -1;
+            for (int i = 0; i < p.batch; i += 64) b += __popcll(__ballot(i + lane < p.batch && p.query_start[i + lane] * group / TILE_ROWS + i + lane <= place));
+            if (b < 0) continue;
+            tile = place - p.query_start[b] * group / TILE_ROWS - b;
+        } else {
+            at -= tile_units;
+            run = at % token_cut.most;
+            at /= token_cut.most;
+            h = at % p.n_kv;
+            at /= p.n_kv;
+            b = at / slots;
+            token = at - b * slots;
+        }
         const int start = p.query_start[b], end = min(p.query_start[b + 1], p.tokens), q_len = end - start;
-        if (start < 0 || i >= q_len || q_len > slots) return;
-        token_run<T, G, 4, 4>(p, *reinterpret_cast<TokenShared<G, 4> *>(smem), token_cut, start + i, b, p.kv_lens[b], end, h, h * group, group, run, item);
+        if (start < 0) continue;
+        if (token < 0) {
+            if (q_len <= slots || tile < 0 || tile * TILE_ROWS >= q_len * group) continue;
+            const int item = (start * group / TILE_ROWS + b + tile) * p.n_kv + h;
+            tile_run<T>(p, *reinterpret_cast<TileShared<T> *>(smem), tile_cut, b, start, q_len, p.kv_lens[b], h, tile * TILE_ROWS, run, item);
+        } else {
+            if (token >= q_len || q_len > slots) continue;
+            token_run<T, G, 4, 4>(p, *reinterpret_cast<TokenShared<G, 4> *>(smem), token_cut, start + token, b, p.kv_lens[b], end, h, h * group, group, run,
+                                  (b * slots + token) * p.n_kv + h);
+        }
     }
 }
 
 template <class T, int G>
 int32_t tokens_go(agpu_ctx *ctx, const PagedAttn &p, int64_t longest) {
     const int64_t items = (int64_t)p.tokens * p.n_kv * ceil_div(p.n_heads / p.n_kv, G);
-    constexpr int part = G * (DH + 2);
-    const paged::Cut cut = paged::cut_keys(items, longest, 2048, 128, 64, part * sizeof(float), ctx->ws_bytes / 2, ctx->n_counters - 1);
-    const Runs runs = {cut.shortest, cut.runs, reinterpret_cast<float *>(ctx->workspace), part, ctx->counters};
-    hipLaunchKernelGGL((paged_tokens_kernel<T, G, 4, 4>), dim3((unsigned)items, cut.runs), dim3(256), 0, ctx->stream, p, runs);
+    constexpr int part = G * (DH + 2), least = 128;
+    const bool listed = p.tokens <= kListed;
+    const int most = paged::most_runs(items, longest, listed ? least : 1024, part * sizeof(float), ctx->ws_bytes / 2, ctx->n_counters - 1);
+    const Runs cut = {1024, most, reinterpret_cast<float *>(ctx->workspace), part, ctx->counters};
+    hipLaunchKernelGGL((paged_tokens_kernel<T, G, 4, 4>), dim3((unsigned)std::min<int64_t>(items * most, TOKG * ctx->num_cus)), dim3(256), 0, ctx->stream, p, cut,
+                       FILL * ctx->num_cus, least, (int)listed);
     return AGPU_LAUNCH_CHECK(ctx, "paged_tokens_kernel");
 }
 template <class T, int G>
@@ -763,14 +950,17 @@ int32_t rows_go(agpu_ctx *ctx, const PagedAttn &p, int64_t longest) {
     const int tile_places = (int)((int64_t)p.tokens * group / TILE_ROWS) + p.batch;
     const int64_t tiles = (int64_t)tile_places * p.n_kv, tokens = (int64_t)p.batch * slots * p.n_kv;
     constexpr int tile_part = TILE_ROWS * (DH + 2), token_part = G * (DH + 2);
-    // a quarter of the scratch and of the tickets each
-    const size_t space = ctx->ws_bytes / 4;
+    const size_t space = ctx->ws_bytes / 4 * 3;  // of the scratch, for tiles; the rest, and half of the tickets each
     const int64_t tickets = (ctx->n_counters - 1) / 2;
-    const paged::Cut a = paged::cut_keys(tiles, longest, 1024, 256, 64, tile_part * sizeof(float), space, tickets);
-    const paged::Cut b = paged::cut_keys(tokens, longest, 2048, 128, 64, token_part * sizeof(float), space, tickets);
-    const Runs tile_cut = {a.shortest, a.runs, reinterpret_cast<float *>(ctx->workspace), tile_part, ctx->counters};
-    const Runs token_cut = {b.shortest, b.runs, reinterpret_cast<float *>(ctx->workspace + space), token_part, ctx->counters + tickets};
-    hipLaunchKernelGGL((paged_rows_kernel<T, G>), dim3((unsigned)(tiles * a.runs + tokens * b.runs)), dim3(256), 0, ctx->stream, p, tile_cut, token_cut, tile_places, slots);
+    const bool listed = p.batch <= kListed;
+    const int tile_most = paged::most_runs(tiles, longest, listed ? 256 : 2048, tile_part * sizeof(float), space, tickets);
+    const int token_most = paged::most_runs(tokens, longest, listed ? 128 : 1024, token_part * sizeof(float), ctx->ws_bytes - space, tickets);
+    const Runs tile_cut = {2048, tile_most, reinterpret_cast<float *>(ctx->workspace), tile_part, ctx->counters};
+    const Runs token_cut = {1024, token_most, reinterpret_cast<float *>(ctx->workspace + space), token_part, ctx->counters + tickets};
+    const int64_t units = tiles * tile_most + tokens * token_most;
+    if (units > INT32_MAX) return agpu_fail(ctx, AGPU_ERR_UNSUPPORTED, "paged_attention: %d tokens of %d requests are too many", p.tokens, p.batch);
+    hipLaunchKernelGGL((paged_rows_kernel<T, G>), dim3((unsigned)std::min<int64_t>(units, ROWG * ctx->num_cus)), dim3(256), 0, ctx->stream, p, tile_cut, token_cut, tile_places,
+                       slots, ctx->num_cus, (int)listed);
     return AGPU_LAUNCH_CHECK(ctx, "paged_rows_kernel");
 }
 template <class T>

@@ -11,7 +11,7 @@ ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 @pytest.fixture(scope="module")
 def rules(tmp_path_factory):
     """A program that answers a line of numbers with a line of numbers: `div size n`, `vis pos kv held window sinks` (keys that are seen),
-    `cut items longest fill shortest most item_bytes space tickets`, `run count shortest most`, and the refusals."""
+    `most items longest least item_bytes space tickets`, `run count run most`, `for work fill least longest most`, and the refusals."""
     d = tmp_path_factory.mktemp("paged")
     src, exe = d / "rules.cpp", d / "rules"
     src.write_text('''
@@ -34,10 +34,12 @@ int main() {
             for (int i = 0; i < v.count; ++i) std::printf("%d ", v.key(i));
             std::printf("\\n");
         } else if (!std::strcmp(what, "run")) {
-            std::printf("%d\\n", paged::run_of_keys((int)a[0], (int)a[1], (int)a[2]));
-        } else if (!std::strcmp(what, "cut")) {
-            const paged::Cut cut = paged::cut_keys(a[0], a[1], a[2], a[3], a[4], (size_t)a[5], (size_t)a[6], a[7]);
-            std::printf("%d %d\\n", cut.shortest, cut.runs);
+            const paged::RunsOf r = paged::runs_of((int)a[0], (int)a[1], (int)a[2]);
+            std::printf("%d %d\\n", r.runs, r.keys);
+        } else if (!std::strcmp(what, "for")) {
+            std::printf("%d\\n", paged::run_for((float)a[0], (float)a[1], (int)a[2], (int)a[3], (int)a[4]));
+        } else if (!std::strcmp(what, "most")) {
+            std::printf("%d\\n", paged::most_runs(a[0], a[1], a[2], (size_t)a[3], (size_t)a[4], a[5]));
         } else if (!std::strcmp(what, "cache")) {
             std::printf("%d\\n", paged::refuse_cache(a[0], a[1], a[2], a[3], (int)a[4], (int)a[5], (int)a[6], (int)a[7], (int)a[8]).code);
         } else if (!std::strcmp(what, "attention")) {
@@ -82,19 +84,26 @@ def test_what_a_query_sees(rules):
 
 
 def test_runs_cover_all_keys(rules):
-    """However a call is cut, its runs hold every key that a row sees, partial results fit their space, and items of several runs have tickets."""
-    calls = [(items, longest, bytes_, space, tickets) for items in (1, 12, 200, 1536, 70000) for longest in (1, 31, 777, 4128, 32768, 2**30)
-             for bytes_ in (264, 2112, 33792) for space in (1 << 19, 48 << 20) for tickets in (16383, 65535)]
-    cuts = rules([f"cut {i} {n} 2048 128 64 {b} {s} {t}" for i, n, b, s, t in calls])
-    lines, whose = [], []
-    for (items, longest, bytes_, space, tickets), (shortest, runs) in zip(calls, cuts):
-        assert shortest % 32 == 0 and 128 <= shortest <= 1024 and 1 <= runs <= 64
-        assert runs == 1 or (items <= tickets and items * runs * bytes_ <= space)
-        for count in sorted({0, 1, min(longest, 33), min(longest, 1000), longest}):
-            lines.append(f"run {count} {shortest} {runs}")
-            whose.append((count, shortest, runs))
-    for (run,), (count, shortest, runs) in zip(rules(lines), whose):
-        assert run % 32 == 0 and run >= shortest and run * runs >= count
+    """However a call is cut, its runs hold every key that a row sees, and more keys never make fewer runs: a request's runs are counted with the most that a
+    row of it sees, and every row's own have to be among them."""
+    asked = [(n, run, most) for run in (128, 160, 256, 1024, 4096) for most in (1, 2, 5, 7, 64) for n in [*range(0, 3000, 7), *range(3000, 70000, 999), 2**30 - 1, 2**30]]
+    got = rules([f"run {n} {run} {most}" for n, run, most in asked])
+    before = None
+    for (n, run, most), (runs, keys) in zip(asked, got):
+        assert 1 <= runs <= most and keys % 32 == 0 and runs * keys >= n
+        if before and before[:2] == (run, most):
+            assert runs >= before[2]
+        before = (run, most, runs)
+
+
+def test_runs_keep_to_scratch_and_tickets(rules):
+    calls = [(items, longest, least, bytes_, space, tickets) for items in (1, 12, 200, 1536, 70000) for longest in (1, 31, 777, 4128, 32768, 2**30) for least in (128, 1024)
+             for bytes_ in (264, 2112, 33792) for space in (1 << 18, 24 << 20) for tickets in (8191, 65534)]
+    for (items, longest, least, bytes_, space, tickets), (most,) in zip(calls, rules(["most " + " ".join(map(str, c)) for c in calls])):
+        assert 1 <= most <= 64 and (most == 1 or (items <= tickets and items * most * bytes_ <= space and (most - 1) * least < longest))
+    asked = [(work, fill, 128, longest, most) for work in (0, 1, 1000, 10**6, 10**9, 10**15) for fill in (1, 512, 1024) for longest in (1, 129, 4000, 2**30) for most in (1, 3, 64)]
+    for (work, fill, least, longest, most), (run,) in zip(asked, rules(["for " + " ".join(map(str, a)) for a in asked])):
+        assert run % 32 == 0 and least <= run and run * most >= longest and run <= max(least, work / fill, longest / most + 1, 1) + 32
 
 
 SHAPE, UNSUPPORTED = -1, -5
