@@ -270,11 +270,6 @@ __device__ __forceinline__ void token_run(const PagedAttn &p, TokenShared<G, W> 
     }
 }
 
-#ifndef TOKG
-#define TOKG 6
-#define FILL 4.0f
-#define ROWG 2
-#endif
 constexpr int kListed = 256;
 // The work of up to 256 entries (requests, or tokens), in LDS: running sums of their units.  A workgroup numbers all units, entry by entry, and takes
 // those of its own number, that plus the number of workgroups, and so on.
@@ -935,13 +930,14 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(const PagedAttn p, R
 
 template <class T, int G>
 int32_t tokens_go(agpu_ctx *ctx, const PagedAttn &p, int64_t longest) {
-    const int64_t items = (int64_t)p.tokens * p.n_kv * ceil_div(p.n_heads / p.n_kv, G);
+    const int64_t items = (int64_t)p.tokens * p.n_kv * ceil_div(p.n_heads / p.n_kv, G), places = 6 * ctx->num_cus;
     constexpr int part = G * (DH + 2), least = 128;
-    const bool listed = p.tokens <= kListed;
-    const int most = paged::most_runs(items, longest, listed ? least : 1024, part * sizeof(float), ctx->ws_bytes / 2, ctx->n_counters - 1);
-    const Runs cut = {1024, most, reinterpret_cast<float *>(ctx->workspace), part, ctx->counters};
-    hipLaunchKernelGGL((paged_tokens_kernel<T, G, 4, 4>), dim3((unsigned)std::min<int64_t>(items * most, TOKG * ctx->num_cus)), dim3(256), 0, ctx->stream, p, cut,
-                       FILL * ctx->num_cus, least, (int)listed);
+    // Where all the runs there could be find place at once, there is nothing to be counted: that takes 1.8 us (1 token of 12 heads, 777 keys: 10.0 / 8.2).
+    const bool few = items * ((longest + least - 1) / least) <= places, listed = !few && p.tokens <= kListed;
+    const int most = paged::most_runs(items, longest, few || listed ? least : 1024, part * sizeof(float), ctx->ws_bytes / 2, ctx->n_counters - 1);
+    const Runs cut = {few ? least : 1024, most, reinterpret_cast<float *>(ctx->workspace), part, ctx->counters};
+    hipLaunchKernelGGL((paged_tokens_kernel<T, G, 4, 4>), dim3((unsigned)std::min<int64_t>(items * most, places)), dim3(256), 0, ctx->stream, p, cut,
+                       4.0f * ctx->num_cus, least, (int)listed);
     return AGPU_LAUNCH_CHECK(ctx, "paged_tokens_kernel");
 }
 template <class T, int G>
@@ -959,7 +955,7 @@ int32_t rows_go(agpu_ctx *ctx, const PagedAttn &p, int64_t longest) {
     const Runs token_cut = {1024, token_most, reinterpret_cast<float *>(ctx->workspace + space), token_part, ctx->counters + tickets};
     const int64_t units = tiles * tile_most + tokens * token_most;
     if (units > INT32_MAX) return agpu_fail(ctx, AGPU_ERR_UNSUPPORTED, "paged_attention: %d tokens of %d requests are too many", p.tokens, p.batch);
-    hipLaunchKernelGGL((paged_rows_kernel<T, G>), dim3((unsigned)std::min<int64_t>(units, ROWG * ctx->num_cus)), dim3(256), 0, ctx->stream, p, tile_cut, token_cut, tile_places,
+    hipLaunchKernelGGL((paged_rows_kernel<T, G>), dim3((unsigned)std::min<int64_t>(units, 2 * ctx->num_cus)), dim3(256), 0, ctx->stream, p, tile_cut, token_cut, tile_places,
                        slots, ctx->num_cus, (int)listed);
     return AGPU_LAUNCH_CHECK(ctx, "paged_rows_kernel");
 }

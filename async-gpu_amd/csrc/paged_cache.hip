@@ -18,33 +18,45 @@ struct PlanArgs {
 
 constexpr int PLAN_THREADS = 256, PLAN_WAVES = PLAN_THREADS / 64;
 
+// Sums that stay at their largest value once they reach it (what they are compared with is below 2^31).
 struct PlanSums {
-    long long freed, pages, tokens;
+    uint32_t freed, pages, tokens;
     __device__ __forceinline__ void add(const PlanSums &o) {
-        freed += o.freed;
-        pages += o.pages;
-        tokens += o.tokens;
+        freed = __builtin_elementwise_add_sat(freed, o.freed);
+        pages = __builtin_elementwise_add_sat(pages, o.pages);
+        tokens = __builtin_elementwise_add_sat(tokens, o.tokens);
+    }
+    template <int CTRL, int ROWS>
+    __device__ __forceinline__ void add_moved() {
+        auto move = [](uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false); };
+        add({move(freed), move(pages), move(tokens)});
+    }
+    // over the lanes up to this one
+    __device__ __forceinline__ void scan() {
+        add_moved<0x111, 0xf>();  // row_shr 1, 2, 4, 8: within rows of 16
+        add_moved<0x112, 0xf>();
+        add_moved<0x114, 0xf>();
+        add_moved<0x118, 0xf>();
+        add_moved<0x142, 0xa>();  // row_bcast 15: row 0 to 1, 2 to 3
+        add_moved<0x143, 0xc>();  // row_bcast 31: rows 0 and 1 to 2 and 3
     }
 };
-__device__ __forceinline__ long long shift_up(long long v, int by, int lane) {
-    const long long o = __shfl_up(v, by, kWave);
-    return lane >= by ? o : 0;
-}
 
 // What a request asks for: its positions so far, the pages that they are on, new tokens and pages (none where its table row is too short).
 struct Ask {
     int cached, have, tokens, pages;
     bool ended;
-    __device__ __forceinline__ Ask(const PlanArgs &p, int b) {
-        const int n = p.new_lens[b];
-        cached = min(max(p.cached_lens[b], 0), p.width * p.div.size);
+    __device__ __forceinline__ Ask() : cached(0), have(0), tokens(0), pages(0), ended(false) {}
+    __device__ __forceinline__ Ask(const PlanArgs &p, int cached_, int n) {
+        const int held = p.width * p.div.size;
+        cached = min(max(cached_, 0), held);
         ended = n < 0;
-        have = (int)(((long long)cached + p.div.size - 1) / p.div.size);
-        const long long total = (long long)cached + max(n, 0);
-        const bool fits = !ended && total <= (long long)p.width * p.div.size;
+        have = p.div.page(cached + p.div.size - 1);
+        const bool fits = !ended && n <= held - cached;
         tokens = fits ? n : 0;
-        pages = fits ? (int)((total + p.div.size - 1) / p.div.size) - have : 0;
+        pages = fits ? p.div.page(cached + n + p.div.size - 1) - have : 0;
     }
+    __device__ __forceinline__ PlanSums sums() const { return {ended ? (uint32_t)have : 0u, (uint32_t)pages, (uint32_t)tokens}; }
 };
 
 // The last entry of at[0 .. n - 1] (ascending, at[0] = 0) that is not above x.
@@ -57,47 +69,51 @@ __device__ __forceinline__ int entry_of(const int *at, int n, int x) {
 // Every workgroup adds up all requests for itself (they are few, and nobody waits for anybody), then the workgroups share what there is to write.
 // Nothing is read that another one writes: table entries of pages held so far, and the stack below n_free; new pages are looked up where they
 // came from.  What bounds it: a chain of loads, sums and searches, 16 bytes a token at the largest.
+// EACH: requests of a thread.
+template <int EACH>
 __global__ __launch_bounds__(PLAN_THREADS) void paged_plan_kernel(const PlanArgs p) {
     extern __shared__ int s_plan[];  // of every request: pages freed before it, pages taken before it, tokens before it
     __shared__ PlanSums s_wave[PLAN_WAVES];
-    __shared__ long long s_used[2][PLAN_WAVES];
+    __shared__ uint32_t s_used[2][PLAN_WAVES];
     int *const s_freed = s_plan, *const s_pages = s_plan + p.batch, *const s_start = s_plan + 2 * p.batch;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int each = (p.batch + PLAN_THREADS - 1) / PLAN_THREADS, b0 = tid * each, b1 = min(b0 + each, p.batch);
-    const int n_free = min(max(*p.n_free, 0), p.stack_size);
-    PlanSums mine = {0, 0, 0};
-    for (int b = b0; b < b1; ++b) {
-        const Ask a(p, b);
-        mine.add({a.ended ? a.have : 0, a.pages, a.tokens});
-    }
-    PlanSums run = mine;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, b0 = tid * EACH;
+    int cached[EACH], fresh[EACH];
 #pragma unroll
-    for (int by = 1; by < 64; by <<= 1) run.add({shift_up(run.freed, by, lane), shift_up(run.pages, by, lane), shift_up(run.tokens, by, lane)});
+    for (int e = 0; e < EACH; ++e) {
+        cached[e] = b0 + e < p.batch ? p.cached_lens[b0 + e] : 0;
+        fresh[e] = b0 + e < p.batch ? p.new_lens[b0 + e] : 0;
+    }
+    const int n_free = min(max(*p.n_free, 0), p.stack_size);
+    Ask ask[EACH];
+    PlanSums run = {0, 0, 0};
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+        ask[e] = Ask(p, cached[e], fresh[e]);
+        run.add(ask[e].sums());
+    }
+    run.scan();
     if (lane == 63) s_wave[wave] = run;
+    // the lanes before this one
+    PlanSums before = {(uint32_t)__shfl_up((int)run.freed, 1, kWave), (uint32_t)__shfl_up((int)run.pages, 1, kWave), (uint32_t)__shfl_up((int)run.tokens, 1, kWave)};
+    if (lane == 0) before = {0, 0, 0};
     __syncthreads();
-    run.add({-mine.freed, -mine.pages, -mine.tokens});
-    PlanSums all = {0, 0, 0};
+    uint32_t freed = 0;
 #pragma unroll
     for (int w = 0; w < PLAN_WAVES; ++w) {
-        if (w < wave) run.add(s_wave[w]);
-        all.add(s_wave[w]);
+        if (w < wave) before.add(s_wave[w]);
+        freed = __builtin_elementwise_add_sat(freed, s_wave[w].freed);
     }
-    const int top = (int)min((long long)n_free + all.freed, (long long)p.stack_size);  // the stack with what was freed on it
+    const uint32_t top = min(__builtin_elementwise_add_sat((uint32_t)n_free, freed), (uint32_t)p.stack_size);  // the stack with what was freed on it
     // Requests are served while the sums with their own are within what there is; sums only grow, so that the first one that is not is the last.
-    long long used_pages = 0, used_tokens = 0;
-    {
-        PlanSums at = run;
-        for (int b = b0; b < b1; ++b) {
-            const Ask a(p, b);
-            at.add({a.ended ? a.have : 0, a.pages, a.tokens});
-            if (at.pages <= top && at.tokens <= p.max_tokens) used_pages = at.pages, used_tokens = at.tokens;
-        }
-    }
+    uint32_t used_pages = 0, used_tokens = 0;
+    run = before;
 #pragma unroll
-    for (int by = 32; by > 0; by >>= 1) {
-        used_pages = max(used_pages, __shfl_xor(used_pages, by, kWave));
-        used_tokens = max(used_tokens, __shfl_xor(used_tokens, by, kWave));
+    for (int e = 0; e < EACH; ++e) {
+        run.add(ask[e].sums());
+        if (run.pages <= top && run.tokens <= (uint32_t)p.max_tokens) used_pages = run.pages, used_tokens = run.tokens;
     }
+    used_pages = wave_minmax_u32<true>(used_pages);
+    used_tokens = wave_minmax_u32<true>(used_tokens);
     if (lane == 0) s_used[0][wave] = used_pages, s_used[1][wave] = used_tokens;
     __syncthreads();
 #pragma unroll
@@ -105,18 +121,20 @@ __global__ __launch_bounds__(PLAN_THREADS) void paged_plan_kernel(const PlanArgs
         used_pages = max(used_pages, s_used[0][w]);
         used_tokens = max(used_tokens, s_used[1][w]);
     }
-    const int taken = (int)used_pages, tokens = (int)used_tokens, left = top - taken;
+    const int taken = (int)used_pages, tokens = (int)used_tokens, left = (int)top - taken;
     const bool writes = blockIdx.x == 0;
-    for (int b = b0; b < b1; ++b) {
-        const Ask a(p, b);
-        const PlanSums before = run;
-        run.add({a.ended ? a.have : 0, a.pages, a.tokens});
-        const bool served = run.pages <= top && run.tokens <= p.max_tokens;
-        s_freed[b] = (int)min(before.freed, (long long)INT32_MAX);
-        s_pages[b] = (int)min(before.pages, used_pages);
-        s_start[b] = (int)min(before.tokens, used_tokens);
+    run = before;
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+        const int b = b0 + e;
+        if (b >= p.batch) break;
+        s_freed[b] = (int)min(run.freed, (uint32_t)INT32_MAX);
+        s_pages[b] = (int)min(run.pages, used_pages);
+        s_start[b] = (int)min(run.tokens, used_tokens);
+        run.add(ask[e].sums());
         if (writes) {
-            p.kv_lens[b] = a.ended ? 0 : a.cached + (served ? a.tokens : 0);
+            const bool served = run.pages <= top && run.tokens <= (uint32_t)p.max_tokens;
+            p.kv_lens[b] = ask[e].ended ? 0 : ask[e].cached + (served ? ask[e].tokens : 0);
             p.query_start[b] = s_start[b];
         }
     }
@@ -126,17 +144,18 @@ __global__ __launch_bounds__(PLAN_THREADS) void paged_plan_kernel(const PlanArgs
     }
     __syncthreads();
     const int at = blockIdx.x * PLAN_THREADS + tid, stride = gridDim.x * PLAN_THREADS;
+    auto positions = [&](int b) { return min(max(p.cached_lens[b], 0), p.width * p.div.size); };
     auto freed_page = [&](int i) {
         const int b = entry_of(s_freed, p.batch, i);
         return p.tables[(size_t)b * p.width + (i - s_freed[b])];
     };
     auto new_page = [&](int i) {  // page i that this step takes
-        const int place = top - 1 - i;
+        const int place = (int)top - 1 - i;
         return place < n_free ? p.free_pages[place] : freed_page(place - n_free);
     };
     for (int i = at; i < max(taken, left - n_free); i += stride) {
         if (i < taken) {
-            const int b = entry_of(s_pages, p.batch, i), have = p.div.page(min(max(p.cached_lens[b], 0), p.width * p.div.size) + p.div.size - 1);
+            const int b = entry_of(s_pages, p.batch, i), have = p.div.page(positions(b) + p.div.size - 1);
             p.tables[(size_t)b * p.width + have + (i - s_pages[b])] = new_page(i);
         }
         if (i < left - n_free) p.free_pages[n_free + i] = freed_page(i);
@@ -144,7 +163,7 @@ __global__ __launch_bounds__(PLAN_THREADS) void paged_plan_kernel(const PlanArgs
     for (int t = at; t < p.max_tokens; t += stride) {
         int slot = -1, pos = 0;
         if (t < tokens) {
-            const int b = entry_of(s_start, p.batch, t), cached = min(max(p.cached_lens[b], 0), p.width * p.div.size);
+            const int b = entry_of(s_start, p.batch, t), cached = positions(b);
             pos = cached + (t - s_start[b]);
             const int k = p.div.page(pos), have = p.div.page(cached + p.div.size - 1);
             const int page = k < have ? p.tables[(size_t)b * p.width + k] : new_page(s_pages[b] + k - have);
@@ -216,8 +235,12 @@ AGPU_EXPORT int32_t agpu_paged_plan(agpu_ctx *ctx, const int32_t *cached_lens, c
     if (here.rc != AGPU_OK) return here.rc;
     const PlanArgs p = {cached_lens, new_lens, n_free, block_tables, free_pages, kv_lens, query_start, slots, positions, n_free_out, batch, table_width, stack_size,
                         max_tokens, PageDiv::of(page_size)};
-    const int wgs = std::max(1, std::min(ceil_div(std::max(max_tokens, batch), 4 * PLAN_THREADS), ctx->num_cus));
-    hipLaunchKernelGGL(paged_plan_kernel, dim3(wgs), dim3(PLAN_THREADS), (3 * batch + 1) * sizeof(int), ctx->stream, p);
+    const int wgs = std::max(1, std::min(ceil_div(std::max(max_tokens, batch), PLAN_THREADS), ctx->num_cus));
+    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(wgs), dim3(PLAN_THREADS), (3 * batch + 1) * sizeof(int), ctx->stream, p); };
+    static_assert(paged::kMaxRequests <= 16 * PLAN_THREADS && 3 * paged::kMaxRequests * sizeof(int) <= 65536 - 1024, "");
+    if (batch <= PLAN_THREADS) go(paged_plan_kernel<1>);
+    else if (batch <= 4 * PLAN_THREADS) go(paged_plan_kernel<4>);
+    else go(paged_plan_kernel<16>);
     return AGPU_LAUNCH_CHECK(ctx, "paged_plan_kernel");
 }
 
