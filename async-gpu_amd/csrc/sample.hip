@@ -3,18 +3,18 @@
 // Each filter keeps a first part of the ranking (the k first; those before which less than p of the k's sum lies; w >= min_p), so that what is kept is the
 // shortest of the three parts, and all that the draw needs of it is its sum Z: the token is the first rank whose running sum exceeds u Z.
 //
-// Sums decide, next to borders, which token comes out, and there are tens of thousands of terms: weights are whole numbers, w 2^46 at
-// 50257 logits, from an exponential in 64-bit floats (off by 4e-14 of itself), and their sums are exact in any order.  (With fp32 exponentials a row of
-// 50257 logits would go wrong about once in a thousand draws.)
+// Sums decide, next to borders, which token comes out, and there are tens of thousands of terms: weights are whole numbers, 2^45 for a weight of
+// one at 50257 logits, from an exponential in 64-bit floats (off by 4e-14 of itself), and their sums are exact in any order.  (With fp32 exponentials a row
+// of 50257 logits would go wrong about once in a thousand draws.)
 //
-// Three launches, of a few workgroups a row each, which take a part of it; what they find they add to the row's state in memory, and the last one of a
-// row to finish draws the conclusion.
-//   sample_top_kernel    the parts' maxima
-//   sample_bins_kernel   sums (and counts, where top_k asks for them) of the weights in 2048 bins of log2 w.  From their running sums follows in which bins the
-//                        filters' borders lie, between which sums Z then is, and in which bins the drawn rank can be: up to three ranges of bins
-//   sample_draw_kernel   what is in those bins, a few hundred elements, is gathered, put in order by counting, and searched
-// When the bins hold too many (thousands of equal logits, a large temperature), the last workgroup looks for each border by itself, in bins cut into
-// 2048 by the bits of (value, index), which are never the same twice, until a piece fits the list.
+// sample_rows_kernel, a workgroup a row, one launch, no scratch:
+//   general   One pass over the row adds up the weights in bins of 1/32 of an octave, each in units of its bin's middle (a polynomial of degree five is then exact to
+//             3e-15), so that the largest logit need not be known before: 64 octaves fit, and the first 4096 elements say where they lie.  Which bin an element
+//             went to stays in LDS.  From the bins' running sums follows in which bins the filters' borders lie, between which sums Z then is, and in which
+//             bins the drawn rank can be: only what is in those, a few hundred elements, is gathered, put in order by counting, and searched.
+//   top_k up to 256   The top_k-th largest of the threads' maxima is a bound that hardly more than top_k elements reach: the list is those.
+// When the bins hold more than the list (thousands of equal logits, a large temperature), each border is looked for by itself, in the elements of
+// its bin cut into 512 by the bits of (value, index), which are never the same twice, until a piece fits.
 #include "agpu_internal.h"
 #include "sampling.h"
 
@@ -24,10 +24,14 @@ namespace {
 
 typedef unsigned long long u64;
 
-constexpr int SM_THREADS = 512, SM_WAVES = SM_THREADS / 64;
-constexpr int SM_BINS = 2048, SM_LIST = 512, SM_MAX_PARTS = 32, SM_PARTS = 256;  // SM_PARTS: workgroups of a launch, about
-constexpr int SM_AHEAD = 4;  // runs of four elements that a thread has on their way at a time
-constexpr int kIndexBits = 20;  // n <= 2^20
+constexpr int SM_THREADS = 1024, SM_WAVES = SM_THREADS / 64;
+constexpr int SM_BINS = 2048, SM_OCTAVE = 32;  // bins, and how many an octave has
+constexpr int SM_LIST = 512, SM_TOP_K = 256;
+constexpr int SM_IDS = 57344;  // elements whose bins LDS has room for
+constexpr int SM_AHEAD = 4;    // runs of four elements that a thread has on their way at a time
+constexpr int kIndexBits = 20, kKeyBits = 52;  // n <= 2^20; of a value and its index
+constexpr int kIdShift = 5;  // an element's bin is kept as that many bits further up, where 16 bits wrap as the bins do
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 
 struct SampleArgs {
     const float *logits, *u;
@@ -36,7 +40,7 @@ struct SampleArgs {
     float temperature, top_p, min_p;
     int top_k;
     int *tokens;
-    int n, bits;  // bits of a weight of one: sums of n weights stay below 2^62, and of one below 2^51
+    int n, bits;  // a weight of one is 2^bits: sums of n weights stay below 2^62, and one below 2^51
 };
 
 // 2^f on [-1/2, 1/2], through 2^f at nine Chebyshev nodes and 1 at zero: off by 3.7e-14
@@ -52,96 +56,67 @@ __device__ __forceinline__ double exp2_part(double f) {
     y = fma(y, f, 6.931471805599453e-01);
     return fma(y, f, 1.0);
 }
+__device__ __forceinline__ double exp2_wide(double t) {
+    const double k = __builtin_rint(t);
+    return __builtin_amdgcn_ldexp(exp2_part(t - k), (int)k);
+}
 
+// The bin of a logit and its weight in units of its bin: 32 log2 of it is t = (x - origin) per, its bin the whole number next to t, and its weight 2^f, f the rest / 32.
 struct Scale {
-    double top, per, least;  // the largest logit; log2(e) / T; log2 of what is no weight any more, less than half a unit
-    float bins_per_octave;   // so that the last bin is not passed
-    int bits;
-    __device__ __forceinline__ Scale(float top_, float temperature, int bits_)
-        : top(top_), per(1.4426950408889634 / ((double)temperature > 1e-8 ? (double)temperature : 1e-8)), least(-(bits_ + 1)),
-          bins_per_octave((SM_BINS - 0.125f) / (bits_ + 1)), bits(bits_) {}
-    __device__ __forceinline__ double log2_of(float x) const { return ((double)x - top) * per; }
-    __device__ __forceinline__ bool counts(double t) const { return t > least; }  // (NaN does not)
-    // To the nearest whole number.  1.5 2^52 more leaves the nearest one of t, and 2^52 more that of the weight, in the low bits.
-    __device__ __forceinline__ u64 weight(double t) const {
-        const double shifted = t + 0x1.8p52;
-        const u64 y = __builtin_bit_cast(u64, exp2_part(t - (shifted - 0x1.8p52)));
-        const u64 exponent = (u64)((uint32_t)__builtin_bit_cast(u64, shifted) + (uint32_t)bits) << 52;
-        return __builtin_bit_cast(u64, __builtin_bit_cast(double, y + exponent) + 0x1p52) & ((1ull << 52) - 1);
+    double per, origin, one;
+    float low, high;  // what counts: within 48 octaves below the origin and 15 above it (NaN does not), 2017 bins of the 2048
+    static constexpr int kNone = -48 * SM_OCTAVE - 8;  // a bin that nothing has
+    __device__ __forceinline__ void set(double at, double temperature, int bits) {
+        per = SM_OCTAVE * 1.4426950408889634 / temperature;
+        origin = at;
+        one = (double)(1ull << bits);
+        const double least = at - 48 * SM_OCTAVE / per, most = at + 15 * SM_OCTAVE / per;  // to the inside, whose ends a number may lie hundreds of octaves off
+        low = (float)least;
+        high = (float)most;
+        if (low < least) low = key_value(order_key(low) + 1);
+        if (high > most) high = key_value(order_key(high) - 1);
     }
-    __device__ __forceinline__ int bin(double t) const { return (int)((float)-t * bins_per_octave); }
+    __device__ __forceinline__ bool counts(float x) const { return x >= low && x <= high; }
+    static constexpr double kWhole = 0x1.8p52;  // added to it, a number's low bits are the whole number next to it
+    __device__ __forceinline__ int bin(float x, u64 &weight) const {
+        const double d = (double)x - origin, v = fma(d, per, kWhole), f = fma(d, per, kWhole - v);
+        // (ln 2 / 32)^k / k!; the next term is below 3e-15
+        double y = 3.9737099845494154e-11;
+        y = fma(y, f, 9.172562701824643e-09);
+        y = fma(y, f, 1.6938509724371819e-06);
+        y = fma(y, f, 2.3459619820224677e-04);
+        y = fma(y, f, 2.166084939249829e-02);
+        y = fma(y, f, 1.0);
+        weight = __builtin_bit_cast(u64, fma(y, one, 0x1p52)) & ((1ull << 52) - 1);  // to the nearest whole number
+        return (int)(uint32_t)__builtin_bit_cast(u64, v);
+    }
+    __device__ __forceinline__ int bin(float x) const { return (int)(uint32_t)__builtin_bit_cast(u64, fma((double)x - origin, per, kWhole)); }
+    __device__ __forceinline__ u64 weight(float x) const {
+        u64 w;
+        bin(x, w);
+        return w;
+    }
 };
+// a sum of weights in bin j, `scale` = 2^(-j / 32), in units of bin 0: never smaller for a larger sum
+__device__ __forceinline__ u64 in_units(u64 sum, double scale) { return (u64)__builtin_rint((double)sum * scale); }
+__device__ __forceinline__ double units(int j) { return exp2_wide(-(double)j / SM_OCTAVE); }
 
 __device__ __forceinline__ u64 composite(float x, int i) { return (u64)order_key(x) << kIndexBits | (u64)((1 << kIndexBits) - 1 - i); }
 __device__ __forceinline__ float value_of(u64 c) { return key_value((uint32_t)(c >> kIndexBits)); }
 __device__ __forceinline__ int index_of(u64 c) { return (1 << kIndexBits) - 1 - (int)(c & ((1 << kIndexBits) - 1)); }
 
-// What the launches leave for one another of a row.
-struct RowState {
-    u64 sum[SM_BINS], min_p_sum;  // of the bins; of the weights from min_p on
+struct Shared {
+    u64 sum[SM_BINS];
     uint32_t count[SM_BINS];
-    float top[SM_MAX_PARTS];
-    int ranges, first[3], last[3];  // bins where borders and the drawn rank can be
-    u64 more_sum[3];                // the running sum and count before a range less what the list holds before it
-    uint32_t more_count[3];
-    u64 all;                        // sum and number of all candidates
-    uint32_t candidates;
-    uint32_t fill;
-    u64 list[SM_LIST];
+    uint16_t id[SM_IDS];
+    u64 list[SM_LIST], ranked[SM_LIST], prefix[SM_LIST];
+    int place[SM_LIST];
+    u64 wave_sum[SM_WAVES], answer_sum, kept_of_min_p, piece_sum;
+    uint32_t wave_count[SM_WAVES], answer_index, piece_count;
+    float wave_top[SM_WAVES];
+    uint32_t top[SM_THREADS];
+    int hit[2], from[4], to[4], fill, piece;
 };
-struct Parts {
-    int n, each, row0;  // parts of a row and elements of each (a multiple of four); the first row of the launch
-    RowState *rows;
-    unsigned int *tickets;
-    int strict;
-};
-
-struct Bins {
-    u64 sum[SM_BINS], wave_sum[SM_WAVES], hit_sum[2];
-    uint32_t count[SM_BINS], wave_count[SM_WAVES], hit_count[2];
-    int hit[2];
-};
-
-// Sums and counts become running ones from bin 0 on.  Whole workgroup; barriers before and after.
-__device__ __forceinline__ void running(Bins &s, int tid, int lane, int wave) {
-    constexpr int EACH = SM_BINS / SM_THREADS;
-    __syncthreads();
-    u64 w[EACH];
-    uint32_t c[EACH];
-#pragma unroll
-    for (int e = 0; e < EACH; ++e) {
-        w[e] = s.sum[EACH * tid + e] + (e ? w[e - 1] : 0);
-        c[e] = s.count[EACH * tid + e] + (e ? c[e - 1] : 0);
-    }
-    u64 before = w[EACH - 1];
-    uint32_t count_before = c[EACH - 1];
-#pragma unroll
-    for (int by = 1; by < 64; by <<= 1) {
-        const u64 o = __shfl_up(before, by, kWave);
-        const uint32_t oc = __shfl_up(count_before, by, kWave);
-        if (lane >= by) {
-            before += o;
-            count_before += oc;
-        }
-    }
-    if (lane == 63) {
-        s.wave_sum[wave] = before;
-        s.wave_count[wave] = count_before;
-    }
-    __syncthreads();
-    before -= w[EACH - 1];
-    count_before -= c[EACH - 1];
-    for (int v = 0; v < wave; ++v) {
-        before += s.wave_sum[v];
-        count_before += s.wave_count[v];
-    }
-#pragma unroll
-    for (int e = 0; e < EACH; ++e) {
-        s.sum[EACH * tid + e] = before + w[e];
-        s.count[EACH * tid + e] = count_before + c[e];
-    }
-    __syncthreads();
-}
 
 // What is asked for: the first rank whose running sum exceeds `past`, or, by count, rank number past + 1.
 struct Target {
@@ -152,427 +127,494 @@ struct Target {
     }
 };
 
-// The bins of running sums (which begin at sum0 and count0) where two targets lie: s.hit, and the sum and count before them.  A barrier at the end.
-__device__ __forceinline__ void find(Bins &s, u64 sum0, uint32_t count0, const Target &a, const Target &b, int tid) {
-#pragma unroll 1
-    for (int x = tid; x < SM_BINS; x += SM_THREADS) {
-        const u64 s0 = sum0 + (x ? s.sum[x - 1] : 0), s1 = sum0 + s.sum[x];
-        const uint32_t c0 = count0 + (x ? s.count[x - 1] : 0), c1 = count0 + s.count[x];
-        auto look = [&](int i, const Target &to) {
-            if (!to.within(s0, c0, s1, c1)) return;
-            s.hit[i] = x;
-            s.hit_sum[i] = s0;
-            s.hit_count[i] = c0;
-        };
-        look(0, a);
-        look(1, b);
-    }
-    __syncthreads();
-}
-
 // The settings of a row, and what they ask for.
 struct Row {
     float temperature, top_p, min_p, u;
     int top_k;
-    u64 one;
     bool by_p;
     __device__ __forceinline__ Row(const SampleArgs &p, int r)
         : temperature(p.temperatures ? p.temperatures[r] : p.temperature), top_p(p.top_ps ? p.top_ps[r] : p.top_p), min_p(p.min_ps ? p.min_ps[r] : p.min_p),
-          u(p.u[r]), top_k(p.top_ks ? p.top_ks[r] : p.top_k), one(1ull << p.bits), by_p(top_p < 1.0f && top_p > 0.0f) {}
-    // Stages 0: the last of top_k, 1: the last that top_p keeps of the sum `kept`, 2: the drawn one of it
-    __device__ __forceinline__ bool asked(int stage, uint32_t candidates) const {
-        return stage == 0 ? top_k > 0 && (uint32_t)top_k < candidates : stage == 1 ? by_p : true;
+          u(p.u[r]), top_k(p.top_ks ? p.top_ks[r] : p.top_k), by_p(top_p < 1.0f && top_p > 0.0f) {}
+    __device__ __forceinline__ Target k_target() const { return Target{true, (u64)(top_k - 1)}; }
+    // the last that top_p keeps of a sum, and the drawn one
+    __device__ __forceinline__ Target p_target(u64 sum) const {
+        const double share = __builtin_ceil((double)top_p * (double)sum) - 1;
+        return Target{false, share > 0.0 && sum > 0 ? min((u64)share, sum - 1) : 0ull};
     }
-    __device__ __forceinline__ Target target(int stage, u64 kept, u64 min_p_sum) const {
-        if (stage == 0) return Target{true, (u64)(top_k - 1)};
-        if (stage == 1) {
-            const double share = __builtin_ceil((double)top_p * (double)kept) - 1;
-            return Target{false, share > 0.0 && kept > 0 ? min((u64)share, kept - 1) : 0ull};
-        }
-        if (top_p <= 0.0f) kept = one;
-        if (min_p > 0.0f) kept = min(kept, min_p_sum);
-        kept = max(kept, one);  // the first is always kept
-        const double at = (double)u * (double)kept;
-        return Target{false, at > 0.0 ? min((u64)at, kept - 1) : 0ull};
+    __device__ __forceinline__ Target u_target(u64 sum, u64 first) const {  // first: the weight of the first, which is always kept
+        sum = max(top_p <= 0.0f ? first : sum, first);
+        const double at = (double)u * (double)sum;
+        return Target{false, at > 0.0 ? min((u64)at, sum - 1) : 0ull};
     }
 };
 
-// The elements lo .. hi - 1 of a row, four in a run, SM_AHEAD runs on their way at a time: visit(i, four of them), where those behind the last are NaN.
-// (Few copies of visit: code comes cold from memory at every launch.)
-template <int THREADS, class F>
-__device__ __forceinline__ void for_runs(const float *row, int lo, int hi, int tid, F &&visit) {
-    const int whole = hi - (hi - lo) % 4, step = 4 * THREADS;
-    if (lo >= hi) return;
+// The row's elements, four in a run, SM_AHEAD runs on their way at a time: visit(i, four of them), where those behind the last are NaN.
+struct Runs {
+    static constexpr int kStep = 4 * SM_THREADS;
+    const float *row;
+    int n, tid;
     float4 x[SM_AHEAD];
-    const int back = max(whole - 4, lo);
-    auto load = [&](int i) { return whole > lo ? load4(row + min(i, back)) : make_float4(0.f, 0.f, 0.f, 0.f); };
-    int i = lo + 4 * tid;
+    __device__ __forceinline__ float4 load(int i) const {
+        const int whole = n & ~3;
+        return whole > 0 ? load4(row + min(i, max(whole - 4, 0))) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+    }
+    __device__ __forceinline__ Runs(const float *row, int n, int tid) : row(row), n(n), tid(tid) {
 #pragma unroll
-    for (int a = 0; a < SM_AHEAD; ++a) x[a] = load(i + a * step);
+        for (int a = 0; a < SM_AHEAD; ++a) x[a] = load(4 * tid + a * kStep);
+    }
+    template <class F>
+    __device__ __forceinline__ void each(F &&visit) {
+        const int whole = n & ~3;
 #pragma unroll 1
-    for (; i < whole; i += SM_AHEAD * step)
+        for (int i = 4 * tid; i < whole; i += SM_AHEAD * kStep)
 #pragma unroll
-        for (int a = 0; a < SM_AHEAD; ++a) {
-            if (i + a * step < whole) visit(i + a * step, x[a]);
-            x[a] = load(i + (SM_AHEAD + a) * step);
+            for (int a = 0; a < SM_AHEAD; ++a) {
+                if (i + a * kStep < whole) visit(i + a * kStep, x[a]);
+                x[a] = load(i + (SM_AHEAD + a) * kStep);
+            }
+        if (whole < n && tid == SM_THREADS - 1) {
+            const float nan = __builtin_nanf("");
+            visit(whole, make_float4(row[whole], whole + 1 < n ? row[whole + 1] : nan, whole + 2 < n ? row[whole + 2] : nan, nan));
         }
-    if (whole < hi && tid == 0) {
-        const float nan = __builtin_nanf("");
-        visit(whole, make_float4(row[whole], whole + 1 < hi ? row[whole + 1] : nan, whole + 2 < hi ? row[whole + 2] : nan, nan));
     }
-}
-// Of a largest logit of infinity only its equals count: they are zeros, the others infinitely less.
-__device__ __forceinline__ void values(const float4 &run, bool infinite, float (&x)[4]) {
-    x[0] = run.x; x[1] = run.y; x[2] = run.z; x[3] = run.w;
-    if (__builtin_expect(infinite, 0)) {
-        asm volatile("");  // (a branch, not four selections a run)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = x[e] == INFINITY ? 0.0f : -INFINITY;
-    }
-}
+};
+__device__ __forceinline__ float max_of_run(const float4 &x) { return fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w)); }
 
-// The last workgroup of a row to arrive (whole workgroup; `ticket` in LDS).
-__device__ __forceinline__ bool last_of_row(const Parts &parts, int r, uint32_t &ticket, int tid) {
-    if (parts.n == 1) return true;
-    partials_published(parts.strict);
-    __syncthreads();
-    if (tid == 0) {
-        ticket = take_ticket(&parts.tickets[r], parts.strict);
-        if (ticket == (unsigned)(parts.n - 1)) __hip_atomic_store(&parts.tickets[r], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
-    __syncthreads();
-    if (ticket != (unsigned)(parts.n - 1)) return false;
-    if (parts.strict) __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
-    return true;
-}
-
-// grid (parts, rows) here and below: the maximum of a part, and zeros for its share of the bins
-__global__ __launch_bounds__(SM_THREADS) void sample_top_kernel(const SampleArgs p, const Parts parts) {
-    __shared__ float s_top[SM_WAVES];
-    const int tid = threadIdx.x, part = blockIdx.x, r = blockIdx.y;
-    RowState &state = parts.rows[r];
-    for (int i = part * SM_THREADS + tid; i < SM_BINS; i += parts.n * SM_THREADS) {
-        state.sum[i] = 0;
-        state.count[i] = 0;
-    }
-    if (part == 0 && tid == 0) {
-        state.min_p_sum = 0;
-        state.fill = 0;
-    }
-    float top = -INFINITY;
-    const int lo = min(part * parts.each, p.n);
-    for_runs<SM_THREADS>(p.logits + (size_t)(parts.row0 + r) * p.n, lo, min(lo + parts.each, p.n), tid,
-                         [&](int, const float4 &x) { top = fmaxf(top, fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w))); });
-    top = wave_max(top);
-    if ((tid & 63) == 0) s_top[tid >> 6] = top;
-    __syncthreads();
-    if (tid == 0) {
-#pragma unroll
-        for (int w = 1; w < SM_WAVES; ++w) top = fmaxf(top, s_top[w]);
-        state.top[part] = top;
-    }
-}
-
-__global__ __launch_bounds__(SM_THREADS) void sample_bins_kernel(const SampleArgs p, const Parts parts) {
-    __shared__ Bins s;
-    __shared__ u64 s_min_p_sum;
-    __shared__ uint32_t s_ticket;
-    __shared__ int s_from[3], s_to[3];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = blockIdx.y;
-    const float *logits = p.logits + (size_t)(parts.row0 + r) * p.n;
-    RowState &state = parts.rows[r];
-    const Row row(p, parts.row0 + r);
-    const float top = wave_max(lane < parts.n ? state.top[lane] : -INFINITY);
-    if (top == -INFINITY) return;  // nothing to draw from (the whole row)
-    const bool infinite = top == INFINITY, counts = row.top_k > 0;
-    const Scale scale(infinite ? 0.0f : top, row.temperature, p.bits);
-    for (int i = tid; i < SM_BINS; i += SM_THREADS) {
-        s.sum[i] = 0;
-        s.count[i] = 0;
-    }
-    if (tid == 0) s_min_p_sum = 0;
-    __syncthreads();
-    const u64 least = row.min_p > 0.0f ? (u64)__builtin_ceil(fmin((double)row.min_p, 2.0) * (double)row.one) : ~0ull;
-    u64 above = 0;  // sum of the weights from min_p on
-    const int lo = min((int)blockIdx.x * parts.each, p.n);
-    for_runs<SM_THREADS>(logits, lo, min(lo + parts.each, p.n), tid, [&](int, const float4 &run) {
-        float x[4];
-        values(run, infinite, x);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const double t = scale.log2_of(x[e]);
-            if (!scale.counts(t)) continue;
-            const u64 w = scale.weight(t);
-            const int b = scale.bin(t);
-            atomicAdd(&s.sum[b], w);
-            if (counts) atomicAdd(&s.count[b], 1u);
-            above += w >= least ? w : 0;
-        }
-    });
-    if (row.min_p > 0.0f) {
-#pragma unroll
-        for (int by = 32; by > 0; by >>= 1) above += __shfl_xor(above, by, kWave);
-        if (lane == 0) atomicAdd(&s_min_p_sum, above);
-    }
-    __syncthreads();
-    for (int i = tid; i < SM_BINS; i += SM_THREADS)
-        if (s.sum[i] != 0 || s.count[i] != 0) {
-            __hip_atomic_fetch_add(&state.sum[i], s.sum[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            if (counts) __hip_atomic_fetch_add(&state.count[i], s.count[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        }
-    if (tid == 0 && row.min_p > 0.0f) __hip_atomic_fetch_add(&state.min_p_sum, s_min_p_sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    if (!last_of_row(parts, r, s_ticket, tid)) return;
-    if (parts.n > 1) {
-        for (int i = tid; i < SM_BINS; i += SM_THREADS) {
-            s.sum[i] = __hip_atomic_load(&state.sum[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            s.count[i] = counts ? __hip_atomic_load(&state.count[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
-        }
-        if (tid == 0) s_min_p_sum = __hip_atomic_load(&state.min_p_sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
-    running(s, tid, lane, wave);
-    auto sum_before = [&](int b) { return b > 0 ? s.sum[b - 1] : 0; };
-    u64 least_sum = s.sum[SM_BINS - 1], most_sum = least_sum;  // between which what is kept so far adds up to
-    const uint32_t candidates = s.count[SM_BINS - 1];
-#pragma unroll 1
-    for (int stage = 0; stage < 3; ++stage) {
-        if (!row.asked(stage, candidates)) continue;  // uniform
-        find(s, 0, 0, row.target(stage, least_sum, s_min_p_sum), row.target(stage, most_sum, s_min_p_sum), tid);
-        least_sum = min(least_sum, sum_before(s.hit[0]));
-        most_sum = min(most_sum, s.sum[s.hit[1]]);
-        if (tid == 0) s_from[stage] = s.hit[0], s_to[stage] = s.hit[1];
+__global__ __launch_bounds__(SM_THREADS) void sample_rows_kernel(const SampleArgs p) {
+    __shared__ __align__(16) Shared s;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = blockIdx.x, n = p.n;
+    const float *logits = p.logits + (size_t)r * n;
+    const Row row(p, r);
+    const double temperature = (double)row.temperature > 1e-8 ? fmin((double)row.temperature, 1e39) : 1e-8;
+    auto all_max = [&](float v) {  // of the workgroup
+        v = wave_max(v);
         __syncthreads();
-    }
-    if (tid != 0) return;
-    // What is drawn does not come behind the last that top_p keeps, nor that behind the last of top_k: the ranges are in order.  Those that meet are one.
-    int n = 0, begin = 0, end = -2;
-    u64 sum = 0;
-    uint32_t count = 0;
-#pragma unroll 1
-    for (int stage = 2; stage >= 0; --stage) {
-        if (!row.asked(stage, candidates)) continue;
-        const int a = max(s_from[stage], 0), b = s_to[stage];
-        if (n > 0 && a <= end + 1) {
-            end = max(end, b);
-            state.last[n - 1] = end;
-            continue;
-        }
-        if (n > 0) {  // the range before is complete
-            sum += s.sum[end] - sum_before(begin);
-            count += s.count[end] - (begin ? s.count[begin - 1] : 0);
-        }
-        begin = a;
-        state.first[n] = a;
-        state.last[n] = end = b;
-        state.more_sum[n] = sum_before(a) - sum;
-        state.more_count[n] = (a ? s.count[a - 1] : 0) - count;
-        ++n;
-    }
-    state.ranges = n;
-    state.all = s.sum[SM_BINS - 1];
-    state.candidates = candidates;
-}
-
-__global__ __launch_bounds__(SM_THREADS, 4) void sample_draw_kernel(const SampleArgs p, const Parts parts) {
-    __shared__ Bins s;  // (for rows whose list does not hold what it should)
-    __shared__ u64 s_list[SM_LIST], s_ranked[SM_LIST], s_answer_sum;
-    __shared__ int s_place[SM_LIST];
-    __shared__ uint32_t s_fill, s_base, s_ticket, s_answer;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = blockIdx.y, n = p.n;
-    const float *logits = p.logits + (size_t)(parts.row0 + r) * n;
-    int *const token = p.tokens + parts.row0 + r;
-    RowState &state = parts.rows[r];
-    const Row row(p, parts.row0 + r);
-    const float top = wave_max(lane < parts.n ? state.top[lane] : -INFINITY);
-    if (top == -INFINITY) {  // the whole row
-        if (tid == 0 && blockIdx.x == 0) *token = -1;
-        return;
-    }
-    const bool infinite = top == INFINITY;
-    const Scale scale(infinite ? 0.0f : top, row.temperature, p.bits);
-    struct Ranges {
-        int n, first[3], last[3];
-    };
-    // visit(i, x, t, bin) of the part's (or the row's) elements in bins first[q] .. last[q] of the ranges q < n
-    auto for_bins = [&](const Ranges &of, int lo, int hi, auto &&visit) {
-        // What cannot be in them is told apart by its value alone: a hair beyond the bins' ends (t and the ends round by 2^-23 at most).
-        float below[3], above[3];
-        const double slack = 1e-5, width = 1.0 / scale.bins_per_octave, by = 1.0 / scale.per;
-        auto beyond = [](float x, float by) { return fabsf(x) < INFINITY ? x + fabsf(x) * by : x; };
+        if (lane == 0) s.wave_top[wave] = v;
+        __syncthreads();
 #pragma unroll
-        for (int q = 0; q < 3; ++q) {
-            below[q] = beyond((float)(scale.top - ((of.last[q] + 1) * width * (1 + slack) + slack) * by), -1e-6f);
-            above[q] = of.first[q] == 0 ? INFINITY : beyond((float)(scale.top - (of.first[q] * width * (1 - slack) - slack) * by), 1e-6f);
-            if (q >= of.n) below[q] = INFINITY, above[q] = -INFINITY;
+        for (int w = 0; w < SM_WAVES; ++w) v = fmaxf(v, s.wave_top[w]);
+        return v;
+    };
+    float top = -INFINITY;
+    bool infinite = false;  // of a largest logit of infinity only its equals count: they are zeros, the others infinitely less
+    auto value = [&](float x) { return !infinite ? x : x == INFINITY ? 0.0f : -INFINITY; };
+    Scale scale;
+    bool listed = false;  // the list is a first part of the ranking by itself (top_k), or bins of it
+    if (tid == 0) s.fill = 0;
+    if (tid < SM_LIST) s.place[tid] = 0;
+
+    // ---- the list of a small top_k ----
+    if (row.top_k > 0 && row.top_k <= SM_TOP_K && row.top_k < n) {
+        Runs(logits, n, tid).each([&](int, const float4 &x) { top = fmaxf(top, max_of_run(x)); });
+        s.top[tid] = order_key(top);
+        top = all_max(top);
+        if (wave == 0) {  // the upper 20 bits of the top_k-th largest maximum, from the first bit on that not all share
+            uint32_t mine[SM_WAVES], most = 0u, least = 0xffffffffu;
+#pragma unroll
+            for (int i = 0; i < SM_WAVES; ++i) {
+                mine[i] = s.top[64 * i + lane];
+                most = max(most, mine[i]);
+                least = min(least, mine[i]);
+            }
+            most = wave_minmax_u32<true>(most);
+            least = wave_minmax_u32<false>(least);
+            const int bits = 31 - __builtin_clz((most ^ least) | 1u);
+            uint32_t b = bits >= 31 ? 0u : most & ~((2u << bits) - 1u);
+#pragma unroll 1
+            for (int bit = bits; bit >= 12; --bit) {
+                const uint32_t higher = b | (1u << bit);
+                int c = 0;
+#pragma unroll
+                for (int i = 0; i < SM_WAVES; ++i) c += __popcll(__ballot(mine[i] >= higher));
+                if (c >= row.top_k) b = higher;
+                if (c == row.top_k) break;
+            }
+            if (lane == 0) s.hit[0] = (int)(b & 0xfffff000u);
         }
-        const float lowest = fminf(below[0], fminf(below[1], below[2]));
-        for_runs<SM_THREADS>(logits, lo, hi, tid, [&](int i, const float4 &run) {
-            float x[4];
-            values(run, infinite, x);
-            if (!(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) >= lowest)) return;
-            unsigned near = 0;
+        __syncthreads();
+        const uint32_t bound = (uint32_t)s.hit[0];
+        const float floor = key_value(bound);  // (a key between two numbers', or below all of them: NaN, which nothing is below)
+        Runs(logits, n, tid).each([&](int i, const float4 &x) {
+            if (max_of_run(x) < floor) return;
+            const float of[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                near |= ((x[e] >= below[0] && x[e] <= above[0]) || (x[e] >= below[1] && x[e] <= above[1]) || (x[e] >= below[2] && x[e] <= above[2])) ? 1u << e : 0u;
-#pragma unroll 1
-            for (; near != 0; near &= near - 1) {
-                const int e = __builtin_ctz(near);
-                const float y = e < 2 ? (e == 0 ? x[0] : x[1]) : e == 2 ? x[2] : x[3];
-                const double t = scale.log2_of(y);
-                const int b = scale.counts(t) ? scale.bin(t) : SM_BINS;
-                if ((b >= of.first[0] && b <= of.last[0]) || (of.n > 1 && b >= of.first[1] && b <= of.last[1]) || (of.n > 2 && b >= of.first[2] && b <= of.last[2]))
-                    visit(i + e, y, t);
-            }
+                if (order_key(of[e]) >= bound && of[e] > -INFINITY) {
+                    const int at = atomicAdd(&s.fill, 1);
+                    if (at < SM_LIST) s.list[at] = 1ull << kKeyBits | composite(of[e], i + e);
+                }
         });
-    };
-    if (tid == 0) s_fill = 0;
-    if (tid < SM_LIST) s_place[tid] = 0;
-    __syncthreads();
-    const Ranges of = {state.ranges, {state.first[0], state.first[1], state.first[2]}, {state.last[0], state.last[1], state.last[2]}};
-    const int lo = min((int)blockIdx.x * parts.each, n);
-    for_bins(of, lo, min(lo + parts.each, n), [&](int i, float x, double) {
-        const uint32_t at = atomicAdd(&s_fill, 1u);
-        if (at < SM_LIST) s_list[at] = composite(x, i);
-    });
-    __syncthreads();
-    uint32_t listed = s_fill;
-    if (parts.n > 1) {
-        if (tid == 0) s_base = __hip_atomic_fetch_add(&state.fill, listed, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         __syncthreads();
-        for (uint32_t i = tid; i < listed && s_base + i < SM_LIST; i += SM_THREADS)
-            __hip_atomic_store(&state.list[s_base + i], s_list[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        if (!last_of_row(parts, r, s_ticket, tid)) return;
-        listed = __hip_atomic_load(&state.fill, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        for (uint32_t i = tid; i < min(listed, (uint32_t)SM_LIST); i += SM_THREADS) s_list[i] = __hip_atomic_load(&state.list[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        listed = s.fill <= SM_LIST && top > -INFINITY && top < INFINITY;
+        if (listed) scale.set(top, temperature, p.bits);
         __syncthreads();
+        if (!listed && tid == 0) s.fill = 0;
     }
-    const bool fits = listed <= SM_LIST;
-    u64 my_run = 0, my_weight = 0, mine = 0;  // of the list's rank tid
-    uint32_t my_rank = 0;
-    const u64 min_p_sum = __hip_atomic_load(&state.min_p_sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    if (fits) {
-        // the place of an element is the number of elements before it, which `helpers` threads count a part of each
-        const int per = listed > 1 ? 1 << (32 - __builtin_clz(listed - 1)) : 1, helpers = SM_THREADS / per, which = tid & (per - 1), helper = tid / per;
-        if (which < (int)listed) {
-            const u64 c = s_list[which];
-            int before = 0;
-            for (int o = helper; o < (int)listed; o += helpers) before += s_list[o] > c ? 1 : 0;
-            atomicAdd(&s_place[which], before);
-        }
-        __syncthreads();
-        if (tid < (int)listed) s_ranked[s_place[tid]] = s_list[tid];
-        __syncthreads();
-        int q = 0;
-        if (tid < (int)listed) {
-            mine = s_ranked[tid];
-            const double t = scale.log2_of(value_of(mine));
-            const int b = scale.bin(t);
-            q = of.n > 2 && b >= of.first[2] ? 2 : of.n > 1 && b >= of.first[1] ? 1 : 0;
-            my_weight = scale.weight(t);
-        }
-        u64 w = my_weight;
-#pragma unroll
-        for (int by = 1; by < 64; by <<= 1) {
-            const u64 o = __shfl_up(w, by, kWave);
-            if (lane >= by) w += o;
-        }
-        if (lane == 63) s.wave_sum[wave] = w;
-        __syncthreads();
-        for (int v = 0; v < wave; ++v) w += s.wave_sum[v];
-        my_run = w + state.more_sum[q];
-        my_rank = (uint32_t)tid + state.more_count[q];
-    }
-    // the bins' running sums again, where the whole row has to be gone through
-    auto load_bins = [&]() {
-        __syncthreads();
-        for (int i = tid; i < SM_BINS; i += SM_THREADS) {
-            s.sum[i] = __hip_atomic_load(&state.sum[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            s.count[i] = __hip_atomic_load(&state.count[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        }
-        running(s, tid, lane, wave);
-    };
-    u64 kept = ~0ull;
-    uint32_t candidates = ~0u;
-    if (!fits) {
-        load_bins();
-        kept = s.sum[SM_BINS - 1];
-        candidates = s.count[SM_BINS - 1];
-        __syncthreads();
-    } else {
-        kept = state.all;
-        candidates = state.candidates;
-    }
-#pragma unroll 1
-    for (int stage = 0; stage < 3; ++stage) {
-        if (!row.asked(stage, candidates)) continue;
-        const Target to = row.target(stage, kept, min_p_sum);
-        if (fits) {
-            if (tid < (int)listed && to.within(my_run - my_weight, my_rank, my_run, my_rank + 1)) {
-                s_answer = (uint32_t)index_of(mine);
-                s_answer_sum = my_run;
-            }
-            __syncthreads();
-            kept = min(kept, s_answer_sum);
-            __syncthreads();
-            continue;
-        }
-        load_bins();
-        find(s, 0, 0, to, to, tid);
-        const int b = s.hit[0];
-        u64 prefix = 0, sum0 = s.hit_sum[0];
-        uint32_t count0 = s.hit_count[0], in_piece = SM_LIST + 1;  // (counts there are only where top_k asks for them)
-        const Ranges bin = {1, {b, 0, 0}, {b, 0, 0}};
-        int known = 52;  // the bits of a composite; those from `known` on are the same, `prefix`
-        while (in_piece > SM_LIST && known > 0) {
-            const int shift = max(known - 11, 0);
-            __syncthreads();
+
+    // ---- the bins ----
+    int q_top = 0;  // the bin of the largest logit; bin number j from there on down is j in what follows
+    const bool by_k_bins = row.top_k > 0 && row.top_k < n;
+    if (!listed) {
+        for (int attempt = 0;; ++attempt) {
             for (int i = tid; i < SM_BINS; i += SM_THREADS) {
                 s.sum[i] = 0;
                 s.count[i] = 0;
             }
+            Runs runs(logits, n, tid);
+            float seen = attempt == 0 ? max_of_run(runs.x[0]) : top;  // of the first 4096, and then of all
+            if (attempt == 0) seen = all_max(seen);
+            infinite = seen == INFINITY;
+            scale.set(infinite || seen == -INFINITY ? 0.0 : (double)seen, temperature, p.bits);
             __syncthreads();
-            for_bins(bin, 0, n, [&](int i, float x, double t) {
-                const u64 c = composite(x, i);
-                if (c >> known != prefix) return;
-                const int d = SM_BINS - 1 - (int)((c >> shift) & ((1ull << (known - shift)) - 1));
-                atomicAdd(&s.sum[d], scale.weight(t));
-                atomicAdd(&s.count[d], 1u);
-            });
-            running(s, tid, lane, wave);
-            find(s, sum0, count0, to, to, tid);
-            const int d = s.hit[0];
-            in_piece = s.count[d] - (d ? s.count[d - 1] : 0);
-            sum0 = s.hit_sum[0];
-            count0 = s.hit_count[0];
-            prefix = prefix << (known - shift) | (u64)(SM_BINS - 1 - d);
-            known = shift;
-        }
-        if (tid == 0) s_fill = 0;
-        __syncthreads();
-        for_bins(bin, 0, n, [&](int i, float x, double) {
-            const u64 c = composite(x, i);
-            if (c >> known == prefix) s_list[min(atomicAdd(&s_fill, 1u), (uint32_t)SM_LIST - 1)] = c;
-        });
-        __syncthreads();
-        if (tid < (int)in_piece) {
-            const u64 c = s_list[tid];
-            u64 before = sum0;
-            uint32_t rank = count0;
-            for (int o = 0; o < (int)in_piece; ++o)
-                if (s_list[o] > c) {
-                    before += scale.weight(scale.log2_of(value_of(s_list[o])));
-                    ++rank;
+            top = -INFINITY;
+            runs.each([&](int i, const float4 &run) {
+                float x[4] = {run.x, run.y, run.z, run.w};
+                top = fmaxf(top, max_of_run(run));
+                if (__builtin_expect(infinite, 0)) {
+                    asm volatile("");  // (a branch, not four selections a run)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[e] = value(x[e]);
                 }
-            const u64 run = before + scale.weight(scale.log2_of(value_of(c)));
-            if (to.within(before, rank, run, rank + 1)) {
-                s_answer = (uint32_t)index_of(c);
-                s_answer_sum = run;
+                uint32_t id[4];
+                u64 weight[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int q = scale.bin(x[e], weight[e]);
+                    id[e] = (uint32_t)(scale.counts(x[e]) ? q : Scale::kNone);
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (id[e] != (uint32_t)Scale::kNone) {
+                        atomicAdd(&s.sum[id[e] & (SM_BINS - 1)], weight[e]);
+                        if (by_k_bins) atomicAdd(&s.count[id[e] & (SM_BINS - 1)], 1u);
+                    }
+                auto two = [&](uint32_t a, uint32_t b) { return (a << kIdShift & 0xffffu) | b << (16 + kIdShift); };
+                if (i < SM_IDS) *reinterpret_cast<uint2 *>(&s.id[i]) = make_uint2(two(id[0], id[1]), two(id[2], id[3]));
+            });
+            top = all_max(top);
+            if (top == -INFINITY) {  // nothing to draw from
+                if (tid == 0) p.tokens[r] = -1;
+                return;
+            }
+            // (the bins are right, unless the largest is beyond them or has infinite company)
+            if (seen > -INFINITY && infinite == (top == INFINITY) && (infinite || top <= scale.high)) break;
+        }
+        if (infinite) top = 0.0f;
+        q_top = scale.bin(top);
+        // running sums, in units of the largest logit's bin, from there on down
+        u64 w[2];
+        uint32_t c[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int j = 2 * tid + e;
+            w[e] = in_units(s.sum[(q_top - j) & (SM_BINS - 1)], units(j)) + (e ? w[0] : 0);
+            c[e] = s.count[(q_top - j) & (SM_BINS - 1)] + (e ? c[0] : 0);
+        }
+        u64 before = w[1];
+        uint32_t count_before = c[1];
+#pragma unroll
+        for (int by = 1; by < 64; by <<= 1) {
+            const u64 o = __shfl_up(before, by, kWave);
+            const uint32_t oc = __shfl_up(count_before, by, kWave);
+            if (lane >= by) {
+                before += o;
+                count_before += oc;
+            }
+        }
+        if (lane == 63) {
+            s.wave_sum[wave] = before;
+            s.wave_count[wave] = count_before;
+        }
+        __syncthreads();
+        before -= w[1];
+        count_before -= c[1];
+#pragma unroll
+        for (int v = 0; v < SM_WAVES - 1; ++v) {
+            before += v < wave ? s.wave_sum[v] : 0;
+            count_before += v < wave ? s.wave_count[v] : 0;
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            s.sum[2 * tid + e] = before + w[e];
+            s.count[2 * tid + e] = count_before + c[e];
+        }
+        __syncthreads();
+    } else {
+        q_top = scale.bin(top);
+    }
+    const u64 first_weight = scale.weight(top);
+    auto sum_before = [&](int j) { return !listed && j > 0 ? s.sum[j - 1] : 0; };
+    auto count_before = [&](int j) { return !listed && j > 0 ? s.count[j - 1] : 0; };
+    // min_p keeps what has at least that weight; in bins m_first .. m_last it is decided
+    const bool by_m = row.min_p > 0.0f;
+    auto min_p_keeps = [&](float x) { return exp2_wide(fmax(((double)x - top) * (1.4426950408889634 / temperature), -1000.0)) >= (double)row.min_p; };
+    // bins of the running sums where two targets lie (s.hit)
+    auto find = [&](const Target &a, const Target &b) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int j = 2 * tid + e;
+            if (a.within(sum_before(j), count_before(j), s.sum[j], s.count[j])) s.hit[0] = j;
+            if (b.within(sum_before(j), count_before(j), s.sum[j], s.count[j])) s.hit[1] = j;
+        }
+        __syncthreads();
+    };
+    const uint32_t candidates = listed ? (uint32_t)s.fill : s.count[SM_BINS - 1];
+    const bool by_k = by_k_bins && (uint32_t)row.top_k < candidates;
+    int m_first = 0, m_last = 0;
+    if (!listed) {
+        u64 least = s.sum[SM_BINS - 1], most = least;  // between which what is kept so far adds up to
+        int ranges = 0;
+        auto range = [&](int from, int to) {
+            least = min(least, sum_before(from));
+            most = min(most, s.sum[to]);
+            if (tid == 0) s.from[ranges] = from, s.to[ranges] = to;
+            ++ranges;
+            __syncthreads();
+        };
+        if (by_k) {
+            find(row.k_target(), row.k_target());
+            range(s.hit[0], s.hit[1]);
+        }
+        if (row.by_p) {
+            find(row.p_target(least), row.p_target(most));
+            range(s.hit[0], s.hit[1]);
+        }
+        if (by_m) {  // (32 times the fp32 logarithm is off by less than 1e-2)
+            const double t = ((double)top - scale.origin) * scale.per + SM_OCTAVE * (double)__log2f(fminf(row.min_p, 1.0f));
+            auto at = [&](double bin) { return max(q_top - (int)__builtin_rint(fmax(bin, -48.0 * SM_OCTAVE)), 0); };
+            m_first = at(t + 1e-2);
+            m_last = at(t - 1e-2);
+            range(m_first, m_last);
+        }
+        find(row.u_target(least, first_weight), row.u_target(most, first_weight));
+        range(s.hit[0], s.hit[1]);
+        // what is in those bins
+        // (two elements' bins at a time: how far above a range's last bin a bin lies, less the range's length, is 0 within it)
+        u16x2 last[4], length[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int of = min(q, ranges - 1);
+            last[q] = (u16x2)(uint16_t)((uint32_t)(q_top - s.to[of]) << kIdShift);
+            length[q] = (u16x2)(uint16_t)((s.to[of] - s.from[of]) << kIdShift);
+        }
+        auto outside = [&](uint32_t two) {
+            const u16x2 ids = __builtin_bit_cast(u16x2, two);
+            auto of = [&](int q) { return __builtin_elementwise_sub_sat((u16x2)(ids - last[q]), length[q]); };
+            u16x2 o = of(0);
+            if (ranges > 1) o = __builtin_elementwise_min(o, of(1));
+            if (ranges > 2) o = __builtin_elementwise_min(__builtin_elementwise_min(o, of(2)), of(3));
+            return o;
+        };
+        auto put = [&](int i) {
+            const int at = atomicAdd(&s.fill, 1);
+            if (at < SM_LIST) s.ranked[at] = (u64)i;
+        };
+#pragma unroll 1
+        for (int i = 8 * tid; i < min(n, SM_IDS); i += 8 * SM_THREADS) {
+            const uint4 ids = *reinterpret_cast<const uint4 *>(&s.id[i]);
+            const uint32_t of[4] = {ids.x, ids.y, ids.z, ids.w};
+            unsigned hits = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const u16x2 o = outside(of[e]);
+                hits |= (o.x == 0 ? 1u : 0u) << (2 * e) | (o.y == 0 ? 2u : 0u) << (2 * e);
+            }
+            for (; hits != 0; hits &= hits - 1)
+                if (i + __builtin_ctz(hits) < n) put(i + __builtin_ctz(hits));
+        }
+#pragma unroll 1
+        for (int i = SM_IDS + tid; i < n; i += SM_THREADS) {
+            const float x = value(logits[i]);
+            if (scale.counts(x) && outside((uint32_t)scale.bin(x) << kIdShift & 0xffffu).x == 0) put(i);
+        }
+        __syncthreads();
+        if (tid < min(s.fill, SM_LIST)) {  // their values, all on their way at once
+            const int i = (int)s.ranked[tid];
+            const float x = value(logits[i]);
+            s.list[tid] = (u64)(SM_BINS - 2 - (q_top - scale.bin(x))) << kKeyBits | composite(x, i);  // the bins' order is that of the list too
+        }
+        __syncthreads();
+    }
+
+    // ---- the list in order ----
+    const int in_list = min(s.fill, SM_LIST);
+    const bool fits = s.fill <= SM_LIST;
+    u64 mine = 0, my_before = 0, my_run = 0;  // of the list's rank tid: the running sums without it and with it
+    uint32_t my_rank = 0;
+    float my_x = 0.0f;
+    if (fits) {
+        // the place of an element is the number of elements before it, which `helpers` threads count a part of each
+        const int size = in_list > 1 ? 1 << (32 - __builtin_clz(in_list - 1)) : 1, helpers = SM_THREADS / size, which = tid & (size - 1), helper = tid / size;
+        if (which < in_list) {
+            // (as the bits of positive 64-bit floats, whose order is the same: one instruction)
+            const double *list = reinterpret_cast<const double *>(s.list), c = list[which];
+            int before = 0;
+            const int part = (size + helpers - 1) / helpers, last = min((helper + 1) * part, in_list);
+#pragma unroll 4
+            for (int o = helper * part; o < last; ++o) before += list[o] > c ? 1 : 0;
+            if (before) atomicAdd(&s.place[which], before);
+        }
+        __syncthreads();
+        if (tid < in_list) s.ranked[s.place[tid]] = s.list[tid];
+        __syncthreads();
+        u64 weight = 0;
+        int j = 0;
+        if (tid < in_list) {
+            mine = s.ranked[tid];
+            my_x = value_of(mine);
+            if (scale.counts(my_x)) {
+                j = q_top - scale.bin(my_x, weight);
+                if (listed) weight = in_units(weight, units(j));  // one by one; otherwise by bins
+            }
+        }
+        u64 w = weight;
+        if (tid < SM_LIST) {
+#pragma unroll
+            for (int by = 1; by < 64; by <<= 1) {
+                const u64 o = __shfl_up(w, by, kWave);
+                if (lane >= by) w += o;
+            }
+            if (lane == 63) s.wave_sum[wave] = w;
+        }
+        __syncthreads();
+        if (tid < SM_LIST) {
+            for (int v = 0; v < wave; ++v) w += s.wave_sum[v];
+            s.prefix[tid] = w;
+        }
+        __syncthreads();
+        if (tid < in_list) {
+            if (listed) {
+                my_run = w;
+                my_before = w - weight;
+                my_rank = (uint32_t)tid;
+            } else {
+                int begin = tid;  // of its bin: the first with the same upper bits
+                for (int step = SM_LIST / 2; step > 0; step >>= 1)
+                    if (begin - step >= 0 && s.ranked[begin - step] >> kKeyBits == mine >> kKeyBits) begin -= step;
+                const double by = units(j);
+                const u64 in_bin = w - (begin > 0 ? s.prefix[begin - 1] : 0);
+                my_run = sum_before(j) + in_units(in_bin, by);
+                my_before = sum_before(j) + in_units(in_bin - weight, by);
+                my_rank = count_before(j) + (uint32_t)(tid - begin);
+            }
+        }
+    }
+
+    // ---- top_k, top_p of its sum, min_p, the draw ----
+    u64 kept = listed ? s.prefix[max(in_list - 1, 0)] : s.sum[SM_BINS - 1];
+#pragma unroll 1
+    for (int stage = 0; stage < 4; ++stage) {
+        if (!(stage == 0 ? by_k : stage == 1 ? row.by_p : stage == 2 ? by_m : true)) continue;  // uniform
+        __syncthreads();  // the last answer has been read
+        if (stage == 2) {
+            if (tid == 0) s.kept_of_min_p = sum_before(m_first);
+            __syncthreads();
+            if (fits) {
+                if (tid < in_list && min_p_keeps(my_x)) atomicMax(&s.kept_of_min_p, my_run);
+            } else {
+                for (int j = m_first; j <= m_last; ++j) {  // the weights of the bin that are kept
+                    __syncthreads();
+                    if (tid == 0) s.piece_sum = 0;
+                    __syncthreads();
+                    for (int i = tid; i < n; i += SM_THREADS) {
+                        const float x = value(logits[i]);
+                        if (scale.counts(x) && scale.bin(x) == q_top - j && min_p_keeps(x)) atomicAdd(&s.piece_sum, scale.weight(x));
+                    }
+                    __syncthreads();
+                    if (tid == 0 && s.piece_sum > 0) s.kept_of_min_p = sum_before(j) + in_units(s.piece_sum, units(j));
+                }
+            }
+            __syncthreads();
+            kept = min(kept, s.kept_of_min_p);
+            continue;
+        }
+        const Target to = stage == 0 ? row.k_target() : stage == 1 ? row.p_target(kept) : row.u_target(kept, first_weight);
+        if (fits) {
+            if (tid < in_list && to.within(my_before, my_rank, my_run, my_rank + 1)) {
+                s.answer_index = (uint32_t)index_of(mine);
+                s.answer_sum = my_run;
+            }
+        } else {
+            find(to, to);
+            const int j = s.hit[0];
+            const double by = units(j);
+            const u64 base = sum_before(j);
+            const uint32_t rank0 = count_before(j);
+            // the pieces of the bin: elements whose composite's bits from `known` on are `prefix`; before them in the bin lie sum0 and count0
+            u64 prefix = 0, sum0 = 0;
+            uint32_t count0 = 0, size = SM_LIST + 1;
+            int known = kKeyBits;
+            auto for_piece = [&](auto &&visit) {
+                for (int i = tid; i < n; i += SM_THREADS) {
+                    if (i < SM_IDS && s.id[i] != (uint16_t)((uint32_t)(q_top - j) << kIdShift)) continue;
+                    const float x = value(logits[i]);
+                    if (!scale.counts(x) || scale.bin(x) != q_top - j) continue;
+                    const u64 c = composite(x, i);
+                    if (c >> known == prefix) visit(c, x);
+                }
+            };
+            while (size > SM_LIST && known > 0) {
+                const int shift = max(known - 9, 0);
+                __syncthreads();
+                if (tid < SM_LIST) {
+                    s.prefix[tid] = 0;
+                    s.place[tid] = 0;
+                }
+                __syncthreads();
+                for_piece([&](u64 c, float x) {
+                    const int d = SM_LIST - 1 - (int)((c >> shift) & ((1ull << (known - shift)) - 1));
+                    atomicAdd(&s.prefix[d], scale.weight(x));
+                    atomicAdd(&s.place[d], 1);
+                });
+                __syncthreads();
+                if (tid == 0) {  // (rare, and 512 steps)
+                    u64 sum = sum0;
+                    uint32_t count = count0;
+                    for (int d = 0; d < SM_LIST; ++d) {
+                        const u64 next = sum + s.prefix[d];
+                        const uint32_t more = count + (uint32_t)s.place[d];
+                        if (to.within(base + in_units(sum, by), rank0 + count, base + in_units(next, by), rank0 + more)) {
+                            s.piece = d;
+                            s.piece_sum = sum;
+                            s.piece_count = count;
+                            break;
+                        }
+                        sum = next;
+                        count = more;
+                    }
+                }
+                __syncthreads();
+                size = (uint32_t)s.place[s.piece];
+                sum0 = s.piece_sum;
+                count0 = s.piece_count;
+                prefix = prefix << (known - shift) | (u64)(SM_LIST - 1 - s.piece);
+                known = shift;
+            }
+            __syncthreads();
+            if (tid == 0) s.piece = 0;
+            __syncthreads();
+            for_piece([&](u64 c, float) { s.list[min(atomicAdd(&s.piece, 1), SM_LIST - 1)] = c; });
+            __syncthreads();
+            if (tid < (int)size) {
+                const u64 c = s.list[tid];
+                u64 sum = sum0;
+                uint32_t rank = count0;
+                for (int o = 0; o < (int)size; ++o)
+                    if (s.list[o] > c) {
+                        sum += scale.weight(value_of(s.list[o]));
+                        ++rank;
+                    }
+                const u64 with = sum + scale.weight(value_of(c));
+                if (to.within(base + in_units(sum, by), rank0 + rank, base + in_units(with, by), rank0 + rank + 1)) {
+                    s.answer_index = (uint32_t)index_of(c);
+                    s.answer_sum = base + in_units(with, by);
+                }
             }
         }
         __syncthreads();
-        kept = min(kept, s_answer_sum);
-        __syncthreads();
+        kept = min(kept, s.answer_sum);
     }
-    if (tid == 0) *token = (int)s_answer;
+    if (tid == 0) p.tokens[r] = (int)s.answer_index;
 }
 
 }  // namespace
@@ -588,17 +630,8 @@ AGPU_EXPORT int32_t agpu_sample(agpu_ctx *ctx, const float *logits, const float 
     if (!logits || !u || !tokens_out) return agpu_fail(ctx, AGPU_ERR_NULL_POINTER, "sample: null pointer");
     agpu_on_device here(ctx);
     if (here.rc != AGPU_OK) return here.rc;
-    const int bits = std::min(62 - (n > 1 ? 32 - __builtin_clz(n - 1) : 0), 50);
+    const int bits = std::min(61 - (n > 1 ? 32 - __builtin_clz(n - 1) : 0), 50);
     const SampleArgs p = {logits, u, temperatures, top_ps, min_ps, top_ks, temperature, top_p, min_p, top_k, tokens_out, n, bits};
-    // Rows by as many as the scratch holds the states of; parts of 2048 elements at least.
-    const int at_once = (int)std::min<size_t>({(size_t)rows, ctx->ws_bytes / 2 / sizeof(RowState), (size_t)ctx->n_counters - 1, 65535});
-    const int count = std::max(1, std::min({SM_PARTS / at_once, n / 2048, SM_MAX_PARTS}));
-    for (int row0 = 0; row0 < rows; row0 += at_once) {
-        const Parts parts = {count, (ceil_div(n, count) + 3) & ~3, row0, reinterpret_cast<RowState *>(ctx->workspace), ctx->counters, ctx->strict_sync};
-        const dim3 grid(count, std::min(at_once, rows - row0));
-        hipLaunchKernelGGL(sample_top_kernel, grid, dim3(SM_THREADS), 0, ctx->stream, p, parts);
-        hipLaunchKernelGGL(sample_bins_kernel, grid, dim3(SM_THREADS), 0, ctx->stream, p, parts);
-        hipLaunchKernelGGL(sample_draw_kernel, grid, dim3(SM_THREADS), 0, ctx->stream, p, parts);
-    }
-    return AGPU_LAUNCH_CHECK(ctx, "sample kernels");
+    hipLaunchKernelGGL(sample_rows_kernel, dim3(rows), dim3(SM_THREADS), 0, ctx->stream, p);
+    return AGPU_LAUNCH_CHECK(ctx, "sample_rows_kernel");
 }
