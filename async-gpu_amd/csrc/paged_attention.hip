@@ -264,7 +264,14 @@ __device__ __forceinline__ void token_run(const PagedAttn &p, TokenShared<G, W> 
             const float mr = r0 + lane < runs ? load(r0 + lane, DH) : -INFINITY, f = mr == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mr - top);
             sum += wave_sum(r0 + lane < runs ? load(r0 + lane, DH + 1) * f : 0.0f);
             const int n = min(64, runs - r0);
-            for (int r = 0; r < n; ++r) acc = fmaf(load(r0 + r, lane), __shfl(f, r, kWave), acc);
+            for (int r = 0; r < n; r += 8) {  // eight on their way at a time, which the compiler would take one by one
+                float x[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = load(r0 + min(r + e, n - 1), lane);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) acc = r + e < n ? fmaf(x[e], __shfl(f, r + e, kWave), acc) : acc;
+            }
         }
         out[g * DH] = sum == 0.0f ? 0.0f : acc / sum;
     }
@@ -803,28 +810,31 @@ __device__ __forceinline__ void tile_run(const PagedAttn &p, TileShared<T> &s, c
         y = __uint_as_float((uint32_t)(v >> 32));
     };
     m = -INFINITY;
-    for (int r = 0; r < runs; ++r) {
-        float mr, lr;
-        load(r, DH, mr, lr);
-        m = fmaxf(m, mr);
-    }
     l = 0.0f;
     o[0] = o[1] = floatx16{};
+    // All loads of a run on their way at a time (the compiler would take them one by one: 5 us a run).
 #pragma unroll 1
     for (int r = 0; r < runs; ++r) {
         float mr, lr;
+        floatx16 x[2];
         load(r, DH, mr, lr);
-        const float a = mr == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mr - m);
-        l = fmaf(lr, a, l);
 #pragma unroll
         for (int db = 0; db < 2; ++db)
 #pragma unroll
             for (int e = 0; e < 16; e += 2) {
-                float x, y;
-                load(r, 32 * db + 8 * (e >> 2) + 4 * h2 + (e & 3), x, y);
-                o[db][e] = fmaf(x, a, o[db][e]);
-                o[db][e + 1] = fmaf(y, a, o[db][e + 1]);
+                float a, d;
+                load(r, 32 * db + 8 * (e >> 2) + 4 * h2 + (e & 3), a, d);
+                x[db][e] = a;
+                x[db][e + 1] = d;
             }
+        __builtin_amdgcn_sched_barrier(0);
+        const float now = fmaxf(m, mr), keep = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - now), a = mr == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mr - now);
+        m = now;
+        l = fmaf(lr, a, l * keep);
+#pragma unroll
+        for (int db = 0; db < 2; ++db)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[db][e] = fmaf(x[db][e], a, o[db][e] * keep);
     }
     store(l);
 }
