@@ -289,11 +289,12 @@ struct Units {
         for (int j = 0; j < 4; ++j) {
             if (64 * j >= entries) break;  // uniform
             int v = units[j];
-#pragma unroll
-            for (int by = 1; by < 64; by <<= 1) {
-                const int o = __shfl_up(v, by, kWave);
-                v += lane >= by ? o : 0;
-            }
+            v += (int)dpp_move_u32<0x111, 0xf>(0, v);  // row_shr 1, 2, 4, 8, then row_bcast 15 and 31: sums over the lanes up to this one
+            v += (int)dpp_move_u32<0x112, 0xf>(0, v);
+            v += (int)dpp_move_u32<0x114, 0xf>(0, v);
+            v += (int)dpp_move_u32<0x118, 0xf>(0, v);
+            v += (int)dpp_move_u32<0x142, 0xa>(0, v);
+            v += (int)dpp_move_u32<0x143, 0xc>(0, v);
             incl[64 * j + lane] = v + all;
             all += __builtin_amdgcn_readlane(v, 63);
         }
@@ -382,7 +383,7 @@ __global__ __launch_bounds__(64 * W) void paged_tokens_kernel(const PagedAttn p,
 
 // ---- tiles of rows on the matrix cores ----
 // S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_32x32x16 with 32 keys and 32 rows: what a 32 x 32 result holds of a column (a row of q) in its two
-// half waves is what the second product takes, if V's keys come in the order tile_key.
+// half waves is what the second product takes, if V's keys come in the order 16 step + 8 (e / 4) + 4 half + e mod 4.
 //   fp32 cache   every operand is the exact sum of three bf16 numbers (8 bits each, cut off one after the other); of the nine products of pieces the six that
 //                reach 2^-24 are formed, the smallest first
 //   bf16 cache   K and V as they are, q and the weights in three pieces: three products
@@ -392,7 +393,9 @@ constexpr int TILE_ROWS = 128, TILE_KEYS = 32;
 constexpr int kFrag = 4 * 2 * 32;  // 16-byte fragments of a piece of 32 keys of K, and of V
 typedef float floatx16 __attribute__((ext_vector_type(16)));
 
-__device__ __forceinline__ int tile_key(int step, int half, int e) { return 16 * step + 8 * (e >> 2) + 4 * half + (e & 3); }
+// Where in LDS the 16 elements `part` of the row of V of a key lie, in bytes: 128 a key, its four parts in an order by which eight keys' parts, which are
+// read at a time, come from different banks.
+__device__ __forceinline__ int tile_v_at(int key, int part) { return 128 * key + 32 * (part ^ (key & 2) ^ (key >> 2 & 1)); }
 
 __device__ __forceinline__ uint32_t upper_halves(float a, float b) { return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u); }
 __device__ __forceinline__ float without_top(float x) { return x - __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
@@ -440,7 +443,7 @@ struct Tiles<F16> {
     }
 };
 
-// Eight elements of K (of one key) or of V (one dimension of eight keys) on their way from the cache to LDS.
+// Eight elements of a key's row of K or V on their way from the cache to LDS.
 template <class T>
 struct Staged;
 template <>
@@ -450,13 +453,10 @@ struct Staged<F32> {
         const float4 a = *reinterpret_cast<const float4 *>(p), b = *reinterpret_cast<const float4 *>(p + 16);
         x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
     }
-    __device__ __forceinline__ void element(int e, const char *p) { x[e] = *reinterpret_cast<const float *>(p); }
-    __device__ __forceinline__ void clear_row() {
+    __device__ __forceinline__ void clear() {
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] = 0.0f;
     }
-    __device__ __forceinline__ void clear_element(int e) { x[e] = 0.0f; }
-    __device__ __forceinline__ void pack() {}
     __device__ __forceinline__ bool odd() const {  // one of them is infinite or no number
         float t = 0.0f;
 #pragma unroll
@@ -483,18 +483,12 @@ struct Staged<F32> {
 };
 template <class T>
 struct Staged16 {
-    uint32_t x[8];  // a row, or elements that have been packed: the first four, two elements each; before: one each
+    uint32_t x[4];  // two elements each
     __device__ __forceinline__ void row(const char *p) {
         const uint4 a = *reinterpret_cast<const uint4 *>(p);
         x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
     }
-    __device__ __forceinline__ void element(int e, const char *p) { x[e] = *reinterpret_cast<const unsigned short *>(p); }
-    __device__ __forceinline__ void clear_row() { x[0] = x[1] = x[2] = x[3] = 0; }
-    __device__ __forceinline__ void clear_element(int e) { x[e] = 0; }
-    __device__ __forceinline__ void pack() {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = x[2 * e] | x[2 * e + 1] << 16;
-    }
+    __device__ __forceinline__ void clear() { x[0] = x[1] = x[2] = x[3] = 0; }
     __device__ __forceinline__ bool odd() const {  // an exponent of ones and one more is the sign bit
         constexpr uint32_t ones = T::kExponent * 0x10001u, one = (T::kExponent & (0u - T::kExponent)) * 0x10001u;
         uint32_t t = 0;
@@ -521,7 +515,7 @@ struct Staged<F16> : Staged16<F16> {};
 
 template <class T>
 struct TileShared {
-    uint4 k[2][Tiles<T>::KP][kFrag], v[2][Tiles<T>::KP][kFrag];  // [buffer][piece]: K [d step of 16][half][key], V [32 dimensions][key step][half][dimension]
+    uint4 k[2][Tiles<T>::KP][kFrag], v[2][Tiles<T>::KP][kFrag];  // [buffer][piece]: K [d step of 16][half][key], V [key][dimension], what tile_v_at says
     long long at[4][TILE_KEYS], at_v[4][TILE_KEYS];  // of a tile's keys: where their rows of K and V begin, in bytes (0 for those that are not there)
     uint32_t seen[4];             // which of them are there
     uint32_t odd_k[4], odd_v[4];  // of which something is infinite or not a number
@@ -571,6 +565,36 @@ __device__ __forceinline__ void tile_run(const PagedAttn &p, TileShared<T> &s, c
     // key number v is seen if v <= v_last and (v > v_low or v < v_first)
     const int v_last = pos - gap, v_low = p.window > 0 ? pos - p.window - gap : -1, v_first = p.window > 0 ? max(first, p.sinks - gap) : 0;
 
+    // keys of tile i are lo + 32 i ..; places of a tile are looked up two tiles ahead
+    const int tiles = (hi - lo + TILE_KEYS - 1) / TILE_KEYS;
+    const int *table = p.tables + (size_t)b * p.width;
+    auto look_up = [&](int i, int &id, int &off) {  // the first 32 threads
+        const int v = lo + TILE_KEYS * i + c;
+        id = -1;
+        off = 0;
+        if (v < hi) {
+            const int j = v < first ? v : v + gap, page = p.div.page(j);
+            id = table[page];
+            off = j - page * p.div.size;
+        }
+    };
+    auto leave = [&](int i, int id, int off) {
+        const bool ok = (unsigned)id < (unsigned)p.n_pages;
+        const long long at = (long long)(h * p.div.size + off) * DH;
+        s.at[i & 3][c] = ok ? (id * p.k_page + at) * kBytes : 0;
+        s.at_v[i & 3][c] = ok ? (id * p.v_page + at) * kBytes : 0;
+        const uint64_t who = __ballot(ok);
+        if (lane == 0) {
+            s.seen[i & 3] = (uint32_t)who;
+            s.odd_k[i & 3] = s.odd_v[i & 3] = 0;
+        }
+    };
+    int id0 = -1, off0 = 0, id1 = -1, off1 = 0, id = -1, off = 0;
+    if (tid < 32) {
+        look_up(0, id0, off0);
+        look_up(1, id1, off1);
+        look_up(2, id, off);
+    }
     const float *q_row = p.q + (size_t)(start + token) * p.q_row + (size_t)head * p.q_head;
     uint4 q[4][QP];
     float unit = 1.0f;  // of the scores
@@ -599,51 +623,28 @@ __device__ __forceinline__ void tile_run(const PagedAttn &p, TileShared<T> &s, c
         for (int ds = 0; ds < 4; ++ds) pieces_of(x[ds], q[ds]);
     }
 
-    // keys of tile i are lo + 32 i ..; places of a tile are looked up two tiles ahead
-    const int tiles = (hi - lo + TILE_KEYS - 1) / TILE_KEYS;
-    const int *table = p.tables + (size_t)b * p.width;
-    auto look_up = [&](int i, int &id, int &off) {  // the first 32 threads
-        const int v = lo + TILE_KEYS * i + c;
-        id = -1;
-        off = 0;
-        if (v < hi) {
-            const int j = v < first ? v : v + gap, page = p.div.page(j);
-            id = table[page];
-            off = j - page * p.div.size;
-        }
-    };
-    auto leave = [&](int i, int id, int off) {
-        const bool ok = (unsigned)id < (unsigned)p.n_pages;
-        const long long at = (long long)(h * p.div.size + off) * DH;
-        s.at[i & 3][c] = ok ? (id * p.k_page + at) * kBytes : 0;
-        s.at_v[i & 3][c] = ok ? (id * p.v_page + at) * kBytes : 0;
-        const uint64_t who = __ballot(ok);
-        if (lane == 0) {
-            s.seen[i & 3] = (uint32_t)who;
-            s.odd_k[i & 3] = s.odd_v[i & 3] = 0;
-        }
-    };
-    int id = -1, off = 0;
     if (tid < 32) {
-        look_up(0, id, off);
-        leave(0, id, off);
-        look_up(1, id, off);
-        leave(1, id, off);
-        look_up(2, id, off);
+        leave(0, id0, off0);
+        leave(1, id1, off1);
     }
     __syncthreads();
     const char *const kb = static_cast<const char *>(p.k), *const vb = static_cast<const char *>(p.v);
     Staged<T> sk, sv;
-    // What this thread fetches: eight elements of K of key c, and eight keys of dimension `lane` of V, the same ones for the whole wave.
-    const int k_byte = (16 * wave + 8 * h2) * kBytes, v_step = wave & 1, v_half = wave >> 1;
+    // What this thread fetches: eight elements of K and of V of key c.
+    const int row_byte = (16 * wave + 8 * h2) * kBytes, v_at = tile_v_at(c, wave) + 16 * h2;
     auto fetch = [&](int i) {
-        sk.row(kb + s.at[i & 3][c] + k_byte);
-        const long long at = s.at_v[i & 3][tile_key(v_step, v_half, lane & 7)];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const uint32_t low = __builtin_amdgcn_readlane((int)(uint32_t)at, e), high = __builtin_amdgcn_readlane((int)(at >> 32), e);
-            sv.element(e, vb + (long long)((uint64_t)high << 32 | low) + lane * kBytes);
-        }
+        sk.row(kb + s.at[i & 3][c] + row_byte);
+        sv.row(vb + s.at_v[i & 3][c] + row_byte);
+    };
+    // The operand of V: of dimension 32 db + c the keys tile_key(st, h2, 0..7), four rows at a time that ds_read_b64_tr_b16 turns (16 lanes read four rows of 16
+    // elements, a row in four lanes, and each gets a column).
+    const int turned = tile_v_at(4 * h2 + ((lane & 15) >> 2), c >> 4) + 8 * (lane & 3);
+    auto v_operand = [&](const uint4 *piece, int st, int db) {
+        typedef short four __attribute__((ext_vector_type(4)));
+        const char *const at = reinterpret_cast<const char *>(piece) + (turned ^ (64 * db)) + 2048 * st;
+        typedef __attribute__((address_space(3))) four *lds;
+        const uint2 a = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds)at)), d = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds)(at + 1024)));
+        return make_uint4(a.x, a.y, d.x, d.y);
     };
     if (tiles > 0) fetch(0);
 
@@ -653,21 +654,17 @@ __device__ __forceinline__ void tile_run(const PagedAttn &p, TileShared<T> &s, c
         const int buf = i & 1;
         const uint32_t there = s.seen[i & 3];
         if (there != 0xffffffffu) {  // uniform; zeros instead of what is not there
-            if (!(there >> c & 1)) sk.clear_row();
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (!(there >> tile_key(v_step, v_half, e) & 1)) sv.clear_element(e);
+            if (!(there >> c & 1)) {
+                sk.clear();
+                sv.clear();
+            }
         }
-        sv.pack();
         if (__builtin_expect(__any(sk.odd() || sv.odd()), 0)) {
             if (sk.clean()) atomicOr(&s.odd_k[i & 3], 1u << c);
-            const uint32_t odd = sv.clean();
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (odd >> e & 1) atomicOr(&s.odd_v[i & 3], 1u << tile_key(v_step, v_half, e));
+            if (sv.clean()) atomicOr(&s.odd_v[i & 3], 1u << c);
         }
         sk.store(&s.k[buf][0][(2 * wave + h2) * 32 + c]);
-        sv.store(&s.v[buf][0][((2 * h2 + v_step) * 2 + v_half) * 32 + c]);
+        sv.store(&s.v[buf][0][v_at / 16]);
         if (i + 1 < tiles) fetch(i + 1);
         if (tid < 32) {
             leave(i + 2, id, off);
@@ -750,7 +747,7 @@ __device__ __forceinline__ void tile_run(const PagedAttn &p, TileShared<T> &s, c
 #pragma unroll
                     for (int st = 0; st < 2; ++st)
 #pragma unroll
-                        for (int db = 0; db < 2; ++db) o[db] = Tiles<T>::mfma(s.v[buf][kp][((2 * db + st) * 2 + h2) * 32 + c], w[st][level - kp], o[db]);
+                        for (int db = 0; db < 2; ++db) o[db] = Tiles<T>::mfma(v_operand(s.v[buf][kp], st, db), w[st][level - kp], o[db]);
         if (__builtin_expect(odd_v != 0, 0))
 #pragma unroll 1
             for (int kk = 0; kk < TILE_KEYS; ++kk) {
