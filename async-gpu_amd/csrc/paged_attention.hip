@@ -21,7 +21,7 @@ struct PagedAttn {
     const int *tables, *kv_lens, *query_start;
     float *o;  // [tokens][n_heads][64]
     int tokens, batch, n_heads, n_kv, n_pages, width, held, window, sinks;
-    PageDiv div;
+    PageDiv div, group;  // by the page size, and by the heads of a K/V head
     int strict;
 };
 
@@ -546,9 +546,9 @@ __device__ __forceinline__ void tile_run(const PagedAttn &p, TileShared<T> &s, c
     constexpr int KP = Tiles<T>::KP, QP = Tiles<T>::QP;
     constexpr int kBytes = 16 / T::EL;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 31, h2 = lane >> 5;
-    const int group = p.n_heads / p.n_kv, rows = q_len * group, last_row = min(first_row + TILE_ROWS, rows) - 1;
+    const int group = p.group.size, rows = q_len * group, last_row = min(first_row + TILE_ROWS, rows) - 1;
     // all keys that a row of the tile sees, numbered without a gap
-    const int pos0 = kv_len - q_len + first_row / group, pos1 = kv_len - q_len + last_row / group;
+    const int pos0 = kv_len - q_len + p.group.page(first_row), pos1 = kv_len - q_len + p.group.page(last_row);
     int end = min(min(pos1 + 1, kv_len), p.held);
     end = max(end, 0);
     int low = p.window > 0 ? max(pos0 + 1 - p.window, 0) : 0;
@@ -558,10 +558,10 @@ __device__ __forceinline__ void tile_run(const PagedAttn &p, TileShared<T> &s, c
     if (run >= runs) return;
     const int lo = run * cuts.keys, hi = min(count, lo + cuts.keys);
     // this lane's row; rows behind the last one repeat it
-    const int row = min(first_row + 32 * wave + c, last_row), token = row / group, head = h * group + (row - token * group);
+    const int row = min(first_row + 32 * wave + c, last_row), token = p.group.page(row), head = h * group + (row - token * group);
     const bool mine = first_row + 32 * wave + c <= last_row, any = first_row + 32 * wave <= last_row;
     const int pos = kv_len - q_len + token;
-    const int wave_pos0 = kv_len - q_len + min(first_row + 32 * wave, last_row) / group, wave_pos1 = kv_len - q_len + min(first_row + 32 * wave + 31, last_row) / group;
+    const int wave_pos0 = kv_len - q_len + p.group.page(min(first_row + 32 * wave, last_row)), wave_pos1 = kv_len - q_len + p.group.page(min(first_row + 32 * wave + 31, last_row));
     // key number v is seen if v <= v_last and (v > v_low or v < v_first)
     const int v_last = pos - gap, v_low = p.window > 0 ? pos - p.window - gap : -1, v_first = p.window > 0 ? max(first, p.sinks - gap) : 0;
 
@@ -848,7 +848,8 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(const PagedAttn p, R
     };
     __shared__ __align__(16) char smem[sizeof(Shared)];
     __shared__ Units tile_list, token_list;
-    const int lane = threadIdx.x & 63, group = p.n_heads / p.n_kv;
+    __shared__ int starts[kListed], lens[kListed], kvs[kListed];
+    const int lane = threadIdx.x & 63, group = p.group.size;
     int tile_units = tile_places * p.n_kv * tile_cut.most, all = tile_units + p.batch * slots * p.n_kv * token_cut.most;
     if (listed) {
         int tiles[4], tokens[4], keys[4], longest = 0;
@@ -857,9 +858,12 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(const PagedAttn p, R
         for (int j = 0; j < 4; ++j) {
             tiles[j] = tokens[j] = keys[j] = 0;
             if (64 * j + lane < p.batch) {
-                const int start = p.query_start[64 * j + lane], q_len = min(p.query_start[64 * j + lane + 1], p.tokens) - start;
+                const int start = p.query_start[64 * j + lane], q_len = min(p.query_start[64 * j + lane + 1], p.tokens) - start, kv_len = p.kv_lens[64 * j + lane];
+                starts[64 * j + lane] = start;
+                lens[64 * j + lane] = q_len;
+                kvs[64 * j + lane] = kv_len;
                 if (start >= 0 && q_len > 0) {
-                    keys[j] = max(keys_seen(p, p.kv_lens[64 * j + lane], q_len > slots ? min(q_len, TILE_ROWS / group + 2) : 1), 1);
+                    keys[j] = max(keys_seen(p, kv_len, q_len > slots ? min(q_len, p.group.page(TILE_ROWS) + 2) : 1), 1);
                     if (q_len > slots) tiles[j] = (q_len * group + TILE_ROWS - 1) / TILE_ROWS;
                     else tokens[j] = q_len;
                 }
@@ -888,16 +892,16 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(const PagedAttn p, R
                 const int each = tile_units >> 3, rest = tile_units & 7, xcd = at & 7;
                 at = xcd * each + min(xcd, rest) + (at >> 3);
                 b = tile_list.entry(at, lane);
-                const int q_len = min(p.query_start[b + 1], p.tokens) - p.query_start[b], n = (q_len * group + TILE_ROWS - 1) / TILE_ROWS;
-                const int runs = paged::runs_of(max(keys_seen(p, p.kv_lens[b], min(q_len, TILE_ROWS / group + 2)), 1), tile_cut.run, tile_cut.most).runs;
-                h = at / (n * runs);
-                at -= h * n * runs;
-                tile = n - 1 - at / runs;
-                run = at % runs;
+                const int q_len = lens[b], n = (q_len * group + TILE_ROWS - 1) / TILE_ROWS;
+                const int runs = paged::runs_of(max(keys_seen(p, kvs[b], min(q_len, p.group.page(TILE_ROWS) + 2)), 1), tile_cut.run, tile_cut.most).runs;
+                const int place = at / runs;
+                run = at - place * runs;
+                h = place / n;
+                tile = n - 1 - (place - h * n);
             } else {
                 at -= tile_units;
                 b = token_list.entry(at, lane);
-                const int runs = paged::runs_of(max(keys_seen(p, p.kv_lens[b], 1), 1), token_cut.run, token_cut.most).runs;
+                const int runs = paged::runs_of(max(keys_seen(p, kvs[b], 1), 1), token_cut.run, token_cut.most).runs;
                 token = at / (runs * p.n_kv);
                 at -= token * runs * p.n_kv;
                 run = at / p.n_kv;
@@ -921,15 +925,16 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(const PagedAttn p, R
             b = at / slots;
             token = at - b * slots;
         }
-        const int start = p.query_start[b], end = min(p.query_start[b + 1], p.tokens), q_len = end - start;
+        const int start = listed ? starts[b] : p.query_start[b], q_len = listed ? lens[b] : min(p.query_start[b + 1], p.tokens) - start;
+        const int kv_len = listed ? kvs[b] : p.kv_lens[b], end = start + q_len;
         if (start < 0) continue;
         if (token < 0) {
             if (q_len <= slots || tile < 0 || tile * TILE_ROWS >= q_len * group) continue;
             const int item = (start * group / TILE_ROWS + b + tile) * p.n_kv + h;
-            tile_run<T>(p, *reinterpret_cast<TileShared<T> *>(smem), tile_cut, b, start, q_len, p.kv_lens[b], h, tile * TILE_ROWS, run, item);
+            tile_run<T>(p, *reinterpret_cast<TileShared<T> *>(smem), tile_cut, b, start, q_len, kv_len, h, tile * TILE_ROWS, run, item);
         } else {
             if (token >= q_len || q_len > slots) continue;
-            token_run<T, G, 4, 4>(p, *reinterpret_cast<TokenShared<G, 4> *>(smem), token_cut, start + token, b, p.kv_lens[b], end, h, h * group, group, run,
+            token_run<T, G, 4, 4>(p, *reinterpret_cast<TokenShared<G, 4> *>(smem), token_cut, start + token, b, kv_len, end, h, h * group, group, run,
                                   (b * slots + token) * p.n_kv + h);
         }
     }
@@ -1001,6 +1006,7 @@ AGPU_EXPORT int32_t agpu_paged_attention(agpu_ctx *ctx, const float *q, int64_t 
     p.tokens = tokens; p.batch = batch; p.n_heads = n_heads; p.n_kv = n_kv_heads; p.n_pages = n_pages;
     p.width = table_width; p.held = table_width * page_size; p.window = window; p.sinks = sinks;
     p.div = PageDiv::of(page_size);
+    p.group = PageDiv::of(n_heads / n_kv_heads);
     p.strict = ctx->strict_sync;
     const int64_t longest = paged::longest_row(p.held, window, sinks);
     return cache_type == AGPU_CACHE_F32 ? attention_go<F32>(ctx, p, longest) : cache_type == AGPU_CACHE_F16 ? attention_go<F16>(ctx, p, longest) : attention_go<BF16>(ctx, p, longest);
