@@ -392,24 +392,36 @@ __global__ __launch_bounds__(64 * W) void paged_tokens_kernel(const PagedAttn p,
 constexpr int TILE_ROWS = 128, TILE_KEYS = 32;
 constexpr int kFrag = 4 * 2 * 32;  // 16-byte fragments of a piece of 32 keys of K, and of V
 typedef float floatx16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
 // Where in LDS the 16 elements `part` of the row of V of a key lie, in bytes: 128 a key, its four parts in an order by which eight keys' parts, which are
 // read at a time, come from different banks.
 __device__ __forceinline__ int tile_v_at(int key, int part) { return 128 * key + 32 * (part ^ (key & 2) ^ (key >> 2 & 1)); }
 
 __device__ __forceinline__ uint32_t upper_halves(float a, float b) { return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u); }
-__device__ __forceinline__ float without_top(float x) { return x - __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
+// x without the first or the second of two bf16 numbers: a product of pairs with (-1, 0) or (0, -1), which is exact.  (The constants come in registers: as
+// literals the compiler takes them for the -1 that stands for both halves.)
+__device__ __forceinline__ float without(uint32_t two, uint32_t which, float x) {
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, two), __builtin_bit_cast(bf16x2, which), x, false);
+}
 // Eight floats -> their three pieces, the largest first
 __device__ __forceinline__ void pieces_of(const float (&v)[8], uint4 (&piece)[3]) {
-    float r[8], t[8];
+    uint32_t first = 0x0000bf80u, second = 0xbf800000u, p[3][4];
+    asm("" : "+s"(first));
+    asm("" : "+s"(second));
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        r[e] = without_top(v[e]);
-        t[e] = without_top(r[e]);
+    for (int i = 0; i < 4; ++i) {
+        float a = v[2 * i], b = v[2 * i + 1];
+#pragma unroll
+        for (int level = 0; level < 3; ++level) {
+            p[level][i] = upper_halves(a, b);
+            a = without(p[level][i], first, a);
+            b = without(p[level][i], second, b);
+        }
     }
-    piece[0] = make_uint4(upper_halves(v[0], v[1]), upper_halves(v[2], v[3]), upper_halves(v[4], v[5]), upper_halves(v[6], v[7]));
-    piece[1] = make_uint4(upper_halves(r[0], r[1]), upper_halves(r[2], r[3]), upper_halves(r[4], r[5]), upper_halves(r[6], r[7]));
-    piece[2] = make_uint4(upper_halves(t[0], t[1]), upper_halves(t[2], t[3]), upper_halves(t[4], t[5]), upper_halves(t[6], t[7]));
+#pragma unroll
+    for (int level = 0; level < 3; ++level) piece[level] = make_uint4(p[level][0], p[level][1], p[level][2], p[level][3]);
 }
 __device__ __forceinline__ void pieces_of(const float (&v)[8], uint4 (&piece)[2]) {  // f16
     f16x8 hi, lo;
@@ -460,7 +472,7 @@ struct Staged<F32> {
     __device__ __forceinline__ bool odd() const {  // one of them is infinite or no number
         float t = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) t = fmaf(x[e], 0.0f, t);
+        for (int e = 0; e < 8; e += 2) t = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, upper_halves(x[e], x[e + 1])), bf16x2{}, t, false);
         return t != 0.0f;
     }
     // Zeros in place of those; which there were.
@@ -489,12 +501,14 @@ struct Staged16 {
         x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
     }
     __device__ __forceinline__ void clear() { x[0] = x[1] = x[2] = x[3] = 0; }
-    __device__ __forceinline__ bool odd() const {  // an exponent of ones and one more is the sign bit
-        constexpr uint32_t ones = T::kExponent * 0x10001u, one = (T::kExponent & (0u - T::kExponent)) * 0x10001u;
-        uint32_t t = 0;
+    __device__ __forceinline__ bool odd() const {
+        float t = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) t |= (x[e] & ones) + one;
-        return (t & 0x80008000u) != 0;
+        for (int e = 0; e < 4; ++e) {
+            if constexpr (T::kExponent == 0x7c00) t = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, x[e]), f16x2{}, t, false);
+            else t = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, x[e]), bf16x2{}, t, false);
+        }
+        return t != 0.0f;
     }
     __device__ __forceinline__ uint32_t clean() {
         uint32_t odd = 0;
@@ -516,9 +530,9 @@ struct Staged<F16> : Staged16<F16> {};
 template <class T>
 struct TileShared {
     uint4 k[2][Tiles<T>::KP][kFrag], v[2][Tiles<T>::KP][kFrag];  // [buffer][piece]: K [d step of 16][half][key], V [key][dimension], what tile_v_at says
-    long long at[4][TILE_KEYS], at_v[4][TILE_KEYS];  // of a tile's keys: where their rows of K and V begin, in bytes (0 for those that are not there)
-    uint32_t seen[4];             // which of them are there
-    uint32_t odd_k[4], odd_v[4];  // of which something is infinite or not a number
+    long long at[2][8][TILE_KEYS];  // of the keys of eight tiles: where their rows of K and of V begin, in bytes (0 for those that are not there)
+    uint32_t seen[8];               // which of them are there
+    uint32_t odd_k[8], odd_v[8];    // of which something is infinite or not a number
     unsigned int ticket;
 };
 
@@ -565,10 +579,11 @@ __device__ __forceinline__ void tile_run(const PagedAttn &p, TileShared<T> &s, c
     // key number v is seen if v <= v_last and (v > v_low or v < v_first)
     const int v_last = pos - gap, v_low = p.window > 0 ? pos - p.window - gap : -1, v_first = p.window > 0 ? max(first, p.sinks - gap) : 0;
 
-    // keys of tile i are lo + 32 i ..; places of a tile are looked up two tiles ahead
+    // keys of tile i are lo + 32 i ..; their places are looked up for four tiles at a time, one a wave, long before they are fetched
     const int tiles = (hi - lo + TILE_KEYS - 1) / TILE_KEYS;
     const int *table = p.tables + (size_t)b * p.width;
-    auto look_up = [&](int i, int &id, int &off) {  // the first 32 threads
+    int id, off;
+    auto look_up = [&](int i) {
         const int v = lo + TILE_KEYS * i + c;
         id = -1;
         off = 0;
@@ -578,23 +593,17 @@ __device__ __forceinline__ void tile_run(const PagedAttn &p, TileShared<T> &s, c
             off = j - page * p.div.size;
         }
     };
-    auto leave = [&](int i, int id, int off) {
+    auto leave = [&](int i) {  // a half wave for K, the other for V
         const bool ok = (unsigned)id < (unsigned)p.n_pages;
-        const long long at = (long long)(h * p.div.size + off) * DH;
-        s.at[i & 3][c] = ok ? (id * p.k_page + at) * kBytes : 0;
-        s.at_v[i & 3][c] = ok ? (id * p.v_page + at) * kBytes : 0;
+        s.at[h2][i & 7][c] = ok ? (id * (h2 ? p.v_page : p.k_page) + (long long)(h * p.div.size + off) * DH) * kBytes : 0;
         const uint64_t who = __ballot(ok);
         if (lane == 0) {
-            s.seen[i & 3] = (uint32_t)who;
-            s.odd_k[i & 3] = s.odd_v[i & 3] = 0;
+            s.seen[i & 7] = (uint32_t)who;
+            s.odd_k[i & 7] = s.odd_v[i & 7] = 0;
         }
     };
-    int id0 = -1, off0 = 0, id1 = -1, off1 = 0, id = -1, off = 0;
-    if (tid < 32) {
-        look_up(0, id0, off0);
-        look_up(1, id1, off1);
-        look_up(2, id, off);
-    }
+    look_up(wave);
+
     const float *q_row = p.q + (size_t)(start + token) * p.q_row + (size_t)head * p.q_head;
     uint4 q[4][QP];
     float unit = 1.0f;  // of the scores
@@ -623,18 +632,16 @@ __device__ __forceinline__ void tile_run(const PagedAttn &p, TileShared<T> &s, c
         for (int ds = 0; ds < 4; ++ds) pieces_of(x[ds], q[ds]);
     }
 
-    if (tid < 32) {
-        leave(0, id0, off0);
-        leave(1, id1, off1);
-    }
+    leave(wave);
+    look_up(4 + wave);
     __syncthreads();
     const char *const kb = static_cast<const char *>(p.k), *const vb = static_cast<const char *>(p.v);
     Staged<T> sk, sv;
     // What this thread fetches: eight elements of K and of V of key c.
     const int row_byte = (16 * wave + 8 * h2) * kBytes, v_at = tile_v_at(c, wave) + 16 * h2;
     auto fetch = [&](int i) {
-        sk.row(kb + s.at[i & 3][c] + row_byte);
-        sv.row(vb + s.at_v[i & 3][c] + row_byte);
+        sk.row(kb + s.at[0][i & 7][c] + row_byte);
+        sv.row(vb + s.at[1][i & 7][c] + row_byte);
     };
     // The operand of V: of dimension 32 db + c the keys tile_key(st, h2, 0..7), four rows at a time that ds_read_b64_tr_b16 turns (16 lanes read four rows of 16
     // elements, a row in four lanes, and each gets a column).
@@ -652,7 +659,7 @@ __device__ __forceinline__ void tile_run(const PagedAttn &p, TileShared<T> &s, c
     float m = -INFINITY, l = 0.0f;
     for (int i = 0; i < tiles; ++i) {
         const int buf = i & 1;
-        const uint32_t there = s.seen[i & 3];
+        const uint32_t there = s.seen[i & 7];
         if (there != 0xffffffffu) {  // uniform; zeros instead of what is not there
             if (!(there >> c & 1)) {
                 sk.clear();
@@ -660,17 +667,17 @@ __device__ __forceinline__ void tile_run(const PagedAttn &p, TileShared<T> &s, c
             }
         }
         if (__builtin_expect(__any(sk.odd() || sv.odd()), 0)) {
-            if (sk.clean()) atomicOr(&s.odd_k[i & 3], 1u << c);
-            if (sv.clean()) atomicOr(&s.odd_v[i & 3], 1u << c);
+            if (sk.clean()) atomicOr(&s.odd_k[i & 7], 1u << c);
+            if (sv.clean()) atomicOr(&s.odd_v[i & 7], 1u << c);
         }
         sk.store(&s.k[buf][0][(2 * wave + h2) * 32 + c]);
         sv.store(&s.v[buf][0][v_at / 16]);
         if (i + 1 < tiles) fetch(i + 1);
-        if (tid < 32) {
-            leave(i + 2, id, off);
-            look_up(i + 3, id, off);
-        }
         __syncthreads();
+        if ((i & 3) == 0) {
+            leave(i + 4 + wave);
+            look_up(i + 8 + wave);
+        }
         const int v0 = lo + TILE_KEYS * i;
         if (!any || (v0 >= first && v0 > wave_pos1 - gap)) continue;  // (the next tile goes to the other buffer)
         floatx16 x = {};
@@ -686,12 +693,12 @@ __device__ __forceinline__ void tile_run(const PagedAttn &p, TileShared<T> &s, c
             for (int r = 0; r < 16; ++r) x[r] *= unit;
         // Keys with something infinite in them, or no number, went as zeros, which no row's other keys notice; their scores are formed in fp32 here, and
         // their values are added below, for the rows that see them.
-        const uint32_t odd_k = s.odd_k[i & 3], odd_v = s.odd_v[i & 3];
+        const uint32_t odd_k = s.odd_k[i & 7], odd_v = s.odd_v[i & 7];
         if (__builtin_expect(odd_k != 0, 0))
 #pragma unroll 1
             for (int kk = 0; kk < TILE_KEYS; ++kk) {
                 if (!(odd_k >> kk & 1)) continue;
-                const size_t at = (size_t)s.at[i & 3][kk];
+                const size_t at = (size_t)s.at[0][i & 7][kk];
                 float d = 0.0f;
 #pragma unroll 1
                 for (int e = 0; e < 32; ++e) d = fmaf(q_row[32 * h2 + e] * kQueryScale, T::one(kb + at, 32 * h2 + e), d);
@@ -758,7 +765,7 @@ __device__ __forceinline__ void tile_run(const PagedAttn &p, TileShared<T> &s, c
 #pragma unroll
                 for (int r = 0; r < 16; ++r) weight = 8 * (r >> 2) + 4 * h2 + (r & 3) == kk ? x[r] : weight;
                 weight = sum_of_halves(weight);  // (one of them is zero)
-                const size_t at = (size_t)s.at_v[i & 3][kk];
+                const size_t at = (size_t)s.at[1][i & 7][kk];
 #pragma unroll
                 for (int db = 0; db < 2; ++db)
 #pragma unroll
