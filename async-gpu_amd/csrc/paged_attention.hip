@@ -392,36 +392,24 @@ __global__ __launch_bounds__(64 * W) void paged_tokens_kernel(const PagedAttn p,
 constexpr int TILE_ROWS = 128, TILE_KEYS = 32;
 constexpr int kFrag = 4 * 2 * 32;  // 16-byte fragments of a piece of 32 keys of K, and of V
 typedef float floatx16 __attribute__((ext_vector_type(16)));
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
 // Where in LDS the 16 elements `part` of the row of V of a key lie, in bytes: 128 a key, its four parts in an order by which eight keys' parts, which are
 // read at a time, come from different banks.
 __device__ __forceinline__ int tile_v_at(int key, int part) { return 128 * key + 32 * (part ^ (key & 2) ^ (key >> 2 & 1)); }
 
 __device__ __forceinline__ uint32_t upper_halves(float a, float b) { return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u); }
-// x without the first or the second of two bf16 numbers: a product of pairs with (-1, 0) or (0, -1), which is exact.  (The constants come in registers: as
-// literals the compiler takes them for the -1 that stands for both halves.)
-__device__ __forceinline__ float without(uint32_t two, uint32_t which, float x) {
-    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, two), __builtin_bit_cast(bf16x2, which), x, false);
-}
+__device__ __forceinline__ float without_top(float x) { return x - __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
 // Eight floats -> their three pieces, the largest first
 __device__ __forceinline__ void pieces_of(const float (&v)[8], uint4 (&piece)[3]) {
-    uint32_t first = 0x0000bf80u, second = 0xbf800000u, p[3][4];
-    asm("" : "+s"(first));
-    asm("" : "+s"(second));
+    float r[8], t[8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        float a = v[2 * i], b = v[2 * i + 1];
-#pragma unroll
-        for (int level = 0; level < 3; ++level) {
-            p[level][i] = upper_halves(a, b);
-            a = without(p[level][i], first, a);
-            b = without(p[level][i], second, b);
-        }
+    for (int e = 0; e < 8; ++e) {
+        r[e] = without_top(v[e]);
+        t[e] = without_top(r[e]);
     }
-#pragma unroll
-    for (int level = 0; level < 3; ++level) piece[level] = make_uint4(p[level][0], p[level][1], p[level][2], p[level][3]);
+    piece[0] = make_uint4(upper_halves(v[0], v[1]), upper_halves(v[2], v[3]), upper_halves(v[4], v[5]), upper_halves(v[6], v[7]));
+    piece[1] = make_uint4(upper_halves(r[0], r[1]), upper_halves(r[2], r[3]), upper_halves(r[4], r[5]), upper_halves(r[6], r[7]));
+    piece[2] = make_uint4(upper_halves(t[0], t[1]), upper_halves(t[2], t[3]), upper_halves(t[4], t[5]), upper_halves(t[6], t[7]));
 }
 __device__ __forceinline__ void pieces_of(const float (&v)[8], uint4 (&piece)[2]) {  // f16
     f16x8 hi, lo;
@@ -472,7 +460,7 @@ struct Staged<F32> {
     __device__ __forceinline__ bool odd() const {  // one of them is infinite or no number
         float t = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 8; e += 2) t = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, upper_halves(x[e], x[e + 1])), bf16x2{}, t, false);
+        for (int e = 0; e < 8; ++e) t = fmaf(x[e], 0.0f, t);
         return t != 0.0f;
     }
     // Zeros in place of those; which there were.
@@ -501,14 +489,12 @@ struct Staged16 {
         x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
     }
     __device__ __forceinline__ void clear() { x[0] = x[1] = x[2] = x[3] = 0; }
-    __device__ __forceinline__ bool odd() const {
-        float t = 0.0f;
+    __device__ __forceinline__ bool odd() const {  // an exponent of ones and one more is the sign bit
+        constexpr uint32_t ones = T::kExponent * 0x10001u, one = (T::kExponent & (0u - T::kExponent)) * 0x10001u;
+        uint32_t t = 0;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            if constexpr (T::kExponent == 0x7c00) t = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, x[e]), f16x2{}, t, false);
-            else t = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, x[e]), bf16x2{}, t, false);
-        }
-        return t != 0.0f;
+        for (int e = 0; e < 4; ++e) t |= (x[e] & ones) + one;
+        return (t & 0x80008000u) != 0;
     }
     __device__ __forceinline__ uint32_t clean() {
         uint32_t odd = 0;
