@@ -203,21 +203,34 @@ __device__ __forceinline__ void token_run(const PagedAttn &p, TokenShared<G, W> 
             }
         }
     }
-    // the wave's keys together, then the waves
+    // The wave's keys together: the rows of 16 lanes are added in two steps that halve the values a lane has, so that each row ends with a quarter of them;
+    // then the waves.
+    constexpr int N = G * EL;
+    float y[N];
 #pragma unroll
     for (int g = 0; g < G; ++g) {
         const float top = over_keys<LPK>(m[g], [](float a, float c) { return fmaxf(a, c); });
         const float f = m[g] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[g] - top);
         const float sum = over_keys<LPK>(l[g] * f, [](float a, float c) { return a + c; });
-#pragma unroll
-        for (int e = 0; e < EL; ++e) {
-            const float x = over_keys<LPK>(o[g][e] * f, [](float a, float c) { return a + c; });
-            if (own == 0) s.o[wave][g][EL * sub + e] = x;
-        }
         if (lane == 0) {
             s.m[wave][g] = top;
             s.l[wave][g] = sum;
         }
+#pragma unroll
+        for (int e = 0; e < EL; ++e) y[g * EL + e] = o[g][e] * f;
+    }
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(y[i]), __float_as_uint(y[i + N / 2]), false, false);
+        y[i] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(y[i]), __float_as_uint(y[i + N / 4]), false, false);
+        y[i] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+        if (LPK == 8) y[i] += dpp_move<0x128, 0xf>(0.0f, y[i]);  // row_ror:8
+        const int n = i + N / 4 * (lane >> 4 & 1) + N / 2 * (lane >> 5);
+        if (LPK == 16 || (lane & 8) == 0) s.o[wave][n / EL][EL * sub + n % EL] = y[i];
     }
     __syncthreads();
     auto place = [&](int r, int g) { return cut.partial + ((size_t)item * cut.most + r) * cut.part + g * (DH + 2); };
@@ -329,6 +342,7 @@ template <class T, int G, int W, int PASS>
 __global__ __launch_bounds__(64 * W) void paged_tokens_kernel(const PagedAttn p, Runs cut, float fill, int least, int listed) {
     __shared__ TokenShared<G, W> s;
     __shared__ Units list;
+    __shared__ int owners[kListed], ends[kListed], kvs[kListed];
     const int lane = threadIdx.x & 63, heads_all = p.n_heads / p.n_kv, blocks = (heads_all + G - 1) / G;  // (G is the power of two that covers them, up to 8)
     const int per_token = p.n_kv * blocks;
     int all = p.tokens * per_token * cut.most;
@@ -351,7 +365,12 @@ __global__ __launch_bounds__(64 * W) void paged_tokens_kernel(const PagedAttn p,
                     }
                     b = lo;
                 }
-                units[j] = b < p.batch ? max(keys_seen(p, p.kv_lens[b], 1), 1) : 0;
+                if (b < p.batch) {
+                    owners[row] = b;
+                    ends[row] = p.query_start ? p.query_start[b + 1] : row + 1;
+                    kvs[row] = p.kv_lens[b];
+                    units[j] = max(keys_seen(p, kvs[row], 1), 1);
+                }
             }
             work += (float)units[j];
             longest = max(longest, units[j]);
@@ -363,21 +382,26 @@ __global__ __launch_bounds__(64 * W) void paged_tokens_kernel(const PagedAttn p,
     }
     for (int unit = blockIdx.x; unit < all; unit += gridDim.x) {
         __syncthreads();  // the numbers, and what the last unit left
-        int at = unit, t, run, hb;
+        int at = unit, t, run, hb, b, kv_len, end;
         if (listed) {
             t = list.entry(at, lane);
             run = at / per_token;
             hb = at - run * per_token;
+            b = owners[t];
+            kv_len = kvs[t];
+            end = ends[t];
         } else {
             run = at % cut.most;
             at /= cut.most;
             t = at / per_token;
             hb = at - t * per_token;
+            b = request_of(p.query_start, p.batch, t, lane);
+            if (b >= p.batch) continue;
+            kv_len = p.kv_lens[b];
+            end = p.query_start ? p.query_start[b + 1] : t + 1;
         }
-        const int h = hb / blocks, g0 = (hb - h * blocks) * G, b = request_of(p.query_start, p.batch, t, lane);
-        if (b >= p.batch) continue;
-        const int end = p.query_start ? p.query_start[b + 1] : t + 1;
-        token_run<T, G, W, PASS>(p, s, cut, t, b, p.kv_lens[b], end, h, h * heads_all + g0, min(G, heads_all - g0), run, t * per_token + hb);
+        const int h = hb / blocks, g0 = (hb - h * blocks) * G;
+        token_run<T, G, W, PASS>(p, s, cut, t, b, kv_len, end, h, h * heads_all + g0, min(G, heads_all - g0), run, t * per_token + hb);
     }
 }
 
@@ -942,7 +966,7 @@ int32_t tokens_go(agpu_ctx *ctx, const PagedAttn &p, int64_t longest) {
     const int most = paged::most_runs(items, longest, few || listed ? least : 1024, part * sizeof(float), ctx->ws_bytes / 2, ctx->n_counters - 1);
     const Runs cut = {few ? least : 1024, most, reinterpret_cast<float *>(ctx->workspace), part, ctx->counters};
     hipLaunchKernelGGL((paged_tokens_kernel<T, G, 4, 4>), dim3((unsigned)std::min<int64_t>(items * most, places)), dim3(256), 0, ctx->stream, p, cut,
-                       4.0f * ctx->num_cus, least, (int)listed);
+                       2.0f * ctx->num_cus, least, (int)listed);
     return AGPU_LAUNCH_CHECK(ctx, "paged_tokens_kernel");
 }
 template <class T, int G>
