@@ -370,6 +370,61 @@ def test_a_cache_beyond_32_bits(agpu, dev):
     check(got, *attend64(q, kc[ids], vc[ids], np.vectorize(lambda p: small.get(p, -1))(tables), lens, start))
 
 
+@pytest.mark.parametrize("type_", ["float32", "bfloat16"])
+@pytest.mark.parametrize("heads,kv_heads", [(2, 2), (6, 1)])
+@pytest.mark.parametrize("kind", ["tokens", "tokens of a few requests", "mixed"])
+def test_more_requests_than_are_numbered(agpu, dev, type_, heads, kv_heads, kind):
+    """Hundreds of requests, whose work a workgroup no longer counts before it begins."""
+    import torch
+    from async_gpu_amd import ops
+    rng, g = np.random.default_rng(heads), torch.Generator(device=dev).manual_seed(1)
+    B, page = 311, 16
+    lens = rng.integers(0, 90, B)
+    lens[[5, 200]] = 2500, 1300
+    if kind == "tokens":
+        new = np.ones(B, int)
+    elif kind == "tokens of a few requests":
+        new = (rng.random(B) < 0.9).astype(int)
+    else:
+        new = np.minimum(rng.choice([0, 1, 1, 3, 9, 60, 140], B), lens)
+        new[5] = 290
+    lens = np.maximum(lens, new)
+    pages = int((-(-lens // page)).sum()) + 1
+    kc, vc = _cache(torch, g, dev, pages, kv_heads, page, type_)
+    tables, start = _tables(rng, lens.tolist(), page, pages), np.concatenate([[0], np.cumsum(new)]).tolist()
+    i32 = lambda x: torch.tensor(np.asarray(x), dtype=torch.int32, device=dev)  # noqa: E731
+    q = torch.randn((start[-1] + 3, heads, 64), generator=g, device=dev)
+    for window, sinks in ((0, 0), (30, 2)):
+        out = torch.full_like(q, 7.0)
+        ops.paged_attention(q, kc, vc, i32(tables), i32(lens), i32(start), window, sinks, out=out)
+        check(out[:start[-1]], *attend64(q[:start[-1]], kc, vc, tables, lens.tolist(), start, window, sinks))
+        assert (out[start[-1]:] == 7.0).all()
+
+
+@pytest.mark.parametrize("type_", TYPES)
+def test_little_scratch(agpu, dev, type_):
+    """With a scratch of 1 MiB rows are cut into fewer runs; the results are as good."""
+    import torch
+    from async_gpu_amd import ops
+    rng, g = np.random.default_rng(5), torch.Generator(device=dev).manual_seed(2)
+    lens, new = [3000, 2100, 1700, 40, 1200], [1, 300, 5, 40, 140]
+    kc, vc = _cache(torch, g, dev, 600, 4, 16, type_)
+    tables, start = _tables(rng, lens, 16, 600), np.concatenate([[0], np.cumsum(new)]).tolist()
+    q = torch.randn((start[-1], 8, 64), generator=g, device=dev)
+    i32 = lambda x: torch.tensor(np.asarray(x), dtype=torch.int32, device=dev)  # noqa: E731
+    args = (kc, vc, i32(tables), i32(lens))
+    small = torch.empty(1 << 20, dtype=torch.uint8, device=dev)
+    c = ops.context(0)
+    c.call("agpu_ctx_set_workspace", small.data_ptr(), small.numel())
+    try:
+        rows, tokens = ops.paged_attention(q, *args, i32(start)), ops.paged_attention(q[:5], *args)
+        torch.cuda.synchronize()
+    finally:
+        c.call("agpu_ctx_set_workspace", None, 0)
+    check(rows, *attend64(q, kc, vc, tables, lens, start))
+    check(tokens, *attend64(q[:5], kc, vc, tables, lens, [0, 1, 2, 3, 4, 5]))
+
+
 def test_hand_over_of_runs_under_the_memory_model(agpu, dev):
     """With fences around the tickets the results are the same bits, and tickets are left as they were found."""
     import torch

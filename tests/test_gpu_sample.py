@@ -158,3 +158,76 @@ def test_odd_addresses(agpu, dev):
         t = torch.empty(3 * 9001 + off, device=dev)[off:].view(3, 9001)
         t.copy_(torch.tensor(x))
         assert ops.sample(t, torch.tensor(u, device=dev), 1.0, 0, 0.9).tolist() == draw64(x, u, 1.0, 0, 0.9, 0.0)
+
+
+@pytest.mark.parametrize("case", ["a little later", "much later", "masked first", "nan first", "infinite later", "lowest first", "steps", "16 bits"])
+@pytest.mark.parametrize("n", [9001, 70001])
+def test_where_the_largest_lies(agpu, dev, case, n):
+    """Largest logits far behind the row's first few thousand, by less and by more than the sums of weights have room for, and steps of many octaves."""
+    rng = np.random.default_rng(n)
+    rows = 5
+    x = _logits(rng, rows, n)
+    if case == "a little later":
+        x[:, n - 700:] += 6
+    elif case == "much later":
+        x[:, 8000] += 300
+        x[::2, n - 5:] += 301
+    elif case == "masked first":
+        x[:, :8500] = -np.inf
+    elif case == "nan first":
+        x[:, :8500] = np.nan
+        x[0, 8700:] = np.nan
+    elif case == "infinite later":
+        x[:, 8600] = np.inf
+        x[1, 8700] = np.inf
+        x[2, :8192] = -np.inf
+    elif case == "lowest first":
+        x[:, :8500] = np.finfo(np.float32).min
+    elif case == "steps":
+        x = (-rng.integers(0, 60, (rows, n)) * 0.5 * np.log(2)).astype(np.float32)
+    elif case == "16 bits":
+        x = (x.view(np.uint32) & 0xffff0000).view(np.float32)
+    for settings in SETTINGS + [(0.01, 0, 1.0, 0.0), (1.0, 300, 0.9, 0.01)]:
+        for u in (rng.random(rows).astype(np.float32), np.full(rows, 1 - 2.0**-24, np.float32)):
+            assert _draw(dev, x, u, *settings) == draw64(x, u, *settings), settings
+
+
+@pytest.mark.parametrize("ties", [False, True])
+@pytest.mark.parametrize("k", [2, 63, 64, 255, 256, 257, 511, 512, 513, 1023])
+def test_top_k_at_the_ends_of_its_ways(agpu, dev, k, ties):
+    rng = np.random.default_rng(k)
+    for n in (k, k + 1, 1024, 5000):
+        if n < k:
+            continue
+        x = _logits(rng, 3, n)
+        if ties:
+            x = np.round(x)
+        u = np.array([0.0, 0.5, 1 - 2.0**-24], np.float32)
+        for p, m in ((1.0, 0.0), (0.9, 0.0), (1.0, 0.01)):
+            assert _draw(dev, x, u, 1.2, k, p, m) == draw64(x, u, 1.2, k, p, m), (n, p, m)
+
+
+def test_draws_of_a_graph_and_of_two_streams(agpu, dev):
+    import torch
+    from async_gpu_amd import ops
+    rng = np.random.default_rng(12)
+    rows, n = 40, 30011
+    settings = [(0.8, 40, 1.0, 0.0), (1.0, 0, 0.9, 0.01)]
+    x, u = torch.zeros((rows, n), device=dev), torch.zeros(rows, device=dev)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        for s in settings:
+            ops.sample(x, u, *s)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        made = [ops.sample(x, u, *s) for s in settings]
+    for _ in range(4):
+        x.copy_(torch.tensor(_logits(rng, rows, n)))
+        u.copy_(torch.tensor(rng.random(rows).astype(np.float32)))
+        torch.cuda.synchronize()
+        graph.replay()
+        here = [ops.sample(x, u, *s) for s in settings]
+        torch.cuda.synchronize()
+        want = [draw64(x.cpu().numpy(), u.cpu().numpy(), *s) for s in settings]
+        assert [m.tolist() for m in made] == want and [m.tolist() for m in here] == want
