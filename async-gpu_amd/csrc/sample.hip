@@ -8,8 +8,8 @@
 // of 50257 logits would go wrong about once in a thousand draws.)
 //
 // sample_rows_kernel, a workgroup a row, one launch, no scratch:
-//   general   One pass over the row adds up the weights in bins of 1/32 of an octave, each in units of its bin's middle (a polynomial of degree five is then exact to
-//             3e-15), so that the largest logit need not be known before: 64 octaves fit, and the first 4096 elements say where they lie.  Which bin an element
+//   general   One pass over the row adds up the weights in bins of 1/32 of an octave, each in units of its bin's middle (a polynomial of degree four is then exact to
+//             8e-14), so that the largest logit need not be known before: 64 octaves fit, and the first 4096 elements say where they lie.  Which bin an element
 //             went to stays in LDS.  From the bins' running sums follows in which bins the filters' borders lie, between which sums Z then is, and in which
 //             bins the drawn rank can be: only what is in those, a few hundred elements, is gathered, put in order by counting, and searched.
 //   top_k up to 256   The top_k-th largest of the threads' maxima is a bound that hardly more than top_k elements reach: the list is those.
@@ -69,7 +69,7 @@ struct Scale {
     __device__ __forceinline__ void set(double at, double temperature, int bits) {
         per = SM_OCTAVE * 1.4426950408889634 / temperature;
         origin = at;
-        one = (double)(1ull << bits);
+        one = __builtin_bit_cast(double, 1ull << bits);  // 2^(bits - 1074)
         const double least = at - 48 * SM_OCTAVE / per, most = at + 15 * SM_OCTAVE / per;  // to the inside, whose ends a number may lie hundreds of octaves off
         low = (float)least;
         high = (float)most;
@@ -78,16 +78,20 @@ struct Scale {
     }
     __device__ __forceinline__ bool counts(float x) const { return x >= low && x <= high; }
     static constexpr double kWhole = 0x1.8p52;  // added to it, a number's low bits are the whole number next to it
+    // a b + c with c in scalar registers, where it stays (left to itself the compiler copies it into the result first)
+    static __device__ __forceinline__ double fma_of(double a, double b, double c) {
+        asm("v_fma_f64 %0, %1, %2, %3" : "=v"(a) : "v"(a), "v"(b), "s"(c));
+        return a;
+    }
     __device__ __forceinline__ int bin(float x, u64 &weight) const {
+        const double fourth = 9.172562701824643e-09;
         const double d = (double)x - origin, v = fma(d, per, kWhole), f = fma(d, per, kWhole - v);
-        // (ln 2 / 32)^k / k!; the next term is below 3e-15
-        double y = 3.9737099845494154e-11;
-        y = fma(y, f, 9.172562701824643e-09);
-        y = fma(y, f, 1.6938509724371819e-06);
-        y = fma(y, f, 2.3459619820224677e-04);
-        y = fma(y, f, 2.166084939249829e-02);
+        // 2^(f / 32) for |f| <= 1/2: the series to the fifth power, that one through the fifth Chebyshev polynomial as the first and the third
+        double y = fma_of(f, fourth, 1.6938633902808830e-06);
+        y = fma_of(y, f, 2.3459619820224677e-04);
+        y = fma_of(y, f, 2.1660849391722176e-02);
         y = fma(y, f, 1.0);
-        weight = __builtin_bit_cast(u64, fma(y, one, 0x1p52)) & ((1ull << 52) - 1);  // to the nearest whole number
+        weight = __builtin_bit_cast(u64, y * one);  // a denormal number, whose bits are the whole number that it was rounded to
         return (int)(uint32_t)__builtin_bit_cast(u64, v);
     }
     __device__ __forceinline__ int bin(float x) const { return (int)(uint32_t)__builtin_bit_cast(u64, fma((double)x - origin, per, kWhole)); }
@@ -104,6 +108,20 @@ __device__ __forceinline__ double units(int j) { return exp2_wide(-(double)j / S
 __device__ __forceinline__ u64 composite(float x, int i) { return (u64)order_key(x) << kIndexBits | (u64)((1 << kIndexBits) - 1 - i); }
 __device__ __forceinline__ float value_of(u64 c) { return key_value((uint32_t)(c >> kIndexBits)); }
 __device__ __forceinline__ int index_of(u64 c) { return (1 << kIndexBits) - 1 - (int)(c & ((1 << kIndexBits) - 1)); }
+
+template <int CTRL, int ROWS>
+__device__ __forceinline__ u64 moved(u64 v) {
+    return (u64)dpp_move_u32<CTRL, ROWS>(0, (uint32_t)(v >> 32)) << 32 | dpp_move_u32<CTRL, ROWS>(0, (uint32_t)v);
+}
+// Sum over the lanes up to this one: row_shr 1, 2, 4, 8, then row_bcast 15 and 31.
+__device__ __forceinline__ u64 sum_up_to(u64 v) {
+    v += moved<0x111, 0xf>(v);
+    v += moved<0x112, 0xf>(v);
+    v += moved<0x114, 0xf>(v);
+    v += moved<0x118, 0xf>(v);
+    v += moved<0x142, 0xa>(v);
+    return v + moved<0x143, 0xc>(v);
+}
 
 struct Shared {
     u64 sum[SM_BINS];
@@ -152,21 +170,24 @@ struct Row {
 struct Runs {
     static constexpr int kStep = 4 * SM_THREADS;
     const float *row;
-    int n, tid;
+    int n, tid, first;
     float4 x[SM_AHEAD];
-    __device__ __forceinline__ float4 load(int i) const {
+    static __device__ __forceinline__ float4 load(const float *row, int n, int i) {
         const int whole = n & ~3;
         return whole > 0 ? load4(row + min(i, max(whole - 4, 0))) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
     }
-    __device__ __forceinline__ Runs(const float *row, int n, int tid) : row(row), n(n), tid(tid) {
+    __device__ __forceinline__ float4 load(int i) const { return load(row, n, i); }
+    // without the first `skip` runs of each thread
+    __device__ __forceinline__ Runs(const float *row, int n, int tid, int skip = 0) : row(row), n(n), tid(tid), first(4 * tid + skip * kStep) {
+        if (skip * kStep < n)
 #pragma unroll
-        for (int a = 0; a < SM_AHEAD; ++a) x[a] = load(4 * tid + a * kStep);
+            for (int a = 0; a < SM_AHEAD; ++a) x[a] = load(first + a * kStep);
     }
     template <class F>
     __device__ __forceinline__ void each(F &&visit) {
         const int whole = n & ~3;
 #pragma unroll 1
-        for (int i = 4 * tid; i < whole; i += SM_AHEAD * kStep)
+        for (int i = first; i < whole; i += SM_AHEAD * kStep)
 #pragma unroll
             for (int a = 0; a < SM_AHEAD; ++a) {
                 if (i + a * kStep < whole) visit(i + a * kStep, x[a]);
@@ -205,7 +226,15 @@ __global__ __launch_bounds__(SM_THREADS) void sample_rows_kernel(const SampleArg
 
     // ---- the list of a small top_k ----
     if (row.top_k > 0 && row.top_k <= SM_TOP_K && row.top_k < n) {
-        Runs(logits, n, tid).each([&](int, const float4 &x) { top = fmaxf(top, max_of_run(x)); });
+        // the row's first elements stay in registers for the second look at them
+        constexpr int kHeld = 12;
+        float4 held[kHeld];
+#pragma unroll
+        for (int a = 0; a < kHeld; ++a) held[a] = Runs::load(logits, n, 4 * tid + a * Runs::kStep);
+#pragma unroll
+        for (int a = 0; a < kHeld; ++a)
+            if (4 * tid + a * Runs::kStep < (n & ~3)) top = fmaxf(top, max_of_run(held[a]));  // (no element counts for two threads)
+        Runs(logits, n, tid, kHeld).each([&](int, const float4 &x) { top = fmaxf(top, max_of_run(x)); });
         s.top[tid] = order_key(top);
         top = all_max(top);
         if (wave == 0) {  // the upper 20 bits of the top_k-th largest maximum, from the first bit on that not all share
@@ -227,14 +256,14 @@ __global__ __launch_bounds__(SM_THREADS) void sample_rows_kernel(const SampleArg
 #pragma unroll
                 for (int i = 0; i < SM_WAVES; ++i) c += __popcll(__ballot(mine[i] >= higher));
                 if (c >= row.top_k) b = higher;
-                if (c == row.top_k) break;
+                if (c >= row.top_k && c <= row.top_k + 24) break;  // (some more than needed do no harm)
             }
             if (lane == 0) s.hit[0] = (int)(b & 0xfffff000u);
         }
         __syncthreads();
         const uint32_t bound = (uint32_t)s.hit[0];
         const float floor = key_value(bound);  // (a key between two numbers', or below all of them: NaN, which nothing is below)
-        Runs(logits, n, tid).each([&](int i, const float4 &x) {
+        auto list = [&](int i, const float4 &x) {
             if (max_of_run(x) < floor) return;
             const float of[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
@@ -243,7 +272,12 @@ __global__ __launch_bounds__(SM_THREADS) void sample_rows_kernel(const SampleArg
                     const int at = atomicAdd(&s.fill, 1);
                     if (at < SM_LIST) s.list[at] = 1ull << kKeyBits | composite(of[e], i + e);
                 }
-        });
+        };
+        Runs more(logits, n, tid, kHeld);
+#pragma unroll
+        for (int a = 0; a < kHeld; ++a)
+            if (4 * tid + a * Runs::kStep < (n & ~3)) list(4 * tid + a * Runs::kStep, held[a]);
+        more.each(list);
         __syncthreads();
         listed = s.fill <= SM_LIST && top > -INFINITY && top < INFINITY;
         if (listed) scale.set(top, temperature, p.bits);
@@ -310,17 +344,8 @@ __global__ __launch_bounds__(SM_THREADS) void sample_rows_kernel(const SampleArg
             w[e] = in_units(s.sum[(q_top - j) & (SM_BINS - 1)], units(j)) + (e ? w[0] : 0);
             c[e] = s.count[(q_top - j) & (SM_BINS - 1)] + (e ? c[0] : 0);
         }
-        u64 before = w[1];
-        uint32_t count_before = c[1];
-#pragma unroll
-        for (int by = 1; by < 64; by <<= 1) {
-            const u64 o = __shfl_up(before, by, kWave);
-            const uint32_t oc = __shfl_up(count_before, by, kWave);
-            if (lane >= by) {
-                before += o;
-                count_before += oc;
-            }
-        }
+        u64 before = sum_up_to(w[1]);
+        uint32_t count_before = (uint32_t)sum_up_to(c[1]);
         if (lane == 63) {
             s.wave_sum[wave] = before;
             s.wave_count[wave] = count_before;
@@ -406,6 +431,7 @@ __global__ __launch_bounds__(SM_THREADS) void sample_rows_kernel(const SampleArg
             return o;
         };
         auto put = [&](int i) {
+            if (i >= n) return;
             const int at = atomicAdd(&s.fill, 1);
             if (at < SM_LIST) s.ranked[at] = (u64)i;
         };
@@ -413,14 +439,12 @@ __global__ __launch_bounds__(SM_THREADS) void sample_rows_kernel(const SampleArg
         for (int i = 8 * tid; i < min(n, SM_IDS); i += 8 * SM_THREADS) {
             const uint4 ids = *reinterpret_cast<const uint4 *>(&s.id[i]);
             const uint32_t of[4] = {ids.x, ids.y, ids.z, ids.w};
-            unsigned hits = 0;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const u16x2 o = outside(of[e]);
-                hits |= (o.x == 0 ? 1u : 0u) << (2 * e) | (o.y == 0 ? 2u : 0u) << (2 * e);
+                if (o.x == 0) put(i + 2 * e);
+                if (o.y == 0) put(i + 2 * e + 1);
             }
-            for (; hits != 0; hits &= hits - 1)
-                if (i + __builtin_ctz(hits) < n) put(i + __builtin_ctz(hits));
         }
 #pragma unroll 1
         for (int i = SM_IDS + tid; i < n; i += SM_THREADS) {
@@ -469,11 +493,7 @@ __global__ __launch_bounds__(SM_THREADS) void sample_rows_kernel(const SampleArg
         }
         u64 w = weight;
         if (tid < SM_LIST) {
-#pragma unroll
-            for (int by = 1; by < 64; by <<= 1) {
-                const u64 o = __shfl_up(w, by, kWave);
-                if (lane >= by) w += o;
-            }
+            w = sum_up_to(w);
             if (lane == 63) s.wave_sum[wave] = w;
         }
         __syncthreads();
