@@ -467,13 +467,13 @@ __global__ __launch_bounds__(SM_THREADS) void sample_rows_kernel(const SampleArg
     uint32_t my_rank = 0;
     float my_x = 0.0f;
     if (fits) {
-        // the place of an element is the number of elements before it, which `helpers` threads count a part of each
-        const int size = in_list > 1 ? 1 << (32 - __builtin_clz(in_list - 1)) : 1, helpers = SM_THREADS / size, which = tid & (size - 1), helper = tid / size;
-        if (which < in_list) {
+        // the place of an element is the number of elements before it, which `helpers` waves count a part of each
+        const int groups = max((in_list + 63) >> 6, 1), helpers = SM_WAVES / groups, helper = __builtin_amdgcn_readfirstlane(wave / groups), which = tid - 64 * groups * helper;
+        if (helper < helpers && which < in_list) {
             // (as the bits of positive 64-bit floats, whose order is the same: one instruction)
             const double *list = reinterpret_cast<const double *>(s.list), c = list[which];
             int before = 0;
-            const int part = (size + helpers - 1) / helpers, last = min((helper + 1) * part, in_list);
+            const int part = (in_list + helpers - 1) / helpers, last = min((helper + 1) * part, in_list);
 #pragma unroll 4
             for (int o = helper * part; o < last; ++o) before += list[o] > c ? 1 : 0;
             if (before) atomicAdd(&s.place[which], before);
