@@ -365,6 +365,7 @@ __global__ __launch_bounds__(64 * W) void paged_tokens_kernel(const PagedAttn p,
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             units[j] = 0;
+            if (64 * j >= p.tokens) continue;  // uniform
             const int row = 64 * j + lane;
             if (row < p.tokens) {
                 // the request of a row that is no request's only one: its first entry of query_start beyond the row
@@ -390,7 +391,8 @@ __global__ __launch_bounds__(64 * W) void paged_tokens_kernel(const PagedAttn p,
         }
         cut.run = paged::run_for(wave_sum(work) * per_token, fill, least, (int)wave_minmax_u32<true>((unsigned)longest), cut.most);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) units[j] = units[j] > 0 ? paged::runs_of(units[j], cut.run, cut.most).runs * per_token : 0;
+        for (int j = 0; j < 4; ++j)
+            if (64 * j < p.tokens) units[j] = units[j] > 0 ? paged::runs_of(units[j], cut.run, cut.most).runs * per_token : 0;
         all = list.number(units, p.tokens, lane);
     }
     for (int unit = blockIdx.x; unit < all; unit += gridDim.x) {
@@ -879,7 +881,7 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(const PagedAttn p, R
     };
     __shared__ __align__(16) char smem[sizeof(Shared)];
     __shared__ Units tile_list, token_list;
-    __shared__ int starts[kListed], lens[kListed], kvs[kListed];
+    __shared__ int starts[kListed], lens[kListed], kvs[kListed], runs_of_each[kListed];
     const int lane = threadIdx.x & 63, group = p.group.size;
     int tile_units = tile_places * p.n_kv * tile_cut.most, all = tile_units + p.batch * slots * p.n_kv * token_cut.most;
     if (listed) {
@@ -888,6 +890,7 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(const PagedAttn p, R
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             tiles[j] = tokens[j] = keys[j] = 0;
+            if (64 * j >= p.batch) continue;  // uniform
             if (64 * j + lane < p.batch) {
                 const int start = p.query_start[64 * j + lane], q_len = min(p.query_start[64 * j + lane + 1], p.tokens) - start, kv_len = p.kv_lens[64 * j + lane];
                 starts[64 * j + lane] = start;
@@ -908,8 +911,11 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(const PagedAttn p, R
         token_cut.run = paged::run_for(wave_sum(token_work) * p.n_kv, 2.0f * cus, 128, longest, token_cut.most);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            tiles[j] = tiles[j] > 0 ? tiles[j] * paged::runs_of(keys[j], tile_cut.run, tile_cut.most).runs * p.n_kv : 0;
-            tokens[j] = tokens[j] > 0 ? tokens[j] * paged::runs_of(keys[j], token_cut.run, token_cut.most).runs * p.n_kv : 0;
+            if (64 * j >= p.batch) continue;  // uniform
+            const int runs = paged::runs_of(keys[j], tiles[j] > 0 ? tile_cut.run : token_cut.run, tiles[j] > 0 ? tile_cut.most : token_cut.most).runs;
+            runs_of_each[64 * j + lane] = runs;
+            tiles[j] *= runs * p.n_kv;
+            tokens[j] *= runs * p.n_kv;
         }
         tile_units = tile_list.number(tiles, p.batch, lane);
         all = tile_units + token_list.number(tokens, p.batch, lane);
@@ -924,7 +930,7 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(const PagedAttn p, R
                 at = xcd * each + min(xcd, rest) + (at >> 3);
                 b = tile_list.entry(at, lane);
                 const int q_len = lens[b], n = (q_len * group + TILE_ROWS - 1) / TILE_ROWS;
-                const int runs = paged::runs_of(max(keys_seen(p, kvs[b], min(q_len, p.group.page(TILE_ROWS) + 2)), 1), tile_cut.run, tile_cut.most).runs;
+                const int runs = runs_of_each[b];
                 const int place = at / runs;
                 run = at - place * runs;
                 h = place / n;
@@ -932,7 +938,7 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(const PagedAttn p, R
             } else {
                 at -= tile_units;
                 b = token_list.entry(at, lane);
-                const int runs = paged::runs_of(max(keys_seen(p, kvs[b], 1), 1), token_cut.run, token_cut.most).runs;
+                const int runs = runs_of_each[b];
                 token = at / (runs * p.n_kv);
                 at -= token * runs * p.n_kv;
                 run = at / p.n_kv;
