@@ -13,6 +13,7 @@ struct PlanArgs {
     int *tables, *free_pages;
     int *kv_lens, *query_start, *slots, *positions, *n_free_out;
     int batch, width, stack_size, max_tokens;
+    int page_groups;  // workgroups that write pages; the others write slots and positions (one alone: both)
     PageDiv div;
 };
 
@@ -69,14 +70,15 @@ __device__ __forceinline__ int entry_of(const int *at, int n, int x) {
 // Every workgroup adds up all requests for itself (they are few, and nobody waits for anybody), then the workgroups share what there is to write.
 // Nothing is read that another one writes: table entries of pages held so far, and the stack below n_free; new pages are looked up where they
 // came from.  What bounds it: a chain of loads, sums and searches, 16 bytes a token at the largest.  8 requests 2.6 us (4.7 a call from Python, which is what
-// the host takes), 512 requests with up to 200 new tokens each 7.6.
+// the host takes), 512 requests with up to 200 new tokens each 5.9 (7.7 where every workgroup has pages and tokens).
 // EACH: requests of a thread.
 template <int EACH>
 __global__ __launch_bounds__(PLAN_THREADS) void paged_plan_kernel(const PlanArgs p) {
-    extern __shared__ int s_plan[];  // of every request: pages freed before it, pages taken before it, tokens before it
+    constexpr bool kept = EACH <= 4;  // positions so far in LDS too (16 requests a thread would be too many)
+    extern __shared__ int s_plan[];   // of every request: pages freed before it, pages taken before it, tokens before it, positions so far
     __shared__ PlanSums s_wave[PLAN_WAVES];
     __shared__ uint32_t s_used[2][PLAN_WAVES];
-    int *const s_freed = s_plan, *const s_pages = s_plan + p.batch, *const s_start = s_plan + 2 * p.batch;
+    int *const s_freed = s_plan, *const s_pages = s_plan + p.batch, *const s_start = s_plan + 2 * p.batch, *const s_cached = s_plan + 3 * p.batch;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, b0 = tid * EACH;
     int cached[EACH], fresh[EACH];
 #pragma unroll
@@ -129,6 +131,7 @@ __global__ __launch_bounds__(PLAN_THREADS) void paged_plan_kernel(const PlanArgs
     for (int e = 0; e < EACH; ++e) {
         const int b = b0 + e;
         if (b >= p.batch) break;
+        if (kept) s_cached[b] = ask[e].cached;
         s_freed[b] = (int)min(run.freed, (uint32_t)INT32_MAX);
         s_pages[b] = (int)min(run.pages, used_pages);
         s_start[b] = (int)min(run.tokens, used_tokens);
@@ -144,8 +147,11 @@ __global__ __launch_bounds__(PLAN_THREADS) void paged_plan_kernel(const PlanArgs
         *p.n_free_out = left;
     }
     __syncthreads();
-    const int at = blockIdx.x * PLAN_THREADS + tid, stride = gridDim.x * PLAN_THREADS;
-    auto positions = [&](int b) { return min(max(p.cached_lens[b], 0), p.width * p.div.size); };
+    // pages and tokens by workgroups of their own, each a chain of searches and loads, unless a single one does it all
+    const bool for_pages = (int)blockIdx.x < p.page_groups, for_tokens = !for_pages || gridDim.x == 1;
+    const int at = ((int)blockIdx.x - (for_pages ? 0 : p.page_groups)) * PLAN_THREADS + tid;
+    const int stride = (for_pages ? p.page_groups : (int)gridDim.x - p.page_groups) * PLAN_THREADS;
+    auto positions = [&](int b) { return kept ? s_cached[b] : min(max(p.cached_lens[b], 0), p.width * p.div.size); };
     auto freed_page = [&](int i) {
         const int b = entry_of(s_freed, p.batch, i);
         return p.tables[(size_t)b * p.width + (i - s_freed[b])];
@@ -154,14 +160,14 @@ __global__ __launch_bounds__(PLAN_THREADS) void paged_plan_kernel(const PlanArgs
         const int place = (int)top - 1 - i;
         return place < n_free ? p.free_pages[place] : freed_page(place - n_free);
     };
-    for (int i = at; i < max(taken, left - n_free); i += stride) {
+    for (int i = at; for_pages && i < max(taken, left - n_free); i += stride) {
         if (i < taken) {
             const int b = entry_of(s_pages, p.batch, i), have = p.div.page(positions(b) + p.div.size - 1);
             p.tables[(size_t)b * p.width + have + (i - s_pages[b])] = new_page(i);
         }
         if (i < left - n_free) p.free_pages[n_free + i] = freed_page(i);
     }
-    for (int t = at; t < p.max_tokens; t += stride) {
+    for (int t = at; for_tokens && t < p.max_tokens; t += stride) {
         int slot = -1, pos = 0;
         if (t < tokens) {
             const int b = entry_of(s_start, p.batch, t), cached = positions(b);
@@ -235,10 +241,13 @@ AGPU_EXPORT int32_t agpu_paged_plan(agpu_ctx *ctx, const int32_t *cached_lens, c
         return agpu_fail(ctx, AGPU_ERR_UNSUPPORTED, "paged_plan: the outputs do not overlap the inputs");
     agpu_on_device here(ctx);
     if (here.rc != AGPU_OK) return here.rc;
+    // as many workgroups as find a CU each; of the pages as many as the tokens could fill
+    auto groups = [](int64_t work, int most) { return (int)std::max<int64_t>(1, std::min<int64_t>((work + PLAN_THREADS - 1) / PLAN_THREADS, most)); };
+    const int page_groups = groups((int64_t)max_tokens / page_size + batch, ctx->num_cus / 4), token_groups = max_tokens <= PLAN_THREADS && page_groups == 1 ? 0 : groups(max_tokens, ctx->num_cus - page_groups);
     const PlanArgs p = {cached_lens, new_lens, n_free, block_tables, free_pages, kv_lens, query_start, slots, positions, n_free_out, batch, table_width, stack_size,
-                        max_tokens, PageDiv::of(page_size)};
-    const int wgs = std::max(1, std::min(ceil_div(std::max(max_tokens, batch), PLAN_THREADS), ctx->num_cus));
-    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(wgs), dim3(PLAN_THREADS), (3 * batch + 1) * sizeof(int), ctx->stream, p); };
+                        max_tokens, page_groups, PageDiv::of(page_size)};
+    const size_t lds = ((batch <= 4 * PLAN_THREADS ? 4 : 3) * batch + 1) * sizeof(int);
+    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(page_groups + token_groups), dim3(PLAN_THREADS), lds, ctx->stream, p); };
     static_assert(paged::kMaxRequests <= 16 * PLAN_THREADS && 3 * paged::kMaxRequests * sizeof(int) <= 65536 - 1024, "");
     if (batch <= PLAN_THREADS) go(paged_plan_kernel<1>);
     else if (batch <= 4 * PLAN_THREADS) go(paged_plan_kernel<4>);
