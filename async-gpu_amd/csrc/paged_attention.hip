@@ -724,6 +724,8 @@ __device__ __forceinline__ void tile_run(const PagedAttn &p, TileShared<T> &s, c
 #pragma unroll 1
             for (int kk = 0; kk < TILE_KEYS; ++kk) {
                 if (!(odd_k >> kk & 1)) continue;
+                int h2 = lane >> 5;
+                asm volatile("" : "+v"(h2));  // (what follows from it is worked out here, and takes no registers all along)
                 const size_t at = (size_t)s.at[0][i & 7][kk];
                 float d = 0.0f;
 #pragma unroll 1
@@ -736,11 +738,12 @@ __device__ __forceinline__ void tile_run(const PagedAttn &p, TileShared<T> &s, c
         const bool whole = there == 0xffffffffu && v0 + TILE_KEYS - 1 <= wave_pos0 - gap &&
                            (p.window == 0 || v0 > wave_pos1 - p.window - gap || v0 + TILE_KEYS <= v_first);
         if (!whole) {
+            auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1; };  // bits 0 .. n - 1
+            const uint32_t see = (there & below(v_last + 1 - v0) & (~below(v_low + 1 - v0) | below(v_first - v0))) >> (4 * h2);
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                const int kk = 8 * (r >> 2) + 4 * h2 + (r & 3), v = v0 + kk;
-                const bool see = (there >> kk & 1) && v <= v_last && (v > v_low || v < v_first);
-                x[r] = see ? x[r] : -INFINITY;
+                const uint32_t all = (uint32_t)((int)(see << (31 - 8 * (r >> 2) - (r & 3))) >> 31);
+                x[r] = __uint_as_float((all & __float_as_uint(x[r])) | (~all & 0xff800000u));
             }
         }
         float top = x[0];
@@ -786,6 +789,8 @@ __device__ __forceinline__ void tile_run(const PagedAttn &p, TileShared<T> &s, c
             for (int kk = 0; kk < TILE_KEYS; ++kk) {
                 const int v = v0 + kk;
                 if (!(odd_v >> kk & 1)) continue;
+                int h2 = lane >> 5;
+                asm volatile("" : "+v"(h2));
                 const bool see = v <= v_last && (v > v_low || v < v_first);
                 float weight = 0.0f;
 #pragma unroll
