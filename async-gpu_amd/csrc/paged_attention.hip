@@ -280,23 +280,22 @@ __device__ __forceinline__ void token_run(const PagedAttn &p, TokenShared<G, W> 
     if (p.strict) __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
     for (int g = wave; g < heads; g += W) {
         auto load = [&](int r, int i) { return __hip_atomic_load(place(r, g) + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
-        // lane r: the weight of run r (and of r + 64, ...)
-        float top = -INFINITY;
-        for (int r = lane; r < runs; r += 64) top = fmaxf(top, load(r, DH));
-        top = wave_max(top);
-        float sum = 0.0f, acc = 0.0f;
-        for (int r0 = 0; r0 < runs; r0 += 64) {
-            const float mr = r0 + lane < runs ? load(r0 + lane, DH) : -INFINITY, f = mr == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mr - top);
-            sum += wave_sum(r0 + lane < runs ? load(r0 + lane, DH + 1) * f : 0.0f);
-            const int n = min(64, runs - r0);
-            for (int r = 0; r < n; r += 8) {  // eight on their way at a time, which the compiler would take one by one
-                float x[8];
+        // lane r: the weight of run r (there are 64 at most).  All that is wanted first goes on its way together, eight runs' sums among it, which the compiler would take
+        // one by one.
+        const float mr = lane < runs ? load(lane, DH) : -INFINITY, lr = lane < runs ? load(lane, DH + 1) : 0.0f;
+        float x[8];
+        auto eight = [&](int r) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = load(r0 + min(r + e, n - 1), lane);
-                __builtin_amdgcn_sched_barrier(0);
+            for (int e = 0; e < 8; ++e) x[e] = load(min(r + e, runs - 1), lane);
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        eight(0);
+        const float top = wave_max(mr), f = mr == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mr - top), sum = wave_sum(lr * f);
+        float acc = 0.0f;
+        for (int r = 0; r < runs; r += 8) {
+            if (r > 0) eight(r);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) acc = r + e < n ? fmaf(x[e], __shfl(f, r + e, kWave), acc) : acc;
-            }
+            for (int e = 0; e < 8; ++e) acc = r + e < runs ? fmaf(x[e], __shfl(f, r + e, kWave), acc) : acc;
         }
         out[g * DH] = sum == 0.0f ? 0.0f : acc / sum;
     }
