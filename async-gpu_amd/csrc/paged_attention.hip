@@ -2,12 +2,12 @@
 //
 // Two kernels, by what the call says about its rows:
 //   tokens <= batch  paged_tokens_kernel: every row by itself on the vector units, as one does with one new token a request.  Bound by the bytes of K and V: 64
-//                    requests of 4096 keys (32 heads over 8, f16) 104 us, 5.2 TB/s; with 1 to 4018 keys (80 MB) 29 us, of which 5 are the launch and the way to the
-//                    first key.  The query heads of a K/V head (up to 8) share what is read of it.
+//                    requests of 4096 keys (32 heads over 8, f16) 105 us, 5.1 TB/s; with 1 to 4018 keys (80 MB) 28 us, of which 5 are the launch and the way to the
+//                    first key; one request of 777 keys, 12 heads, fp32, 7.0, a chain of loads.  The query heads of a K/V head (up to 8) share what is read of it.
 //   otherwise        paged_rows_kernel: requests with more than eight rows of heads a K/V head in tiles of 128 rows on the matrix cores, the others as above.  Bound by
 //                    the instructions of a tile of 32 keys (some 180 vector ones beside 24 matrix products for a 16-bit cache, 330 and 48 for an fp32 one, two waves
-//                    a SIMD): 4 chunks of 512 rows over 2048 keys, 16 heads, fp32, 104 us; 8 x 256 rows in a window of 1024, bf16, 47 us; two prompts of 300 rows
-//                    and 22 tokens, 25 heads, bf16, 26 us.
+//                    a SIMD): 4 chunks of 512 rows over 2048 keys, 16 heads, fp32, 101 us; 8 x 256 rows in a window of 1024, bf16, 44 us; two prompts of 300 rows
+//                    and 22 tokens, 25 heads, bf16, 25 us.
 // The softmax goes along the keys in one pass: maximum m, sum l and sum o of weights 2^(s - m), taken again in units of a new maximum where there is one.  Keys are
 // cut into runs over workgroups, whose (o, m, l) the last one to finish joins (write-through stores, a ticket; the order of the sum is that of the runs, so that
 // results do not depend on who is last).  What has to be known for that, the lengths, is on the device only: a grid of fixed size numbers the runs for itself.
@@ -577,8 +577,8 @@ __device__ __forceinline__ float sum_of_halves(float v) {
 }
 
 // Up to 128 rows of a request (its tokens' heads of one K/V head, token by token) over a run of the keys that any of them sees, by four waves of 32 rows, which
-// share the tiles of 32 keys: what each thread has fetched goes to LDS as operands while the next tile is on its way, one barrier a tile (some 3800 cycles: 450
-// to leave an operand, 460 for the scores, 1000 for weights and products, the rest on the way between).
+// share the tiles of 32 keys: what each thread has fetched goes to LDS as operands while the next tile is on its way, one barrier a tile (3200 cycles for a
+// 16-bit cache, 4900 for an fp32 one).
 // first_row: of the rows of the request and K/V head.
 template <class T>
 __device__ __forceinline__ void tile_run(const PagedAttn &p, TileShared<T> &s, const Runs &cut, int b, int start, int q_len, int kv_len, int h, int first_row, int run, int item) {

@@ -69,8 +69,8 @@ __device__ __forceinline__ int entry_of(const int *at, int n, int x) {
 
 // Every workgroup adds up all requests for itself (they are few, and nobody waits for anybody), then the workgroups share what there is to write.
 // Nothing is read that another one writes: table entries of pages held so far, and the stack below n_free; new pages are looked up where they
-// came from.  What bounds it: a chain of loads, sums and searches, 16 bytes a token at the largest.  8 requests 2.6 us (4.7 a call from Python, which is what
-// the host takes), 512 requests with up to 200 new tokens each 5.9 (7.7 where every workgroup has pages and tokens).
+// came from.  What bounds it: a chain of loads, sums and searches, 16 bytes a token at the largest.  8 requests 2.8 us (4.9 a call from Python, which is what
+// the host takes), 512 requests with up to 200 new tokens each 5.8 (7.7 where every workgroup has pages and tokens).
 // EACH: requests of a thread.
 template <int EACH>
 __global__ __launch_bounds__(PLAN_THREADS) void paged_plan_kernel(const PlanArgs p) {

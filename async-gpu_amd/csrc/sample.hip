@@ -7,7 +7,7 @@
 // one at 50257 logits, from an exponential in 64-bit floats (off by 8e-14 of itself), and their sums are exact in any order.  (With fp32 exponentials a row
 // of 50257 logits would go wrong about once in a thousand draws.)
 //
-// sample_rows_kernel, a workgroup a row, one launch, no scratch (50257 logits: top 40 of 1 row 12.9 us, 32 rows of all kinds 32, the nucleus of 256 rows 33, of
+// sample_rows_kernel, a workgroup a row, one launch, no scratch (50257 logits: top 40 of 1 row 13 us, 32 rows of all kinds 32, the nucleus of 256 rows 33, of
 // which the read of 51 MB is 11).  Bound by the instructions of the one pass, some 22 a weight of which 9 in 64 bits (12 us with its loads), then by a chain of sums,
 // searches and barriers (10 us).  Several workgroups a row and three launches were 22, 32 and 70 us.
 //   general   One pass over the row adds up the weights in bins of 1/32 of an octave, each in units of its bin's middle (a polynomial of degree four is then exact to
