@@ -7,7 +7,7 @@
 // one at 50257 logits, from an exponential in 64-bit floats (off by 8e-14 of itself), and their sums are exact in any order.  (With fp32 exponentials a row
 // of 50257 logits would go wrong about once in a thousand draws.)
 //
-// sample_rows_kernel, a workgroup a row, one launch, no scratch (50257 logits: top 40 of 1 row 13 us, 32 rows of all kinds 32, the nucleus of 256 rows 33, of
+// sample_rows_kernel, a workgroup a row, one launch, no scratch (50257 logits: top 40 of 1 row 13 us, 32 rows of all kinds 32, the nucleus of 256 rows 35, of
 // which the read of 51 MB is 11).  Bound by the instructions of the one pass, some 22 a weight of which 9 in 64 bits (12 us with its loads), then by a chain of sums,
 // searches and barriers (10 us).  Several workgroups a row and three launches were 22, 32 and 70 us.
 //   general   One pass over the row adds up the weights in bins of 1/32 of an octave, each in units of its bin's middle (a polynomial of degree four is then exact to
@@ -16,7 +16,8 @@
 //             bins the drawn rank can be: only what is in those, a few hundred elements, is gathered, put in order by counting, and searched.
 //   top_k up to 256   The top_k-th largest of the threads' maxima is a bound that hardly more than top_k elements reach: the list is those.
 // When the bins hold more than the list (thousands of equal logits, a large temperature), each border is looked for by itself, in the elements of
-// its bin cut into 512 by the bits of (value, index), which are never the same twice, until a piece fits.
+// its bin cut into 512 by the first bits in which their (value, index), which are never the same twice, differ, until a piece fits: three passes over the row for each border as a rule (64 rows at
+// temperature 5 with a nucleus of 0.9 142 us, rows of equal logits 180 to 300).
 #include "agpu_internal.h"
 #include "sampling.h"
 
@@ -28,8 +29,9 @@ typedef unsigned long long u64;
 
 constexpr int SM_THREADS = 1024, SM_WAVES = SM_THREADS / 64;
 constexpr int SM_BINS = 2048, SM_OCTAVE = 32;  // bins, and how many an octave has
-constexpr int SM_LIST = 512, SM_TOP_K = 256;
-constexpr int SM_IDS = 57344;  // elements whose bins LDS has room for
+constexpr int SM_LIST = 1024, SM_TOP_K = 256;  // (an element a thread)
+constexpr int SM_PIECES = 512, SM_PIECE = 256;  // of a bin that does not fit: into how many it is cut, and what a piece may have
+constexpr int SM_IDS = 56832;  // elements whose bins LDS has room for
 constexpr int SM_AHEAD = 4;    // runs of four elements that a thread has on their way at a time
 constexpr int kIndexBits = 20, kKeyBits = 52;  // n <= 2^20; of a value and its index
 constexpr int kIdShift = 5;  // an element's bin is kept as that many bits further up, where 16 bits wrap as the bins do
@@ -129,9 +131,9 @@ struct Shared {
     u64 sum[SM_BINS];
     uint32_t count[SM_BINS];
     uint16_t id[SM_IDS];
-    u64 list[SM_LIST], ranked[SM_LIST], prefix[SM_LIST];
+    u64 list[SM_LIST], ranked[SM_LIST];  // elements in any order, and in that of the ranking; then list: running sums
     int place[SM_LIST];
-    u64 wave_sum[SM_WAVES], answer_sum, kept_of_min_p, piece_sum;
+    u64 wave_sum[SM_WAVES], answer_sum, kept_of_min_p, piece_sum, least, most;
     uint32_t wave_count[SM_WAVES], answer_index, piece_count;
     float wave_top[SM_WAVES];
     uint32_t top[SM_THREADS];
@@ -433,7 +435,7 @@ __global__ __launch_bounds__(SM_THREADS) void sample_rows_kernel(const SampleArg
             return o;
         };
         auto put = [&](int i) {
-            if (i >= n) return;
+            if (i >= n || *(volatile int *)&s.fill > SM_LIST) return;  // (no more of them when they do not fit anyway)
             const int at = atomicAdd(&s.fill, 1);
             if (at < SM_LIST) s.ranked[at] = (u64)i;
         };
@@ -463,26 +465,36 @@ __global__ __launch_bounds__(SM_THREADS) void sample_rows_kernel(const SampleArg
     }
 
     // ---- the list in order ----
+    auto in_order = [&](int count) {  // list -> ranked
+        // the place of an element is the number of elements before it, which `helpers` waves count a part of each
+        const int groups = max((count + 63) >> 6, 1), helpers = SM_WAVES / groups, helper = __builtin_amdgcn_readfirstlane(wave / groups), which = tid - 64 * groups * helper;
+        if (helper < helpers && which < count) {
+            // (as the bits of positive 64-bit floats, whose order is the same: one instruction)
+            const double *list = reinterpret_cast<const double *>(s.list), c = list[which];
+            int before = 0;
+            const int part = (count + helpers - 1) / helpers, last = min((helper + 1) * part, count);
+#pragma unroll 4
+            for (int o = helper * part; o < last; ++o) before += list[o] > c ? 1 : 0;
+            if (before) atomicAdd(&s.place[which], before);
+        }
+        __syncthreads();
+        if (tid < count) s.ranked[s.place[tid]] = s.list[tid];
+        __syncthreads();
+    };
+    auto scanned = [&](u64 w) {  // the sum over the threads up to this one
+        w = sum_up_to(w);
+        if (lane == 63) s.wave_sum[wave] = w;
+        __syncthreads();
+        for (int v = 0; v < wave; ++v) w += s.wave_sum[v];
+        return w;
+    };
     const int in_list = min(s.fill, SM_LIST);
     const bool fits = s.fill <= SM_LIST;
     u64 mine = 0, my_before = 0, my_run = 0;  // of the list's rank tid: the running sums without it and with it
     uint32_t my_rank = 0;
     float my_x = 0.0f;
     if (fits) {
-        // the place of an element is the number of elements before it, which `helpers` waves count a part of each
-        const int groups = max((in_list + 63) >> 6, 1), helpers = SM_WAVES / groups, helper = __builtin_amdgcn_readfirstlane(wave / groups), which = tid - 64 * groups * helper;
-        if (helper < helpers && which < in_list) {
-            // (as the bits of positive 64-bit floats, whose order is the same: one instruction)
-            const double *list = reinterpret_cast<const double *>(s.list), c = list[which];
-            int before = 0;
-            const int part = (in_list + helpers - 1) / helpers, last = min((helper + 1) * part, in_list);
-#pragma unroll 4
-            for (int o = helper * part; o < last; ++o) before += list[o] > c ? 1 : 0;
-            if (before) atomicAdd(&s.place[which], before);
-        }
-        __syncthreads();
-        if (tid < in_list) s.ranked[s.place[tid]] = s.list[tid];
-        __syncthreads();
+        in_order(in_list);
         u64 weight = 0;
         int j = 0;
         if (tid < in_list) {
@@ -493,16 +505,8 @@ __global__ __launch_bounds__(SM_THREADS) void sample_rows_kernel(const SampleArg
                 if (listed) weight = in_units(weight, units(j));  // one by one; otherwise by bins
             }
         }
-        u64 w = weight;
-        if (tid < SM_LIST) {
-            w = sum_up_to(w);
-            if (lane == 63) s.wave_sum[wave] = w;
-        }
-        __syncthreads();
-        if (tid < SM_LIST) {
-            for (int v = 0; v < wave; ++v) w += s.wave_sum[v];
-            s.prefix[tid] = w;
-        }
+        const u64 w = scanned(weight);
+        s.list[tid] = w;
         __syncthreads();
         if (tid < in_list) {
             if (listed) {
@@ -514,7 +518,7 @@ __global__ __launch_bounds__(SM_THREADS) void sample_rows_kernel(const SampleArg
                 for (int step = SM_LIST / 2; step > 0; step >>= 1)
                     if (begin - step >= 0 && s.ranked[begin - step] >> kKeyBits == mine >> kKeyBits) begin -= step;
                 const double by = units(j);
-                const u64 in_bin = w - (begin > 0 ? s.prefix[begin - 1] : 0);
+                const u64 in_bin = w - (begin > 0 ? s.list[begin - 1] : 0);
                 my_run = sum_before(j) + in_units(in_bin, by);
                 my_before = sum_before(j) + in_units(in_bin - weight, by);
                 my_rank = count_before(j) + (uint32_t)(tid - begin);
@@ -522,8 +526,31 @@ __global__ __launch_bounds__(SM_THREADS) void sample_rows_kernel(const SampleArg
         }
     }
 
+    // What is in bins first .. last, read from the row again: visit(index, value, bin)
+    auto for_bins = [&](int tid, int first, int last, auto &&visit) {
+        const int whole = n & ~3;
+        float4 next = Runs::load(logits, n, 4 * tid);
+#pragma unroll 1
+        for (int i = 4 * tid; i < n; i += Runs::kStep) {
+            float4 run = next;
+            next = Runs::load(logits, n, i + Runs::kStep);
+            if (i >= whole) {
+                const float nan = __builtin_nanf("");
+                run = make_float4(logits[i], i + 1 < n ? logits[i + 1] : nan, i + 2 < n ? logits[i + 2] : nan, nan);
+            }
+            const float of[4] = {run.x, run.y, run.z, run.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float x = value(of[e]);
+                if (!scale.counts(x)) continue;
+                const int j = q_top - scale.bin(x);
+                if (j >= first && j <= last) visit(i + e, x, j);
+            }
+        }
+    };
+
     // ---- top_k, top_p of its sum, min_p, the draw ----
-    u64 kept = listed ? s.prefix[max(in_list - 1, 0)] : s.sum[SM_BINS - 1];
+    u64 kept = listed ? s.list[max(in_list - 1, 0)] : s.sum[SM_BINS - 1];
 #pragma unroll 1
     for (int stage = 0; stage < 4; ++stage) {
         if (!(stage == 0 ? by_k : stage == 1 ? row.by_p : stage == 2 ? by_m : true)) continue;  // uniform
@@ -534,17 +561,18 @@ __global__ __launch_bounds__(SM_THREADS) void sample_rows_kernel(const SampleArg
             if (fits) {
                 if (tid < in_list && min_p_keeps(my_x)) atomicMax(&s.kept_of_min_p, my_run);
             } else {
-                for (int j = m_first; j <= m_last; ++j) {  // the weights of the bin that are kept
-                    __syncthreads();
-                    if (tid == 0) s.piece_sum = 0;
-                    __syncthreads();
-                    for (int i = tid; i < n; i += SM_THREADS) {
-                        const float x = value(logits[i]);
-                        if (scale.counts(x) && scale.bin(x) == q_top - j && min_p_keeps(x)) atomicAdd(&s.piece_sum, scale.weight(x));
-                    }
-                    __syncthreads();
-                    if (tid == 0 && s.piece_sum > 0) s.kept_of_min_p = sum_before(j) + in_units(s.piece_sum, units(j));
-                }
+                // the weights that are kept in each of these bins (two at most)
+                if (tid < SM_PIECES) s.list[tid] = 0;
+                __syncthreads();
+                int me = tid;
+                asm volatile("" : "+v"(me));  // (what follows from it is worked out here, and takes no registers all along)
+                for_bins(me, m_first, m_last, [&](int, float x, int j) {
+                    if (min_p_keeps(x)) atomicAdd(&s.list[min(j - m_first, SM_PIECES - 1)], scale.weight(x));
+                });
+                __syncthreads();
+                if (tid == 0)
+                    for (int j = m_first; j <= min(m_last, m_first + SM_PIECES - 1); ++j)
+                        if (s.list[j - m_first] > 0) s.kept_of_min_p = sum_before(j) + in_units(s.list[j - m_first], units(j));
             }
             __syncthreads();
             kept = min(kept, s.kept_of_min_p);
@@ -562,75 +590,77 @@ __global__ __launch_bounds__(SM_THREADS) void sample_rows_kernel(const SampleArg
             const double by = units(j);
             const u64 base = sum_before(j);
             const uint32_t rank0 = count_before(j);
-            // the pieces of the bin: elements whose composite's bits from `known` on are `prefix`; before them in the bin lie sum0 and count0
-            u64 prefix = 0, sum0 = 0;
-            uint32_t count0 = 0, size = SM_LIST + 1;
-            int known = kKeyBits;
+            // A piece of the bin: composites from `low` to `high`; before it in the bin lie sum0 and count0.  It is cut by the first nine bits in which its own differ.
+            int me = tid;
+            asm volatile("" : "+v"(me));
+            u64 low = 0, high = ~0ull, sum0 = 0;
+            uint32_t count0 = 0;
+            int size, shift;
             auto for_piece = [&](auto &&visit) {
-                for (int i = tid; i < n; i += SM_THREADS) {
-                    if (i < SM_IDS && s.id[i] != (uint16_t)((uint32_t)(q_top - j) << kIdShift)) continue;
-                    const float x = value(logits[i]);
-                    if (!scale.counts(x) || scale.bin(x) != q_top - j) continue;
+                for_bins(me, j, j, [&](int i, float x, int) {
                     const u64 c = composite(x, i);
-                    if (c >> known == prefix) visit(c, x);
-                }
+                    if (c >= low && c <= high) visit(c, x);
+                });
             };
-            while (size > SM_LIST && known > 0) {
-                const int shift = max(known - 9, 0);
+            do {
                 __syncthreads();
-                if (tid < SM_LIST) {
-                    s.prefix[tid] = 0;
+                if (tid < SM_PIECES) {
+                    s.list[tid] = 0;
                     s.place[tid] = 0;
                 }
+                if (tid == 0) {
+                    s.least = ~0ull;
+                    s.most = 0;
+                }
                 __syncthreads();
+                u64 least = ~0ull, most = 0;
+                for_piece([&](u64 c, float) {
+                    least = min(least, c);
+                    most = max(most, c);
+                });
+                if (least <= most) {
+                    atomicMin(&s.least, least);
+                    atomicMax(&s.most, most);
+                }
+                __syncthreads();
+                least = s.least;
+                const int bit = 63 - __builtin_clzll((least ^ s.most) | 1ull);
+                shift = max(bit - 8, 0);
+                const u64 mask = (2ull << (bit - shift)) - 1, common = least >> shift & ~mask;
                 for_piece([&](u64 c, float x) {
-                    const int d = SM_LIST - 1 - (int)((c >> shift) & ((1ull << (known - shift)) - 1));
-                    atomicAdd(&s.prefix[d], scale.weight(x));
+                    const int d = SM_PIECES - 1 - (int)(c >> shift & mask);
+                    atomicAdd(&s.list[d], scale.weight(x));
                     atomicAdd(&s.place[d], 1);
                 });
                 __syncthreads();
-                if (tid == 0) {  // (rare, and 512 steps)
-                    u64 sum = sum0;
-                    uint32_t count = count0;
-                    for (int d = 0; d < SM_LIST; ++d) {
-                        const u64 next = sum + s.prefix[d];
-                        const uint32_t more = count + (uint32_t)s.place[d];
-                        if (to.within(base + in_units(sum, by), rank0 + count, base + in_units(next, by), rank0 + more)) {
-                            s.piece = d;
-                            s.piece_sum = sum;
-                            s.piece_count = count;
-                            break;
-                        }
-                        sum = next;
-                        count = more;
-                    }
+                const u64 mine = tid < SM_PIECES ? s.list[tid] : 0;
+                const uint32_t count = tid < SM_PIECES ? (uint32_t)s.place[tid] : 0;
+                const u64 upto = sum0 + scanned(mine);
+                __syncthreads();
+                const uint32_t counted = count0 + (uint32_t)scanned(count);
+                if (count > 0 && to.within(base + in_units(upto - mine, by), rank0 + counted - count, base + in_units(upto, by), rank0 + counted)) {
+                    s.piece = tid;
+                    s.piece_sum = upto - mine;
+                    s.piece_count = counted - count;
                 }
                 __syncthreads();
-                size = (uint32_t)s.place[s.piece];
+                size = s.place[s.piece];
                 sum0 = s.piece_sum;
                 count0 = s.piece_count;
-                prefix = prefix << (known - shift) | (u64)(SM_LIST - 1 - s.piece);
-                known = shift;
-            }
+                low = (common | (u64)(SM_PIECES - 1 - s.piece)) << shift;
+                high = low + ((1ull << shift) - 1);
+            } while (size > SM_PIECE && shift > 0);
             __syncthreads();
-            if (tid == 0) s.piece = 0;
+            if (tid == 0) s.fill = 0;
+            s.place[tid] = 0;
             __syncthreads();
-            for_piece([&](u64 c, float) { s.list[min(atomicAdd(&s.piece, 1), SM_LIST - 1)] = c; });
+            for_piece([&](u64 c, float) { s.list[min(atomicAdd(&s.fill, 1), SM_LIST - 1)] = 1ull << kKeyBits | c; });
             __syncthreads();
-            if (tid < (int)size) {
-                const u64 c = s.list[tid];
-                u64 sum = sum0;
-                uint32_t rank = count0;
-                for (int o = 0; o < (int)size; ++o)
-                    if (s.list[o] > c) {
-                        sum += scale.weight(value_of(s.list[o]));
-                        ++rank;
-                    }
-                const u64 with = sum + scale.weight(value_of(c));
-                if (to.within(base + in_units(sum, by), rank0 + rank, base + in_units(with, by), rank0 + rank + 1)) {
-                    s.answer_index = (uint32_t)index_of(c);
-                    s.answer_sum = base + in_units(with, by);
-                }
+            in_order(size);
+            const u64 c = tid < size ? s.ranked[tid] : 0, weight = tid < size ? scale.weight(value_of(c)) : 0, with = sum0 + scanned(weight);
+            if (tid < size && to.within(base + in_units(with - weight, by), rank0 + count0 + (uint32_t)tid, base + in_units(with, by), rank0 + count0 + (uint32_t)tid + 1)) {
+                s.answer_index = (uint32_t)index_of(c);
+                s.answer_sum = base + in_units(with, by);
             }
         }
         __syncthreads();
