@@ -231,3 +231,15 @@ def test_draws_of_a_graph_and_of_two_streams(agpu, dev):
         torch.cuda.synchronize()
         want = [draw64(x.cpu().numpy(), u.cpu().numpy(), *s) for s in settings]
         assert [m.tolist() for m in made] == want and [m.tolist() for m in here] == want
+
+
+@pytest.mark.parametrize("n", [5000, 50257, 60001])
+@pytest.mark.parametrize("temperature", [2.0, 5.0, 20.0])
+def test_borders_among_many(agpu, dev, n, temperature):
+    """Borders in bins of hundreds to thousands of candidates, some of them equal, more than one list holds."""
+    rng = np.random.default_rng(n)
+    x = _logits(rng, 4, n)
+    x[2:] = (x[2:].view(np.uint32) & 0xfff00000).view(np.float32)
+    for k, p, m in ((0, 0.9, 0.0), (0, 1.0, 0.0), (n // 2, 0.8, 0.0), (n // 3, 1.0, 0.02), (0, 0.97, 0.1)):
+        u = rng.random(4).astype(np.float32)
+        assert _draw(dev, x, u, temperature, k, p, m) == draw64(x, u, temperature, k, p, m), (k, p, m)
