@@ -7,7 +7,8 @@
 //   otherwise        paged_rows_kernel: requests with more than eight rows of heads a K/V head in tiles of 128 rows on the matrix cores, the others as above.  Bound by
 //                    the instructions of a tile of 32 keys (some 180 vector ones beside 24 matrix products for a 16-bit cache, 330 and 48 for an fp32 one, two waves
 //                    a SIMD): 4 chunks of 512 rows over 2048 keys, 16 heads, fp32, 101 us; 8 x 256 rows in a window of 1024, bf16, 44 us; two prompts of 300 rows
-//                    and 22 tokens, 25 heads, bf16, 25 us.
+//                    and 22 tokens, 25 heads, bf16, 24 us; a prompt of 2048 rows from the first on, 16 heads, fp32, 88 us, of 8192, bf16, 450 (644 where every workgroup
+//                    goes through its tiles in the same order).
 // The softmax goes along the keys in one pass: maximum m, sum l and sum o of weights 2^(s - m), taken again in units of a new maximum where there is one.  Keys are
 // cut into runs over workgroups, whose (o, m, l) the last one to finish joins (write-through stores, a ticket; the order of the sum is that of the runs, so that
 // results do not depend on who is last).  What has to be known for that, the lengths, is on the device only: a grid of fixed size numbers the runs for itself.
@@ -889,16 +890,16 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(const PagedAttn p, R
     const int lane = threadIdx.x & 63, group = p.group.size;
     int tile_units = tile_places * p.n_kv * tile_cut.most, all = tile_units + p.batch * slots * p.n_kv * token_cut.most;
     if (listed) {
-        int tiles[4], tokens[4], keys[4], longest = 0;
-        float tile_work = 0.0f, token_work = 0.0f;
+        int tiles[4], tokens[4], keys[4], rows[4], longest = 0;
+        float tile_most = 0.0f, tile_work = 0.0f, token_work = 0.0f;  // (a prompt's tiles see one more than the other: the longest, and on average)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            tiles[j] = tokens[j] = keys[j] = 0;
+            tiles[j] = tokens[j] = keys[j] = rows[j] = 0;
             if (64 * j >= p.batch) continue;  // uniform
             if (64 * j + lane < p.batch) {
                 const int start = p.query_start[64 * j + lane], q_len = min(p.query_start[64 * j + lane + 1], p.tokens) - start, kv_len = p.kv_lens[64 * j + lane];
                 starts[64 * j + lane] = start;
-                lens[64 * j + lane] = q_len;
+                lens[64 * j + lane] = rows[j] = q_len;
                 kvs[64 * j + lane] = kv_len;
                 if (start >= 0 && q_len > 0) {
                     keys[j] = max(keys_seen(p, kv_len, q_len > slots ? min(q_len, p.group.page(TILE_ROWS) + 2) : 1), 1);
@@ -906,12 +907,29 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(const PagedAttn p, R
                     else tokens[j] = q_len;
                 }
             }
-            tile_work += (float)tiles[j] * (float)keys[j];
+            tile_most += (float)tiles[j] * (float)keys[j];
+            tile_work += (float)tiles[j] * ((float)keys[j] - (p.window > 0 ? 0.0f : 0.5f * (float)min(rows[j], keys[j])));
             token_work += (float)tokens[j] * (float)keys[j];
             longest = max(longest, keys[j]);
         }
         longest = (int)wave_minmax_u32<true>((unsigned)longest);
-        tile_cut.run = paged::run_for(wave_sum(tile_work) * p.n_kv, 2.0f * cus, 256, longest, tile_cut.most);
+        // Runs for tiles as long as the longest, or as on average, which makes more of them: what takes less time, if that is the length of a run where all of them find a
+        // place at once, and that of the average otherwise, and what a run takes besides (2048 rows from the first on, 16 heads, fp32: 124 us with the longest, 88; 3 x
+        // 700 rows behind 300, 12 heads: 51 with the longest, 68).
+        tile_work = wave_sum(tile_work) * p.n_kv;
+        const float places = 2.0f * cus;
+        auto time_of = [&](int run) {
+            float units = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (64 * j < p.batch && tiles[j] > 0) units += (float)(tiles[j] * paged::runs_of(keys[j], run, tile_cut.most).runs);
+            units = fmaxf(wave_sum(units) * p.n_kv, 1.0f);
+            const float rounds = __builtin_ceilf(units / places);
+            return rounds > 1.0f ? rounds * (tile_work / units + 192.0f) : (float)run + 192.0f;
+        };
+        const int by_longest = paged::run_for(wave_sum(tile_most) * p.n_kv, places, 256, longest, tile_cut.most);
+        const int by_average = paged::run_for(tile_work, places, 256, longest, tile_cut.most);
+        tile_cut.run = by_average != by_longest && time_of(by_average) < time_of(by_longest) ? by_average : by_longest;
         token_cut.run = paged::run_for(wave_sum(token_work) * p.n_kv, 2.0f * cus, 128, longest, token_cut.most);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -924,7 +942,11 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(const PagedAttn p, R
         tile_units = tile_list.number(tiles, p.batch, lane);
         all = tile_units + token_list.number(tokens, p.batch, lane);
     }
-    for (int unit = blockIdx.x; unit < all; unit += gridDim.x) {
+    // Every second time in the opposite order, XCD by XCD: tiles come the longest first, so that who had the longest then has the shortest.
+    for (int round = 0; round < (all + (int)gridDim.x - 1) / (int)gridDim.x; ++round) {
+        const int turned = (int)gridDim.x - 8 - ((int)blockIdx.x & ~7) + ((int)blockIdx.x & 7);
+        const int unit = round * (int)gridDim.x + ((round & 1) && gridDim.x % 8 == 0 ? turned : (int)blockIdx.x);
+        if (unit >= all) continue;
         __syncthreads();  // the numbers, and what the last unit left
         int at = unit, b, h, run, tile = -1, token = -1;
         if (listed) {

@@ -401,6 +401,24 @@ def test_more_requests_than_are_numbered(agpu, dev, type_, heads, kv_heads, kind
         assert (out[start[-1]:] == 7.0).all()
 
 
+@pytest.mark.parametrize("type_", ["float32", "float16"])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (260, 3)])
+def test_more_tiles_than_find_a_place_at_once(agpu, dev, type_, window, sinks):
+    """Prompts of so many rows that a workgroup takes several tiles, the second time in the opposite order."""
+    import torch
+    from async_gpu_amd import ops
+    rng, g = np.random.default_rng(21), torch.Generator(device=dev).manual_seed(21)
+    lens, new, heads, page = [1100, 1400, 30, 900, 1], [1100, 900, 2, 300, 1], 24, 16
+    kc, vc = _cache(torch, g, dev, 230, heads, page, type_)
+    tables, start = _tables(rng, lens, page, 230), np.concatenate([[0], np.cumsum(new)]).tolist()
+    q = torch.randn((start[-1], heads, 64), generator=g, device=dev)
+    i32 = lambda x: torch.tensor(np.asarray(x), dtype=torch.int32, device=dev)  # noqa: E731
+    args = (q, kc, vc, i32(tables), i32(lens), i32(start), window, sinks)
+    got = ops.paged_attention(*args)
+    check(got, *attend64(q, kc, vc, tables, lens, start, window, sinks))
+    assert all(torch.equal(got, ops.paged_attention(*args)) for _ in range(3))
+
+
 @pytest.mark.parametrize("type_", TYPES)
 def test_little_scratch(agpu, dev, type_):
     """With a scratch of 1 MiB rows are cut into fewer runs; the results are as good."""
