@@ -50,6 +50,30 @@ AGPU_HD Visible visible(int pos, int kv_len, int held, int window, int sinks) {
     return {first, first + rest, low - first};
 }
 
+// The keys that rows at the positions pos0 .. pos1 see together, numbered without a gap: number v is key v for the v of the first tokens that stay visible
+// (`first`), and key v + gap behind them.  Windows may be as large as 32 bits go, and rows may lie before position 0: compared before subtracted.
+struct TileKeys {
+    int first, count, gap;
+    AGPU_HD int key(int v) const { return v < first ? v : v + gap; }
+};
+AGPU_HD TileKeys tile_keys(int pos0, int pos1, int held, int window, int sinks) {
+    int end = pos1 < held ? pos1 + 1 : held;
+    end = end > 0 ? end : 0;
+    const int low = window > 0 && pos0 >= window ? pos0 - window + 1 : 0;
+    int first = sinks < low ? sinks : low;
+    first = first < end ? first : end;
+    return {first, first + (end > low ? end - low : 0), low - first};
+}
+// Which of these numbers the row at `pos` sees.
+struct RowKeys {
+    int last, low, first;
+    AGPU_HD bool sees(int v) const { return v <= last && (v > low || v < first); }
+};
+AGPU_HD RowKeys row_keys(const TileKeys &tile, int pos, int window, int sinks) {
+    const int stay = sinks - tile.gap;
+    return {pos - tile.gap, window > 0 && pos >= window ? pos - window - tile.gap : -1, window > 0 && stay > tile.first ? stay : tile.first};
+}
+
 // `count` keys over workgroups: about as many runs as there are `run` keys in them, `most` at most, of `keys` each (a multiple of 32; the last ones may be
 // empty).  More keys never make fewer runs.
 struct RunsOf {

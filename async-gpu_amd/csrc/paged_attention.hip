@@ -589,21 +589,20 @@ __device__ __forceinline__ void tile_run(const PagedAttn &p, TileShared<T> &s, c
     const int group = p.group.size, rows = q_len * group, last_row = min(first_row + TILE_ROWS, rows) - 1;
     // all keys that a row of the tile sees, numbered without a gap
     const int pos0 = kv_len - q_len + p.group.page(first_row), pos1 = kv_len - q_len + p.group.page(last_row);
-    int end = min(min(pos1 + 1, kv_len), p.held);
-    end = max(end, 0);
-    int low = p.window > 0 ? max(pos0 + 1 - p.window, 0) : 0;
-    const int first = min(min(p.sinks, low), end), gap = low - first, count = first + max(end - low, 0);
-    const paged::RunsOf cuts = paged::runs_of(count, cut.run, cut.most);
+    const paged::TileKeys keys = paged::tile_keys(pos0, pos1, p.held, p.window, p.sinks);
+    const int gap = keys.gap;
+    const paged::RunsOf cuts = paged::runs_of(keys.count, cut.run, cut.most);
     const int runs = cuts.runs;
     if (run >= runs) return;
-    const int lo = run * cuts.keys, hi = min(count, lo + cuts.keys);
+    const int lo = run * cuts.keys, hi = min(keys.count, lo + cuts.keys);
     // this lane's row; rows behind the last one repeat it
     const int row = min(first_row + 32 * wave + c, last_row), token = p.group.page(row), head = h * group + (row - token * group);
     const bool mine = first_row + 32 * wave + c <= last_row, any = first_row + 32 * wave <= last_row;
     const int pos = kv_len - q_len + token;
     const int wave_pos0 = kv_len - q_len + p.group.page(min(first_row + 32 * wave, last_row)), wave_pos1 = kv_len - q_len + p.group.page(min(first_row + 32 * wave + 31, last_row));
-    // key number v is seen if v <= v_last and (v > v_low or v < v_first)
-    const int v_last = pos - gap, v_low = p.window > 0 ? pos - p.window - gap : -1, v_first = p.window > 0 ? max(first, p.sinks - gap) : 0;
+    // which keys the row sees, and below which of those that are no sinks its wave's last row sees none
+    const paged::RowKeys see = paged::row_keys(keys, pos, p.window, p.sinks);
+    const int wave_low = paged::row_keys(keys, wave_pos1, p.window, p.sinks).low;
 
     // keys of tile i are lo + 32 i ..; their places are looked up for four tiles at a time, one a wave, long before they are fetched
     const int tiles = (hi - lo + TILE_KEYS - 1) / TILE_KEYS;
@@ -614,7 +613,7 @@ __device__ __forceinline__ void tile_run(const PagedAttn &p, TileShared<T> &s, c
         id = -1;
         off = 0;
         if (v < hi) {
-            const int j = v < first ? v : v + gap, page = p.div.page(j);
+            const int j = keys.key(v), page = p.div.page(j);
             id = table[page];
             off = j - page * p.div.size;
         }
@@ -705,7 +704,7 @@ __device__ __forceinline__ void tile_run(const PagedAttn &p, TileShared<T> &s, c
             look_up(i + 8 + wave);
         }
         const int v0 = lo + TILE_KEYS * i;
-        if (!any || (v0 >= first && v0 > wave_pos1 - gap)) continue;  // (the next tile goes to the other buffer)
+        if (!any || (v0 >= keys.first && v0 > wave_pos1 - gap)) continue;  // (the next tile goes to the other buffer)
         floatx16 x = {};
 #pragma unroll
         for (int level = QP - 1; level >= 0; --level)
@@ -736,13 +735,13 @@ __device__ __forceinline__ void tile_run(const PagedAttn &p, TileShared<T> &s, c
             }
         // only tiles at the ends of what rows see hide anything (uniform over the wave)
         const bool whole = there == 0xffffffffu && v0 + TILE_KEYS - 1 <= wave_pos0 - gap &&
-                           (p.window == 0 || v0 > wave_pos1 - p.window - gap || v0 + TILE_KEYS <= v_first);
+                           (v0 > wave_low || v0 + TILE_KEYS <= see.first);
         if (!whole) {
             auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1; };  // bits 0 .. n - 1
-            const uint32_t see = (there & below(v_last + 1 - v0) & (~below(v_low + 1 - v0) | below(v_first - v0))) >> (4 * h2);
+            const uint32_t seen = (there & below(see.last + 1 - v0) & (~below(see.low + 1 - v0) | below(see.first - v0))) >> (4 * h2);
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                const uint32_t all = (uint32_t)((int)(see << (31 - 8 * (r >> 2) - (r & 3))) >> 31);
+                const uint32_t all = (uint32_t)((int)(seen << (31 - 8 * (r >> 2) - (r & 3))) >> 31);
                 x[r] = __uint_as_float((all & __float_as_uint(x[r])) | (~all & 0xff800000u));
             }
         }
@@ -791,7 +790,7 @@ __device__ __forceinline__ void tile_run(const PagedAttn &p, TileShared<T> &s, c
                 if (!(odd_v >> kk & 1)) continue;
                 int h2 = lane >> 5;
                 asm volatile("" : "+v"(h2));
-                const bool see = v <= v_last && (v > v_low || v < v_first);
+                const bool in_sight = see.sees(v);
                 float weight = 0.0f;
 #pragma unroll
                 for (int r = 0; r < 16; ++r) weight = 8 * (r >> 2) + 4 * h2 + (r & 3) == kk ? x[r] : weight;
@@ -802,7 +801,7 @@ __device__ __forceinline__ void tile_run(const PagedAttn &p, TileShared<T> &s, c
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
                         const float y = T::one(vb + at, 32 * db + 8 * (r >> 2) + 4 * h2 + (r & 3));
-                        o[db][r] += see && !(fabsf(y) < INFINITY) ? weight * y : 0.0f;
+                        o[db][r] += in_sight && !(fabsf(y) < INFINITY) ? weight * y : 0.0f;
                     }
             }
     }

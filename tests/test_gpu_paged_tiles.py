@@ -1,0 +1,38 @@
+"""paged_attention where tiles of rows and single rows could differ: windows at the end of 32 bits, magnitudes far from one, rows of nobody at either end of the
+calls, and many heads a K/V head in many requests."""
+import numpy as np
+import pytest
+from test_gpu_paged import TYPES, _cache, _tables, attend64, check
+
+pytestmark = pytest.mark.gpu
+
+
+def _i32(dev):
+    import torch
+    return lambda x: torch.tensor(np.asarray(x), dtype=torch.int32, device=dev)
+
+
+def _call(dev, q, kc, vc, tables, lens, start, window=0, sinks=0, **kw):
+    from async_gpu_amd import ops
+    i32 = _i32(dev)
+    return ops.paged_attention(q, kc, vc, i32(tables), i32(lens), i32(start), window, sinks, **kw)
+
+
+@pytest.mark.parametrize("type_", TYPES)
+@pytest.mark.parametrize("window", [2**31 - 1, 2**31 - 12, 2**31 - 30, 2**30])
+@pytest.mark.parametrize("sinks", [0, 3, 2**31 - 1])
+def test_windows_as_large_as_numbers_go(agpu, dev, type_, window, sinks):
+    """Requests with fewer positions than rows, whose first rows lie before position 0 and see nothing, under a window that hides nothing."""
+    import torch
+    lens, new = [5, 33, 1, 0, 200], [12, 40, 30, 20, 200]
+    rng, g = np.random.default_rng(2), torch.Generator(device=dev).manual_seed(3)
+    kc, vc = _cache(torch, g, dev, 40, 2, 16, type_)
+    tables, start = _tables(rng, lens, 16, 40), np.concatenate([[0], np.cumsum(new)]).tolist()
+    q = torch.randn((start[-1], 4, 64), generator=g, device=dev)
+    got = _call(dev, q, kc, vc, tables, lens, start, window, sinks)
+    check(got, *attend64(q, kc, vc, tables, lens, start, window, sinks))
+    assert torch.equal(got, _call(dev, q, kc, vc, tables, lens, start))
+    # the same rows one by one
+    for b in (0, 1):
+        one = _call(dev, q[start[b]:start[b] + 2], kc, vc, tables[[b, b]], [lens[b] - new[b] + 1, 0], [0, 1, 1], window, sinks)
+        check(one[:1], *(x[:1] for x in attend64(q[start[b]:start[b] + 2], kc, vc, tables[[b, b]], [lens[b] - new[b] + 1, 0], [0, 1, 1], window, sinks)))
