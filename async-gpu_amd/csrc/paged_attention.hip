@@ -59,7 +59,7 @@ struct F32 {
 };
 struct BF16 {
     static constexpr int EL = 8;
-    static constexpr uint32_t kExponent = 0x7f80;
+    static constexpr uint32_t kExponent = 0x7f80, kOdd = 217 << 7;  // the exponents' bits; those from which on an element is odd: 2^90
     static __device__ __forceinline__ float one(const void *p, size_t i) { return __uint_as_float((uint32_t)static_cast<const unsigned short *>(p)[i] << 16); }
     static __device__ __forceinline__ void floats(const uint4 &x, float (&f)[8]) {
         const uint32_t w[4] = {x.x, x.y, x.z, x.w};
@@ -72,7 +72,7 @@ struct BF16 {
 };
 struct F16 {
     static constexpr int EL = 8;
-    static constexpr uint32_t kExponent = 0x7c00;
+    static constexpr uint32_t kExponent = 0x7c00, kOdd = 0x7c00;
     static __device__ __forceinline__ float one(const void *p, size_t i) { return (float)static_cast<const _Float16 *>(p)[i]; }
     static __device__ __forceinline__ void floats(const uint4 &x, float (&f)[8]) {
         const uint32_t w[4] = {x.x, x.y, x.z, x.w};
@@ -496,13 +496,13 @@ struct Staged<F32> {
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] = 0.0f;
     }
-    __device__ __forceinline__ bool odd() const {  // one of them is infinite or no number
+    __device__ __forceinline__ bool odd() const {  // one of them is infinite, no number, or larger than 2^91 (none of them, if all are below 2^87)
         float t = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) t = fmaf(x[e], 0.0f, t);
-        return t != 0.0f;
+        for (int e = 0; e < 8; ++e) t = fmaf(x[e], 0x1p38f, t);
+        return !(fabsf(t) < INFINITY);
     }
-    // Zeros in place of those; which there were.
+    // Zeros in place of what is infinite or no number; which they were.
     __device__ __forceinline__ uint32_t clean() {
         uint32_t odd = 0;
 #pragma unroll
@@ -528,11 +528,11 @@ struct Staged16 {
         x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
     }
     __device__ __forceinline__ void clear() { x[0] = x[1] = x[2] = x[3] = 0; }
-    __device__ __forceinline__ bool odd() const {  // an exponent of ones and one more is the sign bit
-        constexpr uint32_t ones = T::kExponent * 0x10001u, one = (T::kExponent & (0u - T::kExponent)) * 0x10001u;
+    __device__ __forceinline__ bool odd() const {  // with what is left up to the sign bit added, an exponent from kOdd on reaches it
+        constexpr uint32_t ones = T::kExponent * 0x10001u, rest = (0x8000u - T::kOdd) * 0x10001u;
         uint32_t t = 0;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) t |= (x[e] & ones) + one;
+        for (int e = 0; e < 4; ++e) t |= (x[e] & ones) + rest;
         return (t & 0x80008000u) != 0;
     }
     __device__ __forceinline__ uint32_t clean() {
@@ -557,7 +557,7 @@ struct TileShared {
     uint4 k[2][Tiles<T>::KP][kFrag], v[2][Tiles<T>::KP][kFrag];  // [buffer][piece]: K [d step of 16][half][key], V [key][dimension], what tile_v_at says
     long long at[2][8][TILE_KEYS];  // of the keys of eight tiles: where their rows of K and of V begin, in bytes (0 for those that are not there)
     uint32_t seen[8];               // which of them are there
-    uint32_t odd_k[8], odd_v[8];    // of which something is infinite or not a number
+    uint32_t odd_k[8], odd_v[8];    // of which something is infinite or not a number, or of V so large that weights above one could take it beyond the largest number
     unsigned int ticket;
 };
 
@@ -693,7 +693,8 @@ __device__ __forceinline__ void tile_run(const PagedAttn &p, TileShared<T> &s, c
         }
         if (__builtin_expect(__any(sk.odd() || sv.odd()), 0)) {
             if (sk.clean()) atomicOr(&s.odd_k[i & 7], 1u << c);
-            if (sv.clean()) atomicOr(&s.odd_v[i & 7], 1u << c);
+            if (sv.odd()) atomicOr(&s.odd_v[i & 7], 1u << c);
+            sv.clean();
         }
         sk.store(&s.k[buf][0][(2 * wave + h2) * 32 + c]);
         sv.store(&s.v[buf][0][v_at / 16]);
@@ -749,7 +750,10 @@ __device__ __forceinline__ void tile_run(const PagedAttn &p, TileShared<T> &s, c
 #pragma unroll
         for (int r = 1; r < 16; ++r) top = fmaxf(top, x[r]);
         top = max_of_halves(top);
-        if (__any(top > m + 6.0f)) {  // weights may grow to 2^6 before everything is rescaled
+        // Weights may grow to 2^6 before everything is rescaled, but not beside values from 2^91 on: those go in with weights of one at most, as they do row by
+        // row, so that their sums are finite where |v| times the keys is below 2^128.  (Sums of 2^30 smaller ones are finite anyway, and f16 values are small.)
+        const float slack = std::is_same_v<T, F16> || odd_v == 0 ? 6.0f : 0.0f;
+        if (__any(top > m + slack)) {
             const float now = fmaxf(m, top), a = now == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - now);
             m = now;
             l *= a;

@@ -36,3 +36,26 @@ def test_windows_as_large_as_numbers_go(agpu, dev, type_, window, sinks):
     for b in (0, 1):
         one = _call(dev, q[start[b]:start[b] + 2], kc, vc, tables[[b, b]], [lens[b] - new[b] + 1, 0], [0, 1, 1], window, sinks)
         check(one[:1], *(x[:1] for x in attend64(q[start[b]:start[b] + 2], kc, vc, tables[[b, b]], [lens[b] - new[b] + 1, 0], [0, 1, 1], window, sinks)))
+
+
+@pytest.mark.parametrize("type_", ["float32", "bfloat16"])
+@pytest.mark.parametrize("large", [1e36, 1e37, 3e37])
+@pytest.mark.parametrize("step", [5.9, 3.0, -5.9])
+def test_large_values_behind_rising_scores(agpu, dev, type_, large, step):
+    """Scores that rise by a little less than 6 octaves from tile to tile of 32 keys, and values whose sums with weights of one stay finite."""
+    import torch
+    kv, rows, page = 192 + 40, 40, 16
+    kc, vc = (torch.zeros((15, 1, page, 64), dtype=getattr(torch, type_), device=dev) for _ in range(2))
+    tables = np.arange(15, dtype=np.int32)[None]
+    flat_k, flat_v = kc.view(-1, 64), vc.view(-1, 64)
+    for t in range(6):
+        flat_k[32 * t:32 * t + 32, 0] = step * t / 1.4426950408889634
+        flat_v[32 * t:32 * t + 32, 1] = 0.5
+        flat_v[32 * t + 3:32 * t + 6, 0] = large
+        flat_v[32 * t + 7, 2:4] = -large
+    q = torch.zeros((rows, 2, 64), device=dev)
+    q[:, :, 0] = 8.0
+    want, tol = attend64(q, kc, vc, tables, [kv], [0, rows])
+    assert torch.isfinite(want).all() and want.abs().max() > large / 50
+    check(_call(dev, q, kc, vc, tables, [kv], [0, rows]), want, tol)
+    check(_call(dev, q[:1], kc, vc, tables, [kv - rows + 1], [0, 1]), want[:1], tol[:1])
