@@ -737,9 +737,12 @@ __device__ __forceinline__ void tile_run(const PagedAttn &p, TileShared<T> &s, c
         // only tiles at the ends of what rows see hide anything (uniform over the wave)
         const bool whole = there == 0xffffffffu && v0 + TILE_KEYS - 1 <= wave_pos0 - gap &&
                            (v0 > wave_low || v0 + TILE_KEYS <= see.first);
-        if (!whole) {
+        auto in_sight = [&] {  // of this row, one bit a key
             auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1; };  // bits 0 .. n - 1
-            const uint32_t seen = (there & below(see.last + 1 - v0) & (~below(see.low + 1 - v0) | below(see.first - v0))) >> (4 * h2);
+            return there & below(see.last + 1 - v0) & (~below(see.low + 1 - v0) | below(see.first - v0));
+        };
+        if (!whole) {
+            const uint32_t seen = in_sight() >> (4 * h2);
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 const uint32_t all = (uint32_t)((int)(seen << (31 - 8 * (r >> 2) - (r & 3))) >> 31);
@@ -752,9 +755,12 @@ __device__ __forceinline__ void tile_run(const PagedAttn &p, TileShared<T> &s, c
         top = max_of_halves(top);
         // Weights may grow to 2^6 before everything is rescaled, but not beside values from 2^91 on: those go in with weights of one at most, as they do row by
         // row, so that their sums are finite where |v| times the keys is below 2^128.  (Sums of 2^30 smaller ones are finite anyway, and f16 values are small.)
-        const float slack = std::is_same_v<T, F16> || odd_v == 0 ? 6.0f : 0.0f;
-        if (__any(top > m + slack)) {
-            const float now = fmaxf(m, top), a = now == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - now);
+        // Each row by what it sees itself: its bits do not depend on the others'.
+        float slack = 6.0f;
+        if (__builtin_expect(!std::is_same_v<T, F16> && odd_v != 0, 0)) slack = (odd_v & in_sight()) != 0 ? 0.0f : slack;
+        const bool rises = top > m + slack;
+        if (__any(rises)) {
+            const float now = rises ? top : m, a = now == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - now);
             m = now;
             l *= a;
 #pragma unroll
@@ -794,7 +800,7 @@ __device__ __forceinline__ void tile_run(const PagedAttn &p, TileShared<T> &s, c
                 if (!(odd_v >> kk & 1)) continue;
                 int h2 = lane >> 5;
                 asm volatile("" : "+v"(h2));
-                const bool in_sight = see.sees(v);
+                const bool sees = see.sees(v);
                 float weight = 0.0f;
 #pragma unroll
                 for (int r = 0; r < 16; ++r) weight = 8 * (r >> 2) + 4 * h2 + (r & 3) == kk ? x[r] : weight;
@@ -805,7 +811,7 @@ __device__ __forceinline__ void tile_run(const PagedAttn &p, TileShared<T> &s, c
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
                         const float y = T::one(vb + at, 32 * db + 8 * (r >> 2) + 4 * h2 + (r & 3));
-                        o[db][r] += in_sight && !(fabsf(y) < INFINITY) ? weight * y : 0.0f;
+                        o[db][r] += sees && !(fabsf(y) < INFINITY) ? weight * y : 0.0f;
                     }
             }
     }

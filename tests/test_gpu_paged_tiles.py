@@ -59,3 +59,34 @@ def test_large_values_behind_rising_scores(agpu, dev, type_, large, step):
     assert torch.isfinite(want).all() and want.abs().max() > large / 50
     check(_call(dev, q, kc, vc, tables, [kv], [0, rows]), want, tol)
     check(_call(dev, q[:1], kc, vc, tables, [kv - rows + 1], [0, 1]), want[:1], tol[:1])
+
+
+@pytest.mark.parametrize("type_", TYPES)
+@pytest.mark.parametrize("what", ["scores", "infinite scores", "nan", "values", "infinite values"])
+def test_keys_of_later_rows_change_no_bits(agpu, dev, type_, what):
+    """Rows of a tile share the keys that are fetched for them; what only later ones see leaves the bits of the earlier ones as they are."""
+    import torch
+    lens, new, heads, page = [500, 130], [200, 130], 2, 16
+    rng, g = np.random.default_rng(3), torch.Generator(device=dev).manual_seed(11)
+    kc, vc = _cache(torch, g, dev, 42, heads, page, type_)
+    tables, start = _tables(rng, lens, page, 42), np.concatenate([[0], np.cumsum(new)]).tolist()
+    q = torch.randn((start[-1], heads, 64), generator=g, device=dev).abs()
+    want = _call(dev, q, kc, vc, tables, lens, start)
+    for b, from_ in ((0, 340), (0, 417), (1, 77)):
+        k, v = kc.clone(), vc.clone()
+        for p in range(from_, lens[b]):
+            at = (tables[b, p // page], slice(None), p % page)
+            if what == "values":
+                v[at] = 60000.0 if type_ == "float16" else 1e36
+            elif what == "infinite values":
+                v[at] = float("inf")
+            else:
+                k[at] = {"scores": 4.0, "infinite scores": float("inf"), "nan": float("nan")}[what]
+        got = _call(dev, q, k, v, tables, lens, start)
+        first = start[b] + from_ - (lens[b] - new[b])
+        others = torch.ones(start[-1], dtype=torch.bool)
+        others[first:start[b + 1]] = False
+        assert torch.equal(got[others], want[others])
+        assert not (got[first:start[b + 1]] == want[first:start[b + 1]]).all()
+        if what in ("scores", "values"):
+            check(got, *attend64(q, k, v, tables, lens, start))
