@@ -103,13 +103,13 @@ __device__ __forceinline__ float over_keys(float v, F op) {
     return op(__uint_as_float(s[0]), __uint_as_float(s[1]));
 }
 
-// The request that token t belongs to (uniform; `batch`: behind the last one).
+// The request that token t belongs to (uniform; `batch`: behind the last one, or before the first).
 __device__ __forceinline__ int request_of(const int *query_start, int batch, int t, int lane) {
     if (!query_start) return t;
     if (t < batch && query_start[t] == t && query_start[t + 1] == t + 1) return t;  // one token each so far, as a rule
     int b = 0;
     for (int i = 0; i < batch; i += 64) b += __popcll(__ballot(i + lane < batch && query_start[i + lane + 1] <= t));
-    return b;
+    return t < query_start[0] ? batch : b;
 }
 
 // What a workgroup of W waves needs in LDS for a token's G query heads.
@@ -377,7 +377,7 @@ __global__ __launch_bounds__(64 * W) void paged_tokens_kernel(const PagedAttn p,
                         if (p.query_start[mid + 1] <= row) lo = mid + 1;
                         else hi = mid;
                     }
-                    b = lo;
+                    b = row < p.query_start[0] ? p.batch : lo;
                 }
                 if (b < p.batch) {
                     owners[row] = b;

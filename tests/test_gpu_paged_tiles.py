@@ -90,3 +90,28 @@ def test_keys_of_later_rows_change_no_bits(agpu, dev, type_, what):
         assert not (got[first:start[b + 1]] == want[first:start[b + 1]]).all()
         if what in ("scores", "values"):
             check(got, *attend64(q, k, v, tables, lens, start))
+
+
+@pytest.mark.parametrize("type_", ["float32", "float16"])
+@pytest.mark.parametrize("batch", [3, 300])
+@pytest.mark.parametrize("kind", ["tokens", "chunks"])
+def test_rows_before_the_first_request(agpu, dev, type_, batch, kind):
+    """query_start may begin behind row 0: the rows before it are nobody's and stay as they were, like those behind the last request's."""
+    import torch
+    rng, g = np.random.default_rng(batch), torch.Generator(device=dev).manual_seed(7)
+    new = np.ones(batch, int) if kind == "tokens" else np.where(np.arange(batch) % 7 == 2, 40, 1)
+    if kind == "tokens":
+        new[batch // 2:] = 0  # room for rows of nobody in a call of as many rows as requests
+    lens = rng.integers(40, 90, batch)
+    first, behind = 1, 0 if kind == "tokens" else 2
+    start = (first + np.concatenate([[0], np.cumsum(new)])).tolist()
+    pages = int((-(-lens // 16)).sum())
+    kc, vc = _cache(torch, g, dev, pages, 2, 16, type_)
+    tables = _tables(rng, lens.tolist(), 16, pages)
+    q = torch.randn((start[-1] + behind, 2, 64), generator=g, device=dev)
+    assert (len(q) <= batch) == (kind == "tokens")
+    out = torch.full_like(q, 7.0)
+    _call(dev, q, kc, vc, tables, lens, start, out=out)
+    want, tol = attend64(q, kc, vc, tables, lens.tolist(), start)
+    check(out, want, tol)
+    assert (out[:first] == 7.0).all() and (out[start[-1]:] == 7.0).all()
