@@ -120,13 +120,13 @@ struct TokenShared {
 };
 
 // Up to G query heads of a token that share a K/V head over a run of its keys, by 64 W threads.  LPK lanes share a key, 16 bytes each.
-// h: K/V head, head0: first of the query heads, heads: how many; end: the row behind the request's last; item: place among the partial results.
+// pos: the token's position in request b; h: K/V head, head0: first of the query heads, heads: how many; item: place among the partial results.
 template <class T, int G, int W, int PASS>
-__device__ __forceinline__ void token_run(const PagedAttn &p, TokenShared<G, W> &s, const Runs &cut, int t, int b, int kv_len, int end, int h, int head0, int heads, int run, int item) {
+__device__ __forceinline__ void token_run(const PagedAttn &p, TokenShared<G, W> &s, const Runs &cut, int t, int b, int pos, int h, int head0, int heads, int run, int item) {
     constexpr int EL = T::EL, LPK = DH / EL, KEYS = 64 / LPK;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int sub = lane % LPK, own = lane / LPK;
-    const Visible vis = paged::visible(kv_len - end + t, kv_len, p.held, p.window, p.sinks);
+    const Visible vis = paged::visible(pos, pos + 1, p.held, p.window, p.sinks);
     const paged::RunsOf cuts = paged::runs_of(vis.count, cut.run, cut.most);
     const int runs = cuts.runs;
     if (run >= runs) return;
@@ -355,7 +355,7 @@ template <class T, int G, int W, int PASS>
 __global__ __launch_bounds__(64 * W) void paged_tokens_kernel(const PagedAttn p, Runs cut, float fill, int least, int listed) {
     __shared__ TokenShared<G, W> s;
     __shared__ Units list;
-    __shared__ int owners[kListed], ends[kListed], kvs[kListed];
+    __shared__ int owners[kListed], positions[kListed];
     const int lane = threadIdx.x & 63, heads_all = p.n_heads / p.n_kv, blocks = (heads_all + G - 1) / G;  // (G is the power of two that covers them, up to 8)
     const int per_token = p.n_kv * blocks;
     int all = p.tokens * per_token * cut.most;
@@ -380,10 +380,10 @@ __global__ __launch_bounds__(64 * W) void paged_tokens_kernel(const PagedAttn p,
                     b = row < p.query_start[0] ? p.batch : lo;
                 }
                 if (b < p.batch) {
+                    const int kv_len = max(p.kv_lens[b], 0);
                     owners[row] = b;
-                    ends[row] = p.query_start ? p.query_start[b + 1] : row + 1;
-                    kvs[row] = p.kv_lens[b];
-                    units[j] = max(keys_seen(p, kvs[row], 1), 1);
+                    positions[row] = kv_len - (p.query_start ? p.query_start[b + 1] : row + 1) + row;
+                    units[j] = max(keys_seen(p, kv_len, 1), 1);
                 }
             }
             work += (float)units[j];
@@ -397,14 +397,13 @@ __global__ __launch_bounds__(64 * W) void paged_tokens_kernel(const PagedAttn p,
     }
     for (int unit = blockIdx.x; unit < all; unit += gridDim.x) {
         __syncthreads();  // the numbers, and what the last unit left
-        int at = unit, t, run, hb, b, kv_len, end;
+        int at = unit, t, run, hb, b, pos;
         if (listed) {
             t = list.entry(at, lane);
             run = at / per_token;
             hb = at - run * per_token;
             b = owners[t];
-            kv_len = kvs[t];
-            end = ends[t];
+            pos = positions[t];
         } else {
             run = at % cut.most;
             at /= cut.most;
@@ -412,11 +411,10 @@ __global__ __launch_bounds__(64 * W) void paged_tokens_kernel(const PagedAttn p,
             hb = at - t * per_token;
             b = request_of(p.query_start, p.batch, t, lane);
             if (b >= p.batch) continue;
-            kv_len = p.kv_lens[b];
-            end = p.query_start ? p.query_start[b + 1] : t + 1;
+            pos = max(p.kv_lens[b], 0) - (p.query_start ? p.query_start[b + 1] : t + 1) + t;
         }
         const int h = hb / blocks, g0 = (hb - h * blocks) * G;
-        token_run<T, G, W, PASS>(p, s, cut, t, b, kv_len, end, h, h * heads_all + g0, min(G, heads_all - g0), run, t * per_token + hb);
+        token_run<T, G, W, PASS>(p, s, cut, t, b, pos, h, h * heads_all + g0, min(G, heads_all - g0), run, t * per_token + hb);
     }
 }
 
@@ -580,15 +578,15 @@ __device__ __forceinline__ float sum_of_halves(float v) {
 // Up to 128 rows of a request (its tokens' heads of one K/V head, token by token) over a run of the keys that any of them sees, by four waves of 32 rows, which
 // share the tiles of 32 keys: what each thread has fetched goes to LDS as operands while the next tile is on its way, one barrier a tile (3200 cycles for a
 // 16-bit cache, 4900 for an fp32 one).
-// first_row: of the rows of the request and K/V head.
+// pos_first: position of the request's first row; first_row: of the rows of the request and K/V head.
 template <class T>
-__device__ __forceinline__ void tile_run(const PagedAttn &p, TileShared<T> &s, const Runs &cut, int b, int start, int q_len, int kv_len, int h, int first_row, int run, int item) {
+__device__ __forceinline__ void tile_run(const PagedAttn &p, TileShared<T> &s, const Runs &cut, int b, int start, int q_len, int pos_first, int h, int first_row, int run, int item) {
     constexpr int KP = Tiles<T>::KP, QP = Tiles<T>::QP;
     constexpr int kBytes = 16 / T::EL;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 31, h2 = lane >> 5;
     const int group = p.group.size, rows = q_len * group, last_row = min(first_row + TILE_ROWS, rows) - 1;
     // all keys that a row of the tile sees, numbered without a gap
-    const int pos0 = kv_len - q_len + p.group.page(first_row), pos1 = kv_len - q_len + p.group.page(last_row);
+    const int pos0 = pos_first + p.group.page(first_row), pos1 = pos_first + p.group.page(last_row);
     const paged::TileKeys keys = paged::tile_keys(pos0, pos1, p.held, p.window, p.sinks);
     const int gap = keys.gap;
     const paged::RunsOf cuts = paged::runs_of(keys.count, cut.run, cut.most);
@@ -598,8 +596,8 @@ __device__ __forceinline__ void tile_run(const PagedAttn &p, TileShared<T> &s, c
     // this lane's row; rows behind the last one repeat it
     const int row = min(first_row + 32 * wave + c, last_row), token = p.group.page(row), head = h * group + (row - token * group);
     const bool mine = first_row + 32 * wave + c <= last_row, any = first_row + 32 * wave <= last_row;
-    const int pos = kv_len - q_len + token;
-    const int wave_pos0 = kv_len - q_len + p.group.page(min(first_row + 32 * wave, last_row)), wave_pos1 = kv_len - q_len + p.group.page(min(first_row + 32 * wave + 31, last_row));
+    const int pos = pos_first + token;
+    const int wave_pos0 = pos_first + p.group.page(min(first_row + 32 * wave, last_row)), wave_pos1 = pos_first + p.group.page(min(first_row + 32 * wave + 31, last_row));
     // which keys the row sees, and below which of those that are no sinks its wave's last row sees none
     const paged::RowKeys see = paged::row_keys(keys, pos, p.window, p.sinks);
     const int wave_low = paged::row_keys(keys, wave_pos1, p.window, p.sinks).low;
@@ -895,7 +893,7 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(const PagedAttn p, R
     };
     __shared__ __align__(16) char smem[sizeof(Shared)];
     __shared__ Units tile_list, token_list;
-    __shared__ int starts[kListed], lens[kListed], kvs[kListed], runs_of_each[kListed];
+    __shared__ int starts[kListed], lens[kListed], positions[kListed], runs_of_each[kListed];
     const int lane = threadIdx.x & 63, group = p.group.size;
     int tile_units = tile_places * p.n_kv * tile_cut.most, all = tile_units + p.batch * slots * p.n_kv * token_cut.most;
     if (listed) {
@@ -906,10 +904,10 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(const PagedAttn p, R
             tiles[j] = tokens[j] = keys[j] = rows[j] = 0;
             if (64 * j >= p.batch) continue;  // uniform
             if (64 * j + lane < p.batch) {
-                const int start = p.query_start[64 * j + lane], q_len = min(p.query_start[64 * j + lane + 1], p.tokens) - start, kv_len = p.kv_lens[64 * j + lane];
+                const int start = p.query_start[64 * j + lane], end = p.query_start[64 * j + lane + 1], q_len = min(end, p.tokens) - start, kv_len = max(p.kv_lens[64 * j + lane], 0);
                 starts[64 * j + lane] = start;
                 lens[64 * j + lane] = rows[j] = q_len;
-                kvs[64 * j + lane] = kv_len;
+                positions[64 * j + lane] = kv_len - (end - start);
                 if (start >= 0 && q_len > 0) {
                     keys[j] = max(keys_seen(p, kv_len, q_len > slots ? min(q_len, p.group.page(TILE_ROWS) + 2) : 1), 1);
                     if (q_len > slots) tiles[j] = (q_len * group + TILE_ROWS - 1) / TILE_ROWS;
@@ -997,16 +995,17 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(const PagedAttn p, R
             b = at / slots;
             token = at - b * slots;
         }
+        // (the rows that the call has of the request, which may have more: positions are theirs)
         const int start = listed ? starts[b] : p.query_start[b], q_len = listed ? lens[b] : min(p.query_start[b + 1], p.tokens) - start;
-        const int kv_len = listed ? kvs[b] : p.kv_lens[b], end = start + q_len;
+        const int pos_first = listed ? positions[b] : max(p.kv_lens[b], 0) - (p.query_start[b + 1] - start);
         if (start < 0) continue;
         if (token < 0) {
             if (q_len <= slots || tile < 0 || tile * TILE_ROWS >= q_len * group) continue;
             const int item = (start * group / TILE_ROWS + b + tile) * p.n_kv + h;
-            tile_run<T>(p, *reinterpret_cast<TileShared<T> *>(smem), tile_cut, b, start, q_len, kv_len, h, tile * TILE_ROWS, run, item);
+            tile_run<T>(p, *reinterpret_cast<TileShared<T> *>(smem), tile_cut, b, start, q_len, pos_first, h, tile * TILE_ROWS, run, item);
         } else {
             if (token >= q_len || q_len > slots) continue;
-            token_run<T, G, 4, 4>(p, *reinterpret_cast<TokenShared<G, 4> *>(smem), token_cut, start + token, b, kv_len, end, h, h * group, group, run,
+            token_run<T, G, 4, 4>(p, *reinterpret_cast<TokenShared<G, 4> *>(smem), token_cut, start + token, b, pos_first + token, h, h * group, group, run,
                                   (b * slots + token) * p.n_kv + h);
         }
     }

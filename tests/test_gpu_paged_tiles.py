@@ -115,3 +115,23 @@ def test_rows_before_the_first_request(agpu, dev, type_, batch, kind):
     want, tol = attend64(q, kc, vc, tables, lens.tolist(), start)
     check(out, want, tol)
     assert (out[:first] == 7.0).all() and (out[start[-1]:] == 7.0).all()
+
+
+@pytest.mark.parametrize("type_", TYPES)
+@pytest.mark.parametrize("batch", [4, 260])
+def test_fewer_rows_than_the_requests_have(agpu, dev, type_, batch):
+    """A call with the first rows only: each is at the position that query_start gives it, whichever way it is worked out."""
+    import torch
+    rng, g = np.random.default_rng(9), torch.Generator(device=dev).manual_seed(8)
+    new = np.full(batch, 1 if batch > 100 else 3)
+    new[-1] = 150
+    lens = new + rng.integers(0, 60, batch)
+    start = np.concatenate([[0], np.cumsum(new)]).tolist()
+    pages = int((-(-lens // 16)).sum())
+    kc, vc = _cache(torch, g, dev, pages, 2, 16, type_)
+    tables = _tables(rng, lens.tolist(), 16, pages)
+    q = torch.randn((start[-1], 4, 64), generator=g, device=dev)
+    want, tol = attend64(q, kc, vc, tables, lens.tolist(), start)
+    for rows in (start[-1] - 20, start[-2] + 3, start[-2], 2):
+        got = _call(dev, q[:rows], kc, vc, tables, lens, start)
+        check(got, want[:rows], tol[:rows])
