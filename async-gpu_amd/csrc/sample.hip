@@ -105,8 +105,8 @@ struct Scale {
         return w;
     }
 };
-// a sum of weights in bin j, `scale` = 2^(-j / 32), in units of bin 0: never smaller for a larger sum
-__device__ __forceinline__ u64 in_units(u64 sum, double scale) { return (u64)__builtin_rint((double)sum * scale); }
+// a sum of weights in bin j, `scale` = 2^(-j / 32), in units of bin 0: never smaller for a larger sum, and bin 0's as it is
+__device__ __forceinline__ u64 in_units(u64 sum, double scale) { return scale == 1.0 ? sum : (u64)__builtin_rint((double)sum * scale); }
 __device__ __forceinline__ double units(int j) { return exp2_wide(-(double)j / SM_OCTAVE); }
 
 __device__ __forceinline__ u64 composite(float x, int i) { return (u64)order_key(x) << kIndexBits | (u64)((1 << kIndexBits) - 1 - i); }
@@ -140,6 +140,22 @@ struct Shared {
     int hit[2], from[4], to[4], fill, piece;
 };
 
+// share times sum, 0 < share < 1, cut off, and whether nothing was: sums have more bits than 64-bit floats, in which a border between equal weights would be missed.
+__device__ __forceinline__ u64 mostof(float share, u64 sum, bool &whole) {
+    const uint32_t bits = __float_as_uint(share), exponent = bits >> 23;
+    const u64 digits = exponent > 0 ? (bits & 0x7fffffu) | 0x800000u : bits & 0x7fffffu;
+    const int down = 150 - max((int)exponent, 1);  // share = digits / 2^down, 24 <= down <= 149
+    const u64 low = digits * sum, high = __umul64hi(digits, sum);
+    if (down < 64) {
+        whole = (low << (64 - down)) == 0;
+        return high << (64 - down) | low >> down;
+    }
+    const int rest = down - 64;
+    const u64 most = rest < 32 ? high >> rest : 0;  // (high is below 2^22)
+    whole = low == 0 && (rest < 32 ? most << rest == high : high == 0);
+    return most;
+}
+
 // What is asked for: the first rank whose running sum exceeds `past`, or, by count, rank number past + 1.
 struct Target {
     bool by_count;
@@ -158,15 +174,16 @@ struct Row {
         : temperature(p.temperatures ? p.temperatures[r] : p.temperature), top_p(p.top_ps ? p.top_ps[r] : p.top_p), min_p(p.min_ps ? p.min_ps[r] : p.min_p),
           u(p.u[r]), top_k(p.top_ks ? p.top_ks[r] : p.top_k), by_p(top_p < 1.0f && top_p > 0.0f) {}
     __device__ __forceinline__ Target k_target() const { return Target{true, (u64)(top_k - 1)}; }
-    // the last that top_p keeps of a sum, and the drawn one
+    // the last that top_p keeps of a sum (by_p: 0 < top_p < 1), which the sum that reaches its share ends with, and the drawn one
     __device__ __forceinline__ Target p_target(u64 sum) const {
-        const double share = __builtin_ceil((double)top_p * (double)sum) - 1;
-        return Target{false, share > 0.0 && sum > 0 ? min((u64)share, sum - 1) : 0ull};
+        bool whole;
+        const u64 share = mostof(top_p, sum, whole);
+        return Target{false, whole && share > 0 ? share - 1 : share};
     }
     __device__ __forceinline__ Target u_target(u64 sum, u64 first) const {  // first: the weight of the first, which is always kept
         sum = max(top_p <= 0.0f ? first : sum, first);
-        const double at = (double)u * (double)sum;
-        return Target{false, at > 0.0 ? min((u64)at, sum - 1) : 0ull};
+        bool whole;
+        return Target{false, u >= 1.0f ? sum - 1 : u > 0.0f ? mostof(u, sum, whole) : 0ull};
     }
 };
 
