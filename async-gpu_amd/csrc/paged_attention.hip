@@ -1,7 +1,8 @@
 // Attention over a KV cache in pages, d_head = 64: o = softmax(q k / 8) v for the rows of several requests, each over the keys of its own block table.
 //
 // Two kernels, by what the call says about its rows:
-//   tokens <= batch  paged_tokens_kernel: every row by itself on the vector units, as one does with one new token a request.  Bound by the bytes of K and V: 64
+//   tokens <= batch  paged_tokens_kernel: every row by itself on the vector units, which suits one new token a request; the lengths are on the device, so that a
+//                    chunk of many rows beside many requests without any comes here too, and reads its keys once a row.  Bound by the bytes of K and V: 64
 //                    requests of 4096 keys (32 heads over 8, f16) 105 us, 5.1 TB/s; with 1 to 4018 keys (80 MB) 28 us, of which 5 are the launch and the way to the
 //                    first key; one request of 777 keys, 12 heads, fp32, 7.0, a chain of loads.  The query heads of a K/V head (up to 8) share what is read of it.
 //   otherwise        paged_rows_kernel: requests with more than eight rows of heads a K/V head in tiles of 128 rows on the matrix cores, the others as above.  Bound by
@@ -421,11 +422,13 @@ __global__ __launch_bounds__(64 * W) void paged_tokens_kernel(const PagedAttn p,
 // ---- tiles of rows on the matrix cores ----
 // S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_32x32x16 with 32 keys and 32 rows: what a 32 x 32 result holds of a column (a row of q) in its two
 // half waves is what the second product takes, if V's keys come in the order 16 step + 8 (e / 4) + 4 half + e mod 4.
-//   fp32 cache   every operand is the exact sum of three bf16 numbers (8 bits each, cut off one after the other); of the nine products of pieces the six that
-//                reach 2^-24 are formed, the smallest first
-//   bf16 cache   K and V as they are, q and the weights in three pieces: three products
+//   fp32 cache   every operand is the exact sum of three bf16 numbers (8 bits each, cut off one after the other); of the nine products of pieces the three
+//                smallest are left out, which come to 2^-21 of the whole at most (2^-24.7 on average, always of its sign); the others, the smallest first.  All nine
+//                would be half as many matrix instructions again for less than what the sums' own roundings are.
+//   bf16 cache   K and V as they are, q and the weights in three pieces: three products, nothing left out
 //   f16 cache    K and V as they are, q (times a power of two per row) and the weights (times 2^9) as two f16 numbers: two products.  q is good to 2^-22 of itself
-//                and 2^-40 of its largest element.
+//                and 2^-39 of its row's largest element, a weight to 2^-22 of itself and 2^-34 of the largest one (f16 has no steps below 2^-24): keys of weights below
+//                that reach the sum of weights, which is fp32, but not o.  A third piece would be half as many products again.
 constexpr int TILE_ROWS = 128, TILE_KEYS = 32;
 constexpr int kFrag = 4 * 2 * 32;  // 16-byte fragments of a piece of 32 keys of K, and of V
 typedef float floatx16 __attribute__((ext_vector_type(16)));

@@ -412,7 +412,11 @@ int32_t agpu_paged_kv_append(agpu_ctx *ctx, const float *k, const float *v, int6
  * position p sees key j <= p, with window > 0 only where p - j < window or j < sinks.  Query head h reads K/V head h / (n_heads / n_kv_heads).
  *   q   row (t, h) of 64 floats at t * q_token_stride + h * q_head_stride elements;  o [tokens][n_heads][64]
  * A row that sees no key gives zeros.  Rows behind the last request's are left as they were.  Keys on a page id outside the cache are not seen.
- * K and V that a row does not see do not reach it, whatever they are.  Scores, weights and sums are fp32. */
+ * K and V that a row does not see do not reach it, whatever they are.  query_start ascends; q may have fewer rows than it says (the first ones are worked
+ * out) or more; rows before query_start[0] are nobody's either.  o overlaps none of the inputs.
+ * Scores, weights and sums are fp32, and sums of weight (1 at most) times |v| over a row's keys have to be: below 2^128.  A request with more than eight
+ * rows of heads a K/V head goes through the matrix cores: products of an fp32 cache are then good to 2^-21 of themselves (2^-24.7 on average); over an f16 cache q
+ * is good to 2^-22 of itself and 2^-39 of its row's largest element, and weights to 2^-22 of themselves and 2^-34 of the largest. */
 int32_t agpu_paged_attention(agpu_ctx *ctx, const float *q, int64_t q_token_stride, int64_t q_head_stride, const void *k_cache,
                              const void *v_cache, int64_t k_page_stride, int64_t v_page_stride, const int32_t *block_tables,
                              const int32_t *kv_lens, const int32_t *query_start, float *o, int32_t tokens, int32_t batch, int32_t n_heads,

@@ -135,3 +135,88 @@ def test_fewer_rows_than_the_requests_have(agpu, dev, type_, batch):
     for rows in (start[-1] - 20, start[-2] + 3, start[-2], 2):
         got = _call(dev, q[:rows], kc, vc, tables, lens, start)
         check(got, want[:rows], tol[:rows])
+
+
+@pytest.mark.parametrize("type_", TYPES)
+def test_magnitudes_far_apart(agpu, dev, type_):
+    """Elements of q and K over 2^24 with scores of ordinary size, rows of q over 2^60, and values over as much as the type has."""
+    import torch
+    lens, new, heads = [300, 40, 1, 90], [140, 40, 1, 3], 3
+    rng, g = np.random.default_rng(4), torch.Generator(device=dev).manual_seed(5)
+    kc, vc = _cache(torch, g, dev, 40, heads, 16, type_)
+    tables, start = _tables(rng, lens, 16, 40), np.concatenate([[0], np.cumsum(new)]).tolist()
+    q = torch.randn((start[-1], heads, 64), generator=g, device=dev)
+    by = 2.0 ** torch.randint(-12, 13, (64,), generator=g, device=dev)
+    far = 2.0 ** torch.randint(-14, 13, vc.shape, generator=g, device=dev) if type_ == "float16" else 10.0 ** torch.randint(-30, 31, vc.shape, generator=g, device=dev).float()
+    args = kc, (vc.float() * far).to(vc.dtype), tables, lens, start
+    check(_call(dev, q, *args), *attend64(q, *args))
+    wide = (kc.float() / by).to(kc.dtype), *args[1:]
+    check(_call(dev, q * by, *wide), *attend64(q * by, *wide))
+    tiny = q * 2.0 ** torch.randint(-60, 1, (start[-1], heads, 1), generator=g, device=dev)
+    check(_call(dev, tiny, *args), *attend64(tiny, *args))
+
+
+@pytest.mark.parametrize("type_", TYPES)
+@pytest.mark.parametrize("octaves", [10, 24, 32, 40])
+def test_many_small_weights_beside_a_large_one(agpu, dev, type_, octaves):
+    """A key with nearly all of the weight and a small value, and a thousand keys of weights 2^-octaves with large ones."""
+    import torch
+    kv, rows, page = 1000, 60, 16
+    g = torch.Generator(device=dev).manual_seed(6)
+    kc = torch.zeros((63, 1, page, 64), dtype=getattr(torch, type_), device=dev)
+    vc = (torch.rand((63, 1, page, 64), generator=g, device=dev) * 3e4 + 3e4).to(kc.dtype)
+    kc.view(-1, 64)[500, 0] = octaves / 1.4426950408889634
+    vc.view(-1, 64)[500] *= 2.0**-20
+    tables = np.arange(63, dtype=np.int32)[None]
+    q = torch.zeros((rows, 1, 64), device=dev)
+    q[:, :, 0] = 8.0
+    want, tol = attend64(q, kc, vc, tables, [kv], [0, rows])
+    if type_ == "float16":
+        # weights times 512 are two f16 numbers there, which no smaller steps than 2^-24 have: half a step is 2^-34 of a weight of one, and the sum of weights at least one
+        tol = tol + 2.0**-34 * vc.double().abs().sum((0, 1, 2)).cpu()
+    check(_call(dev, q, kc, vc, tables, [kv], [0, rows]), want, tol)
+    check(_call(dev, q[:1], kc, vc, tables, [kv - rows + 1], [0, 1]), want[:1], tol[:1])
+
+
+def test_pieces_at_their_worst(agpu, dev):
+    """fp32 caches go to the matrix cores in three pieces, cut off one after the other, and of nine products the three smallest are left out: 2^-7 times 2^-15, twice, and
+    2^-15 squared, 2^-21 of a product of numbers whose last 16 bits are ones.  Scores and outputs of such numbers."""
+    import torch
+    kv, rows, page = 96, 96, 16
+    worst = float(np.uint32(0x3f80ffff).view(np.float32))
+    kc, vc = (torch.zeros((6, 1, page, 64), device=dev) for _ in range(2))
+    kc.view(-1, 64)[::3] = worst
+    kc.view(-1, 64)[1::3] = -worst / 2
+    vc.view(-1, 64)[:, 0] = worst
+    vc.view(-1, 64)[::2, 1] = worst
+    vc.view(-1, 64)[1::2, 2] = worst * 4
+    q = torch.full((rows, 1, 64), worst, device=dev)
+    tables = np.arange(6, dtype=np.int32)[None]
+    want, tol = attend64(q, kc, vc, tables, [kv], [0, rows])
+    got = _call(dev, q, kc, vc, tables, [kv], [0, rows])
+    check(got, want, tol)
+    # what is left out by itself: scores of up to 8.1 octaves' 2^-21 each way, and 2^-21 of the output; and the sums' roundings as above
+    s = 8.0 * worst * worst
+    bound = 2 * s * (2.0**-21 + 64 * 2.0**-24) + 2.0**-21 + 2.0**-20 + 2 * (kv / 16 + 100) * 2.0**-24
+    assert ((got.cpu().double() - want).abs() <= bound * want.abs().amax()).all()
+
+
+@pytest.mark.parametrize("type_", TYPES)
+@pytest.mark.parametrize("heads,kv_heads", [(11, 1), (24, 2), (130, 1)])
+def test_many_heads_in_many_requests(agpu, dev, type_, heads, kv_heads):
+    """More than eight heads a K/V head in more requests than are numbered, rows of every number."""
+    import torch
+    rng, g = np.random.default_rng(heads), torch.Generator(device=dev).manual_seed(1)
+    batch, page = 290, 16
+    new = rng.choice([0, 1, 1, 1, 2, 9], batch)
+    new[[7, 123]] = 40, 17
+    lens = new + rng.integers(0, 40, batch)
+    lens[200] = 900
+    start = np.concatenate([[0], np.cumsum(new)]).tolist()
+    pages = int((-(-lens // page)).sum())
+    kc, vc = _cache(torch, g, dev, pages, kv_heads, page, type_)
+    tables = _tables(rng, lens.tolist(), page, pages)
+    q = torch.randn((start[-1], heads, 64), generator=g, device=dev)
+    assert start[-1] > batch
+    for window, sinks in ((0, 0), (20, 3)):
+        check(_call(dev, q, kc, vc, tables, lens, start, window, sinks), *attend64(q, kc, vc, tables, lens.tolist(), start, window, sinks))
