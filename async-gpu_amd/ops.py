@@ -219,7 +219,7 @@ def paged_attention(q, k_cache, v_cache, block_tables, kv_lens, query_start=None
     """Attention of the new rows of several requests over their pages: q [tokens, n_heads, 64] (any strides of tokens and heads) -> [tokens, n_heads, 64].
     Rows query_start[b] .. query_start[b + 1] - 1 are the last positions of the kv_lens[b] of request b; without query_start each request
     has one row.  A row at position p sees key j <= p, with window > 0 only where p - j < window or j < sinks.  n_heads is a multiple of the
-    cache's heads.  A row that sees nothing gives zeros; rows behind the last request's are not written (`out` keeps them)."""
+    cache's heads.  A row that sees nothing gives zeros; rows of no request, before query_start[0] or behind the last one's, are not written (`out` keeps them)."""
     return _native.paged_attention(q, k_cache, v_cache, block_tables, kv_lens, query_start, window, sinks, out)
 
 

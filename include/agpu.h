@@ -312,7 +312,7 @@ int32_t agpu_top_k_sample(agpu_ctx *ctx, const float *logits, int32_t n, int32_t
  * with the same number it is the one that top_k_sample draws, up to that one's rounding.  A setting is one number for all rows, or where the array
  * behind it is not NULL one number a row (device, [rows]).  NaN ranks with -inf and is never drawn; a row without any logit above -inf gives -1.
  * Weights are good to 2^-43 of themselves and whole multiples of 2^-b of a weight near theirs, b = 61 - ceil(log2 n) or 50 if that is less (45
- * for 50257 logits), and their sums do not depend on an order; candidates below 2^-48 of the first have none.  n <= 2^20. */
+ * for 50257 logits), their sums do not depend on an order, and shares of them are exact; candidates below 2^-48 of the first have none.  n <= 2^20. */
 int32_t agpu_sample(agpu_ctx *ctx, const float *logits, const float *u, int32_t *tokens_out, int32_t rows, int32_t n, float temperature,
                     int32_t top_k, float top_p, float min_p, const float *temperatures, const int32_t *top_ks, const float *top_ps,
                     const float *min_ps);
