@@ -426,7 +426,7 @@ __global__ __launch_bounds__(64 * W) void paged_tokens_kernel(const PagedAttn p,
 // S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_32x32x16 with 32 keys and 32 rows: what a 32 x 32 result holds of a column (a row of q) in its two
 // half waves is what the second product takes, if V's keys come in the order 16 step + 8 (e / 4) + 4 half + e mod 4.
 //   fp32 cache   every operand is the exact sum of three bf16 numbers (8 bits each, cut off one after the other); of the nine products of pieces the three
-//                smallest are left out, which come to 2^-21 of the whole at most (2^-24.7 on average, always of its sign); the others, the smallest first.  All nine
+//                smallest are left out, which come to 2^-21 of the whole at most (2^-24.5 on average, always of its sign); the others, the smallest first.  All nine
 //                would be half as many matrix instructions again for less than what the sums' own roundings are.
 //   bf16 cache   K and V as they are, q and the weights in three pieces: three products, nothing left out
 //   f16 cache    K and V as they are, q (times a power of two per row) and the weights (times 2^9) as two f16 numbers: two products.  q is good to 2^-22 of itself
@@ -759,7 +759,7 @@ __device__ __forceinline__ void tile_run(const PagedAttn &p, TileShared<T> &s, c
         top = max_of_halves(top);
         // Weights may grow to 2^6 before everything is rescaled, but not beside values from 2^91 on: those go in with weights of one at most, as they do row by
         // row, so that their sums are finite where |v| times the keys is below 2^128.  (Sums of 2^30 smaller ones are finite anyway, and f16 values are small.)
-        // Each row by what it sees itself: its bits do not depend on the others'.
+        // Each row by what it sees itself: keys that only other rows of the tile see leave its bits as they are.
         float slack = 6.0f;
         if (__builtin_expect(!std::is_same_v<T, F16> && odd_v != 0, 0)) slack = (odd_v & in_sight()) != 0 ? 0.0f : slack;
         const bool rises = top > m + slack;

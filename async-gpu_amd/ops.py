@@ -198,7 +198,8 @@ def gemm_f32(a, b):
 
 # ---- several requests over a KV cache in pages: a step is paged_plan, then per layer paged_kv_append and paged_attention, then sample.
 # Lengths, tables and slots are int32 device tensors; nothing waits for the host.  A cache is two tensors [n_pages, n_kv_heads, page_size, 64] of
-# float32, float16 or bfloat16 whose pages may lie apart (slices of a larger pool).
+# float32, float16 or bfloat16 whose pages may lie apart (slices of a larger pool).  A captured step keeps the scratch of the stream it was captured on:
+# replays of graphs captured on one stream, and its eager calls, run one after the other.
 
 
 def paged_plan(cached_lens, new_lens, block_tables, free_pages, n_free, page_size, max_tokens):

@@ -374,7 +374,8 @@ int32_t agpu_kv_append(agpu_ctx *ctx, const float *src, float *cache, int32_t n_
 /* No counterpart in the reference, whose cache holds one sequence (KvCache, nn/models/gpt2.rs:1064-1117).  A step of a server:
  * agpu_paged_plan gives the requests their pages and their new tokens their places, agpu_paged_kv_append puts K and V there,
  * agpu_paged_attention reads them, agpu_sample draws the next tokens.  Nothing of it waits for the host: lengths, tables and slots are
- * device data, launch shapes follow from the sizes of the arguments alone, and a step may be captured into a HIP graph.
+ * device data, launch shapes follow from the sizes of the arguments alone, and a step may be captured into a HIP graph.  Graphs captured
+ * from one context share its scratch, as its calls do: they run one after the other, never two at a time.
  *   cache         K and V each [n_pages][n_kv_heads][page_size][64] of cache_type, pages *_page_stride elements apart (a multiple of 16
  *                 bytes, the first at 16 bytes): what may lie between pages is the other one of K and V, or other layers
  *   block_tables  [batch][table_width] int32: position p of request b is on page block_tables[b][p / page_size].  Only entries of
@@ -415,7 +416,7 @@ int32_t agpu_paged_kv_append(agpu_ctx *ctx, const float *k, const float *v, int6
  * K and V that a row does not see do not reach it, whatever they are.  query_start ascends; q may have fewer rows than it says (the first ones are worked
  * out) or more; rows before query_start[0] are nobody's either.  o overlaps none of the inputs.
  * Scores, weights and sums are fp32, and sums of weight (1 at most) times |v| over a row's keys have to be: below 2^128.  A request with more than eight
- * rows of heads a K/V head goes through the matrix cores: products of an fp32 cache are then good to 2^-21 of themselves (2^-24.7 on average); over an f16 cache q
+ * rows of heads a K/V head goes through the matrix cores: products of an fp32 cache are then good to 2^-21 of themselves (2^-24.5 on average); over an f16 cache q
  * is good to 2^-22 of itself and 2^-39 of its row's largest element, and weights to 2^-22 of themselves and 2^-34 of the largest. */
 int32_t agpu_paged_attention(agpu_ctx *ctx, const float *q, int64_t q_token_stride, int64_t q_head_stride, const void *k_cache,
                              const void *v_cache, int64_t k_page_stride, int64_t v_page_stride, const int32_t *block_tables,
