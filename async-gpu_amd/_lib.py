@@ -98,6 +98,10 @@ SIGNATURES = {
     "agpu_paged_plan": (_i32, [_vp] * 11 + [_i32] * 5),
     "agpu_paged_kv_append": (_i32, [_vp] * 3 + [C.c_int64] * 4 + [_vp] * 2 + [C.c_int64] * 2 + [_vp] + [_i32] * 6),
     "agpu_paged_attention": (_i32, [_vp] * 2 + [C.c_int64] * 2 + [_vp] * 2 + [C.c_int64] * 2 + [_vp] * 4 + [_i32] * 11),
+    "agpu_paged_attention_shared": (_i32, [_vp] * 2 + [C.c_int64] * 2 + [_vp] * 2 + [C.c_int64] * 2 + [_vp] * 7 + [_i32] * 13),
+    "agpu_paged_attention_weights": (_i32, [_vp] * 2 + [C.c_int64] * 2 + [_vp] * 2 + [C.c_int64] * 2 + [_vp, C.c_int64] + [_vp] * 4 + [_i32] * 11),
+    "agpu_paged_evict": (_i32, [_vp] * 3 + [C.c_int64] * 2 + [_vp, C.c_int64] + [_vp] * 2 + [_i32] * 11),
+    "agpu_paged_trim": (_i32, [_vp] * 8 + [_i32] * 6),
     "agpu_sample": (_i32, [_vp] * 4 + [_i32] * 2 + [_f, _i32, _f, _f] + [_vp] * 4),
     "agpu_gemm_f32": (_i32, [_vp, _vp, _vp, _vp, _i32, _i32, _i32]),
     # include/agpu_gpt2.h (first argument is the model handle, or the config / context)

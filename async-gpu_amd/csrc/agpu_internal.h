@@ -212,6 +212,17 @@ __device__ __forceinline__ unsigned wave_minmax_u32(unsigned v) {
     return (unsigned)__builtin_amdgcn_readlane((int)v, 63);
 }
 
+// Sum over the lanes up to this one.
+__device__ __forceinline__ int wave_running_sum(int v) {
+    v += (int)dpp_move_u32<0x111, 0xf>(0, v);  // row_shr 1, 2, 4, 8, then row_bcast 15 and 31
+    v += (int)dpp_move_u32<0x112, 0xf>(0, v);
+    v += (int)dpp_move_u32<0x114, 0xf>(0, v);
+    v += (int)dpp_move_u32<0x118, 0xf>(0, v);
+    v += (int)dpp_move_u32<0x142, 0xa>(0, v);
+    v += (int)dpp_move_u32<0x143, 0xc>(0, v);
+    return v;
+}
+
 // n / d and 1 / sqrt(v) from the hardware's estimates (good to 1 ulp) and a correction step each; where that has no number in it (d or v of zero or
 // infinity, n infinite) the estimate stands.  Some 6 and 9 dependent instructions in place of 10 for a division and 22 for 1.0f / sqrtf(v), for
 // chains that a launch waits for.  d is a normal number up to 2^126 (above it the estimate is zero) or infinite.

@@ -106,6 +106,38 @@ inline int most_runs(int64_t items, int64_t longest, int64_t least, size_t item_
 // The most keys a row can see.
 inline int64_t longest_row(int64_t held, int64_t window, int64_t sinks) { return window > 0 && window + sinks < held ? window + sinks : held; }
 
+// The scratch of a prefix's runs, for `rows` rows of heads and `held` keys at most: how many runs there is room for in half of it (0: not even for one), where o
+// of the second and later ones begins, and what all of it takes.  The first 256 bytes are a number's; (m, l) of a row and run are 8 bytes, o is 256.
+struct PrefixRuns {
+    int most;
+    size_t rest, bytes;
+};
+inline PrefixRuns prefix_runs(int64_t rows, int64_t held, size_t scratch) {
+    const size_t all = (size_t)rows, half = scratch / 2;
+    auto up = [](size_t n) { return (n + 255) & ~(size_t)255; };
+    if (256 + up(8 * all) > scratch / 4 * 3) return {0, 0, 0};
+    int64_t runs = (held + 127) / 128;
+    runs = runs < 64 ? runs : 64;
+    const int64_t room = half > 512 ? (int64_t)((half - 512) / (264 * all)) : 0;
+    runs = runs < room ? runs : room;
+    runs = runs < 1 ? 1 : runs;
+    const size_t rest = 256 + up(8 * all * runs);
+    return {(int)runs, rest, rest + up(256 * all * (runs - 1))};
+}
+
+// The scratch of attention that adds up its weights: 8 bytes a row of heads, then, where there is room in half of it (and a K/V head has eight query heads at most),
+// a score for each place and query head.  Where the scores begin (0: none), and what all of it takes (0: it is too small).
+struct WeightsRoom {
+    size_t scores, bytes;
+};
+inline WeightsRoom weights_room(int64_t rows, int64_t places, int group, size_t scratch) {
+    auto up = [](size_t n) { return (n + 255) & ~(size_t)255; };
+    const size_t stats = up(8 * (size_t)rows);
+    if (stats > scratch / 4 * 3) return {0, 0};
+    if (group > 8 || stats + 4 * (size_t)places > scratch / 2) return {0, stats};
+    return {stats, stats + up(4 * (size_t)places)};
+}
+
 // ---- what calls are refused: 0, or the error and why --------------------------------------------
 
 struct Refusal {
@@ -139,6 +171,40 @@ inline Refusal refuse_attention(int32_t tokens, int32_t batch, int32_t n_heads, 
     if ((int64_t)table_width * page_size > kMaxPositions) return {AGPU_ERR_UNSUPPORTED, "a row of the table stands for 2^30 positions at most"};
     if (!query_start && tokens != batch) return {AGPU_ERR_SHAPE_MISMATCH, "without query_start each request has one row"};
     if ((int64_t)tokens * n_heads >= 1 << 23) return {AGPU_ERR_UNSUPPORTED, "2^23 rows of heads or more"};  // (a launch has less than 2^32 threads)
+    return kFine;
+}
+
+constexpr int kMaxPrefixes = 256;  // of a call: what is counted about them lies in LDS
+
+inline Refusal refuse_shared(int32_t n_prefix, int32_t prefix_width, int32_t table_width, int32_t page_size) {
+    if (n_prefix < 0 || prefix_width < 0) return {AGPU_ERR_SHAPE_MISMATCH, "negative sizes"};
+    if (n_prefix > kMaxPrefixes) return {AGPU_ERR_UNSUPPORTED, "256 prefixes at most"};
+    if (((int64_t)prefix_width + table_width) * page_size > kMaxPositions) return {AGPU_ERR_UNSUPPORTED, "a prefix and the row of a table behind it stand for 2^30 positions at most"};
+    return kFine;
+}
+
+inline Refusal refuse_weights(uintptr_t weights, int64_t page_stride, int32_t n_kv_heads, int32_t n_pages, int32_t page_size) {
+    if (n_pages > 1 && page_stride < (int64_t)n_kv_heads * page_size) return {AGPU_ERR_SHAPE_MISMATCH, "pages of the weights overlap"};
+    if (weights % 4) return {AGPU_ERR_UNSUPPORTED, "weights begin at 4 bytes"};
+    return kFine;
+}
+
+// What a request is cut down to.
+inline Refusal refuse_budget(int32_t batch, int32_t table_width, int32_t page_size, int32_t limit, int32_t keep, int32_t recent, int32_t sinks) {
+    if (batch < 0 || table_width < 0 || keep < 0 || recent < 0 || sinks < 0) return {AGPU_ERR_SHAPE_MISMATCH, "negative sizes"};
+    if (page_size <= 0) return {AGPU_ERR_SHAPE_MISMATCH, "page_size is not positive"};
+    if (page_size > kMaxPageSize) return {AGPU_ERR_UNSUPPORTED, "pages of 2^20 positions at most"};
+    if ((int64_t)table_width * page_size > kMaxPositions) return {AGPU_ERR_UNSUPPORTED, "a row of the table stands for 2^30 positions at most"};
+    if (limit < keep) return {AGPU_ERR_SHAPE_MISMATCH, "the limit is below what is kept"};
+    if ((int64_t)recent + sinks > keep) return {AGPU_ERR_SHAPE_MISMATCH, "the first and the last positions are more than what is kept"};
+    return kFine;
+}
+
+constexpr int kMaxEvicted = 1 << 20;  // positions of a request that is cut down: a bit of each lies in LDS
+
+inline Refusal refuse_evict(int32_t batch, int32_t n_kv_heads, int32_t table_width, int32_t page_size) {
+    if ((int64_t)table_width * page_size > kMaxEvicted) return {AGPU_ERR_UNSUPPORTED, "a row of the table stands for 2^20 positions at most"};
+    if ((int64_t)batch * n_kv_heads >= 1 << 23) return {AGPU_ERR_UNSUPPORTED, "2^23 requests times heads or more"};  // (a launch has less than 2^32 threads)
     return kFine;
 }
 

@@ -1,0 +1,239 @@
+// A KV cache that is cut down to a budget by what its keys are worth, d_head = 64: attention that adds up the weight that each key was given (over the rows of a call and the
+// query heads of a K/V head), the eviction of the keys with the least of it, and the pages that this frees.
+//
+// paged_attention_weights: the kernels of paged_attention.hip, and
+//   one row a request   its scores stay in scratch (4 bytes a key and query head beside 128 to 512 of K and V), and the workgroup that joins the row's runs, which knows m
+//                       and l by then, turns them into weights.
+//   more                m and 1 / l of the rows stay in scratch, and paged_weights_kernel forms their scores once more on the matrix cores, a wave's 32 keys in registers
+//                       against all rows that see them, 32 at a time: a key's sum is one wave's, in the order of the rows.
+#include "paged_kernels.h"
+
+namespace {
+
+// ---- what each key was given, by several rows of a request ------------------------------------------
+
+// The rows of a step of 32 in LDS, as operands, double buffered.
+template <class T>
+struct RowsShared {
+    uint4 q[2][Tiles<T>::QP][kFrag];  // [d step of 16][half][row]
+    float unit[2][32];                // f16: of the scores
+};
+
+// Sum over the 32 lanes of a half wave, in each of them.
+__device__ __forceinline__ float half_wave_sum(float v) {
+    v = row16_sum(v);
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// The 128 keys from number `first_key` on of those that the rows of request b see, for K/V head h.  n: rows of the request, `there` of them in the call.
+template <class T>
+__device__ __forceinline__ void weigh_keys(const PagedAttn &p, const More<WEIGHTS> &more, RowsShared<T> &s, int b, int start, int n, int there, int h, int first_key) {
+    constexpr int KP = Tiles<T>::KP, QP = Tiles<T>::QP, kBytes = 16 / T::EL;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 31, h2 = lane >> 5, group = p.group.size;
+    const int kv_len = max(p.kv_lens[b], 0), pos_first = kv_len - n;
+    const paged::TileKeys keys = paged::tile_keys(pos_first, kv_len - 1, p.held, p.window, p.sinks);
+    const int stay = max(p.sinks - keys.gap, keys.first);  // numbers below it are seen whatever the window
+    // this wave's keys
+    const int v0 = first_key + 32 * wave, v = v0 + c, j = keys.key(v);
+    const char *row = static_cast<const char *>(p.k);
+    float *to = more.weights;
+    bool real = false;
+    if (v < keys.count) {
+        const int at = p.div.page(j), place = j - at * p.div.size, page = p.tables[(size_t)b * p.width + at];
+        real = (unsigned)page < (unsigned)p.n_pages;
+        if (real) {
+            row += (page * p.k_page + (long long)(h * p.div.size + place) * DH) * kBytes;
+            to += page * more.page + (long long)h * p.div.size + place;
+        }
+    }
+    const uint32_t held = (uint32_t)__ballot(real);  // (both halves have the same keys)
+    const float old = real && j < pos_first ? *to : 0.0f;
+    uint4 k[4][KP];
+    bool odd = false;
+    {
+        Staged<T> x[4];
+#pragma unroll
+        for (int ds = 0; ds < 4; ++ds) {
+            x[ds].row(row + (16 * ds + 8 * h2) * kBytes);
+            if (!real) x[ds].clear();
+            if (__any(x[ds].odd())) odd |= x[ds].clean() != 0;
+            x[ds].pieces(k[ds]);
+        }
+    }
+    uint32_t odd_k = (uint32_t)__ballot(odd) | (uint32_t)(__ballot(odd) >> 32);
+
+    // Rows from the first that sees a key of the workgroup's to the last that does, in steps of 32.
+    const int last_key = min(first_key + 128, keys.count) - 1;
+    const int from = min(max(keys.key(first_key) - pos_first, 0), there);
+    int upto = there;
+    if (p.window > 0 && first_key >= stay) upto = (int)max(min((long long)there, (long long)keys.key(last_key) + p.window - pos_first), 0ll);
+    const int row_from = from * group & ~31, row_upto = upto * group;
+    const int steps = row_upto > row_from ? (row_upto - row_from + 31) / 32 : 0;
+    // what this thread fetches of a step: eight elements of one of its rows
+    const int own = tid >> 3, part = tid & 7;
+    float4 qa, qd;
+    auto fetch = [&](int i) {
+        const int r = min(row_from + 32 * i + own, row_upto - 1), token = p.group.page(r), head = h * group + (r - token * group);
+        const float *from = p.q + (size_t)(start + token) * p.q_row + (size_t)head * p.q_head + 8 * part;
+        qa = load4(from);
+        qd = load4(from + 4);
+    };
+    if (steps > 0) fetch(0);
+    float acc[16];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[r] = 0.0f;
+    for (int i = 0; i < steps; ++i) {
+        const int buf = i & 1;
+        {
+            float x[8] = {qa.x * kQueryScale, qa.y * kQueryScale, qa.z * kQueryScale, qa.w * kQueryScale, qd.x * kQueryScale, qd.y * kQueryScale, qd.z * kQueryScale, qd.w * kQueryScale};
+            if (QP == 2) {  // as in a tile of rows: into 2^14 .. 2^15
+                float most = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(x[e]));
+                most = fmaxf(most, dpp_move<0xb1, 0xf>(most, most));
+                most = fmaxf(most, dpp_move<0x4e, 0xf>(most, most));
+                most = fmaxf(most, dpp_move<0x141, 0xf>(most, most));  // row_half_mirror: eight lanes have a row
+                const int up = max(min(141 - (int)((__float_as_uint(most) >> 23) & 255u), 100), -112);
+                const float by = __uint_as_float((uint32_t)(up + 127) << 23);
+                if (part == 0) s.unit[buf][own] = __uint_as_float((uint32_t)(127 - up) << 23);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] *= by;
+            }
+            uint4 piece[QP];
+            pieces_of(x, piece);
+#pragma unroll
+            for (int level = 0; level < QP; ++level) s.q[buf][level][part * 32 + own] = piece[level];
+        }
+        if (i + 1 < steps) fetch(i + 1);
+        // this lane's row of the step
+        const int r = row_from + 32 * i + c, r_in = min(r, row_upto - 1), token = p.group.page(r_in), pos = pos_first + token;
+        const float2 stats = more.stats[(size_t)(start + token) * p.n_heads + h * group + (r_in - token * group)];
+        __syncthreads();
+        floatx16 x = {};
+#pragma unroll
+        for (int level = QP - 1; level >= 0; --level)
+#pragma unroll
+            for (int ds = 0; ds < 4; ++ds)
+#pragma unroll
+                for (int kp = KP - 1; kp >= 0; --kp)
+                    if (level - kp >= 0 && level - kp < QP) x = Tiles<T>::mfma(k[ds][kp], s.q[buf][level - kp][(2 * ds + h2) * 32 + c], x);
+        if (QP == 2) {
+            const float unit = s.unit[buf][c];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) x[e] *= unit;
+        }
+        if (__builtin_expect(odd_k != 0, 0)) {  // scores of keys with something infinite or no number, in fp32 (uniform)
+            const float *q_row = p.q + (size_t)(start + token) * p.q_row + (size_t)(h * group + (r_in - token * group)) * p.q_head;
+#pragma unroll 1
+            for (int kk = 0; kk < 32; ++kk) {
+                if (!(odd_k >> kk & 1)) continue;
+                const char *key = reinterpret_cast<const char *>((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(uintptr_t)row, kk) |
+                                                                 (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)((uintptr_t)row >> 32), kk) << 32);
+                float d = 0.0f;
+#pragma unroll 1
+                for (int e = 0; e < 32; ++e) d = fmaf(q_row[32 * h2 + e] * kQueryScale, T::one(key, 32 * h2 + e), d);
+                d = sum_of_halves(d);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) x[e] = 8 * (e >> 2) + 4 * h2 + (e & 3) == kk ? d : x[e];
+            }
+        }
+        const paged::RowKeys see = paged::row_keys(keys, pos, p.window, p.sinks);
+        auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1; };  // bits 0 .. n - 1
+        uint32_t seen = held & below(see.last + 1 - v0) & (~below(see.low + 1 - v0) | below(see.first - v0));
+        if (r >= row_upto) seen = 0;
+        seen >>= 4 * h2;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const float w = __builtin_amdgcn_exp2f(x[e] - stats.x) * stats.y;
+            acc[e] += seen >> (8 * (e >> 2) + (e & 3)) & 1 ? w : 0.0f;
+        }
+    }
+    float mine = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+        const float sum = half_wave_sum(acc[e]);
+        // lane c of the half that has key c's sum
+        mine = 8 * (e >> 2) + (e & 3) == (c & ~4) ? sum : mine;
+    }
+    if (real && (c >> 2 & 1) == h2) *to = old + mine;
+}
+
+// Units: 128 keys of a request and K/V head, for requests of several rows (of one too, where its scores found no room), 256 requests at a time.
+template <class T>
+__global__ __launch_bounds__(256, 2) void paged_weights_kernel(const PagedAttn p, const More<WEIGHTS> more) {
+    __shared__ RowsShared<T> s;
+    __shared__ Units list;
+    __shared__ int starts[kListed], rows[kListed], in_call[kListed];
+    const int lane = threadIdx.x & 63;
+    int before = 0;  // units of the requests so far, modulo the grid
+    for (int b0 = 0; b0 < p.batch; b0 += kListed) {
+        __syncthreads();
+        const int entries = min(p.batch - b0, kListed);
+        int units[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            units[j] = 0;
+            if (64 * j >= entries) continue;  // uniform
+            const int i = 64 * j + lane, b = b0 + i;
+            if (i < entries) {
+                const int start = p.query_start ? p.query_start[b] : b, end = p.query_start ? p.query_start[b + 1] : b + 1, kv_len = max(p.kv_lens[b], 0);
+                const int there = min(end, p.tokens) - start;
+                if (start >= 0 && there > 0 && !more.at_once(end - start, p.group.size)) {
+                    const int count = paged::tile_keys(kv_len - (end - start), kv_len - 1, p.held, p.window, p.sinks).count;
+                    units[j] = (int)min((long long)((count + 127) / 128) * p.n_kv, 1ll << 22);  // (that many are 137 GB of keys at least; their sum stays below 2^31)
+                }
+                starts[i] = start;
+                rows[i] = end - start;
+                in_call[i] = there;
+            }
+        }
+        const int all = list.number(units, entries, lane);
+        __syncthreads();
+        const int grid = gridDim.x, first = (int)blockIdx.x >= before ? (int)blockIdx.x - before : (int)blockIdx.x - before + grid;
+        for (int unit = first; unit < all; unit += grid) {
+            int at = unit;
+            const int i = list.entry(at, lane), h = at % p.n_kv, tile = at / p.n_kv;
+            weigh_keys<T>(p, more, s, b0 + i, starts[i], rows[i], in_call[i], h, 128 * tile);
+            __syncthreads();
+        }
+        before = (int)(((unsigned)before + (unsigned)all % (unsigned)grid) % (unsigned)grid);
+    }
+}
+
+}  // namespace
+
+AGPU_EXPORT int32_t agpu_paged_attention_weights(agpu_ctx *ctx, const float *q, int64_t q_token_stride, int64_t q_head_stride, const void *k_cache,
+                                                 const void *v_cache, int64_t k_page_stride, int64_t v_page_stride, float *weights,
+                                                 int64_t weights_page_stride, const int32_t *block_tables, const int32_t *kv_lens,
+                                                 const int32_t *query_start, float *o, int32_t tokens, int32_t batch, int32_t n_heads,
+                                                 int32_t n_kv_heads, int32_t n_pages, int32_t page_size, int32_t table_width, int32_t window,
+                                                 int32_t sinks, int32_t d_head, int32_t cache_type) {
+    AGPU_REQUIRE_CTX(ctx);
+    const paged::Refusal cache =
+        paged::refuse_cache((uintptr_t)k_cache, (uintptr_t)v_cache, k_page_stride, v_page_stride, n_kv_heads, n_pages, page_size, d_head, cache_type);
+    paged::Refusal no = paged::refuse_attention(tokens, batch, n_heads, n_kv_heads, table_width, page_size, window, sinks, query_start != nullptr);
+    if (no.code == AGPU_OK) no = cache;
+    if (no.code == AGPU_OK) no = paged::refuse_weights((uintptr_t)weights, weights_page_stride, n_kv_heads, n_pages, page_size);
+    if (no.code != AGPU_OK) return agpu_fail(ctx, no.code, "paged_attention_weights: %s", no.why);
+    if (tokens == 0 || batch == 0) return AGPU_OK;
+    if (!q || !k_cache || !v_cache || !weights || !kv_lens || !o || (!block_tables && table_width > 0))
+        return agpu_fail(ctx, AGPU_ERR_NULL_POINTER, "paged_attention_weights: null pointer");
+    agpu_on_device here(ctx);
+    if (here.rc != AGPU_OK) return here.rc;
+    const PagedAttn p = paged_attn(q, q_token_stride, q_head_stride, k_cache, v_cache, k_page_stride, v_page_stride, block_tables, kv_lens, query_start, o, tokens, batch, n_heads,
+                                   n_kv_heads, n_pages, page_size, table_width, window, sinks, ctx->strict_sync);
+    const paged::WeightsRoom room = paged::weights_room((int64_t)tokens * n_heads, (int64_t)n_pages * page_size * n_heads, n_heads / n_kv_heads, ctx->ws_bytes);
+    if (room.bytes == 0) return agpu_fail(ctx, AGPU_ERR_WORKSPACE, "paged_attention_weights: %d rows of %d heads need a larger scratch", tokens, n_heads);
+    More<WEIGHTS> more{};
+    more.weights = weights; more.page = weights_page_stride;
+    more.stats = reinterpret_cast<float2 *>(ctx->workspace);
+    more.scores = room.scores ? reinterpret_cast<float *>(ctx->workspace + room.scores) : nullptr;
+    return of_type(cache_type, [&](auto type) {
+        using T = decltype(type);
+        int32_t rc = attention_go<T, WEIGHTS>(ctx, p, paged::longest_row(p.held, window, sinks), more, ctx->workspace + room.bytes, ctx->ws_bytes - room.bytes);
+        if (rc != AGPU_OK || (!query_start && more.scores)) return rc;
+        hipLaunchKernelGGL((paged_weights_kernel<T>), dim3(2 * ctx->num_cus), dim3(256), 0, ctx->stream, p, more);
+        return AGPU_LAUNCH_CHECK(ctx, "paged_weights_kernel");
+    });
+}

@@ -27,7 +27,8 @@ namespace {
     X(agpu_int4_linear) X(agpu_ln_int4_linear) X(agpu_layer_norm) X(agpu_add_layer_norm_dual) X(agpu_gelu)                    \
     X(agpu_add_inplace) X(agpu_bias_add) X(agpu_softmax_rows) X(agpu_embedding) X(agpu_argmax_rows) X(agpu_split_qkv)         \
     X(agpu_concat_heads) X(agpu_attention) X(agpu_kv_append) X(agpu_gemm_f32) X(agpu_last_error_string)          \
-    X(agpu_paged_plan) X(agpu_paged_kv_append) X(agpu_paged_attention) X(agpu_sample)
+    X(agpu_paged_plan) X(agpu_paged_kv_append) X(agpu_paged_attention) X(agpu_paged_attention_shared)                        \
+    X(agpu_paged_attention_weights) X(agpu_paged_evict) X(agpu_paged_trim) X(agpu_sample)
 struct Lib {
 #define X(f) decltype(&f) f##_ = nullptr;
     AGPU_OPS(X)
@@ -532,6 +533,99 @@ PyObject *paged_attention(PyObject *const *a) {
     return given ? same(a[8]) : wrap(std::move(o));
 }
 
+// What paged_attention and the operators like it have in common: q, k_cache, v_cache; then block_tables, kv_lens, query_start; out behind them.
+struct Attends {
+    const at::Tensor &kc, &vc, &q, &tables, &lens, &start;
+    const bool ragged, given;
+    const int64_t tokens, heads, batch;
+    Attends(PyObject *q_, PyObject *k_, PyObject *v_, PyObject *tables_, PyObject *lens_, PyObject *start_, PyObject *out)
+        : kc(pages(k_, "k_cache [n_pages, n_kv_heads, page_size, d_head]")), vc(pages(v_, "v_cache [n_pages, n_kv_heads, page_size, d_head]")),
+          q(rows(q_, -1, -1, kc.size(3), "q [tokens, n_heads, d_head]")), tables(ints(tables_, {-1, -1}, "block_tables [batch, width]")),
+          lens(ints(lens_, {tables.size(0)}, "kv_lens [batch]")), start(start_ != Py_None ? ints(start_, {tables.size(0) + 1}, "query_start [batch + 1]") : lens),
+          ragged(start_ != Py_None), given(out != Py_None), tokens(q.size(0)), heads(q.size(1)), batch(tables.size(0)) {
+        same_cache(kc, vc);
+        if (!ragged && tokens != batch) shape_err("a row for each of " + str(batch) + " requests without query_start", str(tokens));
+        if (given) {
+            const at::Tensor &o = typed(out, at::kFloat, {tokens, heads, q.size(2)}, "out [tokens, n_heads, d_head]");
+            if (!o.is_contiguous()) shape_err("contiguous out", "strides " + str(o.strides()));
+            for (const at::Tensor *t : {&q, &kc, &vc})
+                if (o.is_alias_of(*t)) shape_err("out with memory of its own", "that of an input");
+        }
+    }
+    // (after what else there is to check of shapes)
+    template <class... T>
+    at::Tensor out(PyObject *o, const T &...others) const {
+        together(q, kc, vc, tables, lens, start, others...);
+        if (given) together(q, tensor(o));
+        return given ? tensor(o) : empty(q.sizes(), q);
+    }
+    const int32_t *starts() const { return ragged ? ip(start) : nullptr; }
+};
+// What each key of a cache was given: [n_pages, n_kv_heads, page_size], a page contiguous, pages anywhere
+const at::Tensor &weights_of(PyObject *o, const at::Tensor &cache) {
+    const int64_t heads = cache.size(1), size = cache.size(2);
+    const at::Tensor &t = typed(o, at::kFloat, {cache.size(0), heads, size}, "weights [n_pages, n_kv_heads, page_size]");
+    if ((size > 1 && t.stride(2) != 1) || (heads > 1 && t.stride(1) != size)) shape_err("contiguous pages of weights [n_kv_heads, page_size]", "strides " + str(t.strides()));
+    return t;
+}
+int64_t weights_stride(const at::Tensor &t) { return t.size(0) > 1 ? t.stride(0) : t.size(1) * t.size(2); }
+
+// q, k_cache, v_cache, prefix_tables, prefix_lens, prefix_of, block_tables, kv_lens, query_start, window, sinks, out
+PyObject *paged_attention_shared(PyObject *const *a) {
+    const Attends c(a[0], a[1], a[2], a[6], a[7], a[8], a[11]);
+    const at::Tensor &prefixes = ints(a[3], {-1, -1}, "prefix_tables [n_prefix, width]");
+    const at::Tensor &lens = ints(a[4], {prefixes.size(0)}, "prefix_lens [n_prefix]"), &of = ints(a[5], {c.batch}, "prefix_of [batch]");
+    at::Tensor o = c.out(a[11], prefixes, lens, of);
+    float *const op = written(o);
+    call(lib.agpu_paged_attention_shared_, context(c.q), data(c.q), c.q.stride(0), c.q.stride(1), c.kc.const_data_ptr(), c.vc.const_data_ptr(), page_stride(c.kc), page_stride(c.vc),
+         ip(prefixes), ip(lens), ip(of), ip(c.tables), ip(c.lens), c.starts(), op, i32(c.tokens), i32(c.batch), i32(c.heads), i32(c.kc.size(1)), i32(c.kc.size(0)), i32(c.kc.size(2)),
+         i32(prefixes.size(0)), i32(prefixes.size(1)), i32(c.tables.size(1)), i32(a[9]), i32(a[10]), i32(c.q.size(2)), cache_type(c.kc));
+    return c.given ? same(a[11]) : wrap(std::move(o));
+}
+
+// q, k_cache, v_cache, weights, block_tables, kv_lens, query_start, window, sinks, out
+PyObject *paged_attention_weights(PyObject *const *a) {
+    const Attends c(a[0], a[1], a[2], a[4], a[5], a[6], a[9]);
+    const at::Tensor &w = weights_of(a[3], c.kc);
+    for (const at::Tensor *t : {&c.q, &c.kc, &c.vc})
+        if (w.is_alias_of(*t)) shape_err("weights with memory of their own", "that of another argument");
+    if (c.given && w.is_alias_of(tensor(a[9]))) shape_err("weights with memory of their own", "that of another argument");
+    at::Tensor o = c.out(a[9], w);
+    float *const op = written(o), *const wp = written(w);
+    call(lib.agpu_paged_attention_weights_, context(c.q), data(c.q), c.q.stride(0), c.q.stride(1), c.kc.const_data_ptr(), c.vc.const_data_ptr(), page_stride(c.kc), page_stride(c.vc), wp,
+         weights_stride(w), ip(c.tables), ip(c.lens), c.starts(), op, i32(c.tokens), i32(c.batch), i32(c.heads), i32(c.kc.size(1)), i32(c.kc.size(0)), i32(c.kc.size(2)),
+         i32(c.tables.size(1)), i32(a[7]), i32(a[8]), i32(c.q.size(2)), cache_type(c.kc));
+    PyObject *const first = c.given ? same(a[9]) : wrap(std::move(o));
+    return Py_BuildValue("(NO)", first, a[3]);
+}
+
+// k_cache, v_cache, weights, block_tables, kv_lens, limit, keep, recent, sinks
+PyObject *paged_evict(PyObject *const *a) {
+    const at::Tensor &kc = pages(a[0], "k_cache [n_pages, n_kv_heads, page_size, d_head]"), &vc = pages(a[1], "v_cache [n_pages, n_kv_heads, page_size, d_head]");
+    same_cache(kc, vc);
+    const at::Tensor &w = weights_of(a[2], kc), &tables = ints(a[3], {-1, -1}, "block_tables [batch, width]"), &lens = ints(a[4], {tables.size(0)}, "kv_lens [batch]");
+    together(kc, vc, w, tables, lens);
+    const int32_t limit = i32(a[5]), keep = i32(a[6]), recent = i32(a[7]), sinks = i32(a[8]);
+    void *const kp = kc.mutable_data_ptr(), *const vp = vc.mutable_data_ptr();
+    float *const wp = written(w);
+    call(lib.agpu_paged_evict_, context(kc), kp, vp, page_stride(kc), page_stride(vc), wp, weights_stride(w), ip(tables), ip(lens), i32(tables.size(0)), i32(kc.size(1)),
+         i32(kc.size(0)), i32(kc.size(2)), i32(tables.size(1)), limit, keep, recent, sinks, i32(kc.size(3)), cache_type(kc));
+    return Py_BuildValue("(OOO)", a[0], a[1], a[2]);
+}
+
+// kv_lens, block_tables, free_pages, n_free, page_size, limit, keep
+PyObject *paged_trim(PyObject *const *a) {
+    const at::Tensor &tables = ints(a[1], {-1, -1}, "block_tables [batch, width]"), &lens = ints(a[0], {tables.size(0)}, "kv_lens [batch]");
+    const at::Tensor &stack = ints(a[2], {-1}, "free_pages [stack_size]"), &n_free = ints(a[3], {1}, "n_free [1]");
+    const int64_t batch = tables.size(0);
+    together(tables, lens, stack, n_free);
+    const int32_t size = i32(a[4]), limit = i32(a[5]), keep = i32(a[6]);
+    std::array<at::Tensor, 3> t = ints_in_one<3>({batch, batch, 1}, tables);
+    int32_t *const sp = iw(stack);
+    call(lib.agpu_paged_trim_, context(tables), ip(lens), ip(tables), sp, ip(n_free), iw(t[0]), iw(t[1]), iw(t[2]), i32(batch), i32(tables.size(1)), i32(stack.numel()), size, limit, keep);
+    return Py_BuildValue("(NNN)", wrap(std::move(t[0])), wrap(std::move(t[1])), wrap(std::move(t[2])));
+}
+
 // A setting of sample: a number for all rows, or a tensor with one a row
 struct PerRow {
     const at::Tensor *t = nullptr;
@@ -614,7 +708,8 @@ PyObject *forget(PyObject *, PyObject *handle) {
 PyMethodDef methods[] = {
     OP(int4_linear, 9), OP(layer_norm, 4), OP(add_layer_norm_dual, 6), OP(gelu, 2), OP(add_inplace, 2), OP(bias_add, 2), OP(softmax_rows, 1),
     OP(embedding, 4), OP(argmax_rows, 2), OP(split_qkv, 3), OP(concat_heads, 1), OP(attention, 6), OP(multi_head_flash_attention, 6),
-    OP(kv_append, 3), OP(gemm_f32, 2), OP(paged_plan, 7), OP(paged_kv_append, 5), OP(paged_attention, 9), OP(sample, 6),
+    OP(kv_append, 3), OP(gemm_f32, 2), OP(paged_plan, 7), OP(paged_kv_append, 5), OP(paged_attention, 9),
+    OP(paged_attention_shared, 12), OP(paged_attention_weights, 10), OP(paged_evict, 9), OP(paged_trim, 7), OP(sample, 6),
     {"bind", bind, METH_VARARGS, nullptr}, {"forget", forget, METH_O, nullptr}, {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_torch_ops", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -224,6 +224,33 @@ def paged_attention(q, k_cache, v_cache, block_tables, kv_lens, query_start=None
     return _native.paged_attention(q, k_cache, v_cache, block_tables, kv_lens, query_start, window, sinks, out)
 
 
+def paged_attention_shared(q, k_cache, v_cache, prefix_tables, prefix_lens, prefix_of, block_tables, kv_lens, query_start=None, window=0, sinks=0, out=None):
+    """paged_attention of requests that begin alike: request b is behind prefix prefix_of[b] (none: -1), whose prefix_lens[i] keys on the pages prefix_tables[i] the
+    cache holds once, and which are read once for all requests behind it.  kv_lens, block_tables and query_start are about the requests' own pages; window and sinks
+    are about positions with the prefix.  256 prefixes at most; their pages are the caller's (no request of paged_plan that ends gives them back)."""
+    return _native.paged_attention_shared(q, k_cache, v_cache, prefix_tables, prefix_lens, prefix_of, block_tables, kv_lens, query_start, window, sinks, out)
+
+
+def paged_attention_weights(q, k_cache, v_cache, weights, block_tables, kv_lens, query_start=None, window=0, sinks=0, out=None):
+    """paged_attention that also adds up, in place, what weight (share of the softmax) each key was given: weights [n_pages, n_kv_heads, page_size] float32, over the rows of the call
+    and the query heads of a K/V head.  Keys of the call's own rows begin at zero.  A page belongs to one request only.  Returns (out, weights)."""
+    return _native.paged_attention_weights(q, k_cache, v_cache, weights, block_tables, kv_lens, query_start, window, sinks, out)
+
+
+def paged_evict(k_cache, v_cache, weights, block_tables, kv_lens, limit, keep, recent=0, sinks=0):
+    """Cuts requests of more than `limit` positions down to `keep`, in place, each K/V head by itself: the first `sinks` stay, the last `recent`, and of the others those with the most
+    weight (of equal ones the first).  What stays keeps its place below `keep`, or moves into that of an evicted one.  For every layer; paged_trim then shortens the
+    lengths.  limit - keep >= recent keeps the latest positions the last ones.  Returns (k_cache, v_cache, weights)."""
+    return _native.paged_evict(k_cache, v_cache, weights, block_tables, kv_lens, limit, keep, recent, sinks)
+
+
+def paged_trim(kv_lens, block_tables, free_pages, n_free, page_size, limit, keep):
+    """Lengths and pages behind paged_evict, once a step: -> (kv_lens [batch], evicted [batch], n_free [1]).  Requests of more than `limit` positions have `keep` now, and the pages behind
+    are on the stack free_pages (in place).  evicted is how many positions went: positions of paged_plan are places, so that a model whose embeddings go by
+    position adds up what was evicted."""
+    return _native.paged_trim(kv_lens, block_tables, free_pages, n_free, page_size, limit, keep)
+
+
 def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     """The next token of each row of logits [..., n] from given numbers u in [0, 1), one a row -> int32 [...].  The settings are numbers, or tensors with
     one a row: temperature, then the top_k first candidates (0: all), of those the nucleus of top_p, of those the ones with at least min_p of the

@@ -423,6 +423,47 @@ int32_t agpu_paged_attention(agpu_ctx *ctx, const float *q, int64_t q_token_stri
                              const int32_t *kv_lens, const int32_t *query_start, float *o, int32_t tokens, int32_t batch, int32_t n_heads,
                              int32_t n_kv_heads, int32_t n_pages, int32_t page_size, int32_t table_width, int32_t window, int32_t sinks,
                              int32_t d_head, int32_t cache_type);
+/* The same, over the keys of a prefix and then of each request's own pages: requests that begin alike hold what they share once, and it is read once for all of them.
+ *   prefix_tables [n_prefix][prefix_width], prefix_lens [n_prefix]   pages and lengths of the prefixes (256 at most), like block_tables and kv_lens
+ *   prefix_of [batch]                                                which of them a request is behind; outside 0 .. n_prefix - 1: none
+ * Place p of a request's own kv_lens is position prefix_lens[prefix_of[b]] + p, for what a row sees: every key up to its own position, with window > 0 only those
+ * nearer than that or among the first `sinks` positions, which are the prefix's.  A prefix is nobody's in agpu_paged_plan's view, or a request of its own that has no new tokens: its
+ * pages stay until the caller gives them back.  The rows of all requests behind a prefix go through the matrix cores there, as those of a request with more than eight do. */
+int32_t agpu_paged_attention_shared(agpu_ctx *ctx, const float *q, int64_t q_token_stride, int64_t q_head_stride, const void *k_cache,
+                                    const void *v_cache, int64_t k_page_stride, int64_t v_page_stride, const int32_t *prefix_tables,
+                                    const int32_t *prefix_lens, const int32_t *prefix_of, const int32_t *block_tables, const int32_t *kv_lens,
+                                    const int32_t *query_start, float *o, int32_t tokens, int32_t batch, int32_t n_heads, int32_t n_kv_heads,
+                                    int32_t n_pages, int32_t page_size, int32_t n_prefix, int32_t prefix_width, int32_t table_width,
+                                    int32_t window, int32_t sinks, int32_t d_head, int32_t cache_type);
+
+/* A cache with a budget.  Per layer agpu_paged_attention_weights in place of agpu_paged_attention, and agpu_paged_evict behind it; then, once a step, agpu_paged_trim.
+ *   weights   [n_pages][n_kv_heads][page_size] float, pages weights_page_stride elements apart: beside K and V of a layer, what weight each key was given so far
+ * agpu_paged_attention that adds up its weights: the weight of key j in a row is its share of the softmax, in 0 .. 1; those of the call's rows, and of the query heads of
+ * a K/V head, are added to what the key has.  Keys of the request's rows (the last query_start[b + 1] - query_start[b] of its kv_lens[b] positions, whether or not q has all of
+ * the rows) begin at zero.  Requests without a row in q, and keys that no row sees, keep what they have.  A page belongs to one request only.  The order of a sum is fixed:
+ * the same call gives the same bits. */
+int32_t agpu_paged_attention_weights(agpu_ctx *ctx, const float *q, int64_t q_token_stride, int64_t q_head_stride, const void *k_cache,
+                                     const void *v_cache, int64_t k_page_stride, int64_t v_page_stride, float *weights,
+                                     int64_t weights_page_stride, const int32_t *block_tables, const int32_t *kv_lens,
+                                     const int32_t *query_start, float *o, int32_t tokens, int32_t batch, int32_t n_heads, int32_t n_kv_heads,
+                                     int32_t n_pages, int32_t page_size, int32_t table_width, int32_t window, int32_t sinks, int32_t d_head,
+                                     int32_t cache_type);
+/* Cuts requests of more than `limit` positions down to `keep` (<= limit): in each K/V head by itself the first `sinks` positions stay, the last `recent` ones, and of the others
+ * those with the most weight, of equal ones the first (no number is less than all numbers, and a page outside the cache less than that).  Those that stay keep their places
+ * below `keep`; the others go, K, V and weight, in order into the places of evicted ones.  Places from `keep` on are left as they were, and kv_lens too: it is agpu_paged_trim that
+ * shortens them, for all layers.  Order among places is lost except that the first `sinks` stay where they are and that what came since the last time is behind the rest:
+ * `recent` means the latest positions as long as limit - keep >= recent, and windows of agpu_paged_attention no longer mean distances.
+ * A page belongs to one request only; a row of the table stands for 2^20 positions at most. */
+int32_t agpu_paged_evict(agpu_ctx *ctx, void *k_cache, void *v_cache, int64_t k_page_stride, int64_t v_page_stride, float *weights,
+                         int64_t weights_page_stride, const int32_t *block_tables, const int32_t *kv_lens, int32_t batch, int32_t n_kv_heads,
+                         int32_t n_pages, int32_t page_size, int32_t table_width, int32_t limit, int32_t keep, int32_t recent, int32_t sinks,
+                         int32_t d_head, int32_t cache_type);
+/* Lengths and pages behind agpu_paged_evict: kv_lens_out [batch] is `keep` where kv_lens is more than `limit` (and kv_lens, within what the table has pages for, elsewhere), evicted
+ * [batch] how many positions that is less, to be added up by a caller whose embeddings go by position; the pages behind `keep` go onto the stack free_pages [stack_size] of n_free [1]
+ * pages, in the order of requests and positions (what has no place there is lost), n_free_out [1] of them.  The outputs do not overlap the inputs.  4096 requests at most. */
+int32_t agpu_paged_trim(agpu_ctx *ctx, const int32_t *kv_lens, const int32_t *block_tables, int32_t *free_pages, const int32_t *n_free, int32_t *kv_lens_out,
+                        int32_t *evicted, int32_t *n_free_out, int32_t batch, int32_t table_width, int32_t stack_size, int32_t page_size, int32_t limit,
+                        int32_t keep);
 
 /* ---- f32 GEMM (the reference model's f32 LM head) --------------------------------------- */
 

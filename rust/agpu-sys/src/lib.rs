@@ -136,6 +136,10 @@ extern "C" {
     pub fn agpu_paged_plan(ctx: *mut agpu_ctx, cached_lens: *const i32, new_lens: *const i32, block_tables: *mut i32, free_pages: *mut i32, n_free: *const i32, kv_lens: *mut i32, query_start: *mut i32, slots: *mut i32, positions: *mut i32, n_free_out: *mut i32, batch: i32, table_width: i32, stack_size: i32, page_size: i32, max_tokens: i32) -> i32;
     pub fn agpu_paged_kv_append(ctx: *mut agpu_ctx, k: *const f32, v: *const f32, k_token_stride: i64, k_head_stride: i64, v_token_stride: i64, v_head_stride: i64, k_cache: *mut c_void, v_cache: *mut c_void, k_page_stride: i64, v_page_stride: i64, slots: *const i32, tokens: i32, n_kv_heads: i32, n_pages: i32, page_size: i32, d_head: i32, cache_type: i32) -> i32;
     pub fn agpu_paged_attention(ctx: *mut agpu_ctx, q: *const f32, q_token_stride: i64, q_head_stride: i64, k_cache: *const c_void, v_cache: *const c_void, k_page_stride: i64, v_page_stride: i64, block_tables: *const i32, kv_lens: *const i32, query_start: *const i32, o: *mut f32, tokens: i32, batch: i32, n_heads: i32, n_kv_heads: i32, n_pages: i32, page_size: i32, table_width: i32, window: i32, sinks: i32, d_head: i32, cache_type: i32) -> i32;
+    pub fn agpu_paged_attention_shared(ctx: *mut agpu_ctx, q: *const f32, q_token_stride: i64, q_head_stride: i64, k_cache: *const c_void, v_cache: *const c_void, k_page_stride: i64, v_page_stride: i64, prefix_tables: *const i32, prefix_lens: *const i32, prefix_of: *const i32, block_tables: *const i32, kv_lens: *const i32, query_start: *const i32, o: *mut f32, tokens: i32, batch: i32, n_heads: i32, n_kv_heads: i32, n_pages: i32, page_size: i32, n_prefix: i32, prefix_width: i32, table_width: i32, window: i32, sinks: i32, d_head: i32, cache_type: i32) -> i32;
+    pub fn agpu_paged_attention_weights(ctx: *mut agpu_ctx, q: *const f32, q_token_stride: i64, q_head_stride: i64, k_cache: *const c_void, v_cache: *const c_void, k_page_stride: i64, v_page_stride: i64, weights: *mut f32, weights_page_stride: i64, block_tables: *const i32, kv_lens: *const i32, query_start: *const i32, o: *mut f32, tokens: i32, batch: i32, n_heads: i32, n_kv_heads: i32, n_pages: i32, page_size: i32, table_width: i32, window: i32, sinks: i32, d_head: i32, cache_type: i32) -> i32;
+    pub fn agpu_paged_evict(ctx: *mut agpu_ctx, k_cache: *mut c_void, v_cache: *mut c_void, k_page_stride: i64, v_page_stride: i64, weights: *mut f32, weights_page_stride: i64, block_tables: *const i32, kv_lens: *const i32, batch: i32, n_kv_heads: i32, n_pages: i32, page_size: i32, table_width: i32, limit: i32, keep: i32, recent: i32, sinks: i32, d_head: i32, cache_type: i32) -> i32;
+    pub fn agpu_paged_trim(ctx: *mut agpu_ctx, kv_lens: *const i32, block_tables: *const i32, free_pages: *mut i32, n_free: *const i32, kv_lens_out: *mut i32, evicted: *mut i32, n_free_out: *mut i32, batch: i32, table_width: i32, stack_size: i32, page_size: i32, limit: i32, keep: i32) -> i32;
     pub fn agpu_sample(ctx: *mut agpu_ctx, logits: *const f32, u: *const f32, tokens_out: *mut i32, rows: i32, n: i32, temperature: f32, top_k: i32, top_p: f32, min_p: f32, temperatures: *const f32, top_ks: *const i32, top_ps: *const f32, min_ps: *const f32) -> i32;
     pub fn agpu_gemm_f32(ctx: *mut agpu_ctx, a: *const f32, b: *const f32, c: *mut f32, M: i32, N: i32, K: i32) -> i32;
     // ---- include/agpu_gpt2.h ----
