@@ -50,7 +50,7 @@ struct More<SHARED> {
     // of all in ml [runs][tokens][n_heads].
     float *rest;
     float2 *ml;
-    int *run, most;  // the length of a run, as the device has chosen it, and how many a prefix may have
+    int *before;  // [batch] how many runs there are of what a request's rows have seen of their prefix
     __device__ __forceinline__ int len(int g) const { return (unsigned)g < (unsigned)n_prefix ? max(min(lens[g], held), 0) : 0; }
 };
 template <>
@@ -133,37 +133,8 @@ __device__ __forceinline__ int request_of(const int *query_start, int batch, int
 // The first positions that stay visible, of those on a request's own pages.
 template <int MODE>
 __device__ __forceinline__ int sinks_of(const PagedAttn &p, const More<MODE> &more, int b) {
-    if constexpr (MODE == SHARED) return max(p.sinks - more.len(more.of[b]), 0);
+    if constexpr (MODE == SHARED) return p.sinks > 0 ? max(p.sinks - more.len(more.of[b]), 0) : 0;
     return p.sinks;
-}
-
-// What the rows of a head of token t have seen of a prefix joined to o (dimension `lane`), m and l of the rest, by a wave.
-__device__ __forceinline__ void join_prefix(const PagedAttn &p, const More<SHARED> &more, int b, int t, int head, int lane, float &acc, float &top, float &sum) {
-    const int len = more.len(more.of[b]);
-    if (len == 0) return;  // uniform
-    const int runs = paged::runs_of(len, *more.run, more.most).runs;
-    const size_t row = (size_t)t * p.n_heads + head, rows = (size_t)p.tokens * p.n_heads;
-    const float2 ml = lane < runs ? more.ml[lane * rows + row] : make_float2(-INFINITY, 0.0f);
-    float x[8];
-    auto eight = [&](int r) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const int i = min(r + e, runs - 1);
-            x[e] = (i == 0 ? p.o + row * DH : more.rest + ((i - 1) * rows + row) * DH)[lane];
-        }
-        __builtin_amdgcn_sched_barrier(0);
-    };
-    eight(0);
-    const float now = fmaxf(top, wave_max(ml.x)), f = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - now);
-    const float keep = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - now);
-    top = now;
-    sum = fmaf(sum, keep, wave_sum(ml.y * f));
-    acc = top == -INFINITY ? 0.0f : acc * keep;
-    for (int r = 0; r < runs; r += 8) {
-        if (r > 0) eight(r);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) acc = r + e < runs ? fmaf(x[e], __shfl(f, r + e, kWave), acc) : acc;
-    }
 }
 
 // What a workgroup of W waves needs in LDS for a token's G query heads.
@@ -206,6 +177,26 @@ __device__ __forceinline__ void token_run(const PagedAttn &p, const More<MODE> &
         l[g] = 0.0f;
 #pragma unroll
         for (int e = 0; e < EL; ++e) o[g][e] = 0.0f;
+    }
+    // What the rows have seen of a prefix counts as keys of the first run: lanes of a key take a run of it each, as many as there are.  Of few heads it is on its way before
+    // the keys are.
+    int before = 0;
+    float2 seen_ml[G];
+    float4 seen_o[G][EL / 4];
+    auto load_seen = [&](int r, int g) {
+        if constexpr (MODE == SHARED) {
+            const size_t rows = (size_t)p.tokens * p.n_heads, row = (size_t)t * p.n_heads + head0 + min(g, heads - 1);
+            const float *from = (r == 0 ? p.o + row * DH : more.rest + ((r - 1) * rows + row) * DH) + EL * sub;
+            seen_ml[g] = more.ml[r * rows + row];
+#pragma unroll
+            for (int e = 0; e < EL / 4; ++e) seen_o[g][e] = *reinterpret_cast<const float4 *>(from + 4 * e);
+        }
+    };
+    if constexpr (MODE == SHARED) {
+        before = run == 0 ? more.before[b] : 0;
+        if (G <= 2 && wave + W * own < before)
+#pragma unroll
+            for (int g = 0; g < G; ++g) load_seen(wave + W * own, g);
     }
     bool at_once = false;
     if constexpr (MODE == WEIGHTS) at_once = more.at_once(p.query_start ? p.query_start[b + 1] - p.query_start[b] : 1, p.group.size);
@@ -281,6 +272,22 @@ __device__ __forceinline__ void token_run(const PagedAttn &p, const More<MODE> &
             }
         }
     }
+    if constexpr (MODE == SHARED)
+        for (int r = wave + W * own; r < before; r += W * KEYS)
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                if (G > 2 || r >= W * KEYS) load_seen(r, g);
+                const float2 ml = seen_ml[g];
+                const float now = fmaxf(m[g], ml.x), keep = m[g] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[g] - now), f = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - now);
+                m[g] = now;
+                l[g] = fmaf(ml.y, f, l[g] * keep);
+#pragma unroll
+                for (int e = 0; e < EL; e += 4) {
+                    const float4 x = seen_o[g][e / 4];
+                    o[g][e] = fmaf(x.x, f, o[g][e] * keep); o[g][e + 1] = fmaf(x.y, f, o[g][e + 1] * keep);
+                    o[g][e + 2] = fmaf(x.z, f, o[g][e + 2] * keep); o[g][e + 3] = fmaf(x.w, f, o[g][e + 3] * keep);
+                }
+            }
     // The wave's keys together: the rows of 16 lanes are added in two steps that halve the values a lane has, so that each row ends with a quarter of them;
     // then the waves.
     constexpr int N = G * EL;
@@ -315,7 +322,6 @@ __device__ __forceinline__ void token_run(const PagedAttn &p, const More<MODE> &
     float *out = p.o + ((size_t)t * p.n_heads + head0) * DH + lane;
     // A head's result, and what there is to do besides.
     auto finish = [&](int g, float acc, float top, float sum) {
-        if constexpr (MODE == SHARED) join_prefix(p, more, b, t, head0 + g, lane, acc, top, sum);
         out[g * DH] = sum == 0.0f ? 0.0f : acc / sum;
         if constexpr (MODE == WEIGHTS) {
             const float unit = top == -INFINITY ? 0.0f : top, share = sum == 0.0f ? 0.0f : 1.0f / sum;
@@ -683,31 +689,17 @@ __device__ __forceinline__ float sum_of_halves(float v) {
 template <int MODE>
 struct TileOf {
     int start, tokens, first;
-    PageDiv group;
     __device__ __forceinline__ int token(int i) const { return start + i; }
     __device__ __forceinline__ int pos(int i) const { return first + i; }
-    // the smallest and the largest position of rows a .. b
-    __device__ __forceinline__ int least(int a, int) const { return first + group.page(a); }
-    __device__ __forceinline__ int most(int, int b) const { return first + group.page(b); }
 };
 // The rows behind a prefix: tokens of any requests, those of this tile (from `first` on) listed in LDS.
 template <>
 struct TileOf<PREFIX> {
     const int *list, *positions;
     int first, tokens;
-    PageDiv group;
     __device__ __forceinline__ int token(int i) const { return list[i - first]; }
     __device__ __forceinline__ int pos(int i) const { return positions[i - first]; }
-    __device__ __forceinline__ int least(int a, int b) const {
-        int v = INT32_MAX;
-        for (int i = group.page(a); i <= group.page(b); ++i) v = min(v, pos(i));
-        return v;
-    }
-    __device__ __forceinline__ int most(int a, int b) const {
-        int v = INT32_MIN;
-        for (int i = group.page(a); i <= group.page(b); ++i) v = max(v, pos(i));
-        return v;
-    }
+    int pos0, pos1;  // the smallest and the largest of the tile's positions
 };
 
 // Up to 128 rows of a request (its tokens' heads of one K/V head, token by token) over a run of the keys that any of them sees, by four waves of 32 rows, which
@@ -724,7 +716,10 @@ __device__ __forceinline__ void tile_run(const PagedAttn &p, const More<MODE> &m
     const int sinks = sinks_of(p, more, b);
     int held = p.held;
     if constexpr (MODE == PREFIX) held = more.len(b);
-    const paged::TileKeys keys = paged::tile_keys(of.least(first_row, last_row), of.most(first_row, last_row), held, p.window, sinks);
+    int pos0, pos1;
+    if constexpr (MODE == PREFIX) pos0 = of.pos0, pos1 = of.pos1;
+    else pos0 = of.first + p.group.page(first_row), pos1 = of.first + p.group.page(last_row);
+    const paged::TileKeys keys = paged::tile_keys(pos0, pos1, held, p.window, sinks);
     const int gap = keys.gap;
     const paged::RunsOf cuts = paged::runs_of(MODE == PREFIX ? held : keys.count, cut.run, cut.most);  // (of a prefix the same for all rows)
     const int runs = cuts.runs;
@@ -734,8 +729,8 @@ __device__ __forceinline__ void tile_run(const PagedAttn &p, const More<MODE> &m
     const int row = min(first_row + 32 * wave + c, last_row), token = p.group.page(row), head = h * group + (row - token * group);
     const bool mine = first_row + 32 * wave + c <= last_row, any = first_row + 32 * wave <= last_row;
     const int t = of.token(token), pos = of.pos(token);
-    const int wave_first = min(first_row + 32 * wave, last_row), wave_last = min(first_row + 32 * wave + 31, last_row);
-    const int wave_pos0 = of.least(wave_first, wave_last), wave_pos1 = of.most(wave_first, wave_last);
+    int wave_pos0 = of.pos(p.group.page(min(first_row + 32 * wave, last_row))), wave_pos1 = of.pos(p.group.page(min(first_row + 32 * wave + 31, last_row)));
+    if constexpr (MODE == PREFIX) wave_pos0 = pos0, wave_pos1 = pos1;  // (those of requests in no order)
     // which keys the row sees, and below which of those that are no sinks its wave's last row sees none
     const paged::RowKeys see = paged::row_keys(keys, pos, p.window, sinks);
     const int wave_low = paged::row_keys(keys, wave_pos1, p.window, sinks).low;
@@ -968,7 +963,7 @@ __device__ __forceinline__ void tile_run(const PagedAttn &p, const More<MODE> &m
     auto store = [&](float sum) {
         if (!mine) return;
         if constexpr (MODE == SHARED) {
-            const int len = more.len(more.of[b]), pre = len > 0 ? paged::runs_of(len, *more.run, more.most).runs : 0;
+            const int pre = more.before[b];
             const size_t rows_all = (size_t)p.tokens * p.n_heads;
             for (int i = 0; i < pre; ++i) {
                 const float2 ml = more.ml[i * rows_all + row_at];
@@ -1175,7 +1170,7 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(const PagedAttn p, R
         if (token < 0) {
             if (q_len <= slots || tile < 0 || tile * TILE_ROWS >= q_len * group) continue;
             const int item = (start * group / TILE_ROWS + b + tile) * p.n_kv + h;
-            tile_run<T>(p, more, *reinterpret_cast<TileShared<T> *>(smem), tile_cut, b, TileOf<MODE>{start, q_len, pos_first, p.group}, h, tile * TILE_ROWS, run, item);
+            tile_run<T>(p, more, *reinterpret_cast<TileShared<T> *>(smem), tile_cut, b, TileOf<MODE>{start, q_len, pos_first}, h, tile * TILE_ROWS, run, item);
         } else {
             if (token >= q_len || q_len > slots) continue;
             token_run<T, G, 4, 4>(p, more, *reinterpret_cast<TokenShared<G, 4> *>(smem), token_cut, start + token, b, pos_first + token, h, h * group, group, run,
