@@ -24,6 +24,7 @@ struct EvictArgs {
 
 // Positions of a thread that are in registers at a time: position e * 512 + tid of a block.
 constexpr int kEvictThreads = 512, kEvictWaves = kEvictThreads / 64, kEvictEach = 8, kEvictListed = 1024;
+constexpr int kBins = 2048, kClose = 64;  // how many are told apart one by one
 
 // Larger for larger weights; zeros of both signs are equal; no number is less than all numbers, and a page outside the cache (0) less than that.
 __device__ __forceinline__ uint32_t order_of(float w) {
@@ -32,9 +33,14 @@ __device__ __forceinline__ uint32_t order_of(float w) {
 }
 
 struct EvictShared {
-    int counts[2][kEvictWaves][3];
-    int ties[kEvictEach * kEvictWaves];  // of each 64 positions of a block: how many weigh the least
-    int before[kEvictThreads], wave_sums[kEvictWaves];
+    int bins[kBins];
+    int wave_sums[kEvictWaves];
+    int found[3];  // the bin that what stays ends in, how many are above it, and in it
+    int n_close;
+    uint32_t close_key[kClose];
+    int close_at[kClose];
+    int ties[kEvictEach * kEvictWaves];  // of each 64 positions of a block
+    int before[kEvictThreads];           // of each 64 positions: places of evicted ones, and in the upper half those that move
     int to[kEvictListed], from[kEvictListed];  // positions
 };
 
@@ -60,7 +66,7 @@ __global__ __launch_bounds__(kEvictThreads) void paged_evict_kernel(const EvictA
     };
     auto middle = [&](int i) { return i >= p.sinks && i < n - p.recent; };
     uint32_t key[kEvictEach];
-    auto load = [&](int block) {
+    auto load = [&](int block) __attribute__((always_inline)) {
         int page[kEvictEach], slot[kEvictEach];
 #pragma unroll
         for (int e = 0; e < kEvictEach; ++e) {
@@ -72,62 +78,61 @@ __global__ __launch_bounds__(kEvictThreads) void paged_evict_kernel(const EvictA
         for (int e = 0; e < kEvictEach; ++e) key[e] = slot[e] >= 0 ? order_of(p.weights[page[e] * p.w_page + slot[e]]) : 0;
     };
     load(0);
-    // The largest `least` that has `need` keys or more from it on.
-    uint32_t least = need > 0 ? 0u : 0xffffffffu;
-    bool exact = need == 0;  // just as many
-    for (int bit = 30; bit >= 0 && !exact; bit -= 2) {
-        int count[3] = {0, 0, 0};
+    // The weight that what stays ends in, 11, 11 and 10 bits at a time: keys of the right upper bits (`least` >> upto) are counted by the next ones, until those that are not decided
+    // are few, or all stay.  (The first 11 bits are a quarter of an octave.)
+    uint32_t least = 0;
+    int upto = 32, left = need, close = n - p.sinks - p.recent;  // of the `close` keys that agree with `least` down to bit `upto`, `left` stay
+    while (left > 0 && left < close && close > kClose && upto > 0) {
+        const int bits = upto > 10 ? 11 : 10, shift = upto - bits, bins = 1 << bits;
+        for (int i = tid; i < bins; i += kEvictThreads) s.bins[i] = 0;
+        __syncthreads();
         for (int block = 0; block < blocks; ++block) {
             if (blocks > 1) load(block);
 #pragma unroll
-            for (int e = 0; e < kEvictEach; ++e)
-#pragma unroll
-                for (int c = 0; c < 3; ++c) count[c] += __popcll(__ballot(key[e] >= (least | (uint32_t)(c + 1) << bit)));
-        }
-        int(&counts)[kEvictWaves][3] = s.counts[bit >> 1 & 1];  // (what the other one holds has been read before the next barrier)
-        if (lane == 0)
-#pragma unroll
-            for (int c = 0; c < 3; ++c) counts[wave][c] = count[c];
-        __syncthreads();
-        int all[3] = {0, 0, 0};
-#pragma unroll
-        for (int w = 0; w < kEvictWaves; ++w)
-#pragma unroll
-            for (int c = 0; c < 3; ++c) all[c] += counts[w][c];
-        const uint32_t low = least;
-#pragma unroll
-        for (int c = 0; c < 3; ++c)
-            if (all[c] >= need) {
-                least = low | (uint32_t)(c + 1) << bit;
-                exact = all[c] == need;
+            for (int e = 0; e < kEvictEach; ++e) {
+                const bool in = middle(block * BLOCK + e * kEvictThreads + tid) && (upto == 32 || key[e] >> (upto & 31) == least >> (upto & 31));
+                if (in) atomicAdd(&s.bins[key[e] >> shift & (bins - 1)], 1);
             }
-    }
-    int ties = 0;  // how many of those that weigh the least stay: the first ones
-    if (!exact) {
-        int more = 0;
-        for (int block = 0; block < blocks; ++block) {
-            if (blocks > 1) load(block);
-#pragma unroll
-            for (int e = 0; e < kEvictEach; ++e) more += __popcll(__ballot(key[e] > least));
         }
         __syncthreads();
-        if (lane == 0) s.counts[0][wave][0] = more;
+        // from the top down: a thread has a few bins
+        const int each = bins / kEvictThreads, first = bins - 1 - each * tid;
+        int own = 0;
+        for (int i = 0; i < each; ++i) own += s.bins[first - i];
+        const int sum = wave_running_sum(own);
+        if (lane == 63) s.wave_sums[wave] = sum;
         __syncthreads();
-        ties = need;
+        int above = sum - own;
 #pragma unroll
-        for (int w = 0; w < kEvictWaves; ++w) ties -= s.counts[0][w][0];
+        for (int w = 0; w < kEvictWaves; ++w) above += w < wave ? s.wave_sums[w] : 0;
+        if (above < left && above + own >= left) {  // (one thread's)
+            int i = 0;
+            while (above + s.bins[first - i] < left) above += s.bins[first - i++];
+            s.found[0] = first - i;
+            s.found[1] = above;
+            s.found[2] = s.bins[first - i];
+        }
+        __syncthreads();
+        least |= (uint32_t)s.found[0] << shift;
+        left -= s.found[1];
+        close = s.found[2];
+        upto = shift;
     }
-    // Who stays, a bit a position.
+    // Who stays, a bit a position: above all that are close; of these none, all, the first of equal ones, or what comes out one by one.
+    const bool all_close = left > 0 && left >= close, one_by_one = left > 0 && !all_close && upto > 0, equal = left > 0 && !all_close && upto == 0;
+    if (tid == 0) s.n_close = 0;
+    int ties = left;
+    __syncthreads();
     for (int block = 0; block < blocks; ++block) {
         if (blocks > 1) load(block);
-        uint64_t equal[kEvictEach];
         int before = 0, all = 0;
-        if (!exact) {
+        uint64_t same[kEvictEach];
+        if (equal) {
             __syncthreads();
 #pragma unroll
             for (int e = 0; e < kEvictEach; ++e) {
-                equal[e] = __ballot(middle(block * BLOCK + e * kEvictThreads + tid) && key[e] == least);
-                if (lane == 0) s.ties[e * kEvictWaves + wave] = __popcll(equal[e]);
+                same[e] = __ballot(middle(block * BLOCK + e * kEvictThreads + tid) && key[e] == least);
+                if (lane == 0) s.ties[e * kEvictWaves + wave] = __popcll(same[e]);
             }
             __syncthreads();
             static_assert(kEvictEach * kEvictWaves == 64, "");
@@ -139,9 +144,15 @@ __global__ __launch_bounds__(kEvictThreads) void paged_evict_kernel(const EvictA
 #pragma unroll
         for (int e = 0; e < kEvictEach; ++e) {
             const int i = block * BLOCK + e * kEvictThreads + tid;
-            bool stay = i < n && (!middle(i) || key[e] > least);
-            if (exact) stay = stay || (middle(i) && key[e] == least);
-            else if (middle(i) && key[e] == least) stay = __builtin_amdgcn_readlane(before, e * kEvictWaves + __builtin_amdgcn_readfirstlane(wave)) + bits_below(equal[e]) < ties;
+            const bool inside = middle(i), near = inside && (upto == 32 || key[e] >> (upto & 31) == least >> (upto & 31));
+            bool stay = i < n && (!inside || (!near && key[e] > least));
+            if (near && all_close) stay = true;
+            if (near && equal) stay = __builtin_amdgcn_readlane(before, e * kEvictWaves + __builtin_amdgcn_readfirstlane(wave)) + bits_below(same[e]) < ties;
+            if (near && one_by_one) {
+                const int at = atomicAdd(&s.n_close, 1);  // (in any order: what comes out does not depend on it)
+                s.close_key[at] = key[e];
+                s.close_at[at] = i;
+            }
             const uint64_t word = __ballot(stay);
             const int chunk = (block * kEvictEach + e) * kEvictWaves + wave;
             if (lane == 0 && chunk < chunks) stays[chunk] = word;
@@ -149,27 +160,40 @@ __global__ __launch_bounds__(kEvictThreads) void paged_evict_kernel(const EvictA
         ties -= all;
     }
     __syncthreads();
+    if (one_by_one) {
+        static_assert(8 * kClose == kEvictThreads, "");
+        const int own = min(tid >> 3, close - 1), at = s.close_at[own];  // eight threads for each
+        const uint32_t mine = s.close_key[own];
+        int before = 0;
+#pragma unroll
+        for (int e = 0; e < kClose / 8; ++e) {
+            const int i = 8 * e + (tid & 7), k = min(i, close - 1);
+            before += i < close && (s.close_key[k] > mine || (s.close_key[k] == mine && s.close_at[k] < at));
+        }
+        before += (int)dpp_move_u32<0xb1, 0xf>(0, before);   // quad_perm [1,0,3,2]
+        before += (int)dpp_move_u32<0x4e, 0xf>(0, before);   // quad_perm [2,3,0,1]
+        before += (int)dpp_move_u32<0x141, 0xf>(0, before);  // row_half_mirror
+        if ((tid & 7) == 0 && tid >> 3 < close && before < left) atomicOr(reinterpret_cast<unsigned int *>(stays) + (at >> 5), 1u << (at & 31));
+        __syncthreads();
+    }
     // Of 64 positions those that are evicted and get another one's key, or those that move.
     auto word = [&](bool hole, int chunk) {
         const uint64_t kept = first_bits(p.keep - 64 * chunk), stay = stays[chunk];
         return hole ? ~stay & kept : stay & ~kept;
     };
-    int moves = 0;  // as many as places of evicted ones
-    for (int chunk = tid; chunk < chunks; chunk += kEvictThreads) moves += __popcll(word(false, chunk));
-    moves = __builtin_amdgcn_readlane(wave_running_sum(moves), 63);
-    if (lane == 0) s.wave_sums[wave] = moves;
-    __syncthreads();
-    moves = 0;
-#pragma unroll
-    for (int w = 0; w < kEvictWaves; ++w) moves += s.wave_sums[w];
-    __syncthreads();
-    // Numbers done .. done + kEvictListed - 1 of one kind, from the chunks `first` on, before which there are `base`.
-    auto list = [&](bool hole, int done, int &first, int &base, int *out) {
+    // Numbers done .. done + kEvictListed - 1 of the ones or the other, or both, of 64 * 512 positions at a time, beginning with the group in which the first of them is.
+    struct Cursor {
+        int group, before;  // and how many there are before that group
+    };
+    Cursor hole = {0, 0}, move = {p.keep / (64 * kEvictThreads), 0};
+    int moves = 1 << 30;  // (known when all positions have been gone through)
+    auto list = [&](bool holes, bool movers, int done) __attribute__((always_inline)) {
         for (;;) {
-            const int chunk = first + tid, count = chunk < chunks ? __popcll(word(hole, chunk)) : 0, upto = wave_running_sum(count);
-            if (lane == 63) s.wave_sums[wave] = upto;
+            const int group = holes ? hole.group : move.group, chunk = group * kEvictThreads + tid;
+            const int own = chunk < chunks ? __popcll(word(true, chunk)) | __popcll(word(false, chunk)) << 16 : 0, sum = wave_running_sum(own);
+            if (lane == 63) s.wave_sums[wave] = sum;
             __syncthreads();
-            int before = base - done + upto - count, all = 0;
+            int before = sum - own, all = 0;
 #pragma unroll
             for (int w = 0; w < kEvictWaves; ++w) {
                 if (w < wave) before += s.wave_sums[w];
@@ -177,53 +201,66 @@ __global__ __launch_bounds__(kEvictThreads) void paged_evict_kernel(const EvictA
             }
             s.before[tid] = before;
             __syncthreads();
-            for (int c = wave; c < kEvictThreads && first + c < chunks; c += kEvictWaves) {
-                const int rank = s.before[c];
-                if (rank >= kEvictListed) break;
-                const uint64_t bits = word(hole, first + c);
-                const int mine = rank + bits_below(bits);
-                if ((bits >> lane & 1) && mine >= 0 && mine < kEvictListed) out[mine] = 64 * (first + c) + lane;
+            const int hole_base = hole.before - done, move_base = move.before - done, all_holes = all & 0xffff, all_moves = (int)((unsigned)all >> 16);
+            for (int c = wave; c < kEvictThreads && group * kEvictThreads + c < chunks; c += kEvictWaves) {
+                const int at = group * kEvictThreads + c, packed = s.before[c];
+                auto note = [&](bool which, int rank, int *out) {
+                    const uint64_t bits = word(which, at);
+                    rank += bits_below(bits);
+                    if ((bits >> lane & 1) && rank >= 0 && rank < kEvictListed) out[rank] = 64 * at + lane;
+                };
+                if (holes) note(true, hole_base + (packed & 0xffff), s.to);
+                if (movers) note(false, move_base + (int)((unsigned)packed >> 16), s.from);
             }
             __syncthreads();
-            if (base + all >= done + kEvictListed || first + kEvictThreads >= chunks) return;
-            first += kEvictThreads;
-            base += all;
+            const bool end = (group + 1) * kEvictThreads >= chunks;
+            if (movers && end) moves = move.before + all_moves;
+            const bool more_holes = holes && !end && hole.before + all_holes < done + kEvictListed, more_moves = movers && !end && move.before + all_moves < done + kEvictListed;
+            if (more_holes) hole = {group + 1, hole.before + all_holes};
+            if (more_moves) move = {group + 1, move.before + all_moves};
+            if (!more_holes && !more_moves) return;
+            holes = more_holes;
+            movers = more_moves;
         }
     };
-    int first_hole = 0, holes_before = 0, first_move = 0, moves_before = 0;
     for (int done = 0; done < moves; done += kEvictListed) {
-        list(true, done, first_hole, holes_before, s.to);
-        list(false, done, first_move, moves_before, s.from);
+        if (hole.group == move.group) {
+            list(true, true, done);
+        } else {
+            list(false, true, done);
+            list(true, false, done);
+        }
         const int now = min(moves - done, kEvictListed);
         constexpr int ROUNDS = 4;
+        typedef uint32_t Piece __attribute__((ext_vector_type(4)));
         for (int base = 0; base < now * ROW; base += ROUNDS * kEvictThreads) {
-            uint4 kx[ROUNDS], vx[ROUNDS];
+            Piece kx[ROUNDS], vx[ROUNDS];
             float w[ROUNDS];
-            int from_page[ROUNDS], to_page[ROUNDS], from[ROUNDS], to[ROUNDS], piece[ROUNDS];
+            int from_page[ROUNDS], to_page[ROUNDS], from[ROUNDS], to[ROUNDS];
+            const int piece = tid % ROW;
             bool ok[ROUNDS];
 #pragma unroll
             for (int r = 0; r < ROUNDS; ++r) {
                 const int i = base + r * kEvictThreads + tid, m = min(i / ROW, now - 1);
-                piece[r] = i % ROW;
                 from[r] = slot_of(s.from[m], from_page[r]);
                 to[r] = slot_of(s.to[m], to_page[r]);
                 ok[r] = i < now * ROW && from[r] >= 0 && to[r] >= 0;
+                if (!ok[r]) from[r] = from_page[r] = 0;  // (loaded all the same, so that all loads are on their way together)
+            }
+#pragma unroll
+            for (int r = 0; r < ROUNDS; ++r) {
+                const long long at = ((long long)from[r] * ROW + piece) * 16;
+                kx[r] = *reinterpret_cast<const Piece *>(p.k + from_page[r] * p.k_page + at);
+                vx[r] = *reinterpret_cast<const Piece *>(p.v + from_page[r] * p.v_page + at);
+                w[r] = p.weights[from_page[r] * p.w_page + from[r]];
             }
 #pragma unroll
             for (int r = 0; r < ROUNDS; ++r)
                 if (ok[r]) {
-                    const long long at = ((long long)from[r] * ROW + piece[r]) * 16;
-                    kx[r] = *reinterpret_cast<const uint4 *>(p.k + from_page[r] * p.k_page + at);
-                    vx[r] = *reinterpret_cast<const uint4 *>(p.v + from_page[r] * p.v_page + at);
-                    if (piece[r] == 0) w[r] = p.weights[from_page[r] * p.w_page + from[r]];
-                }
-#pragma unroll
-            for (int r = 0; r < ROUNDS; ++r)
-                if (ok[r]) {
-                    const long long at = ((long long)to[r] * ROW + piece[r]) * 16;
-                    *reinterpret_cast<uint4 *>(p.k + to_page[r] * p.k_page + at) = kx[r];
-                    *reinterpret_cast<uint4 *>(p.v + to_page[r] * p.v_page + at) = vx[r];
-                    if (piece[r] == 0) p.weights[to_page[r] * p.w_page + to[r]] = w[r];
+                    const long long at = ((long long)to[r] * ROW + piece) * 16;
+                    *reinterpret_cast<Piece *>(p.k + to_page[r] * p.k_page + at) = kx[r];
+                    *reinterpret_cast<Piece *>(p.v + to_page[r] * p.v_page + at) = vx[r];
+                    if (piece == 0) p.weights[to_page[r] * p.w_page + to[r]] = w[r];
                 }
         }
         __syncthreads();  // the lists
