@@ -335,18 +335,35 @@ __device__ __forceinline__ void token_run(const PagedAttn &p, const More<MODE> &
         if constexpr (MODE == WEIGHTS) {
             if (!at_once) return;
             __syncthreads();
-            for (int v = tid; v < vis.count; v += 64 * W) {
-                const int j = vis.key(v), at = p.div.page(j), place = j - at * p.div.size, page = table[at];
-                if ((unsigned)page >= (unsigned)p.n_pages) continue;
-                const float *score = more.scores + (((size_t)page * p.n_kv + h) * p.div.size + place) * heads;
-                float *const to = more.weights + page * more.page + (size_t)h * p.div.size + place;
-                float x[G], sum = 0.0f;
+            constexpr int KEYS_AT_ONCE = 4;  // what is loaded is loaded together
+            for (int v0 = tid; v0 < vis.count; v0 += KEYS_AT_ONCE * 64 * W) {
+                int place[KEYS_AT_ONCE], page[KEYS_AT_ONCE];
+                float x[KEYS_AT_ONCE][G], old[KEYS_AT_ONCE];
 #pragma unroll
-                for (int g = 0; g < G; ++g) x[g] = __hip_atomic_load(score + min(g, heads - 1), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                const float old = j == pos ? 0.0f : *to;
+                for (int k = 0; k < KEYS_AT_ONCE; ++k) {
+                    const int v = v0 + k * 64 * W, j = v < vis.count ? vis.key(v) : 0, at = p.div.page(j);
+                    place[k] = h * p.div.size + (j - at * p.div.size);
+                    page[k] = v < vis.count ? table[at] : -1;
+                }
 #pragma unroll
-                for (int g = 0; g < G; ++g) sum += g < heads ? __builtin_amdgcn_exp2f(x[g] - s.m[0][g]) * s.l[0][g] : 0.0f;
-                *to = old + sum;
+                for (int k = 0; k < KEYS_AT_ONCE; ++k) {
+                    const bool there = (unsigned)page[k] < (unsigned)p.n_pages;
+                    page[k] = there ? page[k] : -1;
+                    const size_t of = there ? page[k] : 0;
+                    const float *const score = more.scores + (of * p.n_kv * p.div.size + place[k]) * heads;
+#pragma unroll
+                    for (int g = 0; g < G; ++g) x[k][g] = __hip_atomic_load(score + min(g, heads - 1), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                    old[k] = more.weights[of * more.page + place[k]];
+                }
+#pragma unroll
+                for (int k = 0; k < KEYS_AT_ONCE; ++k) {
+                    if (page[k] < 0) continue;
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int g = 0; g < G; ++g) sum += g < heads ? __builtin_amdgcn_exp2f(x[k][g] - s.m[0][g]) * s.l[0][g] : 0.0f;
+                    const int v = v0 + k * 64 * W;
+                    more.weights[page[k] * more.page + place[k]] = (vis.key(v) == pos ? 0.0f : old[k]) + sum;
+                }
             }
         }
     };

@@ -12,11 +12,11 @@ namespace {
 
 // ---- what each key was given, by several rows of a request ------------------------------------------
 
-// The rows of a step of 32 in LDS, as operands, double buffered.
+// The rows of a step of twice 32 in LDS, as operands, double buffered.
 template <class T>
 struct RowsShared {
-    uint4 q[2][Tiles<T>::QP][kFrag];  // [d step of 16][half][row]
-    float unit[2][32];                // f16: of the scores
+    uint4 q[2][2][Tiles<T>::QP][kFrag];  // [d step of 16][half][row ^ 2 (twice the step + half): what is written at a time lies in all banks]
+    float unit[2][2][32];                // f16: of the scores
 };
 
 // Sum over the 32 lanes of a half wave, in each of them.
@@ -63,30 +63,40 @@ __device__ __forceinline__ void weigh_keys(const PagedAttn &p, const More<WEIGHT
     }
     uint32_t odd_k = (uint32_t)__ballot(odd) | (uint32_t)(__ballot(odd) >> 32);
 
-    // Rows from the first that sees a key of the workgroup's to the last that does, in steps of 32.
+    // Rows from the first that sees a key of the workgroup's to the last that does, in steps of 64.
     const int last_key = min(first_key + 128, keys.count) - 1;
     const int from = min(max(keys.key(first_key) - pos_first, 0), there);
     int upto = there;
     if (p.window > 0 && first_key >= stay) upto = (int)max(min((long long)there, (long long)keys.key(last_key) + p.window - pos_first), 0ll);
     const int row_from = from * group & ~31, row_upto = upto * group;
-    const int steps = row_upto > row_from ? (row_upto - row_from + 31) / 32 : 0;
-    // what this thread fetches of a step: eight elements of one of its rows
+    const int steps = row_upto > row_from ? (row_upto - row_from + 63) / 64 : 0;
+    // what this thread fetches of a step: eight elements of two of its rows, and what weights of its lane's rows are in units of and divided by
     const int own = tid >> 3, part = tid & 7;
-    float4 qa, qd;
+    float4 qa[2], qd[2];
+    float2 next_stats[2];
     auto fetch = [&](int i) {
-        const int r = min(row_from + 32 * i + own, row_upto - 1), token = p.group.page(r), head = h * group + (r - token * group);
-        const float *from = p.q + (size_t)(start + token) * p.q_row + (size_t)head * p.q_head + 8 * part;
-        qa = load4(from);
-        qd = load4(from + 4);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int own_r = min(row_from + 64 * i + 32 * u + c, row_upto - 1), own_token = p.group.page(own_r);
+            next_stats[u] = more.stats[(size_t)(start + own_token) * p.n_heads + h * group + (own_r - own_token * group)];
+            const int r = min(row_from + 64 * i + 32 * u + own, row_upto - 1), token = p.group.page(r), head = h * group + (r - token * group);
+            const float *from = p.q + (size_t)(start + token) * p.q_row + (size_t)head * p.q_head + 8 * part;
+            qa[u] = load4(from);
+            qd[u] = load4(from + 4);
+        }
     };
     if (steps > 0) fetch(0);
     float acc[16];
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc[r] = 0.0f;
+    const int v_last = v0 + 31;
     for (int i = 0; i < steps; ++i) {
         const int buf = i & 1;
-        {
-            float x[8] = {qa.x * kQueryScale, qa.y * kQueryScale, qa.z * kQueryScale, qa.w * kQueryScale, qd.x * kQueryScale, qd.y * kQueryScale, qd.z * kQueryScale, qd.w * kQueryScale};
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            float x[8] = {qa[u].x, qa[u].y, qa[u].z, qa[u].w, qd[u].x, qd[u].y, qd[u].z, qd[u].w};
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] *= kQueryScale;
             if (QP == 2) {  // as in a tile of rows: into 2^14 .. 2^15
                 float most = 0.0f;
 #pragma unroll
@@ -96,57 +106,78 @@ __device__ __forceinline__ void weigh_keys(const PagedAttn &p, const More<WEIGHT
                 most = fmaxf(most, dpp_move<0x141, 0xf>(most, most));  // row_half_mirror: eight lanes have a row
                 const int up = max(min(141 - (int)((__float_as_uint(most) >> 23) & 255u), 100), -112);
                 const float by = __uint_as_float((uint32_t)(up + 127) << 23);
-                if (part == 0) s.unit[buf][own] = __uint_as_float((uint32_t)(127 - up) << 23);
+                if (part == 0) s.unit[buf][u][own] = __uint_as_float((uint32_t)(127 - up) << 23);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) x[e] *= by;
             }
             uint4 piece[QP];
             pieces_of(x, piece);
 #pragma unroll
-            for (int level = 0; level < QP; ++level) s.q[buf][level][part * 32 + own] = piece[level];
+            for (int level = 0; level < QP; ++level) s.q[buf][u][level][part * 32 + (own ^ 2 * part)] = piece[level];
         }
+        const float2 stats[2] = {next_stats[0], next_stats[1]};
         if (i + 1 < steps) fetch(i + 1);
-        // this lane's row of the step
-        const int r = row_from + 32 * i + c, r_in = min(r, row_upto - 1), token = p.group.page(r_in), pos = pos_first + token;
-        const float2 stats = more.stats[(size_t)(start + token) * p.n_heads + h * group + (r_in - token * group)];
+        // this lane's rows of the step
+        int pos[2], token[2], head[2];
+        const int row0 = row_from + 64 * i;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int r = min(row0 + 32 * u + c, row_upto - 1);
+            token[u] = p.group.page(r);
+            head[u] = h * group + (r - token[u] * group);
+            pos[u] = pos_first + token[u];
+        }
         __syncthreads();
-        floatx16 x = {};
+        floatx16 x[2] = {};
 #pragma unroll
         for (int level = QP - 1; level >= 0; --level)
 #pragma unroll
             for (int ds = 0; ds < 4; ++ds)
 #pragma unroll
                 for (int kp = KP - 1; kp >= 0; --kp)
-                    if (level - kp >= 0 && level - kp < QP) x = Tiles<T>::mfma(k[ds][kp], s.q[buf][level - kp][(2 * ds + h2) * 32 + c], x);
-        if (QP == 2) {
-            const float unit = s.unit[buf][c];
+                    if (level - kp >= 0 && level - kp < QP)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) x[e] *= unit;
-        }
-        if (__builtin_expect(odd_k != 0, 0)) {  // scores of keys with something infinite or no number, in fp32 (uniform)
-            const float *q_row = p.q + (size_t)(start + token) * p.q_row + (size_t)(h * group + (r_in - token * group)) * p.q_head;
-#pragma unroll 1
-            for (int kk = 0; kk < 32; ++kk) {
-                if (!(odd_k >> kk & 1)) continue;
-                const char *key = reinterpret_cast<const char *>((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(uintptr_t)row, kk) |
-                                                                 (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)((uintptr_t)row >> 32), kk) << 32);
-                float d = 0.0f;
-#pragma unroll 1
-                for (int e = 0; e < 32; ++e) d = fmaf(q_row[32 * h2 + e] * kQueryScale, T::one(key, 32 * h2 + e), d);
-                d = sum_of_halves(d);
+                        for (int u = 0; u < 2; ++u) x[u] = Tiles<T>::mfma(k[ds][kp], s.q[buf][u][level - kp][(2 * ds + h2) * 32 + (c ^ 2 * (2 * ds + h2))], x[u]);
+        // only steps at the ends of what rows see hide anything (uniform)
+        const int pos0 = pos_first + p.group.page(row0), pos1 = pos_first + p.group.page(min(row0 + 63, row_upto - 1));
+        const bool whole = held == 0xffffffffu && row0 + 64 <= row_upto && v_last <= pos0 - keys.gap && (v0 > paged::row_keys(keys, pos1, p.window, p.sinks).low || v_last < stay);
 #pragma unroll
-                for (int e = 0; e < 16; ++e) x[e] = 8 * (e >> 2) + 4 * h2 + (e & 3) == kk ? d : x[e];
+        for (int u = 0; u < 2; ++u) {
+            if (QP == 2) {
+                const float unit = s.unit[buf][u][c];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) x[u][e] *= unit;
             }
-        }
-        const paged::RowKeys see = paged::row_keys(keys, pos, p.window, p.sinks);
-        auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1; };  // bits 0 .. n - 1
-        uint32_t seen = held & below(see.last + 1 - v0) & (~below(see.low + 1 - v0) | below(see.first - v0));
-        if (r >= row_upto) seen = 0;
-        seen >>= 4 * h2;
+            if (__builtin_expect(odd_k != 0, 0)) {  // scores of keys with something infinite or no number, in fp32 (uniform)
+                const float *q_row = p.q + (size_t)(start + token[u]) * p.q_row + (size_t)head[u] * p.q_head;
+#pragma unroll 1
+                for (int kk = 0; kk < 32; ++kk) {
+                    if (!(odd_k >> kk & 1)) continue;
+                    const char *key = reinterpret_cast<const char *>((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(uintptr_t)row, kk) |
+                                                                     (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)((uintptr_t)row >> 32), kk) << 32);
+                    float d = 0.0f;
+#pragma unroll 1
+                    for (int e = 0; e < 32; ++e) d = fmaf(q_row[32 * h2 + e] * kQueryScale, T::one(key, 32 * h2 + e), d);
+                    d = sum_of_halves(d);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            const float w = __builtin_amdgcn_exp2f(x[e] - stats.x) * stats.y;
-            acc[e] += seen >> (8 * (e >> 2) + (e & 3)) & 1 ? w : 0.0f;
+                    for (int e = 0; e < 16; ++e) x[u][e] = 8 * (e >> 2) + 4 * h2 + (e & 3) == kk ? d : x[u][e];
+                }
+            }
+            if (whole) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) acc[e] = fmaf(__builtin_amdgcn_exp2f(x[u][e] - stats[u].x), stats[u].y, acc[e]);
+                continue;
+            }
+            const paged::RowKeys see = paged::row_keys(keys, pos[u], p.window, p.sinks);
+            auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1; };  // bits 0 .. n - 1
+            uint32_t seen = held & below(see.last + 1 - v0) & (~below(see.low + 1 - v0) | below(see.first - v0));
+            if (row0 + 32 * u + c >= row_upto) seen = 0;
+            seen >>= 4 * h2;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const float w = __builtin_amdgcn_exp2f(x[u][e] - stats[u].x) * stats[u].y;
+                acc[e] += seen >> (8 * (e >> 2) + (e & 3)) & 1 ? w : 0.0f;
+            }
         }
     }
     float mine = 0.0f;
@@ -188,6 +219,7 @@ __global__ __launch_bounds__(256, 2) void paged_weights_kernel(const PagedAttn p
                 in_call[i] = there;
             }
         }
+        if (!__any(units[0] + units[1] + units[2] + units[3] > 0)) continue;  // uniform: nobody here has several rows
         const int all = list.number(units, entries, lane);
         __syncthreads();
         const int grid = gridDim.x, first = (int)blockIdx.x >= before ? (int)blockIdx.x - before : (int)blockIdx.x - before + grid;
