@@ -38,9 +38,9 @@ struct More<WEIGHTS> {
     float *weights;   // [n_pages][n_kv][page_size]
     long long page;   // elements between pages
     float *scores;    // [n_pages][n_kv][page_size][group]: of requests with one row; null: there is no room for them
-    float2 *stats;    // [tokens][n_heads]: the unit of a row's weights and what they are divided by, of all other requests
-    // Whether a token's weights are added up from its scores by the last workgroup at it; the others' by paged_weights_kernel.
-    __device__ __forceinline__ bool at_once(int rows, int group) const { return rows == 1 && group <= 8 && scores != nullptr; }
+    float2 *stats;    // [tokens][n_heads]: the unit of a row's weights and what they are divided by
+    bool few;         // weights are added up from scores by the last workgroup at a token; otherwise, and without scores, by paged_weights_kernel
+    __device__ __forceinline__ bool scored(int rows, int group) const { return rows == 1 && group <= 8 && scores != nullptr; }
 };
 template <>
 struct More<SHARED> {
@@ -198,8 +198,11 @@ __device__ __forceinline__ void token_run(const PagedAttn &p, const More<MODE> &
 #pragma unroll
             for (int g = 0; g < G; ++g) load_seen(wave + W * own, g);
     }
-    bool at_once = false;
-    if constexpr (MODE == WEIGHTS) at_once = more.at_once(p.query_start ? p.query_start[b + 1] - p.query_start[b] : 1, p.group.size);
+    bool scored = false, at_once = false;
+    if constexpr (MODE == WEIGHTS) {
+        scored = more.scored(p.query_start ? p.query_start[b + 1] - p.query_start[b] : 1, p.group.size);
+        at_once = scored && more.few;
+    }
     int id[PASS], off[PASS];
     auto pages = [&](int first) {
 #pragma unroll
@@ -237,7 +240,7 @@ __device__ __forceinline__ void token_run(const PagedAttn &p, const More<MODE> &
                 x[g][i] = ok[i] ? sum_of_key<LPK>(d) : -INFINITY;
             }
             if constexpr (MODE == WEIGHTS)
-                if (at_once && ok[i] && sub < heads) {  // (lanes of a key have its scores all, and there are at least as many as heads)
+                if (scored && ok[i] && sub < heads) {  // (lanes of a key have its scores all, and there are at least as many as heads)
                     float mine = x[0][i];
 #pragma unroll
                     for (int g = 1; g < G; ++g) mine = sub == g ? x[g][i] : mine;

@@ -190,7 +190,47 @@ __device__ __forceinline__ void weigh_keys(const PagedAttn &p, const More<WEIGHT
     if (real && (c >> 2 & 1) == h2) *to = old + mine;
 }
 
-// Units: 128 keys of a request and K/V head, for requests of several rows (of one too, where its scores found no room), 256 requests at a time.
+// Keys number v0 .. of those that the only row of request b sees, four a thread, from the scores that attention has left.
+constexpr int kScoredKeys = 1024;
+__device__ __forceinline__ void add_scored(const PagedAttn &p, const More<WEIGHTS> &more, int b, int t, int h, int v0) {
+    const int group = p.group.size, kv_len = max(p.kv_lens[b], 0), pos = kv_len - 1;
+    const Visible vis = paged::visible(pos, kv_len, p.held, p.window, p.sinks);
+    const int *table = p.tables + (size_t)b * p.width;
+    const float2 *stats = more.stats + (size_t)t * p.n_heads + h * group;
+    constexpr int EACH = kScoredKeys / 256;
+    int place[EACH], page[EACH];
+#pragma unroll
+    for (int k = 0; k < EACH; ++k) {
+        const int v = v0 + 256 * k + (int)threadIdx.x, j = v < vis.count ? vis.key(v) : 0, at = p.div.page(j);
+        place[k] = h * p.div.size + (j - at * p.div.size);
+        page[k] = v < vis.count ? table[at] : -1;
+    }
+    float sum[EACH], old[EACH];
+    const float *score[EACH];
+    float *to[EACH];
+#pragma unroll
+    for (int k = 0; k < EACH; ++k) {
+        const bool there = (unsigned)page[k] < (unsigned)p.n_pages;
+        const size_t of = there ? page[k] : 0;
+        score[k] = more.scores + (of * p.n_kv * p.div.size + place[k]) * group;
+        to[k] = more.weights + of * more.page + place[k];
+        old[k] = *to[k];
+        sum[k] = 0.0f;
+        if (!there) to[k] = nullptr;
+    }
+    for (int g = 0; g < group; ++g) {
+        const float2 row = stats[g];
+#pragma unroll
+        for (int k = 0; k < EACH; ++k) sum[k] += __builtin_amdgcn_exp2f(score[k][g] - row.x) * row.y;
+    }
+#pragma unroll
+    for (int k = 0; k < EACH; ++k) {
+        const int v = v0 + 256 * k + (int)threadIdx.x;
+        if (to[k] != nullptr) *to[k] = (vis.key(v) == pos ? 0.0f : old[k]) + sum[k];
+    }
+}
+
+// Units: 128 keys of a request and K/V head, or 1024 of one whose scores are there, 256 requests at a time.
 template <class T>
 __global__ __launch_bounds__(256, 2) void paged_weights_kernel(const PagedAttn p, const More<WEIGHTS> more) {
     __shared__ RowsShared<T> s;
@@ -210,9 +250,10 @@ __global__ __launch_bounds__(256, 2) void paged_weights_kernel(const PagedAttn p
             if (i < entries) {
                 const int start = p.query_start ? p.query_start[b] : b, end = p.query_start ? p.query_start[b + 1] : b + 1, kv_len = max(p.kv_lens[b], 0);
                 const int there = min(end, p.tokens) - start;
-                if (start >= 0 && there > 0 && !more.at_once(end - start, p.group.size)) {
-                    const int count = paged::tile_keys(kv_len - (end - start), kv_len - 1, p.held, p.window, p.sinks).count;
-                    units[j] = (int)min((long long)((count + 127) / 128) * p.n_kv, 1ll << 22);  // (that many are 137 GB of keys at least; their sum stays below 2^31)
+                const bool scored = more.scored(end - start, p.group.size);
+                if (start >= 0 && there > 0 && !(scored && more.few)) {
+                    const int count = paged::tile_keys(kv_len - (end - start), kv_len - 1, p.held, p.window, p.sinks).count, each = scored ? kScoredKeys : 128;
+                    units[j] = (int)min((long long)((count + each - 1) / each) * p.n_kv, 1ll << 22);  // (that many are 137 GB of keys at least; their sum stays below 2^31)
                 }
                 starts[i] = start;
                 rows[i] = end - start;
@@ -226,8 +267,12 @@ __global__ __launch_bounds__(256, 2) void paged_weights_kernel(const PagedAttn p
         for (int unit = first; unit < all; unit += grid) {
             int at = unit;
             const int i = list.entry(at, lane), h = at % p.n_kv, tile = at / p.n_kv;
-            weigh_keys<T>(p, more, s, b0 + i, starts[i], rows[i], in_call[i], h, 128 * tile);
-            __syncthreads();
+            if (more.scored(rows[i], p.group.size)) {
+                add_scored(p, more, b0 + i, starts[i], h, kScoredKeys * tile);
+            } else {
+                weigh_keys<T>(p, more, s, b0 + i, starts[i], rows[i], in_call[i], h, 128 * tile);
+                __syncthreads();
+            }
         }
         before = (int)(((unsigned)before + (unsigned)all % (unsigned)grid) % (unsigned)grid);
     }
@@ -261,10 +306,13 @@ AGPU_EXPORT int32_t agpu_paged_attention_weights(agpu_ctx *ctx, const float *q, 
     more.weights = weights; more.page = weights_page_stride;
     more.stats = reinterpret_cast<float2 *>(ctx->workspace);
     more.scores = room.scores ? reinterpret_cast<float *>(ctx->workspace + room.scores) : nullptr;
+    // The last workgroup at a token adds up its weights where other work goes on meanwhile (chunks beside tokens: 37 us, 39 with a launch for them), or where there is so little of it that
+    // a launch more costs as much (12 heads of 777 keys: 10 us, and 4 for the launch where query_start leaves open whether there are chunks); 64 tokens of up to 4096 keys, 8 heads: 43 us that way, 40 with one.
+    more.few = more.scores && (tokens > batch || (int64_t)tokens * n_kv_heads * std::min<int64_t>(paged::longest_row(p.held, window, sinks), kScoredKeys) <= 64 * kScoredKeys);
     return of_type(cache_type, [&](auto type) {
         using T = decltype(type);
         int32_t rc = attention_go<T, WEIGHTS>(ctx, p, paged::longest_row(p.held, window, sinks), more, ctx->workspace + room.bytes, ctx->ws_bytes - room.bytes);
-        if (rc != AGPU_OK || (!query_start && more.scores)) return rc;
+        if (rc != AGPU_OK || (!query_start && more.few)) return rc;
         hipLaunchKernelGGL((paged_weights_kernel<T>), dim3(2 * ctx->num_cus), dim3(256), 0, ctx->stream, p, more);
         return AGPU_LAUNCH_CHECK(ctx, "paged_weights_kernel");
     });
