@@ -435,11 +435,22 @@ __global__ __launch_bounds__(256, 2) void paged_prefix_kernel(const PagedAttn p,
                 if (w < wave) at += s.wave_rows[w];
                 before += s.wave_rows[w];
             }
-            for (int i = max(first - at, 0); i < count && at + i <= last; ++i) {
-                s.token[at + i - first] = r.start + i;
-                s.pos[at + i - first] = len + r.pos + i;
-                pos0 = min(pos0, len + r.pos + i);
-                pos1 = max(pos1, len + r.pos + i);
+            // rows from .. to - 1 of this thread's request are the tile's; its own thread writes them where they are few, and its wave where they are many
+            const int from = max(first - at, 0), to = min(count, last + 1 - at);
+            if (to > from) {
+                pos0 = min(pos0, len + r.pos + from);
+                pos1 = max(pos1, len + r.pos + to - 1);
+            }
+            constexpr int kFew = 4;
+#pragma unroll
+            for (int e = 0; e < kFew; ++e) {
+                const int i = from + e;
+                if (to - from <= kFew && i < to) s.token[at + i - first] = r.start + i, s.pos[at + i - first] = len + r.pos + i;
+            }
+            for (uint64_t many = __ballot(to - from > kFew); many != 0; many &= many - 1) {  // uniform
+                const int who = __builtin_ctzll(many), at_w = __builtin_amdgcn_readlane(at, who), to_w = __builtin_amdgcn_readlane(to, who);
+                const int start_w = __builtin_amdgcn_readlane(r.start, who), pos_w = __builtin_amdgcn_readlane(r.pos, who);
+                for (int i = __builtin_amdgcn_readlane(from, who) + lane; i < to_w; i += 64) s.token[at_w + i - first] = start_w + i, s.pos[at_w + i - first] = len + pos_w + i;
             }
         };
         list_rows(mine);
