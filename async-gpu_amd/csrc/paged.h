@@ -107,22 +107,23 @@ inline int most_runs(int64_t items, int64_t longest, int64_t least, size_t item_
 inline int64_t longest_row(int64_t held, int64_t window, int64_t sinks) { return window > 0 && window + sinks < held ? window + sinks : held; }
 
 // The scratch of a prefix's runs, for `rows` rows of heads and `held` keys at most: how many runs there is room for in half of it (0: not even for one), where their (m, l)
-// begin, which are 8 bytes a row, where o of the second and later ones, which is 256, and what all of it takes.  Before them is a number a request.
+// begin, which are 8 bytes a row, where o of the second and later ones, which is 256 (`apart`: and of the first one behind them), and what all of it takes.  Before them is a number a
+// request.
 struct PrefixRuns {
     int most;
     size_t ml, rest, bytes;
 };
-inline PrefixRuns prefix_runs(int64_t batch, int64_t rows, int64_t held, size_t scratch) {
+inline PrefixRuns prefix_runs(int64_t batch, int64_t rows, int64_t held, bool apart, size_t scratch) {
     auto up = [](size_t n) { return (n + 255) & ~(size_t)255; };
     const size_t all = (size_t)rows, half = scratch / 2, ml = up(4 * (size_t)batch);
-    if (ml + up(8 * all) > scratch / 4 * 3) return {0, 0, 0, 0};
+    if (ml + up((apart ? 264 : 8) * all) > scratch / 4 * 3) return {0, 0, 0, 0};
     int64_t runs = (held + 127) / 128;
     runs = runs < 64 ? runs : 64;
     const int64_t room = half > ml + 512 ? (int64_t)((half - ml - 512) / (264 * all)) : 0;
     runs = runs < room ? runs : room;
     runs = runs < 1 ? 1 : runs;
     const size_t rest = ml + up(8 * all * runs);
-    return {(int)runs, ml, rest, rest + up(256 * all * (runs - 1))};
+    return {(int)runs, ml, rest, rest + up(256 * all * (runs - !apart))};
 }
 
 // The scratch of attention that adds up its weights: 8 bytes a row of heads, then, where there is room in half of it (and a K/V head has eight query heads at most),

@@ -46,9 +46,9 @@ template <>
 struct More<SHARED> {
     const int *tables, *lens, *of;  // of the prefixes [n_prefix][width], [n_prefix]; of the requests
     int n_prefix, width, held;
-    // What rows have seen of their prefix, in runs: o of the first run is where the rows' results go, of the others in rest [runs - 1][tokens][n_heads][64]; (m, l)
-    // of all in ml [runs][tokens][n_heads].
-    float *rest;
+    // What rows have seen of their prefix, in runs: o of the first run is in first [tokens][n_heads][64], which is where the rows' results go if that begins at 16 bytes, of
+    // the others in rest [runs - 1][tokens][n_heads][64]; (m, l) of all in ml [runs][tokens][n_heads].
+    float *first, *rest;
     float2 *ml;
     int *before;  // [batch] how many runs there are of what a request's rows have seen of their prefix
     __device__ __forceinline__ int len(int g) const { return (unsigned)g < (unsigned)n_prefix ? max(min(lens[g], held), 0) : 0; }
@@ -186,7 +186,7 @@ __device__ __forceinline__ void token_run(const PagedAttn &p, const More<MODE> &
     auto load_seen = [&](int r, int g) {
         if constexpr (MODE == SHARED) {
             const size_t rows = (size_t)p.tokens * p.n_heads, row = (size_t)t * p.n_heads + head0 + min(g, heads - 1);
-            const float *from = (r == 0 ? p.o + row * DH : more.rest + ((r - 1) * rows + row) * DH) + EL * sub;
+            const float *from = (r == 0 ? more.first + row * DH : more.rest + ((r - 1) * rows + row) * DH) + EL * sub;
             seen_ml[g] = more.ml[r * rows + row];
 #pragma unroll
             for (int e = 0; e < EL / 4; ++e) seen_o[g][e] = *reinterpret_cast<const float4 *>(from + 4 * e);
@@ -971,7 +971,7 @@ __device__ __forceinline__ void tile_run(const PagedAttn &p, const More<MODE> &m
     if constexpr (MODE == PREFIX) {
         if (!mine) return;
         const size_t rows_all = (size_t)p.tokens * p.n_heads;
-        float *const out = (run == 0 ? p.o + row_at * DH : more.rest + ((run - 1) * rows_all + row_at) * DH) + 4 * h2;
+        float *const out = (run == 0 ? more.first + row_at * DH : more.rest + ((run - 1) * rows_all + row_at) * DH) + 4 * h2;
 #pragma unroll
         for (int db = 0; db < 2; ++db)
 #pragma unroll
@@ -987,7 +987,7 @@ __device__ __forceinline__ void tile_run(const PagedAttn &p, const More<MODE> &m
             const size_t rows_all = (size_t)p.tokens * p.n_heads;
             for (int i = 0; i < pre; ++i) {
                 const float2 ml = more.ml[i * rows_all + row_at];
-                const float *const from = (i == 0 ? p.o + row_at * DH : more.rest + ((i - 1) * rows_all + row_at) * DH) + 4 * h2;
+                const float *const from = (i == 0 ? more.first + row_at * DH : more.rest + ((i - 1) * rows_all + row_at) * DH) + 4 * h2;
                 float4 x[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) x[e] = *reinterpret_cast<const float4 *>(from + 8 * e);

@@ -507,7 +507,7 @@ __global__ __launch_bounds__(256, 2) void paged_prefix_kernel(const PagedAttn p,
                     sum += u.wave.join.l[set + SETS * k][at & 31];
                 }
                 const size_t row_at = (size_t)s.token[token - first] * p.n_heads + head;
-                store4_through((run == 0 ? p.o + row_at * DH : more.rest + ((run - 1) * rows_all + row_at) * DH) + d, all);
+                store4_through((run == 0 ? more.first + row_at * DH : more.rest + ((run - 1) * rows_all + row_at) * DH) + d, all);
                 if (d == 0) store2_through(&more.ml[run * rows_all + row_at].x, u.wave.join.m[set][at & 31], sum);
             }
         };
@@ -544,14 +544,17 @@ AGPU_EXPORT int32_t agpu_paged_attention_shared(agpu_ctx *ctx, const float *q, i
     if (here.rc != AGPU_OK) return here.rc;
     const PagedAttn p = paged_attn(q, q_token_stride, q_head_stride, k_cache, v_cache, k_page_stride, v_page_stride, block_tables, kv_lens, query_start, o, tokens, batch, n_heads,
                              n_kv_heads, n_pages, page_size, table_width, window, sinks, ctx->strict_sync);
-    // Scratch: how many runs there are before each request, (m, l) of the prefix's runs and o of all but the first, half of it at most; then the partial results over own pages.
-    const paged::PrefixRuns room = paged::prefix_runs(batch, (int64_t)tokens * n_heads, (int64_t)prefix_width * page_size, ctx->ws_bytes);
+    // Scratch: how many runs there are before each request, (m, l) of the prefix's runs and o of those that the results have no place for, half of it at most; then the
+    // partial results over own pages.
+    const bool apart = (uintptr_t)o % 16 != 0;
+    const paged::PrefixRuns room = paged::prefix_runs(batch, (int64_t)tokens * n_heads, (int64_t)prefix_width * page_size, apart, ctx->ws_bytes);
     if (room.most == 0) return agpu_fail(ctx, AGPU_ERR_WORKSPACE, "paged_attention_shared: %d rows of %d heads need a larger scratch", tokens, n_heads);
     More<PREFIX> pre{};
     pre.tables = prefix_tables; pre.lens = prefix_lens; pre.of = prefix_of; pre.n_prefix = n_prefix; pre.width = prefix_width; pre.held = prefix_width * page_size;
     pre.before = reinterpret_cast<int *>(ctx->workspace);
     pre.ml = reinterpret_cast<float2 *>(ctx->workspace + room.ml);
     pre.rest = reinterpret_cast<float *>(ctx->workspace + room.rest);
+    pre.first = apart ? pre.rest + (int64_t)(room.most - 1) * tokens * n_heads * DH : o;
     const int64_t tiles = ((int64_t)tokens * p.group.size / TILE_ROWS + n_prefix) * n_kv_heads;
     PagedAttn front = p;
     front.tables = prefix_tables; front.width = prefix_width; front.held = pre.held;

@@ -504,3 +504,64 @@ def test_a_server_with_a_budget(agpu, dev, type_):
         for s, out in ((state, made[-3:]), (eager, made_eager)):
             s["cached"].copy_(out[0]), s["n"].copy_(out[2])
     assert cuts > 5
+
+
+@pytest.mark.parametrize("type_", ["float32", "float16"])
+@pytest.mark.parametrize("heads,kv_heads", [(3, 3), (9, 1), (8, 2)])
+def test_chunks_beside_idle_requests(agpu, dev, type_, heads, kv_heads):
+    """No more rows than requests, but not one each."""
+    new = [0, 9, 0, 0, 40, 0, 1, 0, 2, 0] + [0, 1] * 30
+    lens = [20 + 3 * i for i in range(len(new))]
+    kc, vc, w, tables, start, q = _state(dev, lens, new, heads, kv_heads, 16, type_, 7)
+    for window, sinks in ((0, 0), (30, 4)):
+        own = w.clone()
+        _attend(dev, q, kc, vc, own, tables, lens, start, window, sinks)
+        check(own, *given64(q, kc, w, tables, lens, start, window, sinks))
+
+
+@pytest.mark.parametrize("type_", TYPES)
+@pytest.mark.parametrize("lens", [[3000], [5000] * 20, [70, 1, 9000, 2048, 1024, 1025]])
+def test_tokens_of_long_requests(agpu, dev, type_, lens):
+    """Weights from scores, by the last workgroup at a token or by a launch of their own; with and without query_start the same bits."""
+    import torch
+    kc, vc, w, tables, start, q = _state(dev, lens, [1] * len(lens), 12, 6, 16, type_, 7)
+    own, plain = w.clone(), w.clone()
+    _attend(dev, q, kc, vc, own, tables, lens, start)
+    check(own, *given64(q, kc, w, tables, lens, start))
+    _attend(dev, q, kc, vc, plain, tables, lens, None)
+    assert torch.equal(own, plain)
+
+
+def test_evict_twice_and_in_a_graph(agpu, dev):
+    """What is cut down stays as it is cut down again with the lengths it has now; a graph of both calls gives what eager calls give, replay by replay."""
+    import torch
+    from async_gpu_amd import ops
+    i = _i32(dev)
+    kc, vc, w, tables = _evict_case(dev, [300, 200, 90, 1000], 3, 16, "float16", 3)
+    t, lens, stack, n = i(tables), i([300, 200, 90, 1000]), i(np.full(200, -1)), i([0])
+    first = [x.clone() for x in (kc, vc, w)]
+
+    def both(kc, vc, w, lens, stack):
+        ops.paged_evict(kc, vc, w, t, lens, 120, 100, 10, 2)
+        return ops.paged_trim(lens, t, stack, n, 16, 120, 100)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        both(*[x.clone() for x in first], lens, stack.clone())
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    gl, gs = lens.clone(), stack.clone()
+    with torch.cuda.graph(graph, stream=side):
+        made = both(kc, vc, w, gl, gs)
+    for x, y in zip((kc, vc, w), first):
+        x.copy_(y)
+    for step in ([300, 200, 90, 1000], [120, 121, 90, 700], [100, 100, 90, 100]):
+        gl.copy_(i(step)), lens.copy_(i(step))
+        eager = [x.clone() for x in (kc, vc, w)]
+        es = gs.clone()
+        want = both(*eager, lens, es)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip((*made, kc, vc, w, gs), (*want, *eager, es)))

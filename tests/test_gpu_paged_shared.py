@@ -323,3 +323,57 @@ def test_captured_server(agpu, dev):
             check(want[5][rows], *attend64(qkv[rows, 0], k.transpose(0, 1)[None], v.transpose(0, 1)[None], [[0]], [k.shape[0]], [0, m]))
         for s, out in ((state, made), (eager, want)):
             s["cached"].copy_(out[0]), s["n"].copy_(out[4])
+
+
+@pytest.mark.parametrize("type_", TYPES)
+def test_out_at_any_float(agpu, dev, type_):
+    """Results to memory that begins at any float, behind a prefix of several runs: the same bits."""
+    import torch
+    s = Batch(dev, [900], [(100, 1, 0), (150, 140, 0), (60, 20, -1), (33, 2, 0)], 6, 3, 16, type_)
+    want, buf = s.run(), torch.full((s.q.numel() + 5,), 7.0, device=dev)
+    s.check(want)
+    for odd in (1, 2, 3):
+        buf.fill_(7.0)
+        out = buf[odd:odd + s.q.numel()].view(s.q.shape)
+        assert s.run(out=out) is out and torch.equal(out, want) and (buf[:odd] == 7.0).all() and (buf[odd + s.q.numel():] == 7.0).all()
+
+
+@pytest.mark.parametrize("type_", ["float32", "bfloat16"])
+@pytest.mark.parametrize("heads,kv_heads", [(3, 3), (9, 1)])
+def test_chunks_beside_idle_requests(agpu, dev, type_, heads, kv_heads):
+    """No more rows than requests, but not one each: rows of chunks go one by one over their own pages, and in tiles over the prefix."""
+    new = [0, 9, 0, 0, 40, 0, 1, 0, 0, 0] + [0] * 50
+    s = Batch(dev, [250, 33], [(20 + 3 * i, n, (0, 1, -1)[i % 3]) for i, n in enumerate(new)], heads, kv_heads, 16, type_)
+    s.check(s.run())
+    s.check(s.run(30, 4), 30, 4)
+
+
+@pytest.mark.parametrize("type_", ["float32", "float16"])
+def test_far_apart_magnitudes(agpu, dev, type_):
+    """Runs and waves whose maxima lie far apart, and rows of which one key has all the weight."""
+    import torch
+    s = Batch(dev, [1500], [(20, 1, 0), (40, 30, 0), (70, 1, 0)], 4, 2, 16, type_, scale=8.0)
+    for p in (3, 700, 1499):
+        s.kc[s.ptables[0, p // 16], :, p % 16] *= 6.0
+    s.check(s.run())
+    s.kc *= 0.0
+    got = s.run()  # equal scores: the mean
+    k, v, tables, lens = s.joint()
+    check(got, *attend64(s.q, k, v, tables, lens, s.start))
+
+
+def test_a_cache_beyond_32_bits(agpu, dev):
+    """Elements of a cache beyond number 2^32, of the prefix and of own pages."""
+    import torch
+    page, H = 64, 4
+    pages = (1 << 32) // (page * H * 64) + 40
+    s = Batch(dev, [400], [(200, 1, 0), (150, 140, 0), (90, 3, 0)], 2 * H, H, page, "bfloat16")
+    ids = np.array([pages - 1 - 2 * i if i % 2 else i for i in range(s.kc.shape[0])])
+    big = [torch.empty((pages, H, page, 64), dtype=torch.bfloat16, device=dev) for _ in range(2)]
+    for b, small in zip(big, (s.kc, s.vc)):
+        b[torch.tensor(ids, device=dev)] = small
+    want, small = s.run(), (s.kc, s.vc, s.ptables, s.tables)
+    s.check(want)
+    move = lambda t: np.where((t >= 0) & (t < len(ids)), ids[np.clip(t, 0, len(ids) - 1)], -1)  # noqa: E731
+    s.kc, s.vc, s.ptables, s.tables = *big, move(small[2]), move(small[3])
+    assert torch.equal(s.run(), want)

@@ -12,7 +12,7 @@ BIG = 2**31 - 1
 
 @pytest.fixture(scope="module")
 def rules(tmp_path_factory):
-    """A program that answers a line of numbers with a line of numbers: `runs batch rows held scratch` and `room rows places group scratch` (how scratch is shared out), and the refusals."""
+    """A program that answers a line of numbers with a line of numbers: `runs batch rows held apart scratch` and `room rows places group scratch` (how scratch is shared out), and the refusals."""
     d = tmp_path_factory.mktemp("paged_more")
     src, exe = d / "rules.cpp", d / "rules"
     src.write_text('''
@@ -28,7 +28,7 @@ int main() {
         while (std::scanf("%c", &c) == 1 && c != '\\n')
             if (std::scanf("%lld", &a[n]) == 1) ++n;
         if (!std::strcmp(what, "runs")) {
-            const paged::PrefixRuns r = paged::prefix_runs(a[0], a[1], a[2], (size_t)a[3]);
+            const paged::PrefixRuns r = paged::prefix_runs(a[0], a[1], a[2], a[3] != 0, (size_t)a[4]);
             std::printf("%d %zu %zu %zu\\n", r.most, r.ml, r.rest, r.bytes);
         } else if (!std::strcmp(what, "room")) {
             const paged::WeightsRoom r = paged::weights_room(a[0], a[1], (int)a[2], (size_t)a[3]);
@@ -60,16 +60,16 @@ int main() {
 
 def test_runs_of_a_prefix_keep_to_scratch(rules):
     """Whatever is asked for, (m, l) and o of all runs lie one after the other within the scratch, and leave room for partial results; one run has to be possible for 2^23 rows."""
-    asked = [(batch, rows, held, scratch) for batch in (1, 300, 5000) for rows in (1, 12, 1600, 14400, 131072, 1 << 20, (1 << 23) - 1) for held in (1, 128, 129, 5000, 2**30) for scratch in (1 << 20, 10 << 20, 96 << 20, 1 << 30)]
-    for (batch, rows, held, scratch), (most, ml, rest, size) in zip(asked, rules(["runs " + " ".join(map(str, a)) for a in asked])):
+    asked = [(batch, rows, held, apart, scratch) for apart in (0, 1) for batch in (1, 300, 5000) for rows in (1, 12, 1600, 14400, 131072, 1 << 20, (1 << 23) - 1) for held in (1, 128, 129, 5000, 2**30) for scratch in (1 << 20, 10 << 20, 96 << 20, 1 << 30)]
+    for (batch, rows, held, apart, scratch), (most, ml, rest, size) in zip(asked, rules(["runs " + " ".join(map(str, a)) for a in asked])):
         if most == 0:
-            assert 4 * batch + 8 * rows + 512 > scratch // 4 * 3
+            assert 4 * batch + (264 if apart else 8) * rows + 512 > scratch // 4 * 3
             continue
         assert 4 * batch <= ml and ml % 256 == 0
         assert 1 <= most <= 64 and (most - 1) * 128 < held
-        assert ml + 8 * rows * most <= rest and rest + 256 * rows * (most - 1) <= size <= scratch - (scratch // 4 - 256) and rest % 256 == 0 and size % 256 == 0
-        assert most == 1 or size <= scratch // 2 + 512
-    assert rules([f"runs 4096 {(1 << 23) - 1} 1000 {96 << 20}"])[0][0] == 1
+        assert ml + 8 * rows * most <= rest and rest + 256 * rows * (most - 1 + apart) <= size <= scratch - (scratch // 4 - 256) and rest % 256 == 0 and size % 256 == 0
+        assert most == 1 or size <= scratch // 2 + 512 + 256 * rows * apart
+    assert rules([f"runs 4096 {(1 << 23) - 1} 1000 0 {96 << 20}"])[0][0] == 1
 
 
 def test_scores_keep_to_scratch(rules):
