@@ -64,6 +64,7 @@ __global__ __launch_bounds__(kEvictThreads) void paged_evict_kernel(const EvictA
         page = table[at];
         return (unsigned)page < (unsigned)p.n_pages ? h * p.div.size + (i - at * p.div.size) : -1;
     };
+    auto beyond = [&](int block, int e) { return block * BLOCK + e * kEvictThreads >= n; };  // (uniform: nothing there)
     auto middle = [&](int i) { return i >= p.sinks && i < n - p.recent; };
     uint32_t key[kEvictEach];
     auto load = [&](int block) __attribute__((always_inline)) {
@@ -72,6 +73,7 @@ __global__ __launch_bounds__(kEvictThreads) void paged_evict_kernel(const EvictA
         for (int e = 0; e < kEvictEach; ++e) {
             const int i = block * BLOCK + e * kEvictThreads + tid;
             slot[e] = -1;
+            if (beyond(block, e)) continue;
             if (middle(i)) slot[e] = slot_of(i, page[e]);
         }
 #pragma unroll
@@ -90,6 +92,7 @@ __global__ __launch_bounds__(kEvictThreads) void paged_evict_kernel(const EvictA
             if (blocks > 1) load(block);
 #pragma unroll
             for (int e = 0; e < kEvictEach; ++e) {
+                if (beyond(block, e)) break;
                 const bool in = middle(block * BLOCK + e * kEvictThreads + tid) && (upto == 32 || key[e] >> (upto & 31) == least >> (upto & 31));
                 if (in) atomicAdd(&s.bins[key[e] >> shift & (bins - 1)], 1);
             }
@@ -143,6 +146,7 @@ __global__ __launch_bounds__(kEvictThreads) void paged_evict_kernel(const EvictA
         }
 #pragma unroll
         for (int e = 0; e < kEvictEach; ++e) {
+            if (beyond(block, e)) break;
             const int i = block * BLOCK + e * kEvictThreads + tid;
             const bool inside = middle(i), near = inside && (upto == 32 || key[e] >> (upto & 31) == least >> (upto & 31));
             bool stay = i < n && (!inside || (!near && key[e] > least));
