@@ -1,8 +1,11 @@
 // A KV cache cut down to a budget: which places of a request keep their keys, and the pages behind them.
 //
-// paged_evict_kernel, a workgroup a request and K/V head: weights as integers in the order of the floats, the smallest one that stays found bit by bit from the top (two a step, by
-// counting), equal ones in the order of their places.  Those that stay keep their places, except where that is behind what is kept: these move into places of evicted ones, the first to the
-// first.  So no more is moved than has to be, sources and targets never overlap, and nothing waits for the order of moves.
+// paged_evict_kernel, a workgroup a request and K/V head: weights as integers in the order of the floats, those that stay found by histograms of 11 bits from the top down until what
+// is not decided is few, or all equal, and in the order of the places then.  What stays keeps its place, except where that is behind what is kept: it moves into the place of an
+// evicted one, the first to the first.  So no more is moved than has to be (of 2200 keys cut down to 2000, 200), sources and targets never overlap, and nothing waits for the order of moves.
+// What bounds it: 8 requests of 1000 to 1200 keys, 12 heads, fp32, 10.4 us, a chain: 1.6 to the first weights, 1.4 a histogram, 2 who stays, 1.4 the lists, 2 the moves.  64 requests
+// of up to 4096 keys, 25 heads, bf16, cut to 2000: 58 us where it is done again and 170 MB move, 2.9 TB/s; the first time (3 times as much) the bytes.  Found bit by bit, two a step
+// with a count each, the last weight that stays took 4 to 11 us in place of 3.
 #include "agpu_internal.h"
 #include "paged.h"
 
@@ -282,7 +285,7 @@ struct TrimArgs {
 
 constexpr int TRIM_THREADS = 256;
 
-// Every workgroup adds up the pages of all requests for itself, then they share the stack's new entries.
+// Every workgroup adds up the pages of all requests for itself, then they share the stack's new entries.  8 requests 2.2 us, 512 that give 38000 pages back 4.9.
 __global__ __launch_bounds__(TRIM_THREADS) void paged_trim_kernel(const TrimArgs p) {
     extern __shared__ int s_start[];  // pages given back before each request, and all
     __shared__ uint32_t s_wave[TRIM_THREADS / 64];

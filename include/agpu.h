@@ -424,7 +424,8 @@ int32_t agpu_paged_attention(agpu_ctx *ctx, const float *q, int64_t q_token_stri
                              int32_t n_kv_heads, int32_t n_pages, int32_t page_size, int32_t table_width, int32_t window, int32_t sinks,
                              int32_t d_head, int32_t cache_type);
 /* The same, over the keys of a prefix and then of each request's own pages: requests that begin alike hold what they share once, and it is read once for all of them.
- *   prefix_tables [n_prefix][prefix_width], prefix_lens [n_prefix]   pages and lengths of the prefixes (256 at most), like block_tables and kv_lens
+ *   prefix_tables [n_prefix][prefix_width], prefix_lens [n_prefix]   pages and lengths of the prefixes (256 at most), like block_tables and kv_lens; a length
+ *                                                                    counts as far as the table has pages for it
  *   prefix_of [batch]                                                which of them a request is behind; outside 0 .. n_prefix - 1: none
  * Place p of a request's own kv_lens is position prefix_lens[prefix_of[b]] + p, for what a row sees: every key up to its own position, with window > 0 only those
  * nearer than that or among the first `sinks` positions, which are the prefix's.  A prefix is nobody's in agpu_paged_plan's view, or a request of its own that has no new tokens: its
