@@ -135,7 +135,7 @@ inline WeightsRoom weights_room(int64_t rows, int64_t places, int group, size_t 
     auto up = [](size_t n) { return (n + 255) & ~(size_t)255; };
     const size_t stats = up(8 * (size_t)rows);
     if (stats > scratch / 4 * 3) return {0, 0};
-    if (group > 8 || stats + 4 * (size_t)places > scratch / 2) return {0, stats};
+    if (group > 8 || places >= 0xffffffffll || stats + 4 * (size_t)places > scratch / 2) return {0, stats};
     return {stats, stats + up(4 * (size_t)places)};
 }
 

@@ -192,21 +192,33 @@ __device__ __forceinline__ void token_run(const PagedAttn &p, const More<MODE> &
             id[i] = v < hi ? table[at] : -1;
         }
     };
+    // Scores leave when the next keys are on their way: loads wait for stores before them (64 requests of 4096 keys, 32 heads over 8, f16: 141 us, 126 this way, 110 without scores).
+    float late[PASS];
+    uint32_t late_to[PASS];
+    auto store_late = [&] {
+        if constexpr (MODE == WEIGHTS)
+#pragma unroll
+            for (int i = 0; i < PASS; ++i)
+                if (late_to[i] != 0xffffffffu) __hip_atomic_store(more.scores + late_to[i], late[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    };
+#pragma unroll
+    for (int i = 0; i < PASS; ++i) late_to[i] = 0xffffffffu;
     const int first = lo + wave * KEYS + own;
     pages(first);
     for (int base = first - own; base < hi; base += PASS * W * KEYS) {
         uint4 kx[PASS], vx[PASS];
         bool ok[PASS];
-        size_t key[PASS];  // of all places and K/V heads
+        uint32_t key[PASS];  // of all places and K/V heads: where its scores go (there are less than 2^32 of them)
 #pragma unroll
         for (int i = 0; i < PASS; ++i) {
             ok[i] = (unsigned)id[i] < (unsigned)p.n_pages;
             const size_t row = (size_t)(h * p.div.size + (ok[i] ? off[i] : 0)) * DH, page = ok[i] ? id[i] : 0;
             kx[i] = *reinterpret_cast<const uint4 *>(kb + (page * p.k_page + row) * kBytes);
             vx[i] = *reinterpret_cast<const uint4 *>(vb + (page * p.v_page + row) * kBytes);
-            if constexpr (MODE == WEIGHTS) key[i] = (page * p.n_kv + h) * p.div.size + off[i];
+            if constexpr (MODE == WEIGHTS) key[i] = scored && ok[i] && sub < heads ? ((uint32_t)(page * p.n_kv + h) * (uint32_t)p.div.size + (uint32_t)off[i]) * (uint32_t)heads + sub : 0xffffffffu;
         }
         pages(base + own + PASS * W * KEYS);
+        if constexpr (MODE == WEIGHTS) store_late();
         float x[G][PASS];
 #pragma unroll
         for (int i = 0; i < PASS; ++i) {
@@ -219,13 +231,12 @@ __device__ __forceinline__ void token_run(const PagedAttn &p, const More<MODE> &
                 for (int e = 1; e < EL; ++e) d = fmaf(q[g][e], f[e], d);
                 x[g][i] = ok[i] ? sum_of_key<LPK>(d) : -INFINITY;
             }
-            if constexpr (MODE == WEIGHTS)
-                if (scored && ok[i] && sub < heads) {  // (lanes of a key have its scores all, and there are at least as many as heads)
-                    float mine = x[0][i];
+            if constexpr (MODE == WEIGHTS) {  // (lanes of a key have its scores all, and there are at least as many as heads)
+                late[i] = x[0][i];
 #pragma unroll
-                    for (int g = 1; g < G; ++g) mine = sub == g ? x[g][i] : mine;
-                    __hip_atomic_store(more.scores + key[i] * heads + sub, mine, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                }
+                for (int g = 1; g < G; ++g) late[i] = sub == g ? x[g][i] : late[i];
+                late_to[i] = key[i];
+            }
         }
 #pragma unroll
         for (int g = 0; g < G; ++g) {
@@ -255,6 +266,7 @@ __device__ __forceinline__ void token_run(const PagedAttn &p, const More<MODE> &
             }
         }
     }
+    if constexpr (MODE == WEIGHTS) store_late();
     // What the rows have seen of a prefix counts as keys of the first run: lanes of a key take a run of it each, as many as there are.  (Loaded before the keys it would cost a wave
     // of five on a SIMD: 64 requests, 25 heads 18.6 us, 16.9.)
     if constexpr (MODE == SHARED) {

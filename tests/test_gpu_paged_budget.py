@@ -565,3 +565,23 @@ def test_evict_twice_and_in_a_graph(agpu, dev):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(x, y) for x, y in zip((*made, kc, vc, w, gs), (*want, *eager, es)))
+
+
+def test_evict_under_a_wide_table(agpu, dev):
+    """Tables that stand for 2^20 positions, whose bits take most of a workgroup's LDS."""
+    import torch
+    kc, vc, w, tables = _evict_case(dev, [300, 5000, 20], 2, 16, "float16", 3)
+    wide = np.full((3, 65536), -1, np.int32)
+    wide[:, :tables.shape[1]] = tables
+    _check_evict(dev, kc, vc, w, wide, [300, 5000, 20], 200, 150, 10, 2)
+    from async_gpu_amd import ops
+    i = _i32(dev)
+    with pytest.raises(agpu.AgpuError) as e:
+        ops.paged_evict(kc, vc, w, i(np.zeros((1, 65537))), i([5]), 4, 4)
+    assert e.value.code == -5
+    with pytest.raises(agpu.AgpuError) as e:
+        ops.paged_evict(kc, vc, w, i(tables), i([300, 5000, 20]), 4, 5)
+    assert e.value.code == -1
+    with pytest.raises(agpu.AgpuError) as e:
+        ops.paged_trim(i([300, 5000, 20]), i(tables), i([1]), i([1]), 16, 4, 5)
+    assert e.value.code == -1
