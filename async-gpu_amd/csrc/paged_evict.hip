@@ -127,6 +127,7 @@ __global__ __launch_bounds__(kEvictThreads) void paged_evict_kernel(const EvictA
     // Who stays, a bit a position: above all that are close; of these none, all, the first of equal ones, or what comes out one by one.
     const bool all_close = left > 0 && left >= close, one_by_one = left > 0 && !all_close && upto > 0, equal = left > 0 && !all_close && upto == 0;
     if (tid == 0) s.n_close = 0;
+    if (tid < kClose) s.close_key[tid] = s.close_at[tid] = 0;
     int ties = left;
     __syncthreads();
     for (int block = 0; block < blocks; ++block) {
@@ -157,8 +158,10 @@ __global__ __launch_bounds__(kEvictThreads) void paged_evict_kernel(const EvictA
             if (near && equal) stay = __builtin_amdgcn_readlane(before, e * kEvictWaves + __builtin_amdgcn_readfirstlane(wave)) + bits_below(same[e]) < ties;
             if (near && one_by_one) {
                 const int at = atomicAdd(&s.n_close, 1);  // (in any order: what comes out does not depend on it)
-                s.close_key[at] = key[e];
-                s.close_at[at] = i;
+                if (at < kClose) {                        // (more only where weights change meanwhile, on a page that another request has too)
+                    s.close_key[at] = key[e];
+                    s.close_at[at] = i;
+                }
             }
             const uint64_t word = __ballot(stay);
             const int chunk = (block * kEvictEach + e) * kEvictWaves + wave;
@@ -249,8 +252,9 @@ __global__ __launch_bounds__(kEvictThreads) void paged_evict_kernel(const EvictA
 #pragma unroll
             for (int r = 0; r < ROUNDS; ++r) {
                 const int i = base + r * kEvictThreads + tid, m = min(i / ROW, now - 1);
-                from[r] = slot_of(s.from[m], from_page[r]);
-                to[r] = slot_of(s.to[m], to_page[r]);
+                // (Every position that moves has one to go to, but where weights changed meanwhile; whatever is in the lists then, it is kept to the request's own positions.)
+                from[r] = slot_of((int)min((uint32_t)s.from[m], (uint32_t)n - 1), from_page[r]);
+                to[r] = slot_of((int)min((uint32_t)s.to[m], (uint32_t)n - 1), to_page[r]);
                 ok[r] = i < now * ROW && from[r] >= 0 && to[r] >= 0;
                 if (!ok[r]) from[r] = from_page[r] = 0;  // (loaded all the same, so that all loads are on their way together)
             }

@@ -585,3 +585,18 @@ def test_evict_under_a_wide_table(agpu, dev):
     with pytest.raises(agpu.AgpuError) as e:
         ops.paged_trim(i([300, 5000, 20]), i(tables), i([1]), i([1]), 16, 4, 5)
     assert e.value.code == -1
+
+
+def test_evict_of_pages_that_two_requests_have(agpu, dev):
+    """A page belongs to one request only; where one does not, what becomes of it is left open, but of nothing else."""
+    import torch
+    from async_gpu_amd import ops
+    i = _i32(dev)
+    lens = [9000, 9000, 6000]
+    kc, vc, w, tables = _evict_case(dev, lens, 2, 64, "bfloat16", 3)
+    tables[1] = tables[0]
+    others = torch.as_tensor(np.setdiff1d(np.arange(kc.shape[0]), tables[0]), device=dev)
+    alone = [x.clone() for x in (kc, vc, w)]
+    ops.paged_evict(*alone, i(tables[2:]), i(lens[2:]), 4500, 4000, 100, 4)
+    ops.paged_evict(kc, vc, w, i(tables), i(lens), 4500, 4000, 100, 4)
+    assert all(torch.equal(x[others], y[others]) for x, y in zip((kc, vc, w), alone))
