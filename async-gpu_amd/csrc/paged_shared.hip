@@ -387,7 +387,7 @@ __global__ __launch_bounds__(256, 2) void paged_prefix_kernel(const PagedAttn p,
         if (other.count > 0) atomicAdd(&s.rows[other.g], other.count);
     }
     __syncthreads();
-    auto rows_behind = [&](int g) { return min(s.rows[g], p.tokens) * group; };
+    auto rows_behind = [&](int g) { return min(max(s.rows[g], 0), p.tokens) * group; };  // (query_starts that overlap may count to more than there are, or than an int holds)
     int tiles[4], keys[4], longest = 0;
     float work = 0.0f;
 #pragma unroll
