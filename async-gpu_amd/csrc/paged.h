@@ -127,7 +127,7 @@ inline PrefixRuns prefix_runs(int64_t batch, int64_t rows, int64_t held, bool ap
 }
 
 // The scratch of attention that adds up its weights: 8 bytes a row of heads, then, where there is room in half of it (and a K/V head has eight query heads at most),
-// a score for each place and query head.  Where the scores begin (0: none), and what all of it takes (0: it is too small).
+// a score for each key (place of the cache, or key that a row of a request can see) and query head.  Where the scores begin (0: none), and what all of it takes (0: it is too small).
 struct WeightsRoom {
     size_t scores, bytes;
 };

@@ -37,10 +37,16 @@ template <>
 struct More<WEIGHTS> {
     float *weights;   // [n_pages][n_kv][page_size]
     long long page;   // elements between pages
-    float *scores;    // [n_pages][n_kv][page_size][group]: of requests with one row; null: there is no room for them
+    float *scores;    // of requests with one row: [batch][n_kv][seen][group], or, with seen = 0, [n_pages][n_kv][page_size][group]; null: there is no room for them
+    int seen;         // the most keys that a row sees
     float2 *stats;    // [tokens][n_heads]: the unit of a row's weights and what they are divided by
     bool few;         // weights are added up from scores by the last workgroup at a token; otherwise, and without scores, by paged_weights_kernel
     __device__ __forceinline__ bool scored(int rows, int group) const { return rows == 1 && group <= 8 && scores != nullptr; }
+    // Where the first score of request b's key number v is, which is at position `off` of a page (there are less than 2^32 scores).
+    __device__ __forceinline__ uint32_t score_at(const PagedAttn &p, int b, int h, int v, int page, int off) const {
+        const uint32_t size = seen ? seen : p.div.size;
+        return ((uint32_t)((seen ? b : page) * p.n_kv + h) * size + (uint32_t)(seen ? v : off)) * (uint32_t)p.group.size;
+    }
 };
 template <>
 struct More<SHARED> {
@@ -208,14 +214,14 @@ __device__ __forceinline__ void token_run(const PagedAttn &p, const More<MODE> &
     for (int base = first - own; base < hi; base += PASS * W * KEYS) {
         uint4 kx[PASS], vx[PASS];
         bool ok[PASS];
-        uint32_t key[PASS];  // of all places and K/V heads: where its scores go (there are less than 2^32 of them)
+        uint32_t key[PASS];  // where this lane's score goes
 #pragma unroll
         for (int i = 0; i < PASS; ++i) {
             ok[i] = (unsigned)id[i] < (unsigned)p.n_pages;
             const size_t row = (size_t)(h * p.div.size + (ok[i] ? off[i] : 0)) * DH, page = ok[i] ? id[i] : 0;
             kx[i] = *reinterpret_cast<const uint4 *>(kb + (page * p.k_page + row) * kBytes);
             vx[i] = *reinterpret_cast<const uint4 *>(vb + (page * p.v_page + row) * kBytes);
-            if constexpr (MODE == WEIGHTS) key[i] = scored && ok[i] && sub < heads ? ((uint32_t)(page * p.n_kv + h) * (uint32_t)p.div.size + (uint32_t)off[i]) * (uint32_t)heads + sub : 0xffffffffu;
+            if constexpr (MODE == WEIGHTS) key[i] = scored && ok[i] && sub < heads ? more.score_at(p, b, h, base + own + i * (W * KEYS), id[i], off[i]) + sub : 0xffffffffu;
         }
         pages(base + own + PASS * W * KEYS);
         if constexpr (MODE == WEIGHTS) store_late();
@@ -351,7 +357,7 @@ __device__ __forceinline__ void token_run(const PagedAttn &p, const More<MODE> &
                     const bool there = (unsigned)page[k] < (unsigned)p.n_pages;
                     page[k] = there ? page[k] : -1;
                     const size_t of = there ? page[k] : 0;
-                    const float *const score = more.scores + (of * p.n_kv * p.div.size + place[k]) * heads;
+                    const float *const score = more.scores + more.score_at(p, b, h, min(v0 + k * 64 * W, vis.count - 1), (int)of, place[k] - h * p.div.size);
 #pragma unroll
                     for (int g = 0; g < G; ++g) x[k][g] = __hip_atomic_load(score + min(g, heads - 1), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
                     old[k] = more.weights[of * more.page + place[k]];

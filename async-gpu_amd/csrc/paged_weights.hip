@@ -211,7 +211,7 @@ __device__ __forceinline__ void add_scored(const PagedAttn &p, const More<WEIGHT
     for (int k = 0; k < EACH; ++k) {
         const bool there = (unsigned)page[k] < (unsigned)p.n_pages;
         const size_t of = there ? page[k] : 0;
-        score[k] = more.scores + (of * p.n_kv * p.div.size + place[k]) * group;
+        score[k] = more.scores + more.score_at(p, b, h, min(v0 + 256 * k + (int)threadIdx.x, vis.count - 1), (int)of, place[k] - h * p.div.size);
         to[k] = more.weights + of * more.page + place[k];
         old[k] = *to[k];
         sum[k] = 0.0f;
@@ -299,18 +299,22 @@ AGPU_EXPORT int32_t agpu_paged_attention_weights(agpu_ctx *ctx, const float *q, 
     if (here.rc != AGPU_OK) return here.rc;
     const PagedAttn p = paged_attn(q, q_token_stride, q_head_stride, k_cache, v_cache, k_page_stride, v_page_stride, block_tables, kv_lens, query_start, o, tokens, batch, n_heads,
                                    n_kv_heads, n_pages, page_size, table_width, window, sinks, ctx->strict_sync);
-    const paged::WeightsRoom room = paged::weights_room((int64_t)tokens * n_heads, (int64_t)n_pages * page_size * n_heads, n_heads / n_kv_heads, ctx->ws_bytes);
+    // Scores lie by requests, or by places of the cache, whichever are fewer (a large cache, or tables much wider than requests are long).  Without room for them they are formed again:
+    // 64 tokens of 1 to 4096 keys, 32 heads over 8, f16, 62 us, 41 with scores.
+    const int64_t longest = paged::longest_row(p.held, window, sinks), by_place = (int64_t)n_pages * page_size, by_request = batch * longest;
+    const paged::WeightsRoom room = paged::weights_room((int64_t)tokens * n_heads, std::min(by_place, by_request) * n_heads, n_heads / n_kv_heads, ctx->ws_bytes);
     if (room.bytes == 0) return agpu_fail(ctx, AGPU_ERR_WORKSPACE, "paged_attention_weights: %d rows of %d heads need a larger scratch", tokens, n_heads);
     More<WEIGHTS> more{};
     more.weights = weights; more.page = weights_page_stride;
     more.stats = reinterpret_cast<float2 *>(ctx->workspace);
+    more.seen = by_request < by_place ? (int)longest : 0;
     more.scores = room.scores ? reinterpret_cast<float *>(ctx->workspace + room.scores) : nullptr;
     // The last workgroup at a token adds up its weights where other work goes on meanwhile (chunks beside tokens: 37 us, 39 with a launch for them), or where there is so little of it that
     // a launch more costs as much (12 heads of 777 keys: 10 us, and 4 for the launch where query_start leaves open whether there are chunks); 64 tokens of up to 4096 keys, 8 heads: 43 us that way, 40 with one.
-    more.few = more.scores && (tokens > batch || (int64_t)tokens * n_kv_heads * std::min<int64_t>(paged::longest_row(p.held, window, sinks), kScoredKeys) <= 64 * kScoredKeys);
+    more.few = more.scores && (tokens > batch || (int64_t)tokens * n_kv_heads * std::min<int64_t>(longest, kScoredKeys) <= 64 * kScoredKeys);
     return of_type(cache_type, [&](auto type) {
         using T = decltype(type);
-        int32_t rc = attention_go<T, WEIGHTS>(ctx, p, paged::longest_row(p.held, window, sinks), more, ctx->workspace + room.bytes, ctx->ws_bytes - room.bytes);
+        int32_t rc = attention_go<T, WEIGHTS>(ctx, p, longest, more, ctx->workspace + room.bytes, ctx->ws_bytes - room.bytes);
         if (rc != AGPU_OK || (!query_start && more.few)) return rc;
         hipLaunchKernelGGL((paged_weights_kernel<T>), dim3(2 * ctx->num_cus), dim3(256), 0, ctx->stream, p, more);
         return AGPU_LAUNCH_CHECK(ctx, "paged_weights_kernel");

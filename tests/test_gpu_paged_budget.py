@@ -600,3 +600,23 @@ def test_evict_of_pages_that_two_requests_have(agpu, dev):
     ops.paged_evict(*alone, i(tables[2:]), i(lens[2:]), 4500, 4000, 100, 4)
     ops.paged_evict(kc, vc, w, i(tables), i(lens), 4500, 4000, 100, 4)
     assert all(torch.equal(x[others], y[others]) for x, y in zip((kc, vc, w), alone))
+
+
+@pytest.mark.parametrize("type_", TYPES)
+@pytest.mark.parametrize("heads,kv_heads,window,sinks", [(3, 3, 0, 0), (8, 2, 0, 0), (5, 1, 300, 7), (16, 2, 0, 0)])
+@pytest.mark.parametrize("new", [[1] * 6, [1, 1, 30, 1, 0, 1]])
+def test_tokens_of_a_large_cache(agpu, dev, type_, heads, kv_heads, window, sinks, new):
+    """Where scores wait depends on which are fewer, places of the cache or keys of the requests; what comes out does not."""
+    import torch
+    lens = [3000, 2100, 700, 40, 1200, 1]
+    kc, vc, w, tables, start, q = _state(dev, lens, new, heads, kv_heads, 16, type_, heads)
+    large = [torch.cat([x, torch.full((2000, *x.shape[1:]), float("nan"), device=dev, dtype=x.dtype)]) for x in (kc, vc, w)]
+    wide = np.full((6, 2000), -1, np.int32)
+    wide[:, :tables.shape[1]] = tables
+    got = []
+    for cache, table in (((kc, vc, w.clone()), wide), (large, np.where(tables >= kc.shape[0], -1, tables))):
+        out, weights = _attend(dev, q, *cache, table, lens, start, window, sinks)
+        got.append((out, weights[:kc.shape[0]]))
+        assert torch.isnan(weights[kc.shape[0]:]).all()
+    check(got[0][1], *given64(q, kc, w, tables, lens, start, window, sinks))
+    assert torch.equal(got[0][1], got[1][1]) and torch.equal(got[0][0], got[1][0])
