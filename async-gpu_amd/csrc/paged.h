@@ -106,6 +106,10 @@ inline int most_runs(int64_t items, int64_t longest, int64_t least, size_t item_
 // The most keys a row can see.
 inline int64_t longest_row(int64_t held, int64_t window, int64_t sinks) { return window > 0 && window + sinks < held ? window + sinks : held; }
 
+// Of a request's tiles of keys, how many of each of n_kv heads are numbered at a time, so that 256 requests' numbers stay below 2^31: 2^22 in all, or one a head (of which there are
+// less than 2^23, as there are rows of heads).  Only weights of more than 2^29 keys times heads are numbered more than once.
+AGPU_HD int weight_tiles(int n_kv) { return n_kv < 1 << 22 ? (1 << 22) / n_kv : 1; }
+
 // The scratch of a prefix's runs, for `rows` rows of heads and `held` keys at most: how many runs there is room for in half of it (0: not even for one), where their (m, l)
 // begin, which are 8 bytes a row, where o of the second and later ones, which is 256 (`apart`: and of the first one behind them), and what all of it takes.  Before them is a number a
 // request.

@@ -40,6 +40,7 @@ struct More<WEIGHTS> {
     float *scores;    // of requests with one row: [batch][n_kv][seen][group], or, with seen = 0, [n_pages][n_kv][page_size][group]; null: there is no room for them
     int seen;         // the most keys that a row sees
     float2 *stats;    // [tokens][n_heads]: the unit of a row's weights and what they are divided by
+    int at_once;      // tiles of a head's keys that are numbered at a time
     bool few;         // weights are added up from scores by the last workgroup at a token; otherwise, and without scores, by paged_weights_kernel
     __device__ __forceinline__ bool scored(int rows, int group) const { return rows == 1 && group <= 8 && scores != nullptr; }
     // Where the first score of request b's key number v is, which is at position `off` of a page (there are less than 2^32 scores).

@@ -229,7 +229,7 @@ __device__ __forceinline__ void add_scored(const PagedAttn &p, const More<WEIGHT
     }
 }
 
-// Units: 128 keys of a request and K/V head, or 1024 of one whose scores are there, 256 requests at a time.
+// Units: tiles of 128 keys of a request and K/V head, or of 1024 of one whose scores are there, 256 requests at a time.
 template <class T>
 __global__ __launch_bounds__(256, 2) void paged_weights_kernel(const PagedAttn p, const More<WEIGHTS> more) {
     __shared__ RowsShared<T> s;
@@ -237,10 +237,11 @@ __global__ __launch_bounds__(256, 2) void paged_weights_kernel(const PagedAttn p
     __shared__ int starts[kListed], rows[kListed], in_call[kListed];
     const int lane = threadIdx.x & 63;
     int before = 0;  // units of the requests so far, modulo the grid
-    for (int b0 = 0; b0 < p.batch; b0 += kListed) {
+    for (int b0 = 0, skip = 0; b0 < p.batch;) {  // skip: tiles of each head that are done (where a request has more of them than are numbered at a time)
         __syncthreads();
         const int entries = min(p.batch - b0, kListed);
         int units[4];
+        bool rest = false;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             units[j] = 0;
@@ -252,24 +253,29 @@ __global__ __launch_bounds__(256, 2) void paged_weights_kernel(const PagedAttn p
                 const bool scored = more.scored(end - start, p.group.size);
                 if (start >= 0 && there > 0 && !(scored && more.few)) {
                     const int count = paged::tile_keys(kv_len - (end - start), kv_len - 1, p.held, p.window, p.sinks).count, each = scored ? kScoredKeys : 128;
-                    units[j] = (int)min((long long)((count + each - 1) / each) * p.n_kv, 1ll << 22);  // (that many are 137 GB of keys at least; their sum stays below 2^31)
+                    const int tiles = max((count + each - 1) / each - skip, 0);
+                    units[j] = min(tiles, more.at_once) * p.n_kv;
+                    rest |= tiles > more.at_once;
                 }
                 starts[i] = start;
                 rows[i] = end - start;
                 in_call[i] = there;
             }
         }
+        const int b_now = b0, skip_now = skip;
+        if (__any(rest)) skip += more.at_once;  // uniform, and the same in every wave
+        else b0 += kListed, skip = 0;
         if (!__any(units[0] + units[1] + units[2] + units[3] > 0)) continue;  // uniform: nobody here has several rows
         const int all = list.number(units, entries, lane);
         __syncthreads();
         const int grid = gridDim.x, first = (int)blockIdx.x >= before ? (int)blockIdx.x - before : (int)blockIdx.x - before + grid;
         for (int unit = first; unit < all; unit += grid) {
             int at = unit;
-            const int i = list.entry(at, lane), h = at % p.n_kv, tile = at / p.n_kv;
+            const int i = list.entry(at, lane), h = at % p.n_kv, tile = skip_now + at / p.n_kv;
             if (more.scored(rows[i], p.group.size)) {
-                add_scored(p, more, b0 + i, starts[i], h, kScoredKeys * tile);
+                add_scored(p, more, b_now + i, starts[i], h, kScoredKeys * tile);
             } else {
-                weigh_keys<T>(p, more, s, b0 + i, starts[i], rows[i], in_call[i], h, 128 * tile);
+                weigh_keys<T>(p, more, s, b_now + i, starts[i], rows[i], in_call[i], h, 128 * tile);
                 __syncthreads();
             }
         }
@@ -309,6 +315,7 @@ AGPU_EXPORT int32_t agpu_paged_attention_weights(agpu_ctx *ctx, const float *q, 
     more.stats = reinterpret_cast<float2 *>(ctx->workspace);
     more.seen = by_request < by_place ? (int)longest : 0;
     more.scores = room.scores ? reinterpret_cast<float *>(ctx->workspace + room.scores) : nullptr;
+    more.at_once = paged::weight_tiles(n_kv_heads);
     // The last workgroup at a token adds up its weights where other work goes on meanwhile (chunks beside tokens: 37 us, 39 with a launch for them), or where there is so little of it that
     // a launch more costs as much (12 heads of 777 keys: 10 us, and 4 for the launch where query_start leaves open whether there are chunks); 64 tokens of up to 4096 keys, 8 heads: 43 us that way, 40 with one.
     more.few = more.scores && (tokens > batch || (int64_t)tokens * n_kv_heads * std::min<int64_t>(longest, kScoredKeys) <= 64 * kScoredKeys);
