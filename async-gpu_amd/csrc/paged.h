@@ -143,6 +143,14 @@ inline WeightsRoom weights_room(int64_t rows, int64_t places, int group, size_t 
     return {stats, stats + up(4 * (size_t)places)};
 }
 
+// Of up to 2^15 positions of a request that is cut down, how many are holes (places of evicted ones) and how many move, as one number that may be added up: 2^15 movers are 2^31.
+struct HolesMoves {
+    uint32_t both;
+    static AGPU_HD HolesMoves of(int holes, int moves) { return {(uint32_t)holes | (uint32_t)moves << 16}; }
+    AGPU_HD int holes() const { return (int)(both & 0xffffu); }
+    AGPU_HD int moves() const { return (int)(both >> 16); }
+};
+
 // ---- what calls are refused: 0, or the error and why --------------------------------------------
 
 struct Refusal {

@@ -13,6 +13,7 @@
 
 namespace {
 
+using paged::HolesMoves;
 using paged::PageDiv;
 
 struct EvictArgs {
@@ -37,13 +38,13 @@ __device__ __forceinline__ uint32_t order_of(float w) {
 
 struct EvictShared {
     int bins[kBins];
-    int wave_sums[kEvictWaves];
+    uint32_t wave_sums[kEvictWaves];
     int found[3];  // the bin that what stays ends in, how many are above it, and in it
     int n_close;
     uint32_t close_key[kClose];
     int close_at[kClose];
     int ties[kEvictEach * kEvictWaves];  // of each 64 positions of a block
-    int before[kEvictThreads];           // of each 64 positions: places of evicted ones, and in the upper half those that move
+    HolesMoves before[kEvictThreads];    // in front of each 64 positions of 64 * 512
     int to[kEvictListed], from[kEvictListed];  // positions
 };
 
@@ -106,11 +107,11 @@ __global__ __launch_bounds__(kEvictThreads) void paged_evict_kernel(const EvictA
         int own = 0;
         for (int i = 0; i < each; ++i) own += s.bins[first - i];
         const int sum = wave_running_sum(own);
-        if (lane == 63) s.wave_sums[wave] = sum;
+        if (lane == 63) s.wave_sums[wave] = (uint32_t)sum;
         __syncthreads();
         int above = sum - own;
 #pragma unroll
-        for (int w = 0; w < kEvictWaves; ++w) above += w < wave ? s.wave_sums[w] : 0;
+        for (int w = 0; w < kEvictWaves; ++w) above += w < wave ? (int)s.wave_sums[w] : 0;
         if (above < left && above + own >= left) {  // (one thread's)
             int i = 0;
             while (above + s.bins[first - i] < left) above += s.bins[first - i++];
@@ -200,27 +201,30 @@ __global__ __launch_bounds__(kEvictThreads) void paged_evict_kernel(const EvictA
     auto list = [&](bool holes, bool movers, int done) __attribute__((always_inline)) {
         for (;;) {
             const int group = holes ? hole.group : move.group, chunk = group * kEvictThreads + tid;
-            const int own = chunk < chunks ? __popcll(word(true, chunk)) | __popcll(word(false, chunk)) << 16 : 0, sum = wave_running_sum(own);
+            const uint32_t own = chunk < chunks ? HolesMoves::of(__popcll(word(true, chunk)), __popcll(word(false, chunk))).both : 0;
+            const uint32_t sum = (uint32_t)wave_running_sum((int)own);  // (of a wave 2^28 at most)
             if (lane == 63) s.wave_sums[wave] = sum;
             __syncthreads();
-            int before = sum - own, all = 0;
+            uint32_t before = sum - own;
+            HolesMoves all = {0};
 #pragma unroll
             for (int w = 0; w < kEvictWaves; ++w) {
                 if (w < wave) before += s.wave_sums[w];
-                all += s.wave_sums[w];
+                all.both += s.wave_sums[w];
             }
-            s.before[tid] = before;
+            s.before[tid] = {before};
             __syncthreads();
-            const int hole_base = hole.before - done, move_base = move.before - done, all_holes = all & 0xffff, all_moves = (int)((unsigned)all >> 16);
+            const int hole_base = hole.before - done, move_base = move.before - done, all_holes = all.holes(), all_moves = all.moves();
             for (int c = wave; c < kEvictThreads && group * kEvictThreads + c < chunks; c += kEvictWaves) {
-                const int at = group * kEvictThreads + c, packed = s.before[c];
+                const int at = group * kEvictThreads + c;
+                const HolesMoves front = s.before[c];
                 auto note = [&](bool which, int rank, int *out) {
                     const uint64_t bits = word(which, at);
                     rank += bits_below(bits);
                     if ((bits >> lane & 1) && rank >= 0 && rank < kEvictListed) out[rank] = 64 * at + lane;
                 };
-                if (holes) note(true, hole_base + (packed & 0xffff), s.to);
-                if (movers) note(false, move_base + (int)((unsigned)packed >> 16), s.from);
+                if (holes) note(true, hole_base + front.holes(), s.to);
+                if (movers) note(false, move_base + front.moves(), s.from);
             }
             __syncthreads();
             const bool end = (group + 1) * kEvictThreads >= chunks;

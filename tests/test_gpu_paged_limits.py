@@ -2,7 +2,7 @@
 import numpy as np
 import pytest
 from test_gpu_paged import check
-from test_gpu_paged_budget import _attend, given64
+from test_gpu_paged_budget import _attend, _check_evict, _evict_case, given64
 
 pytestmark = pytest.mark.gpu
 
@@ -25,3 +25,10 @@ def test_weights_of_hundreds_of_millions_of_keys(agpu, dev, type_, page, missing
     assert (tol[4, :, :page // 3] > 0).all()
     _attend(dev, q, kc, vc, w, tables, lens, start)
     check(w, want, tol)
+
+
+@pytest.mark.parametrize("n,limit,keep,recent,sinks", [(100000, 40000, 40000, 40000, 0), (200000, 100000, 100000, 100000, 0), (200000, 150000, 99990, 99980, 4), (140000, 70000, 65536, 0, 65536)])
+def test_evict_where_all_of_a_range_moves(agpu, dev, n, limit, keep, recent, sinks):
+    """2^15 positions in a row of which all are evicted, all move or all stay: the last ones are nearly all that is kept, or the first ones."""
+    kc, vc, w, tables = _evict_case(dev, [n, 3], 1, 100, "bfloat16", keep)
+    _check_evict(dev, kc, vc, w, tables, [n, 3], limit, keep, recent, sinks)
