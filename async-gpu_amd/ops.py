@@ -246,7 +246,7 @@ def paged_evict(k_cache, v_cache, weights, block_tables, kv_lens, limit, keep, r
 
 def paged_trim(kv_lens, block_tables, free_pages, n_free, page_size, limit, keep):
     """Lengths and pages behind paged_evict, once a step: -> (kv_lens [batch], evicted [batch], n_free [1]).  Requests of more than `limit` positions have `keep` now, and the pages behind
-    are on the stack free_pages (in place).  evicted is how many positions went: positions of paged_plan are places, so that a model whose embeddings go by
+    are on the stack free_pages (in place), as the tables have them: they have to be pages of the cache, as those of requests that end in paged_plan.  evicted is how many positions went: positions of paged_plan are places, so that a model whose embeddings go by
     position adds up what was evicted."""
     return _native.paged_trim(kv_lens, block_tables, free_pages, n_free, page_size, limit, keep)
 

@@ -461,7 +461,9 @@ int32_t agpu_paged_evict(agpu_ctx *ctx, void *k_cache, void *v_cache, int64_t k_
                          int32_t d_head, int32_t cache_type);
 /* Lengths and pages behind agpu_paged_evict: kv_lens_out [batch] is `keep` where kv_lens is more than `limit` (and kv_lens, within what the table has pages for, elsewhere), evicted
  * [batch] how many positions that is less, to be added up by a caller whose embeddings go by position; the pages behind `keep` go onto the stack free_pages [stack_size] of n_free [1]
- * pages, in the order of requests and positions (what has no place there is lost), n_free_out [1] of them.  The outputs do not overlap the inputs.  4096 requests at most. */
+ * pages, in the order of requests and positions (what has no place there is lost), n_free_out [1] of them.  They go there as block_tables has them, as those of requests that end do in
+ * agpu_paged_plan: entries from `keep` on have to be pages of the cache.  (An id outside it, whose keys the other operators take for missing, would be given to a request later: what that
+ * one appends there is kept nowhere, and not seen.)  The outputs do not overlap the inputs.  4096 requests at most. */
 int32_t agpu_paged_trim(agpu_ctx *ctx, const int32_t *kv_lens, const int32_t *block_tables, int32_t *free_pages, const int32_t *n_free, int32_t *kv_lens_out,
                         int32_t *evicted, int32_t *n_free_out, int32_t batch, int32_t table_width, int32_t stack_size, int32_t page_size, int32_t limit,
                         int32_t keep);
