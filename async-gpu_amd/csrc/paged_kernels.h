@@ -444,13 +444,7 @@ struct Units {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             if (64 * j >= entries) break;  // uniform
-            int v = units[j];
-            v += (int)dpp_move_u32<0x111, 0xf>(0, v);  // row_shr 1, 2, 4, 8, then row_bcast 15 and 31: sums over the lanes up to this one
-            v += (int)dpp_move_u32<0x112, 0xf>(0, v);
-            v += (int)dpp_move_u32<0x114, 0xf>(0, v);
-            v += (int)dpp_move_u32<0x118, 0xf>(0, v);
-            v += (int)dpp_move_u32<0x142, 0xa>(0, v);
-            v += (int)dpp_move_u32<0x143, 0xc>(0, v);
+            const int v = wave_running_sum(units[j]);
             incl[64 * j + lane] = v + all;
             all += __builtin_amdgcn_readlane(v, 63);
         }
