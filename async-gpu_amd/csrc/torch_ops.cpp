@@ -506,33 +506,6 @@ PyObject *paged_kv_append(PyObject *const *a) {
     return Py_BuildValue("(OO)", a[2], a[3]);
 }
 
-// q, k_cache, v_cache, block_tables, kv_lens, query_start, window, sinks, out
-PyObject *paged_attention(PyObject *const *a) {
-    const at::Tensor &kc = pages(a[1], "k_cache [n_pages, n_kv_heads, page_size, d_head]"), &vc = pages(a[2], "v_cache [n_pages, n_kv_heads, page_size, d_head]");
-    same_cache(kc, vc);
-    const at::Tensor &q = rows(a[0], -1, -1, kc.size(3), "q [tokens, n_heads, d_head]");
-    const at::Tensor &tables = ints(a[3], {-1, -1}, "block_tables [batch, width]");
-    const int64_t tokens = q.size(0), heads = q.size(1), batch = tables.size(0);
-    const at::Tensor &lens = ints(a[4], {batch}, "kv_lens [batch]");
-    const bool ragged = a[5] != Py_None, given = a[8] != Py_None;
-    const at::Tensor &start = ragged ? ints(a[5], {batch + 1}, "query_start [batch + 1]") : lens;
-    if (!ragged && tokens != batch) shape_err("a row for each of " + str(batch) + " requests without query_start", str(tokens));
-    if (given) {
-        const at::Tensor &o = typed(a[8], at::kFloat, {tokens, heads, q.size(2)}, "out [tokens, n_heads, d_head]");
-        if (!o.is_contiguous()) shape_err("contiguous out", "strides " + str(o.strides()));
-        for (const at::Tensor *t : {&q, &kc, &vc})
-            if (o.is_alias_of(*t)) shape_err("out with memory of its own", "that of an input");
-    }
-    together(q, kc, vc, tables, lens, start);
-    at::Tensor o = given ? tensor(a[8]) : empty(q.sizes(), q);
-    together(q, o);
-    float *const op = written(o);
-    call(lib.agpu_paged_attention_, context(q), data(q), q.stride(0), q.stride(1), kc.const_data_ptr(), vc.const_data_ptr(), page_stride(kc), page_stride(vc), ip(tables),
-         ip(lens), ragged ? ip(start) : nullptr, op, i32(tokens), i32(batch), i32(heads), i32(kc.size(1)), i32(kc.size(0)), i32(kc.size(2)), i32(tables.size(1)),
-         i32(a[6]), i32(a[7]), i32(q.size(2)), cache_type(kc));
-    return given ? same(a[8]) : wrap(std::move(o));
-}
-
 // What paged_attention and the operators like it have in common: q, k_cache, v_cache; then block_tables, kv_lens, query_start; out behind them.
 struct Attends {
     const at::Tensor &kc, &vc, &q, &tables, &lens, &start;
@@ -561,6 +534,18 @@ struct Attends {
     }
     const int32_t *starts() const { return ragged ? ip(start) : nullptr; }
 };
+
+// q, k_cache, v_cache, block_tables, kv_lens, query_start, window, sinks, out
+PyObject *paged_attention(PyObject *const *a) {
+    const Attends c(a[0], a[1], a[2], a[3], a[4], a[5], a[8]);
+    at::Tensor o = c.out(a[8]);
+    float *const op = written(o);
+    call(lib.agpu_paged_attention_, context(c.q), data(c.q), c.q.stride(0), c.q.stride(1), c.kc.const_data_ptr(), c.vc.const_data_ptr(), page_stride(c.kc), page_stride(c.vc), ip(c.tables),
+         ip(c.lens), c.starts(), op, i32(c.tokens), i32(c.batch), i32(c.heads), i32(c.kc.size(1)), i32(c.kc.size(0)), i32(c.kc.size(2)), i32(c.tables.size(1)), i32(a[6]), i32(a[7]),
+         i32(c.q.size(2)), cache_type(c.kc));
+    return c.given ? same(a[8]) : wrap(std::move(o));
+}
+
 // What each key of a cache was given: [n_pages, n_kv_heads, page_size], a page contiguous, pages anywhere
 const at::Tensor &weights_of(PyObject *o, const at::Tensor &cache) {
     const int64_t heads = cache.size(1), size = cache.size(2);
