@@ -3,8 +3,11 @@
 //   cache   [n_pages][n_kv_heads][page_size][64], pages page_stride elements apart; a slot is page * page_size + offset
 //   tables  [batch][width] page ids: position p of request b is on page tables[b][p / page_size]
 #pragma once
+#include <algorithm>
 #include <cstddef>
 #include <cstdint>
+#include <initializer_list>
+#include <numeric>
 
 #include "../../include/agpu.h"
 
@@ -200,6 +203,70 @@ inline Refusal refuse_weights(uintptr_t weights, int64_t page_stride, int32_t n_
     if (n_pages > 1 && page_stride < (int64_t)n_kv_heads * page_size) return {AGPU_ERR_SHAPE_MISMATCH, "pages of the weights overlap"};
     if (weights % 4) return {AGPU_ERR_UNSUPPORTED, "weights begin at 4 bytes"};
     return kFine;
+}
+
+// `n` pieces of memory of `bytes` each, `stride` bytes apart: pages of a cache, or rows.
+struct Pieces {
+    uintptr_t at;
+    int64_t n, stride, bytes;
+    static Pieces one(const void *p, int64_t bytes) { return {(uintptr_t)p, 1, 0, bytes}; }
+    static Pieces pages(const void *p, int64_t n, int64_t stride, int64_t bytes) { return n > 1 ? Pieces{(uintptr_t)p, n, stride, bytes} : one(p, n * bytes); }
+    // Rows of q [tokens][heads][64]; at two strides that leave gaps all from the first to the last.
+    static Pieces rows(const float *p, int64_t tokens, int64_t heads, int64_t row, int64_t head) {
+        if (tokens <= 0 || heads <= 0) return one(p, 0);
+        if (row > 0 && (heads == 1 || head == 64)) return pages(p, tokens, 4 * row, 256 * heads);
+        if (head > 0 && (tokens == 1 || row == 64)) return pages(p, heads, 4 * head, 256 * tokens);
+        const int64_t r = row * (tokens - 1), h = head * (heads - 1), low = std::min<int64_t>(r, 0) + std::min<int64_t>(h, 0);
+        return one(p + low, 4 * (std::max<int64_t>(r, 0) + std::max<int64_t>(h, 0) - low + 64));
+    }
+};
+// Whether two have a byte in common.  Those of one stride, and single ones, by a division; of two strides by what is left modulo both, and if that does not tell, piece by piece.
+inline bool share(Pieces a, Pieces b) {
+    typedef __int128 Wide;
+    if (a.n <= 0 || b.n <= 0 || a.bytes <= 0 || b.bytes <= 0) return false;
+    if (a.n == 1 && b.n == 1) return a.at < b.at + (uintptr_t)b.bytes && b.at < a.at + (uintptr_t)a.bytes;
+    // Is there a k in low .. high with more - a.bytes < k * stride < more + b.bytes, where piece k of a begins `more` bytes before b?
+    auto meets = [&](Wide more, Wide low, Wide high, Wide stride) {
+        const Wide from = more - a.bytes, to = more + b.bytes;
+        if (stride <= 0) return low <= high && from < 0 && 0 < to;
+        const Wide down = from >= 0 ? from / stride : -((-from + stride - 1) / stride);     // of from / stride
+        const Wide up = to > 0 ? (to + stride - 1) / stride : -(-to / stride);              // of to / stride, upwards
+        return std::max(low, down + 1) <= std::min(high, up - 1);
+    };
+    const Wide apart = (Wide)b.at - (Wide)a.at;
+    if (apart >= (Wide)(a.n - 1) * a.stride + a.bytes || -apart >= (Wide)(b.n - 1) * b.stride + b.bytes) return false;
+    if (a.n == 1 || b.n == 1 || a.stride == b.stride) {
+        const bool alone = a.n == 1;  // (the stride is the other's then)
+        return meets(apart, -(Wide)(b.n - 1), a.n - 1, alone ? b.stride : a.stride);
+    }
+    const Wide both = std::gcd(a.stride, b.stride);
+    if (both > 0) {
+        const Wide left = (apart % both + both) % both;
+        if (left >= a.bytes && both - left >= b.bytes) return false;
+    }
+    if (a.n > b.n) std::swap(a, b);
+    for (int64_t i = 0; i < a.n; ++i)
+        if (meets((Wide)b.at - (Wide)a.at - (Wide)i * a.stride, -(Wide)(b.n - 1), 0, b.stride)) return true;
+    return false;
+}
+// What is written, and what it must not share memory with.
+inline Refusal refuse_shared_memory(const Pieces &written, std::initializer_list<Pieces> others, const char *why) {
+    for (const Pieces &p : others)
+        if (share(written, p)) return {AGPU_ERR_UNSUPPORTED, why};
+    return kFine;
+}
+
+inline Pieces cache_pages(const void *p, int64_t page_stride, int32_t n_kv_heads, int32_t n_pages, int32_t page_size, int bytes) {
+    return Pieces::pages(p, n_pages, page_stride * bytes, (int64_t)n_kv_heads * page_size * 64 * bytes);
+}
+inline Pieces weight_pages(const float *p, int64_t page_stride, int32_t n_kv_heads, int32_t n_pages, int32_t page_size) {
+    return Pieces::pages(p, n_pages, 4 * page_stride, (int64_t)n_kv_heads * page_size * 4);
+}
+// K and V may be one and the same: then what moves moves twice, to the same place.
+inline Refusal refuse_evicted_memory(const Pieces &k, const Pieces &v, const Pieces &weights) {
+    const Refusal no = refuse_shared_memory(weights, {k, v}, "the weights share memory with K or V");
+    if (no.code != AGPU_OK || (k.at == v.at && k.stride == v.stride)) return no;
+    return refuse_shared_memory(k, {v}, "K and V share memory and are not the same");
 }
 
 // What a request is cut down to.

@@ -361,9 +361,12 @@ AGPU_EXPORT int32_t agpu_paged_evict(agpu_ctx *ctx, void *k_cache, void *v_cache
     const int held = table_width * page_size;
     if (batch == 0 || held <= limit) return AGPU_OK;
     if (!k_cache || !v_cache || !weights || !block_tables || !kv_lens) return agpu_fail(ctx, AGPU_ERR_NULL_POINTER, "paged_evict: null pointer");
+    const int bytes = paged::cache_element_bytes(cache_type);
+    const paged::Pieces k = paged::cache_pages(k_cache, k_page_stride, n_kv_heads, n_pages, page_size, bytes), v = paged::cache_pages(v_cache, v_page_stride, n_kv_heads, n_pages, page_size, bytes);
+    no = paged::refuse_evicted_memory(k, v, paged::weight_pages(weights, weights_page_stride, n_kv_heads, n_pages, page_size));
+    if (no.code != AGPU_OK) return agpu_fail(ctx, no.code, "paged_evict: %s", no.why);
     agpu_on_device here(ctx);
     if (here.rc != AGPU_OK) return here.rc;
-    const int bytes = paged::cache_element_bytes(cache_type);
     const EvictArgs p = {static_cast<char *>(k_cache), static_cast<char *>(v_cache), k_page_stride * bytes, v_page_stride * bytes, weights, weights_page_stride, block_tables, kv_lens,
                          n_kv_heads, n_pages, table_width, held, limit, keep, recent, sinks, PageDiv::of(page_size)};
     const size_t lds = (size_t)((held + 63) / 64) * sizeof(uint64_t);
@@ -387,8 +390,15 @@ AGPU_EXPORT int32_t agpu_paged_trim(agpu_ctx *ctx, const int32_t *kv_lens, const
     if (no.code != AGPU_OK) return agpu_fail(ctx, no.code, "paged_trim: %s", no.why);
     if ((batch > 0 && (!kv_lens || !kv_lens_out || !evicted || (!block_tables && table_width > 0))) || (!free_pages && stack_size > 0) || !n_free || !n_free_out)
         return agpu_fail(ctx, AGPU_ERR_NULL_POINTER, "paged_trim: null pointer");
-    if ((batch > 0 && (kv_lens_out == kv_lens || evicted == kv_lens)) || n_free_out == n_free)
-        return agpu_fail(ctx, AGPU_ERR_UNSUPPORTED, "paged_trim: the outputs do not overlap the inputs");
+    using paged::Pieces;
+    constexpr int64_t kInt = sizeof(int32_t);
+    const Pieces lens = Pieces::one(kv_lens, batch * kInt), tables = Pieces::one(block_tables, (int64_t)batch * table_width * kInt), count = Pieces::one(n_free, kInt);
+    const Pieces out[4] = {Pieces::one(kv_lens_out, batch * kInt), Pieces::one(evicted, batch * kInt), Pieces::one(n_free_out, kInt), Pieces::one(free_pages, stack_size * kInt)};
+    for (int i = 0; i < 4 && no.code == AGPU_OK; ++i) {
+        no = paged::refuse_shared_memory(out[i], {lens, tables, count}, "the outputs do not overlap the inputs");
+        for (int j = 0; j < i && no.code == AGPU_OK; ++j) no = paged::refuse_shared_memory(out[i], {out[j]}, "the outputs do not overlap");
+    }
+    if (no.code != AGPU_OK) return agpu_fail(ctx, no.code, "paged_trim: %s", no.why);
     agpu_on_device here(ctx);
     if (here.rc != AGPU_OK) return here.rc;
     const TrimArgs p = {kv_lens, block_tables, n_free, free_pages, kv_lens_out, evicted, n_free_out, batch, table_width, stack_size, limit, keep, PageDiv::of(page_size)};

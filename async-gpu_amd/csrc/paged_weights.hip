@@ -301,6 +301,12 @@ AGPU_EXPORT int32_t agpu_paged_attention_weights(agpu_ctx *ctx, const float *q, 
     if (tokens == 0 || batch == 0) return AGPU_OK;
     if (!q || !k_cache || !v_cache || !weights || !kv_lens || !o || (!block_tables && table_width > 0))
         return agpu_fail(ctx, AGPU_ERR_NULL_POINTER, "paged_attention_weights: null pointer");
+    const int bytes = paged::cache_element_bytes(cache_type);
+    no = paged::refuse_shared_memory(paged::weight_pages(weights, weights_page_stride, n_kv_heads, n_pages, page_size),
+                                     {paged::cache_pages(k_cache, k_page_stride, n_kv_heads, n_pages, page_size, bytes), paged::cache_pages(v_cache, v_page_stride, n_kv_heads, n_pages, page_size, bytes),
+                                      paged::Pieces::rows(q, tokens, n_heads, q_token_stride, q_head_stride), paged::Pieces::one(o, (int64_t)tokens * n_heads * DH * sizeof(float))},
+                                     "the weights share memory with another argument");
+    if (no.code != AGPU_OK) return agpu_fail(ctx, no.code, "paged_attention_weights: %s", no.why);
     agpu_on_device here(ctx);
     if (here.rc != AGPU_OK) return here.rc;
     const PagedAttn p = paged_attn(q, q_token_stride, q_head_stride, k_cache, v_cache, k_page_stride, v_page_stride, block_tables, kv_lens, query_start, o, tokens, batch, n_heads,

@@ -18,6 +18,7 @@
 #include <vector>
 
 #include "../../include/agpu.h"
+#include "paged.h"
 
 namespace {
 
@@ -506,6 +507,16 @@ PyObject *paged_kv_append(PyObject *const *a) {
     return Py_BuildValue("(OO)", a[2], a[3]);
 }
 
+// Whether two tensors have memory in common, and not only the storage they lie in: caches, their weights and rows may be parts of one arena.  (A lazy clone is of another storage.)
+paged::Pieces memory(const at::Tensor &t) {
+    const int64_t size = t.element_size();
+    const void *const at = t.const_data_ptr();
+    if (t.numel() == 0) return paged::Pieces::one(at, 0);
+    if (t.dim() == 3 && t.scalar_type() == at::kFloat && t.size(2) == 64 && t.stride(2) == 1) return paged::Pieces::rows(static_cast<const float *>(at), t.size(0), t.size(1), t.stride(0), t.stride(1));
+    return paged::Pieces::pages(at, t.size(0), t.stride(0) * size, t.numel() / t.size(0) * size);  // (each contiguous)
+}
+bool share_memory(const at::Tensor &a, const at::Tensor &b) { return a.is_alias_of(b) && paged::share(memory(a), memory(b)); }
+
 // What paged_attention and the operators like it have in common: q, k_cache, v_cache; then block_tables, kv_lens, query_start; out behind them.
 struct Attends {
     const at::Tensor &kc, &vc, &q, &tables, &lens, &start;
@@ -522,7 +533,7 @@ struct Attends {
             const at::Tensor &o = typed(out, at::kFloat, {tokens, heads, q.size(2)}, "out [tokens, n_heads, d_head]");
             if (!o.is_contiguous()) shape_err("contiguous out", "strides " + str(o.strides()));
             for (const at::Tensor *t : {&q, &kc, &vc})
-                if (o.is_alias_of(*t)) shape_err("out with memory of its own", "that of an input");
+                if (share_memory(o, *t)) shape_err("out with memory of its own", "that of an input");
         }
     }
     // (after what else there is to check of shapes)
@@ -573,8 +584,8 @@ PyObject *paged_attention_weights(PyObject *const *a) {
     const Attends c(a[0], a[1], a[2], a[4], a[5], a[6], a[9]);
     const at::Tensor &w = weights_of(a[3], c.kc);
     for (const at::Tensor *t : {&c.q, &c.kc, &c.vc})
-        if (w.is_alias_of(*t)) shape_err("weights with memory of their own", "that of another argument");
-    if (c.given && w.is_alias_of(tensor(a[9]))) shape_err("weights with memory of their own", "that of another argument");
+        if (share_memory(w, *t)) shape_err("weights with memory of their own", "that of another argument");
+    if (c.given && share_memory(w, tensor(a[9]))) shape_err("weights with memory of their own", "that of another argument");
     at::Tensor o = c.out(a[9], w);
     float *const op = written(o), *const wp = written(w);
     call(lib.agpu_paged_attention_weights_, context(c.q), data(c.q), c.q.stride(0), c.q.stride(1), c.kc.const_data_ptr(), c.vc.const_data_ptr(), page_stride(c.kc), page_stride(c.vc), wp,
@@ -589,6 +600,9 @@ PyObject *paged_evict(PyObject *const *a) {
     const at::Tensor &kc = pages(a[0], "k_cache [n_pages, n_kv_heads, page_size, d_head]"), &vc = pages(a[1], "v_cache [n_pages, n_kv_heads, page_size, d_head]");
     same_cache(kc, vc);
     const at::Tensor &w = weights_of(a[2], kc), &tables = ints(a[3], {-1, -1}, "block_tables [batch, width]"), &lens = ints(a[4], {tables.size(0)}, "kv_lens [batch]");
+    for (const at::Tensor *t : {&kc, &vc})
+        if (share_memory(w, *t)) shape_err("weights with memory of their own", "that of a cache");
+    if (share_memory(kc, vc) && (kc.const_data_ptr() != vc.const_data_ptr() || page_stride(kc) != page_stride(vc))) shape_err("k_cache and v_cache apart, or the same", "caches that share memory");
     together(kc, vc, w, tables, lens);
     const int32_t limit = i32(a[5]), keep = i32(a[6]), recent = i32(a[7]), sinks = i32(a[8]);
     void *const kp = kc.mutable_data_ptr(), *const vp = vc.mutable_data_ptr();

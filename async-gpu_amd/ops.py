@@ -233,7 +233,8 @@ def paged_attention_shared(q, k_cache, v_cache, prefix_tables, prefix_lens, pref
 
 def paged_attention_weights(q, k_cache, v_cache, weights, block_tables, kv_lens, query_start=None, window=0, sinks=0, out=None):
     """paged_attention that also adds up, in place, what weight (share of the softmax) each key was given: weights [n_pages, n_kv_heads, page_size] float32, over the rows of the call
-    and the query heads of a K/V head.  Keys of the call's own rows begin at zero.  A page belongs to one request only.  Returns (out, weights)."""
+    and the query heads of a K/V head.  Keys of the call's own rows begin at zero.  A page belongs to one request only.  Caches, weights, rows and out may be parts of one
+    allocation that do not overlap.  Returns (out, weights)."""
     return _native.paged_attention_weights(q, k_cache, v_cache, weights, block_tables, kv_lens, query_start, window, sinks, out)
 
 

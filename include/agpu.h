@@ -442,7 +442,7 @@ int32_t agpu_paged_attention_shared(agpu_ctx *ctx, const float *q, int64_t q_tok
  * agpu_paged_attention that adds up its weights: the weight of key j in a row is its share of the softmax, in 0 .. 1; those of the call's rows, and of the query heads of
  * a K/V head, are added to what the key has.  Keys of the request's rows (the last query_start[b + 1] - query_start[b] of its kv_lens[b] positions, whether or not q has all of
  * the rows) begin at zero.  Requests without a row in q, and keys that no row sees, keep what they have.  A page belongs to one request only.  The order of a sum is fixed:
- * the same call gives the same bits. */
+ * the same call gives the same bits.  The weights share no memory with K, V, q or o; they may lie between pages of K and V. */
 int32_t agpu_paged_attention_weights(agpu_ctx *ctx, const float *q, int64_t q_token_stride, int64_t q_head_stride, const void *k_cache,
                                      const void *v_cache, int64_t k_page_stride, int64_t v_page_stride, float *weights,
                                      int64_t weights_page_stride, const int32_t *block_tables, const int32_t *kv_lens,
@@ -454,7 +454,8 @@ int32_t agpu_paged_attention_weights(agpu_ctx *ctx, const float *q, int64_t q_to
  * below `keep`; the others go, K, V and weight, in order into the places of evicted ones.  Places from `keep` on are left as they were, and kv_lens too: it is agpu_paged_trim that
  * shortens them, for all layers.  Order among places is lost except that the first `sinks` stay where they are and that what came since the last time is behind the rest:
  * `recent` means the latest positions as long as limit - keep >= recent, and windows of agpu_paged_attention no longer mean distances.
- * A page belongs to one request only; a row of the table stands for 2^20 positions at most. */
+ * A page belongs to one request only; a row of the table stands for 2^20 positions at most.  K, V and the weights share no memory (pages of one may lie between those of another), except that
+ * K and V may be one and the same. */
 int32_t agpu_paged_evict(agpu_ctx *ctx, void *k_cache, void *v_cache, int64_t k_page_stride, int64_t v_page_stride, float *weights,
                          int64_t weights_page_stride, const int32_t *block_tables, const int32_t *kv_lens, int32_t batch, int32_t n_kv_heads,
                          int32_t n_pages, int32_t page_size, int32_t table_width, int32_t limit, int32_t keep, int32_t recent, int32_t sinks,
@@ -463,7 +464,7 @@ int32_t agpu_paged_evict(agpu_ctx *ctx, void *k_cache, void *v_cache, int64_t k_
  * [batch] how many positions that is less, to be added up by a caller whose embeddings go by position; the pages behind `keep` go onto the stack free_pages [stack_size] of n_free [1]
  * pages, in the order of requests and positions (what has no place there is lost), n_free_out [1] of them.  They go there as block_tables has them, as those of requests that end do in
  * agpu_paged_plan: entries from `keep` on have to be pages of the cache.  (An id outside it, whose keys the other operators take for missing, would be given to a request later: what that
- * one appends there is kept nowhere, and not seen.)  The outputs do not overlap the inputs.  4096 requests at most. */
+ * one appends there is kept nowhere, and not seen.)  The outputs, free_pages among them, overlap neither the inputs nor one another.  4096 requests at most. */
 int32_t agpu_paged_trim(agpu_ctx *ctx, const int32_t *kv_lens, const int32_t *block_tables, int32_t *free_pages, const int32_t *n_free, int32_t *kv_lens_out,
                         int32_t *evicted, int32_t *n_free_out, int32_t batch, int32_t table_width, int32_t stack_size, int32_t page_size, int32_t limit,
                         int32_t keep);
