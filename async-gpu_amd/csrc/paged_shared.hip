@@ -8,7 +8,8 @@
 // What bounds it: 64 requests of 100 own keys on average, 25 heads, bf16, behind 4000 keys take 33 us, of which the bytes of K and V, each read once, are 13.  The prefix's
 // half is 17: 1 until all workgroups are there, 3 until a tile's rows are known (requests counted by prefix, runs cut, rows listed: loads, sums and divisions that wait for one
 // another), 8 to 10 for 3.5 tiles of 32 keys a wave (2900 cycles one after the other: 800 from LDS to operands, 400 the next tile's request, 460 products, 420 softmax, 900 weights and
-// products; the SIMDs issue a third of the time), 1.5 to join the waves, 0.5 for the last stores.  The other half is what paged_attention takes for the own pages (15) and 2 for the prefix's runs.
+// products; the SIMDs issue a third of the time), 1.5 to join the waves, 0.5 for the last stores.  (Two waves a SIMD, as both ways share one budget of registers; over
+// fp32 20 of them are spilled.  Runs go by the prefix's length: a window leaves them as they are, and those that it hides are empty.)  The other half is what paged_attention takes for the own pages (15) and 2 for the prefix's runs.
 #include "paged_kernels.h"
 
 namespace {

@@ -1,9 +1,9 @@
 // Attention that adds up the weight that each key was given (over the rows of a call and the query heads of a K/V head), d_head = 64: the kernels of paged_attention.hip, and
 //   one row a request   its scores stay in scratch (4 bytes a key and query head beside 128 to 512 of K and V).  The workgroup that joins the row's runs, which knows m and l by then,
-//                       turns them into weights, or, where there are many keys, a launch of its own: 64 tokens of 1 to 4096 keys, 32 heads over 8, f16, 32 + 8 us (attention alone 29).
+//                       turns them into weights, or, where there are many keys, a launch of its own: 64 tokens of 1 to 4096 keys, 32 heads over 8, f16, 41 us (attention alone 28).
 //   more                m and 1 / l of the rows stay in scratch, and paged_weights_kernel forms their scores once more on the matrix cores, a wave's 32 keys in registers
-//                       against all rows that see them, 64 at a time: a key's sum is one wave's, in the order of the rows.  4 chunks of 512 rows over 2048 keys, 16 heads, fp32, 59 us
-//                       beside 106 of attention: matrix instructions 33 % and vector instructions 38 % of the SIMDs' cycles, which overlap little; matrix instructions alone would take 32.
+//                       against all rows that see them, 64 at a time: a key's sum is one wave's, in the order of the rows.  4 chunks of 512 rows over 2048 keys, 16 heads, fp32, 53 us
+//                       beside 102 of attention: matrix instructions 33 % and vector instructions 38 % of the SIMDs' cycles, which overlap little; matrix instructions alone would take 32.
 //                       Half of what it was to begin with went to conflicts between LDS banks (66 us).
 #include "paged_kernels.h"
 
@@ -311,8 +311,8 @@ AGPU_EXPORT int32_t agpu_paged_attention_weights(agpu_ctx *ctx, const float *q, 
     if (here.rc != AGPU_OK) return here.rc;
     const PagedAttn p = paged_attn(q, q_token_stride, q_head_stride, k_cache, v_cache, k_page_stride, v_page_stride, block_tables, kv_lens, query_start, o, tokens, batch, n_heads,
                                    n_kv_heads, n_pages, page_size, table_width, window, sinks, ctx->strict_sync);
-    // Scores lie by requests, or by places of the cache, whichever are fewer (a large cache, or tables much wider than requests are long).  Without room for them they are formed again:
-    // 64 tokens of 1 to 4096 keys, 32 heads over 8, f16, 62 us, 41 with scores.
+    // Scores lie by requests, or by places of the cache, whichever are fewer (a large cache, or tables much wider than requests are long), as far as the arguments' sizes say: lengths are on
+    // the device.  Without room for them they are formed again: 64 tokens of 1 to 4096 keys, 32 heads over 8, f16, 59 us, 41 with scores.
     const int64_t longest = paged::longest_row(p.held, window, sinks), by_place = (int64_t)n_pages * page_size, by_request = batch * longest;
     const paged::WeightsRoom room = paged::weights_room((int64_t)tokens * n_heads, std::min(by_place, by_request) * n_heads, n_heads / n_kv_heads, ctx->ws_bytes);
     if (room.bytes == 0) return agpu_fail(ctx, AGPU_ERR_WORKSPACE, "paged_attention_weights: %d rows of %d heads need a larger scratch", tokens, n_heads);

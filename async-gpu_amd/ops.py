@@ -227,7 +227,8 @@ def paged_attention(q, k_cache, v_cache, block_tables, kv_lens, query_start=None
 def paged_attention_shared(q, k_cache, v_cache, prefix_tables, prefix_lens, prefix_of, block_tables, kv_lens, query_start=None, window=0, sinks=0, out=None):
     """paged_attention of requests that begin alike: request b is behind prefix prefix_of[b] (none: -1), whose prefix_lens[i] keys on the pages prefix_tables[i] the
     cache holds once, and which are read once for all requests behind it.  kv_lens, block_tables and query_start are about the requests' own pages; window and sinks
-    are about positions with the prefix.  256 prefixes at most; their pages are the caller's (no request of paged_plan that ends gives them back)."""
+    are about positions with the prefix.  256 prefixes at most; their pages are the caller's (no request of paged_plan that ends gives them back).  Weights are not added up
+    behind a prefix: such requests have no budget."""
     return _native.paged_attention_shared(q, k_cache, v_cache, prefix_tables, prefix_lens, prefix_of, block_tables, kv_lens, query_start, window, sinks, out)
 
 
@@ -241,7 +242,7 @@ def paged_attention_weights(q, k_cache, v_cache, weights, block_tables, kv_lens,
 def paged_evict(k_cache, v_cache, weights, block_tables, kv_lens, limit, keep, recent=0, sinks=0):
     """Cuts requests of more than `limit` positions down to `keep`, in place, each K/V head by itself: the first `sinks` stay, the last `recent`, and of the others those with the most
     weight (of equal ones the first).  What stays keeps its place below `keep`, or moves into that of an evicted one.  For every layer; paged_trim then shortens the
-    lengths.  limit - keep >= recent keeps the latest positions the last ones.  Returns (k_cache, v_cache, weights)."""
+    lengths.  limit - keep >= recent keeps the latest positions the last ones.  A row of the tables stands for 2^20 positions at most.  Returns (k_cache, v_cache, weights)."""
     return _native.paged_evict(k_cache, v_cache, weights, block_tables, kv_lens, limit, keep, recent, sinks)
 
 

@@ -428,7 +428,7 @@ int32_t agpu_paged_attention(agpu_ctx *ctx, const float *q, int64_t q_token_stri
  *                                                                    counts as far as the table has pages for it
  *   prefix_of [batch]                                                which of them a request is behind; outside 0 .. n_prefix - 1: none
  * Place p of a request's own kv_lens is position prefix_lens[prefix_of[b]] + p, for what a row sees: every key up to its own position, with window > 0 only those
- * nearer than that or among the first `sinks` positions, which are the prefix's.  A prefix is nobody's in agpu_paged_plan's view, or a request of its own that has no new tokens: its
+ * nearer than that or among the first `sinks` positions, which are the prefix's.  Nothing adds up weights behind a prefix (agpu_paged_attention_weights takes none).  A prefix is nobody's in agpu_paged_plan's view, or a request of its own that has no new tokens: its
  * pages stay until the caller gives them back.  The rows of all requests behind a prefix go through the matrix cores there, as those of a request with more than eight do. */
 int32_t agpu_paged_attention_shared(agpu_ctx *ctx, const float *q, int64_t q_token_stride, int64_t q_head_stride, const void *k_cache,
                                     const void *v_cache, int64_t k_page_stride, int64_t v_page_stride, const int32_t *prefix_tables,
