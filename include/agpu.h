@@ -427,7 +427,7 @@ int32_t agpu_paged_attention(agpu_ctx *ctx, const float *q, int64_t q_token_stri
  *   prefix_tables [n_prefix][prefix_width], prefix_lens [n_prefix]   pages and lengths of the prefixes (256 at most), like block_tables and kv_lens; a length
  *                                                                    counts as far as the table has pages for it
  *   prefix_of [batch]                                                which of them a request is behind; outside 0 .. n_prefix - 1: none
- * Place p of a request's own kv_lens is position prefix_lens[prefix_of[b]] + p, for what a row sees: every key up to its own position, with window > 0 only those
+ * Place p of a request's own kv_lens (2^30 at most, which is what a table can stand for) is position prefix_lens[prefix_of[b]] + p, for what a row sees: every key up to its own position, with window > 0 only those
  * nearer than that or among the first `sinks` positions, which are the prefix's.  Nothing adds up weights behind a prefix (agpu_paged_attention_weights takes none).  A prefix is nobody's in agpu_paged_plan's view, or a request of its own that has no new tokens: its
  * pages stay until the caller gives them back.  The rows of all requests behind a prefix go through the matrix cores there, as those of a request with more than eight do. */
 int32_t agpu_paged_attention_shared(agpu_ctx *ctx, const float *q, int64_t q_token_stride, int64_t q_head_stride, const void *k_cache,
